@@ -1,0 +1,520 @@
+// Attention over selected tokens: what follows the selector. Every query token t attends to the cache rows its selection names,
+//   o[t, h] = sum_j p_j v[row_j, h / g] / sum_j p_j,   p_j = exp(scale * q[t, h] . k[row_j, h / g] - max),   row_j = indices[t, j]
+// g query heads to a key head, negative indices left out, a token that names none gets zeros and a log-sum of -inf.
+// k and v are of q's type, or e4m3 with a 32-bit scale per row and head. (The reference ends with the indices.)
+//
+// attend_narrow_kernel, up to 16 query heads to a key head at a time. A row of k or v is used by those heads alone, so reading
+// the rows bounds it: 16 flop a byte at most in 16 bits, 32 in fp8, where the tensor cores want over 200. The rows lie anywhere,
+// and nothing but their own heads shares them, so they go straight from memory into the registers that mma.sync reads, without
+// shared memory in between: a warp takes blocks of keys, 16 at a time, all their bytes in flight at once.
+//   q.k: the contraction's order is free, so a lane's 16-byte piece of a key row serves as B fragments of consecutive steps
+//        and q is loaded in the same order.
+//   p.v: the contraction runs over keys, so B fragments pair two rows' elements: a lane loads the same 16-byte piece of the
+//        four rows its fragments hold and interleaves them (byte permutes); which column a fragment's lane stands for is free too.
+// A warp keeps running maxima and sums (one pass); the warps of a CTA are joined in shared memory, the CTAs of a cluster (few
+// tokens: a token's keys are split over up to 8 CTAs) through distributed shared memory. No workspace.
+//   e4m3 rows are widened to fp16, which holds every code exactly; a row's k scale multiplies its score, its v scale its weight.
+//   Queries are brought to magnitudes below 2 by a power of two per head first (fp16 has fewer exponents than bf16; what is
+//   lost lies 2^-25 below the head's largest). Weights p * v scale become fp16 relative to the largest v scale seen: 2^-12 of a
+//   weight's size, 2^-25 of the largest for the smallest ones. 16-bit caches: weights are rounded to the cache's type.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "../../include/fftopk.h"
+#include "fftopk_host.h"
+#include "fftopk_internal.h"
+#include "fftopk_rows.cuh"
+
+namespace fftopk {
+namespace {
+
+namespace cg = cooperative_groups;
+
+struct AttendParams {
+  const void* q;
+  int64_t q_token, q_head;  // strides, elements
+  const void* k;
+  const void* v;
+  int64_t k_slot, k_head, v_slot, v_head;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t ks_slot, ks_head, vs_slot, vs_head;
+  const int32_t* indices;
+  int64_t idx_row;
+  const int32_t* offsets;
+  void* out;
+  int64_t out_token, out_head;
+  float* lse;  // [T, q heads]
+  int64_t slots;
+  int32_t tokens, kv_heads, group, picks;
+  int32_t head_blocks;  // blocks of 16 query heads per key head
+  float scale_log2;     // softmax scale * log2(e)
+  uint32_t* status;
+};
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kHeadsM = 16;  // query heads a CTA works on: rows of the MMA
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int kMaxCluster = 8;
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(kAll, x, 1));
+  return fmaxf(x, __shfl_xor_sync(kAll, x, 2));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  x += __shfl_xor_sync(kAll, x, 1);
+  return x + __shfl_xor_sync(kAll, x, 2);
+}
+
+// Shared memory of a CTA: the warps' accumulators, maxima, sums; then, joined, the CTA's own.
+template <int D>
+struct JoinSmem {
+  float o[kWarps][kHeadsM][D];
+  float m[kWarps][kHeadsM], l[kWarps][kHeadsM];
+  float joined[kHeadsM][D];
+  float jm[kHeadsM], jl[kHeadsM];
+};
+
+// T: type of q and out, and of the cache where kFp8 is false
+template <typename T, bool kFp8, int D>
+__global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid_constant__ AttendParams p) {
+  using M = typename std::conditional<kFp8, __half, T>::type;  // the MMAs' type
+  constexpr int kCE = kFp8 ? 16 : 8;                            // elements of a 16-byte piece
+  constexpr int kPieces = D / (4 * kCE);                        // pieces of a key row per lane (a quad reads a row)
+  constexpr int kVWords = D * (kFp8 ? 1 : 2) / 32;              // 32-bit words of a value row per lane (8 lanes read a row)
+  constexpr int kKeys = kFp8 ? 32 : 16;                         // keys a warp has in flight
+  constexpr int kSub = kKeys / 16;
+  constexpr int kTiles = D / 8;                                 // columns tiles of the output
+  extern __shared__ unsigned char smem_raw[];
+  JoinSmem<D>& sm = *reinterpret_cast<JoinSmem<D>*>(smem_raw);
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, qd = lane & 3;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  uint32_t unit = blockIdx.x / (uint32_t)ctas;
+  const int hb = (int)(unit % (uint32_t)p.head_blocks);
+  unit /= (uint32_t)p.head_blocks;
+  const int kvh = (int)(unit % (uint32_t)p.kv_heads);
+  const int token = (int)(unit / (uint32_t)p.kv_heads);
+  const int heads = min(kHeadsM, p.group - hb * kHeadsM);
+  const int head0 = kvh * p.group + hb * kHeadsM;
+
+  // q fragments in the order of the key pieces: element pair u of piece i of lane qd
+  uint32_t qa[D / 16][4];
+  float qmul[2];  // what the rows' scores are to be multiplied with
+  {
+    const T* q0 = static_cast<const T*>(p.q) + (int64_t)token * p.q_token + (int64_t)head0 * p.q_head;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const bool have = g + 8 * r < heads;
+      const T* q = q0 + (int64_t)(g + 8 * r) * p.q_head;
+      uint2 w[D / 16];
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m) {
+        const int i = m / (kCE / 4), u = m % (kCE / 4);
+        w[m] = have ? *reinterpret_cast<const uint2*>(q + i * 4 * kCE + qd * kCE + 4 * u) : make_uint2(0u, 0u);
+      }
+      qmul[r] = p.scale_log2;
+      if constexpr (kFp8 && !std::is_same<T, __half>::value) {
+        float amax = 0.f;
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) {
+          const float2 a = widen2(w[m].x, T()), b = widen2(w[m].y, T());
+          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
+        }
+        amax = quad_max(amax);
+        const uint32_t e = __float_as_uint(amax) >> 23;  // amax in [2^(e-127), 2^(e-126)); 255: an infinity
+        const uint32_t ee = e == 255u ? 127u : max(1u, min(e, 253u));
+        const float down = __uint_as_float((254u - ee) << 23), up = __uint_as_float(ee << 23);
+        qmul[r] *= up;
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) {
+          const float2 a = widen2(w[m].x, T()), b = widen2(w[m].y, T());
+          w[m] = make_uint2(narrow2(a.x * down, a.y * down, __half()), narrow2(b.x * down, b.y * down, __half()));
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m) qa[m][r] = w[m].x, qa[m][2 + r] = w[m].y;
+    }
+  }
+
+  float o[kTiles][4];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+  float vref = 0.f;  // fp8: the largest v scale seen; weights are relative to it
+
+  const int32_t* idx = p.indices + (int64_t)token * p.idx_row;
+  const int64_t offset = p.offsets != nullptr ? p.offsets[token] : 0;
+  const char* kbase = static_cast<const char*>(p.k) + (int64_t)kvh * p.k_head * (kFp8 ? 1 : 2) + qd * 16;
+  const char* vbase = static_cast<const char*>(p.v) + (int64_t)kvh * p.v_head * (kFp8 ? 1 : 2) + g * (kVWords >= 4 ? 16 : 8);
+  const int64_t kstep = p.k_slot * (kFp8 ? 1 : 2), vstep = p.v_slot * (kFp8 ? 1 : 2);
+  const int blocks = (p.picks + kKeys - 1) / kKeys;
+  const int stride = ctas * kWarps;
+
+  auto pick = [&](int block) {  // lane's index in a block; -1: none
+    const int j = block * kKeys + (lane & (kKeys - 1));
+    return block < blocks && j < p.picks ? idx[j] : -1;
+  };
+  int block = rank * kWarps + warp;
+  int32_t next = pick(block);
+  for (; block < blocks; block += stride) {
+    int64_t slot = next;
+    next = pick(block + stride);
+    bool ok = slot >= 0;
+    if (ok) {
+      slot += offset;
+      if (slot < 0 || slot >= p.slots) {
+        ok = false;
+        if (p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+      }
+    }
+    const unsigned live = __ballot_sync(kAll, ok) & (kKeys == 16 ? 0xffffu : kAll);
+    if (live == 0u) continue;
+    const int row = ok ? (int)slot : -1;
+    // every byte of the block's rows, asked for before any is used
+    uint4 kw[kSub * 2][kPieces];
+    uint32_t vw[kSub * 4][kVWords];
+#pragma unroll
+    for (int n = 0; n < kSub * 2; ++n) {
+      const int r = __shfl_sync(kAll, row, n * 8 + g);
+      const char* at = kbase + (int64_t)r * kstep;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) kw[n][i] = r >= 0 ? ldg16(at + i * 64) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int n = 0; n < kSub * 4; ++n) {  // keys 16 * (n / 4) + {2 qd, 2 qd + 1, 2 qd + 8, 2 qd + 9}
+      const int r = __shfl_sync(kAll, row, (n >> 2) * 16 + 2 * qd + (n & 1) + ((n & 2) << 2));
+      const char* at = vbase + (int64_t)r * vstep;
+      if constexpr (kVWords >= 4) {
+#pragma unroll
+        for (int i = 0; i < kVWords / 4; ++i) {
+          const uint4 x = r >= 0 ? ldg16(at + i * 128) : make_uint4(0u, 0u, 0u, 0u);
+          vw[n][4 * i] = x.x, vw[n][4 * i + 1] = x.y, vw[n][4 * i + 2] = x.z, vw[n][4 * i + 3] = x.w;
+        }
+      } else {
+        const uint2 x = r >= 0 ? ldg8(at) : make_uint2(0u, 0u);
+        vw[n][0] = x.x, vw[n][1] = x.y;
+      }
+    }
+    float ks = 0.f, vs = 0.f;  // the scales of the lane's key
+    if constexpr (kFp8) {
+      if (ok) {
+        ks = __ldg(p.k_scale + (int64_t)row * p.ks_slot + (int64_t)kvh * p.ks_head);
+        vs = __ldg(p.v_scale + (int64_t)row * p.vs_slot + (int64_t)kvh * p.vs_head);
+      }
+    }
+    // scores, in units of log2
+    float sc[kSub * 2][4];
+#pragma unroll
+    for (int n = 0; n < kSub * 2; ++n) {
+      sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m) {
+        const int i = m / (kCE / 4), u = m % (kCE / 4);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&kw[n][i]);
+        if constexpr (kFp8) {
+          mma16816(sc[n], qa[m], e4m3x2_to_half2((uint16_t)w[u]), e4m3x2_to_half2((uint16_t)(w[u] >> 16)), M());
+        } else {
+          mma16816(sc[n], qa[m], w[2 * u], w[2 * u + 1], M());
+        }
+      }
+    }
+    float bmax[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < kSub * 2; ++n) {
+      const unsigned mask = live >> (n * 8 + 2 * qd);
+      float k0 = 1.f, k1 = 1.f;
+      if constexpr (kFp8) {
+        k0 = __shfl_sync(kAll, ks, n * 8 + 2 * qd);
+        k1 = __shfl_sync(kAll, ks, n * 8 + 2 * qd + 1);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        sc[n][2 * r] = (mask & 1u) ? sc[n][2 * r] * k0 * qmul[r] : -INFINITY;
+        sc[n][2 * r + 1] = (mask & 2u) ? sc[n][2 * r + 1] * k1 * qmul[r] : -INFINITY;
+        bmax[r] = fmaxf(bmax[r], fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
+      }
+    }
+    float grow[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float m = fmaxf(mx[r], quad_max(bmax[r]));
+      grow[r] = mx[r] == m ? 1.f : ex2(mx[r] - m);  // (-inf both: nothing seen yet)
+      mx[r] = m;
+    }
+    if constexpr (kFp8) {
+      float top = vs;
+#pragma unroll
+      for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, i));
+      const float ref = fmaxf(vref, top);
+      const float f = ref > vref ? vref / ref : 1.f;
+      vref = ref;
+      vs = ref > 0.f ? vs / ref : 0.f;
+      if (__any_sync(kAll, grow[0] != 1.f || grow[1] != 1.f || f != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          o[i][0] *= grow[0] * f, o[i][1] *= grow[0] * f;
+          o[i][2] *= grow[1] * f, o[i][3] *= grow[1] * f;
+        }
+      }
+    } else {
+      if (__any_sync(kAll, grow[0] != 1.f || grow[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          o[i][0] *= grow[0], o[i][1] *= grow[0];
+          o[i][2] *= grow[1], o[i][3] *= grow[1];
+        }
+      }
+    }
+    sum[0] *= grow[0];
+    sum[1] *= grow[1];
+    uint32_t pa[kSub][4];
+#pragma unroll
+    for (int n = 0; n < kSub * 2; ++n) {
+      float v0 = 1.f, v1 = 1.f;
+      if constexpr (kFp8) {
+        v0 = __shfl_sync(kAll, vs, n * 8 + 2 * qd);
+        v1 = __shfl_sync(kAll, vs, n * 8 + 2 * qd + 1);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float m = mx[r] == -INFINITY ? 0.f : mx[r];
+        const float a = ex2(sc[n][2 * r] - m), b = ex2(sc[n][2 * r + 1] - m);
+        sum[r] += a + b;
+        pa[n >> 1][(n & 1) * 2 + r] = narrow2(a * v0, b * v1, M());
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) {
+      if constexpr (kFp8) {
+        // columns 4 w .. 4 w + 3 of the lane's piece: bytes of rows 2 qd and 2 qd + 1 side by side
+#pragma unroll
+        for (int w = 0; w < kVWords; ++w) {
+          const uint32_t a = vw[4 * s][w], b = vw[4 * s + 1][w], c = vw[4 * s + 2][w], d = vw[4 * s + 3][w];
+          const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
+          const uint32_t cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
+          mma16816(o[4 * w], pa[s], e4m3x2_to_half2((uint16_t)ab0), e4m3x2_to_half2((uint16_t)cd0), M());
+          mma16816(o[4 * w + 1], pa[s], e4m3x2_to_half2((uint16_t)(ab0 >> 16)), e4m3x2_to_half2((uint16_t)(cd0 >> 16)), M());
+          mma16816(o[4 * w + 2], pa[s], e4m3x2_to_half2((uint16_t)ab1), e4m3x2_to_half2((uint16_t)cd1), M());
+          mma16816(o[4 * w + 3], pa[s], e4m3x2_to_half2((uint16_t)(ab1 >> 16)), e4m3x2_to_half2((uint16_t)(cd1 >> 16)), M());
+        }
+      } else {
+#pragma unroll
+        for (int w = 0; w < kVWords; ++w) {
+          const uint32_t a = vw[4 * s][w], b = vw[4 * s + 1][w], c = vw[4 * s + 2][w], d = vw[4 * s + 3][w];
+          mma16816(o[2 * w], pa[s], __byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), M());
+          mma16816(o[2 * w + 1], pa[s], __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632), M());
+        }
+      }
+    }
+  }
+
+  // ---- join: warps, then CTAs ----
+  sum[0] = quad_sum(sum[0]);
+  sum[1] = quad_sum(sum[1]);
+  if (qd == 0) {
+    sm.m[warp][g] = mx[0], sm.m[warp][g + 8] = mx[1];
+    sm.l[warp][g] = sum[0], sm.l[warp][g + 8] = sum[1];
+  }
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // which column tile t of lane n stands for: see the value pieces above
+      const int n = 2 * qd + (e & 1);
+      const int col = kFp8 ? n * (kVWords * 4) + t : (t >> 3) * 64 + n * 8 + (t & 7);
+      sm.o[warp][g + 8 * (e >> 1)][col] = kFp8 ? o[t][e] * vref : o[t][e];
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < kHeadsM * D; i += kThreads) {
+    const int h = i / D, d = i % D;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm.m[w][h]);
+    float acc = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = sm.m[w][h] == m ? 1.f : ex2(sm.m[w][h] - m);  // (a warp without keys: 0 of both; 0 * NaN stays NaN)
+      acc += f * sm.o[w][h][d];
+      l += f * sm.l[w][h];
+    }
+    sm.joined[h][d] = acc;
+    if (d == 0) sm.jm[h] = m, sm.jl[h] = l;
+  }
+  if (ctas > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  for (int i = tid + rank * kThreads; i < heads * D; i += kThreads * ctas) {
+    const int h = i / D, d = i % D;
+    float m = -INFINITY;
+    for (int c = 0; c < ctas; ++c) m = fmaxf(m, ctas > 1 ? *cluster.map_shared_rank(&sm.jm[h], c) : sm.jm[h]);
+    float acc = 0.f, l = 0.f;
+    for (int c = 0; c < ctas; ++c) {
+      const float cm = ctas > 1 ? *cluster.map_shared_rank(&sm.jm[h], c) : sm.jm[h];
+      const float f = cm == m ? 1.f : ex2(cm - m);
+      acc += f * (ctas > 1 ? *cluster.map_shared_rank(&sm.joined[h][d], c) : sm.joined[h][d]);
+      l += f * (ctas > 1 ? *cluster.map_shared_rank(&sm.jl[h], c) : sm.jl[h]);
+    }
+    T* out = static_cast<T*>(p.out) + (int64_t)token * p.out_token + (int64_t)(head0 + h) * p.out_head + d;
+    const float y = l == 0.f ? 0.f : acc / l;
+    if constexpr (std::is_same<T, __half>::value)
+      *out = __float2half_rn(y);
+    else
+      *out = __float2bfloat16_rn(y);
+    if (d == 0 && p.lse != nullptr)
+      p.lse[(int64_t)token * p.kv_heads * p.group + head0 + h] = l == 0.f ? -INFINITY : m * 0.693147180559945309f + logf(l);
+  }
+  if (ctas > 1) cluster.sync();  // (nobody leaves while its memory is read)
+}
+
+DeviceOnce g_attend_once[kMaxDevices];
+int g_attend_sms[kMaxDevices];
+
+template <typename T, bool kFp8, int D>
+int setup_one() {
+  const cudaError_t e =
+      cudaFuncSetAttribute(attend_narrow_kernel<T, kFp8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(JoinSmem<D>));
+  return e == cudaSuccess ? 0 : cuda_fail(e);
+}
+
+int attend_setup(int& sms) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e);
+  if (dev < 0 || dev >= kMaxDevices) return FFTOPK_EDEVICE;
+  const int rc = g_attend_once[dev].run([&] {
+    const cudaError_t e2 = cudaDeviceGetAttribute(&g_attend_sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    if (e2 != cudaSuccess) return cuda_fail(e2);
+    int r = setup_one<__nv_bfloat16, false, 64>();
+    if (!r) r = setup_one<__nv_bfloat16, false, 128>();
+    if (!r) r = setup_one<__nv_bfloat16, true, 64>();
+    if (!r) r = setup_one<__nv_bfloat16, true, 128>();
+    if (!r) r = setup_one<__half, false, 64>();
+    if (!r) r = setup_one<__half, false, 128>();
+    if (!r) r = setup_one<__half, true, 64>();
+    if (!r) r = setup_one<__half, true, 128>();
+    return r;
+  });
+  sms = g_attend_sms[dev];
+  return rc;
+}
+
+template <typename T, bool kFp8, int D>
+cudaError_t launch_narrow(const AttendParams& p, int ctas, int64_t units, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * ctas), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = sizeof(JoinSmem<D>);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)ctas;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attend_narrow_kernel<T, kFp8, D>, p);
+}
+
+template <typename T>
+cudaError_t launch_narrow(const AttendParams& p, bool fp8, int D, int ctas, int64_t units, cudaStream_t stream) {
+  if (fp8) return D == 64 ? launch_narrow<T, true, 64>(p, ctas, units, stream) : launch_narrow<T, true, 128>(p, ctas, units, stream);
+  return D == 64 ? launch_narrow<T, false, 64>(p, ctas, units, stream) : launch_narrow<T, false, 128>(p, ctas, units, stream);
+}
+
+// rows of 16-byte pieces whatever their token (slot) and head; the stride of a lone one says nothing
+bool on16(const void* p, int64_t n, int64_t a, int64_t heads, int64_t b, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (n <= 1 || a * bytes % 16 == 0) && (heads <= 1 || b * bytes % 16 == 0);
+}
+
+}  // namespace
+}  // namespace fftopk
+
+using namespace fftopk;
+
+extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status, void* cuda_stream) {
+  if (a == nullptr) return FFTOPK_EINVAL;
+  if (a->tokens < 0 || a->kv_heads < 0 || a->q_heads < 0 || a->picks < 0 || a->slots < 0) return FFTOPK_EINVAL;
+  if (a->dtype != FFTOPK_DTYPE_FP16 && a->dtype != FFTOPK_DTYPE_BF16) return FFTOPK_EINVAL;
+  if (a->D != 64 && a->D != 128) return FFTOPK_ERANGE;
+  if (a->tokens == 0 || a->q_heads == 0) return FFTOPK_OK;
+  if (a->kv_heads == 0 || a->q_heads % a->kv_heads != 0) return FFTOPK_EINVAL;
+  const bool fp8 = a->k_scale != nullptr;
+  if (fp8 != (a->v_scale != nullptr)) return FFTOPK_EINVAL;
+  if (!a->q || !a->out) return FFTOPK_EINVAL;
+  if (a->picks > 0 && !a->indices) return FFTOPK_EINVAL;
+  if (a->picks > 0 && a->slots > 0 && (!a->k || !a->v)) return FFTOPK_EINVAL;
+  const int ce = fp8 ? 1 : 2;
+  if (!on16(a->q, a->tokens, a->q_token, a->q_heads, a->q_head, 2) || !on16(a->k, a->slots, a->k_slot, a->kv_heads, a->k_head, ce) ||
+      !on16(a->v, a->slots, a->v_slot, a->kv_heads, a->v_head, ce))
+    return FFTOPK_EINVAL;
+  if ((reinterpret_cast<uintptr_t>(a->out) & 1u) || ((reinterpret_cast<uintptr_t>(a->indices) | reinterpret_cast<uintptr_t>(a->offsets) |
+                                                      reinterpret_cast<uintptr_t>(a->lse) | reinterpret_cast<uintptr_t>(a->k_scale) |
+                                                      reinterpret_cast<uintptr_t>(a->v_scale)) & 3u))
+    return FFTOPK_EINVAL;
+  if (a->slots > 0x7fffffff || a->tokens > 0x7fffffff) return FFTOPK_ERANGE;
+  int sms = 0;
+  const int rc = attend_setup(sms);
+  if (rc) return rc;
+
+  AttendParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = a->q, p.q_token = a->q_token, p.q_head = a->q_head;
+  p.k = a->k, p.v = a->v;
+  p.k_slot = a->k_slot, p.k_head = a->k_head, p.v_slot = a->v_slot, p.v_head = a->v_head;
+  p.k_scale = a->k_scale, p.v_scale = a->v_scale;
+  p.ks_slot = a->ks_slot, p.ks_head = a->ks_head, p.vs_slot = a->vs_slot, p.vs_head = a->vs_head;
+  p.indices = a->indices, p.idx_row = a->idx_row, p.offsets = a->offsets;
+  p.out = a->out, p.out_token = a->out_token, p.out_head = a->out_head, p.lse = a->lse;
+  p.slots = a->slots;
+  p.tokens = (int32_t)a->tokens, p.kv_heads = a->kv_heads, p.group = a->q_heads / a->kv_heads, p.picks = a->picks;
+  p.head_blocks = (p.group + kHeadsM - 1) / kHeadsM;
+  p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
+  p.status = status;
+
+  // CTAs a token: as many as keep the device's SMs busy, and no more than give every warp keys
+  const int64_t units = a->tokens * p.kv_heads * p.head_blocks;
+  const int keys = kWarps * (fp8 ? 32 : 16);
+  int ctas = 1;
+  while (ctas < kMaxCluster && units * ctas * 2 <= sms && (int64_t)ctas * keys < p.picks) ctas *= 2;
+  if (units * ctas > 0x7fffffff) return FFTOPK_ERANGE;
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  const cudaError_t e = a->dtype == FFTOPK_DTYPE_BF16 ? launch_narrow<__nv_bfloat16>(p, fp8, a->D, ctas, units, stream)
+                                                      : launch_narrow<__half>(p, fp8, a->D, ctas, units, stream);
+  return e == cudaSuccess ? FFTOPK_OK : cuda_fail(e);
+}

@@ -1,0 +1,167 @@
+// Eight channels of a head row in a lane's registers: loads, stores, conversions and sums over a row's lanes.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+namespace fftopk {
+
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery, 1994): with s = ceil(log2 d) and
+// m = floor(2^32 (2^s - d) / d) + 1, floor(n / d) = (mulhi(n, m) + n) >> s
+struct FastDiv {
+  uint32_t d = 1, m = 1, s = 0;
+  FastDiv() = default;
+  __host__ explicit FastDiv(uint32_t div) : d(div) {
+    while (((uint64_t)1 << s) < d) ++s;
+    m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - d)) / d + 1);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+#endif
+};
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ float2 widen2(uint32_t v, __nv_bfloat16) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ float2 widen2(uint32_t v, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ uint32_t narrow2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t narrow2(float a, float b, __half) {
+  const __half2 r = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <typename T>
+struct Row8 {  // 16-bit types: 16 bytes
+  uint32_t v[4];
+  __device__ __forceinline__ void zero() { v[0] = v[1] = v[2] = v[3] = 0u; }
+  template <bool kVec>
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kVec) {
+      const uint4 r = *reinterpret_cast<const uint4*>(p);
+      v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+    } else {
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (uint32_t)q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
+    }
+  }
+  template <bool kVec>
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kVec) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+    } else {
+      uint16_t* q = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[2 * i] = (uint16_t)v[i], q[2 * i + 1] = (uint16_t)(v[i] >> 16);
+    }
+  }
+  __device__ __forceinline__ void widen(float (&y)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = widen2(v[i], T());
+      y[2 * i] = f.x, y[2 * i + 1] = f.y;
+    }
+  }
+  __device__ __forceinline__ void narrow(const float (&y)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = narrow2(y[2 * i], y[2 * i + 1], T());
+  }
+};
+
+template <>
+struct Row8<float> {  // 32 bytes
+  float v[8];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  }
+  template <bool kVec>
+  __device__ __forceinline__ void load(const float* p) {
+    if constexpr (kVec) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = p[i];
+    }
+  }
+  template <bool kVec>
+  __device__ __forceinline__ void store(float* p) const {
+    if constexpr (kVec) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = v[i];
+    }
+  }
+  __device__ __forceinline__ void widen(float (&y)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = v[i];
+  }
+  __device__ __forceinline__ void narrow(const float (&y)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = y[i];
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(float (&y)[8], const T* p, bool aligned) {
+  Row8<T> r;
+  if (aligned)
+    r.template load<true>(p);
+  else
+    r.template load<false>(p);
+  r.widen(y);
+}
+
+// The lanes of the calling group, as a mask of its warp: groups of one warp may be at work on parts with different norms, each
+// behind branches of its own, so a group's shuffles name its own lanes alone.
+template <int kLanes>
+__device__ __forceinline__ uint32_t group_mask() {
+  if constexpr (kLanes == 32) return 0xffffffffu;
+  return ((1u << (kLanes & 31)) - 1u) << (threadIdx.x & 31u & ~(uint32_t)(kLanes - 1));
+}
+template <int kLanes>
+__device__ __forceinline__ float group_sum(float x, uint32_t mask) {
+#pragma unroll
+  for (int i = kLanes / 2; i > 0; i >>= 1) x += __shfl_xor_sync(mask, x, i);
+  return x;
+}
+template <int kLanes>
+__device__ __forceinline__ float group_max(float x, uint32_t mask) {
+#pragma unroll
+  for (int i = kLanes / 2; i > 0; i >>= 1) x = fmaxf(x, __shfl_xor_sync(mask, x, i));
+  return x;
+}
+
+// e4m3(y * inv), to nearest even; beyond 448 and infinities become 448, NaN stays NaN
+__device__ __forceinline__ uint2 to_e4m3(const float (&y)[8], float inv) {
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * inv, y[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint16_t v) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
+  return (uint32_t)r.x | (uint32_t)r.y << 16;
+}
+__device__ __forceinline__ void from_e4m3(float (&y)[8], uint2 codes) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = i < 2 ? codes.x : codes.y;
+    const float2 f = widen2(e4m3x2_to_half2((uint16_t)(w >> (16 * (i & 1)))), __half());
+    y[2 * i] = f.x, y[2 * i + 1] = f.y;
+  }
+}
+
+#endif  // __CUDACC__
+
+}  // namespace fftopk

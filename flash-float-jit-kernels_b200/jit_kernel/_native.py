@@ -22,6 +22,7 @@ ST_INTERNAL = 2
 ST_PEER_TIMEOUT = 4
 ST_GUESS_MISSED = 8
 ST_CHECK = 16
+ST_BAD_INDEX = 32
 
 E_RANGE = -4
 
@@ -52,6 +53,9 @@ EXPORTS = (
     "fftopk_indexer_workspace_bytes",
     "fftopk_indexer_topk2048",
     "fftopk_indexer_topk2048_fp8",
+    "fftopk_head_rows",
+    "fftopk_cache_read",
+    "fftopk_sparse_attention",
     "fftopk_probe_read_bandwidth",
     "fftopk_key_of",
     "fftopk_plan",
@@ -158,6 +162,15 @@ def lib() -> ctypes.CDLL:
     L.fftopk_indexer_topk2048_fp8.argtypes = [c.c_void_p, c.c_void_p, c.c_int64, c.c_void_p, c.c_int64, c.c_void_p, c.c_int32,
                                               c.c_int64, c.c_void_p, c.c_void_p, c.c_uint32, c.c_void_p, c.c_int64,
                                               c.c_void_p, c.c_void_p, c.c_size_t, c.c_void_p, c.c_void_p]
+    L.fftopk_head_rows.restype = c.c_int
+    L.fftopk_head_rows.argtypes = [c.c_char_p, c.c_int32, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_void_p, c.c_int64,
+                                   c.c_int32, c.c_int32, c.c_void_p, c.c_void_p]
+    L.fftopk_cache_read.restype = c.c_int
+    L.fftopk_cache_read.argtypes = [c.c_void_p, c.c_int64, c.c_int64, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_int64,
+                                    c.c_int64, c.c_void_p, c.c_int64, c.c_int64, c.c_void_p, c.c_void_p, c.c_int32, c.c_void_p,
+                                    c.c_void_p]
+    L.fftopk_sparse_attention.restype = c.c_int
+    L.fftopk_sparse_attention.argtypes = [c.c_char_p, c.c_void_p, c.c_void_p]
     L.fftopk_probe_read_bandwidth.restype = c.c_int
     L.fftopk_probe_read_bandwidth.argtypes = [c.c_void_p, c.c_size_t, c.c_size_t, c.c_void_p, c.POINTER(c.c_size_t),
                                               c.c_void_p]

@@ -1,0 +1,92 @@
+"""A cache of keys or values in fp8: e4m3 codes [slots, heads, D] with a float32 scale per slot and head, quantised as it is
+written and widened as it is read (no counterpart in the reference). A slot is a token's row; which one a token has is the
+caller's affair (a page table's entry, a sequence's base plus the position). ``sparse_attention`` reads such caches as they are."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _native
+from .norm_rope import _DTYPES, FP8, _check_cache, _check_call, _check_rows, _check_vector, _no_grad, _part, _rows
+from .topk_indexer import _launch
+
+
+def cache_write(
+    k: torch.Tensor,
+    slots: torch.Tensor,
+    k_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v: Optional[torch.Tensor] = None,
+    v_cache: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+) -> None:
+    """
+    Quantise k - and v, in the same launch - into rows `slots` of their caches.
+    Args:
+        k, v: [T, H, D] of one type (float16, bfloat16, float32), CUDA, unit inner stride; D a multiple of 8 up to 256.
+        slots: int32 [T]. A negative slot is padding: that token is not written. A slot beyond the cache is not written either
+            and shows up in kernel_status(). The slots of one call differ from one another.
+        k_cache, v_cache: float8_e4m3fn [slots, H, D], unit inner stride; k_scale, v_scale: float32 [slots, H].
+    A row's largest finite magnitude becomes 448 (scale = amax / 448, codes to nearest even); infinities become the largest code,
+    NaN stays NaN. Rows that no slot names keep what they hold.
+    """
+    if k.dim() != 3:
+        raise RuntimeError("k must be [tokens, heads, D]")
+    T, H, D = k.shape
+    idx = _check_call(k, None, None, D)
+    _check_rows(k, "k", idx, k.dtype, T, D)
+    _check_vector(slots, "slots", idx, T)
+    _check_cache(k_cache, k_scale, "k", idx, H, D)
+    _no_grad(k, v)
+    parts = [_part(k, k_cache, scale=k_scale, slots=slots)]
+    if (v is None) != (v_cache is None) or (v is None) != (v_scale is None):
+        raise RuntimeError("v, v_cache and v_scale go together")
+    if v is not None:
+        _check_rows(v, "v", idx, k.dtype, T, D)
+        _check_cache(v_cache, v_scale, "v", idx, v.size(1), D)
+        parts.append(_part(v, v_cache, scale=v_scale, slots=slots))
+    if T:
+        _rows(idx, parts, T, D, k.dtype, None, None, False)
+
+
+def cache_read(
+    cache: torch.Tensor,
+    scale: torch.Tensor,
+    slots: torch.Tensor,
+    *,
+    offsets: Optional[torch.Tensor] = None,
+    dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """
+    Rows of a quantised cache, gathered and widened.
+    Args:
+        cache, scale: float8_e4m3fn [slots, H, D] and float32 [slots, H], as cache_write fills them.
+        slots: int32 [B, K] or [K], contiguous: the rows to read, -1 for none (zeros) - what the selector hands out, for instance.
+        offsets: int32 [B] (with slots [B, K]): added to the non-negative entries of row b.
+        dtype: float16, bfloat16 or float32.
+    Returns:
+        slots.shape + [H, D], contiguous. A row beyond the cache gives zeros and shows up in kernel_status().
+    """
+    if not cache.is_cuda or cache.dim() != 3:
+        raise RuntimeError("cache must be a CUDA tensor [slots, heads, D]")
+    idx = cache.get_device()
+    n, H, D = cache.shape
+    _check_cache(cache, scale, "", idx, H, D)
+    if D % 8 or not 8 <= D <= 256:
+        raise RuntimeError("D must be a multiple of 8 up to 256")
+    if dtype not in _DTYPES:
+        raise RuntimeError("dtype must be float16, bfloat16 or float32")
+    if slots.dtype != torch.int32 or slots.dim() not in (1, 2) or not slots.is_contiguous() or slots.get_device() != idx:
+        raise RuntimeError("slots must be a contiguous int32 tensor [B, K] or [K] on the cache's device")
+    rows, per_row = (1, slots.size(0)) if slots.dim() == 1 else slots.shape
+    if offsets is not None:
+        if slots.dim() != 2:
+            raise RuntimeError("offsets go with slots [B, K]")
+        _check_vector(offsets, "offsets", idx, rows)
+    out = torch.empty((*slots.shape, H, D), dtype=dtype, device=cache.device)
+    if out.numel():
+        _launch(_native.lib().fftopk_cache_read, "fftopk_cache_read", idx, cache.data_ptr(), cache.stride(0), cache.stride(1), n, H, D,
+                scale.data_ptr(), scale.stride(0), scale.stride(1), slots.data_ptr(), rows, per_row,
+                None if offsets is None else offsets.data_ptr(), out.data_ptr(), _DTYPES[dtype])
+    return out

@@ -46,6 +46,8 @@ enum {
                                /* was selected from scratch (informational, result is exact)   */
   FFTOPK_ST_CHECK = 16,        /* checked build (-DFFTOPK_CHECKED) only: an index the logic     */
                                /* guarantees to be in range was not; the access was skipped    */
+  FFTOPK_ST_BAD_INDEX = 32,    /* a slot, an index or a position beyond its cache or table; the access  */
+                               /* was left out (head rows, cache rows, attention: see there)   */
 };
 
 /* Library version: major*10000 + minor*100 + patch. */
@@ -348,6 +350,102 @@ int fftopk_indexer_topk2048(const void* q, const void* k_cache, int64_t k_rows_p
                             uint32_t margin, float* logits, int64_t logits_stride, int32_t* out_idx,
                             void* d_workspace, size_t workspace_bytes, uint32_t* status,
                             void* cuda_stream);
+
+/*
+ * Head rows: norm, rotation and quantisation of q, k and v in one pass - what lies in front of the indexer and of the
+ * attention behind the selector. No counterpart in the reference, which starts from finished logits.
+ * A call works on up to three parts (q, k, v in any order). A part is [tokens, heads, D] activations; each of its head rows is
+ *   normed     FFTOPK_NORM_RMS: x * rsqrt(mean(x^2) + eps) * weight; FFTOPK_NORM_LAYER: (x - mean) * rsqrt(var + eps) * weight;
+ *              + bias (weight, bias [D] of weight_dtype, NULL: 1 and 0)
+ *   rotated    rotate != 0: its first `rotary` channels, pairs (i, i + rotary/2) - interleaved != 0: (2i, 2i + 1) - by the angle
+ *              whose cosine and sine are cos_sin[position, i] and cos_sin[position, rotary/2 + i]
+ *   written    scale == NULL: in the type it came in; scale != NULL: as e4m3 codes(y * (448 / amax)), amax the row's largest
+ *              finite magnitude (at least 2^-96), with scale[to, head] = amax / 448 (times mul[token, head], contiguous
+ *              [tokens, heads], where given). Infinities become +-448, NaN stays.
+ *              to = token, or slots[token] where slots are given: a negative slot leaves the part's rows of that token out
+ *              (padding); one at or beyond n_slots too, and raises FFTOPK_ST_BAD_INDEX. Slots of one call differ from one
+ *              another (of two tokens with one slot either's codes and scales may stay, in any mixture).
+ * in 32 bits, rounded once. A position outside [0, table_rows) makes the rotated channels NaN and raises FFTOPK_ST_BAD_INDEX.
+ * out may be x itself (same strides); anything else that overlaps is not supported.
+ *   strides      elements (codes: bytes); the D channels of a row are contiguous
+ *   D            a multiple of 8 up to 256; rotary a multiple of 16 up to D (FFTOPK_ERANGE otherwise)
+ *   dtype        of every part's x, and of its out where it is not quantised
+ *   cos_sin      device, fp32 [table_rows, rotary], contiguous, 16-byte aligned; positions int32 [tokens]; both may be NULL
+ *                where no part is rotated
+ *   tokens       tokens * heads may not reach 2^31 - 64 (FFTOPK_ERANGE)
+ * Rows whose addresses are not all multiples of 16 bytes are read and written an element at a time.
+ */
+#define FFTOPK_DTYPE_FP32 2 /* beside FFTOPK_DTYPE_FP16 and FFTOPK_DTYPE_BF16 */
+#define FFTOPK_NORM_NONE 0
+#define FFTOPK_NORM_RMS 1
+#define FFTOPK_NORM_LAYER 2
+typedef struct fftopk_head_part {
+  const void* x;
+  int64_t x_token_stride, x_head_stride;
+  const void* weight;
+  const void* bias;
+  void* out;
+  int64_t out_token_stride, out_head_stride;
+  float* scale;
+  int64_t scale_token_stride, scale_head_stride;
+  const float* mul;
+  const int32_t* slots;
+  int64_t n_slots;
+  int32_t heads, norm, rotate, weight_dtype;
+  float eps;
+  int32_t reserved;
+} fftopk_head_part;
+int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tokens, int32_t D, int32_t dtype,
+                     const int32_t* positions, const float* cos_sin, int64_t table_rows, int32_t rotary, int32_t interleaved,
+                     uint32_t* status, void* cuda_stream);
+
+/*
+ * Rows of a quantised cache, gathered and widened: out[i, j, h, :] = codes[slot, h, :] * scale[slot, h] with
+ * slot = slots[i, j] (+ offsets[i]), slots int32 [rows, per_row] contiguous, offsets int32 [rows] or NULL, out contiguous
+ * [rows, per_row, heads, D] of out_dtype, 16-byte aligned. A negative entry of slots gives zeros; a slot outside [0, n_slots)
+ * zeros and FFTOPK_ST_BAD_INDEX. Strides in elements; D as for fftopk_head_rows.
+ */
+int fftopk_cache_read(const void* cache, int64_t slot_stride, int64_t head_stride, int64_t n_slots, int32_t heads, int32_t D,
+                      const float* scale, int64_t scale_slot_stride, int64_t scale_head_stride, const int32_t* slots, int64_t rows,
+                      int64_t per_row, const int32_t* offsets, void* out, int32_t out_dtype, uint32_t* status, void* cuda_stream);
+
+/*
+ * Attention over selected tokens: the step behind the selector.
+ *   out[t, h] = sum_j p_j v[slot_j, h / group] / sum_j p_j,  p_j = exp(softmax_scale q[t, h] . k[slot_j, h / group] - max),
+ *   slot_j = indices[t, j] (+ offsets[t]), group = q_heads / kv_heads
+ * Negative indices are left out wherever they stand; an index that gives a slot outside [0, slots) too, and raises
+ * FFTOPK_ST_BAD_INDEX. A token that is left with none gets zeros and lse -inf. An index named twice counts twice. Nothing of
+ * rows that no index names is read.
+ *   q, out       [tokens, q_heads, D] of dtype (fp16 or bf16), D 64 or 128 (FFTOPK_ERANGE otherwise)
+ *   k, v         [slots, kv_heads, D] of dtype, or - k_scale and v_scale given, fp32 [slots, kv_heads] - e4m3 codes
+ *   indices      int32 [tokens, picks], rows idx_row elements apart, inner stride 1; offsets int32 [tokens] or NULL
+ *   lse          fp32 [tokens, q_heads], contiguous, or NULL: log of the sum of exponentials
+ *   strides      in elements; rows of q, k and v start on 16 bytes
+ * Sums and maxima are kept in 32 bits; weights are rounded to dtype (16-bit cache) or fp16 (e4m3) for the second product.
+ * The call holds no state and needs no workspace; the first one on a device sets kernel attributes (outside any capture).
+ */
+typedef struct fftopk_attend {
+  const void* q;
+  int64_t q_token, q_head;
+  const void* k;
+  int64_t k_slot, k_head;
+  const void* v;
+  int64_t v_slot, v_head;
+  const float* k_scale;
+  int64_t ks_slot, ks_head;
+  const float* v_scale;
+  int64_t vs_slot, vs_head;
+  const int32_t* indices;
+  int64_t idx_row;
+  const int32_t* offsets;
+  void* out;
+  int64_t out_token, out_head;
+  float* lse;
+  int64_t tokens, slots;
+  int32_t q_heads, kv_heads, D, picks, dtype;
+  float softmax_scale;
+} fftopk_attend;
+int fftopk_sparse_attention(const fftopk_attend* args, uint32_t* status, void* cuda_stream);
 
 /*
  * Measurement aid, not part of the selection path (no reference counterpart): a read-only bandwidth

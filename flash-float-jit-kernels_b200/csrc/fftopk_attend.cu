@@ -28,6 +28,7 @@
 #include "../../include/fftopk.h"
 #include "fftopk_host.h"
 #include "fftopk_internal.h"
+#include "fftopk_attend.cuh"
 #include "fftopk_rows.cuh"
 
 namespace fftopk {
@@ -35,33 +36,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-struct AttendParams {
-  const void* q;
-  int64_t q_token, q_head;  // strides, elements
-  const void* k;
-  const void* v;
-  int64_t k_slot, k_head, v_slot, v_head;
-  const float* k_scale;
-  const float* v_scale;
-  int64_t ks_slot, ks_head, vs_slot, vs_head;
-  const int32_t* indices;
-  int64_t idx_row;
-  const int32_t* offsets;
-  void* out;
-  int64_t out_token, out_head;
-  float* lse;  // [T, q heads]
-  int64_t slots;
-  int32_t tokens, kv_heads, group, picks;
-  int32_t head_blocks;  // blocks of 16 query heads per key head
-  float scale_log2;     // softmax scale * log2(e)
-  uint32_t* status;
-};
-
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kHeadsM = 16;  // query heads a CTA works on: rows of the MMA
-constexpr unsigned kAll = 0xffffffffu;
-constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -72,21 +49,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint2 ldg8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
 }
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(kAll, x, 1));
@@ -428,6 +390,7 @@ int attend_setup(int& sms) {
     if (!r) r = setup_one<__half, false, 128>();
     if (!r) r = setup_one<__half, true, 64>();
     if (!r) r = setup_one<__half, true, 128>();
+    if (!r) r = attend_wide_setup();
     return r;
   });
   sms = g_attend_sms[dev];
@@ -503,17 +466,24 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   p.out = a->out, p.out_token = a->out_token, p.out_head = a->out_head, p.lse = a->lse;
   p.slots = a->slots;
   p.tokens = (int32_t)a->tokens, p.kv_heads = a->kv_heads, p.group = a->q_heads / a->kv_heads, p.picks = a->picks;
-  p.head_blocks = (p.group + kHeadsM - 1) / kHeadsM;
+  const bool wide = p.group > kHeadsM;
+  const int rows = wide ? 128 : kHeadsM;
+  p.head_blocks = (p.group + rows - 1) / rows;
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
+  p.out_vec = on16(a->out, a->tokens, a->out_token, a->q_heads, a->out_head, 2);
   p.status = status;
 
-  // CTAs a token: as many as keep the device's SMs busy, and no more than give every warp keys
+  // CTAs a token: as many as keep the device's SMs busy, and no more than give every warp (wide: every CTA) keys
   const int64_t units = a->tokens * p.kv_heads * p.head_blocks;
-  const int keys = kWarps * (fp8 ? 32 : 16);
+  const int keys = wide ? 128 : kWarps * (fp8 ? 32 : 16);
   int ctas = 1;
-  while (ctas < kMaxCluster && units * ctas * 2 <= sms && (int64_t)ctas * keys < p.picks) ctas *= 2;
+  while (ctas < kAttendMaxCluster && units * ctas * 2 <= sms && (int64_t)ctas * keys < p.picks) ctas *= 2;
   if (units * ctas > 0x7fffffff) return FFTOPK_ERANGE;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  if (wide) {
+    const cudaError_t e = attend_wide(p, a->dtype == FFTOPK_DTYPE_BF16, fp8, a->D, ctas, units, sms, stream);
+    return e == cudaSuccess ? FFTOPK_OK : cuda_fail(e);
+  }
   const cudaError_t e = a->dtype == FFTOPK_DTYPE_BF16 ? launch_narrow<__nv_bfloat16>(p, fp8, a->D, ctas, units, stream)
                                                       : launch_narrow<__half>(p, fp8, a->D, ctas, units, stream);
   return e == cudaSuccess ? FFTOPK_OK : cuda_fail(e);

@@ -1,0 +1,57 @@
+// What the two attention kernels over selected rows share.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace fftopk {
+
+struct AttendParams {
+  const void* q;
+  int64_t q_token, q_head;  // strides, elements
+  const void* k;
+  const void* v;
+  int64_t k_slot, k_head, v_slot, v_head;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t ks_slot, ks_head, vs_slot, vs_head;
+  const int32_t* indices;
+  int64_t idx_row;
+  const int32_t* offsets;
+  void* out;
+  int64_t out_token, out_head;
+  float* lse;  // [T, q heads]
+  int64_t slots;
+  int32_t tokens, kv_heads, group, picks;
+  int32_t head_blocks;  // blocks of query heads per key head: of 16 (narrow) or 128 (wide)
+  float scale_log2;     // softmax scale * log2(e)
+  int32_t out_vec;      // rows of out start on 16 bytes
+  uint32_t* status;
+};
+
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int kAttendMaxCluster = 8;  // CTAs that share a token's keys: the portable cluster size
+
+// fftopk_attend_wide.cu; fp8: e4m3 caches; `units` pieces of work (token, key head, 128 query heads), `ctas` CTAs each
+int attend_wide_setup();
+cudaError_t attend_wide(const AttendParams& p, bool bf16, bool fp8, int D, int ctas, int64_t units, int sms, cudaStream_t stream);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+#endif  // __CUDACC__
+
+}  // namespace fftopk

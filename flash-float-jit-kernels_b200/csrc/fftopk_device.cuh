@@ -10,6 +10,7 @@
 #include "../../include/fftopk.h"
 #include "fftopk_decide.h"
 #include "fftopk_key.h"
+#include "fftopk_tcgen05.cuh"
 #include "fftopk_trace.cuh"
 
 namespace fftopk {
@@ -63,9 +64,6 @@ static __device__ unsigned int g_routes[3];
 // the gather buffer; selected by full histograms
 constexpr int kRouteHeld = 0, kRouteBeyond = 1, kRouteHistograms = 2;
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
 
 // Shared-memory atomics with the state space spelled out. Pointers into the dynamic shared
 // memory block travel through structs and function arguments here, where the compiler no longer

@@ -51,6 +51,7 @@
 #include "fftopk_host.h"
 #include "fftopk_internal.h"
 #include "fftopk_key.h"
+#include "fftopk_tcgen05.cuh"
 
 namespace fftopk {
 
@@ -96,7 +97,6 @@ struct IdxScaleRing {
   static constexpr int kSlots = kFp8 ? IdxFmt<true>::kStages + kIdxBufs : 0;
 };
 constexpr uint32_t kIdxScaleBytes = kIdxTile * 4;
-constexpr unsigned long long kIdxWaitNs = 200ull * 1000 * 1000;
 
 struct IndexerParams {
   const float* w;            // [B, 64] head weights
@@ -116,43 +116,7 @@ struct IndexerParams {
   uint32_t* status;
 };
 
-// ---- mbarrier / TMA / tcgen05 wrappers -----------------------------------------------------------
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0u;
-}
-// Bounded wait: false when the time ran out or another thread of the CTA has given up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
-  if (mbar_try_wait(bar, parity)) return true;
-  unsigned long long t0;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  for (;;) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > kIdxWaitNs) {
-      *abort_flag = 1u;
-      return false;
-    }
-  }
-}
+// ---- TMA / tcgen05 wrappers (mbarriers, descriptors, commits: fftopk_tcgen05.cuh) ------------------
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
@@ -166,17 +130,6 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                    smem_u32(smem_dst)),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
-}
-// Shared-memory matrix descriptor of a K-major operand in the 128-byte-swizzle layout a TMA box of
-// 128 bytes (64 bf16 or 128 fp8) x rows produces: rows of 128 bytes, groups of 8 rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr >> 4) & 0x3fffu);  // start address, 16-byte units
-  d |= (uint64_t)1u << 16;                       // leading byte offset (unused with swizzle): 1
-  d |= (uint64_t)(1024u >> 4) << 32;             // stride byte offset: 8 rows x 128 B
-  d |= (uint64_t)1u << 46;                       // descriptor version of sm_100
-  d |= (uint64_t)2u << 61;                       // layout type: 128-byte swizzle
-  return d;
 }
 template <bool kFp8>
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t accumulate) {
@@ -196,22 +149,6 @@ __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t adesc, uint64_t b
         : "memory");
   }
 }
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr)
-      : "memory");
-}
-
 __device__ __forceinline__ int indexer_row_tiles(const IndexerParams& p, int row, int& len) {
   int64_t len64 = p.lengths[row];
   len64 = len64 < 0 ? 0 : (len64 > p.L ? p.L : len64);

@@ -6,11 +6,13 @@
 //   S[128 heads x 128 keys] = Q K^T    Q, K in shared memory (K-major, 128-byte swizzle), S in tensor memory
 //   O[128 heads x D]       += P V      P in tensor memory (16 bits, over the S it came from), V in shared memory as it lies in the
 //                                      cache, [key][channel]: an MN-major operand
-// 17 warps: two groups of four softmax warps, one thread per head, that take alternate tiles of keys, each with an S, an O and a
-// running maximum of its own, so that one group's exponentials run while the other's products do; eight that gather rows (four
-// k, four v), and one thread that issues the MMAs: QK of tile j + 1, then PV of tile j. The rows lie anywhere: 16-bit ones are
-// copied with cp.async, e4m3 ones go through registers and are widened to fp16 on the way (eight 16-byte loads a thread in
-// flight: as a piece is widened the next tile's takes its registers). Rows that are not there are zeros, and masked in S.
+// 20 warps: two groups of four softmax warps, one thread per head, that take alternate tiles of keys, each with an S, an O and a
+// running maximum of its own, so that one group's exponentials run while the other's products do; one that looks up which rows
+// the tiles to come are made of (and, fp8, their scales) and hands them out as a stream of TileMeta; four that gather k rows and
+// four that gather v rows; two that bring the queries of the next piece of work; and one thread that issues the MMAs: QK of
+// tile n + 1, then PV of tile n. The rows lie anywhere: 16-bit ones are copied with cp.async, e4m3 ones go through registers and
+// are widened to fp16 on the way (eight 16-byte loads a thread in flight: as a piece is widened the next tile's takes its
+// registers). Rows that are not there are zeros, and masked in S.
 //
 // A row's maximum is let stand until a score exceeds it by 2^8 (fp16 and 32-bit sums have the room), so O, which lives in tensor
 // memory, is hardly ever rescaled. fp8: the k scales multiply S, the v scales P, relative to a power of two near the largest v scale that is
@@ -40,64 +42,97 @@ namespace cg = cooperative_groups;
 
 constexpr int kHeadsW = 128;   // rows of the MMAs
 constexpr int kTileKeys = 128; // keys of a tile
-constexpr int kSoftmaxWarps = 8, kGatherWarps = 8;
-constexpr int kMmaWarp = kSoftmaxWarps + kGatherWarps;
-constexpr int kWideThreads = (kMmaWarp + 1) * 32;
+constexpr int kSoftmaxWarps = 8, kGatherWarps = 8, kQueryWarps = 2;
+constexpr int kMmaWarp = kSoftmaxWarps + kGatherWarps, kScoutWarp = kMmaWarp + 1, kQueryWarp = kScoutWarp + 1;
+constexpr int kWideThreads = (kQueryWarp + kQueryWarps) * 32;
+// Registers a thread: 640 threads are launched with 96 each; by warpgroup 2 x 128 (softmax: 64 scores at once), 2 x 80 (gather) and
+// 64 (the rest) are the same 480.
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 128, kRegsGather = 80, kRegsRest = 64;
+static_assert(2 * kRegsSoftmax + 2 * kRegsGather + kRegsRest == kWideThreads / 128 * kRegsLaunch, "no more registers than the block has");
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLetStand = 8.f;  // log2 by which a score may exceed the reference
 
 template <int D>
 struct WideCfg {
   static constexpr uint32_t kTileBytes = kTileKeys * D * 2;  // of Q too
-  static constexpr int kKStages = D == 128 ? 3 : 4, kVStages = D == 128 ? 2 : 4;
-  // Softmax reads a tile's TileMeta after its K stage may have been filled again. The gather of tile n + kKStages + 2 waits for
-  // QK of tile n + 2, which is issued behind PV of tile n, which waits for softmax of tile n: so many places are enough.
-  static constexpr int kMeta = kKStages + 2;
+  static constexpr int kKStages = D == 128 ? 2 : 4, kVStages = D == 128 ? 2 : 4;
 };
-struct TileMeta {  // of a tile's keys
+constexpr int kChunk = 64;    // scores of a row that a softmax thread works on at once
+constexpr int kMeta = 4;      // tiles the scout is ahead at most; a place is free again when its tile's PV is done
+constexpr int kInfo = 4;      // pieces of work it is ahead
+constexpr int kQTiles = 2;    // query tiles
+constexpr int kFirst = 1, kLast = 2, kEnd = 4, kWhole = 8;
+struct TileMeta {             // a tile of 128 keys
+  int32_t row[kTileKeys];     // cache rows; -1: none
   float ks[kTileKeys], vs[kTileKeys];
   uint32_t live[4];
-  float vmax[4];
+  float vtop;                 // largest v scale
+  int32_t flags;              // first, last tile of its piece of work; end of the stream (no tile); all rows are there
+  int32_t j;                  // tile of its piece of work
+  int32_t kvh;
 };
 template <int D>
 struct WideSmem {  // behind the operand tiles
-  TileMeta meta[WideCfg<D>::kMeta];
-  float qmul[2][kHeadsW];    // by parity of the piece of work
+  TileMeta meta[kMeta];
+  float qmul[4][kHeadsW];    // by piece of work: softmax may be two behind the queries
   float2 ml[2][2][kHeadsW];  // by parity of the piece of work, and group: maximum and sum
+  int32_t tiles[kInfo];      // tiles of a piece of work
   uint64_t kfull[WideCfg<D>::kKStages], kempty[WideCfg<D>::kKStages];
   uint64_t vfull[WideCfg<D>::kVStages], vempty[WideCfg<D>::kVStages];
-  uint64_t mfull[WideCfg<D>::kMeta];
-  uint64_t qfull, qempty, oempty, mlbar;
+  uint64_t mfull[kMeta], mempty[kMeta], ifull[kInfo], iempty[kInfo];
+  uint64_t qfull[kQTiles], qempty[kQTiles], oempty, mlbar;
   uint64_t sfull[2], pfull[2], pvdone[2];
   uint32_t tmem, abort_flag;
 };
 template <int D>
 constexpr size_t wide_smem_bytes() {
-  return 1024 + (size_t)WideCfg<D>::kTileBytes * (1 + WideCfg<D>::kKStages + WideCfg<D>::kVStages) + sizeof(WideSmem<D>);
+  return 1024 + (size_t)WideCfg<D>::kTileBytes * (kQTiles + WideCfg<D>::kKStages + WideCfg<D>::kVStages) + sizeof(WideSmem<D>);
 }
 
-// V as it lies in the cache: an MN-major operand, 128-byte swizzle. Blocks of 64 channels x 128 keys, 128 bytes a key; 8 keys are
-// 1024 bytes apart (stride offset), blocks of channels 16 KiB (leading offset).
-__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t smem_addr) {
-  return umma_desc_sw128(smem_addr) & ~((uint64_t)0x3fffu << 16) | (uint64_t)((kTileKeys * 128u) >> 4) << 16;
+// Matrix descriptors as their two halves: only the lower one, address and leading offset, differs from operand to operand, and
+// 16-byte units may be added to it. K-major (Q, K): see umma_desc_sw128. V as it lies in the cache is an MN-major operand, 128-byte
+// swizzle: blocks of 64 channels x 128 keys, 128 bytes a key; 8 keys are 1024 bytes apart (stride offset), blocks of channels 16 KiB
+// (leading offset).
+__device__ __forceinline__ uint32_t desc_k(uint32_t smem_addr) { return (uint32_t)umma_desc_sw128(smem_addr); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t smem_addr) {  // (of a cluster's CTAs, addresses have more bits)
+  return ((smem_addr >> 4) & 0x3fffu) | ((kTileKeys * 128u) >> 4) << 16;
 }
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;  // stride offset, version, 128-byte swizzle
 template <typename M, int N, bool kMnMajorB>
 __host__ __device__ constexpr uint32_t instr_desc() {  // D fp32; A and B fp16 or bf16; M = 128
   constexpr uint32_t f = std::is_same<M, __half>::value ? 0u : 1u;
   return (1u << 4) | (f << 7) | (f << 10) | ((kMnMajorB ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kHeadsW >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -107,14 +142,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
-      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
+__device__ __forceinline__ void load_chunk(uint32_t taddr, float (&s)[64]) {
+  tmem_ld32(taddr, reinterpret_cast<uint32_t(&)[32]>(s[0]));
+  tmem_ld32(taddr + 32u, reinterpret_cast<uint32_t(&)[32]>(s[32]));
+}
+__device__ __forceinline__ void store_chunk(uint32_t taddr, const uint32_t (&v)[32]) {
+  tmem_st16(taddr, reinterpret_cast<const uint32_t(&)[16]>(v[0]));
+  tmem_st16(taddr + 16u, reinterpret_cast<const uint32_t(&)[16]>(v[16]));
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -161,26 +195,17 @@ __device__ __forceinline__ Work work_of(const AttendParams& p, uint32_t unit) {
   return w;
 }
 
-// 32 consecutive scores of a thread's row out of tensor memory: times the k scales (fp8), masked
-template <bool kFp8>
-__device__ __forceinline__ void load_scores(float (&s)[32], uint32_t taddr, const float* ks, uint32_t live) {
-  uint32_t v[32];
-  tmem_ld32(taddr, v);
-  tmem_wait_ld();
+// the largest of a thread's kChunk scores
+__device__ __forceinline__ float top_of(const float (&s)[kChunk]) {
+  float top[4];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(v[i]);
-  if constexpr (kFp8) {
+  for (int i = 0; i < 4; ++i) top[i] = fmaxf(s[2 * i], s[2 * i + 1]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 k = reinterpret_cast<const float4*>(ks)[i];
-      s[4 * i] *= k.x, s[4 * i + 1] *= k.y, s[4 * i + 2] *= k.z, s[4 * i + 3] *= k.w;
-    }
+  for (int i = 8; i < kChunk; i += 8) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(s[i + 2 * e], s[i + 2 * e + 1]));
   }
-  if (live != kAll) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (!(live >> i & 1u)) s[i] = -INFINITY;
-  }
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
 
 template <typename T, int N>
@@ -209,8 +234,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
   extern __shared__ unsigned char wide_raw[];
   const uint32_t pad = (1024u - (smem_u32(wide_raw) & 1023u)) & 1023u;
   unsigned char* base = wide_raw + pad;
-  const uint32_t q_tile = smem_u32(base), k_tiles = q_tile + kTileBytes, v_tiles = k_tiles + kKS * kTileBytes;
-  WideSmem<D>& sm = *reinterpret_cast<WideSmem<D>*>(base + (size_t)kTileBytes * (1 + kKS + kVS));
+  const uint32_t q_tiles = smem_u32(base), k_tiles = q_tiles + kQTiles * kTileBytes, v_tiles = k_tiles + kKS * kTileBytes;
+  WideSmem<D>& sm = *reinterpret_cast<WideSmem<D>*>(base + (size_t)kTileBytes * (kQTiles + kKS + kVS));
   volatile uint32_t* abort_flag = &sm.abort_flag;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -221,9 +246,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
   if (tid == 0) {
     for (int i = 0; i < kKS; ++i) mbar_init(&sm.kfull[i], 4), mbar_init(&sm.kempty[i], 1);
     for (int i = 0; i < kVS; ++i) mbar_init(&sm.vfull[i], 4), mbar_init(&sm.vempty[i], 1);
-    for (int i = 0; i < C::kMeta; ++i) mbar_init(&sm.mfull[i], 4);
-    mbar_init(&sm.qfull, 4);
-    mbar_init(&sm.qempty, 1);
+    for (int i = 0; i < kMeta; ++i) mbar_init(&sm.mfull[i], 1), mbar_init(&sm.mempty[i], 1);
+    for (int i = 0; i < kInfo; ++i) mbar_init(&sm.ifull[i], 1), mbar_init(&sm.iempty[i], kSoftmaxWarps + kQueryWarps);
+    for (int i = 0; i < kQTiles; ++i) mbar_init(&sm.qfull[i], kQueryWarps), mbar_init(&sm.qempty[i], 1);
     mbar_init(&sm.oempty, kSoftmaxWarps);
     mbar_init(&sm.mlbar, kSoftmaxWarps);
     for (int i = 0; i < 2; ++i) mbar_init(&sm.sfull[i], 1), mbar_init(&sm.pfull[i], 4), mbar_init(&sm.pvdone[i], 1);
@@ -238,242 +263,335 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = sm.tmem;
-
-  // Tiles this CTA has been through (it), pieces of work with tiles (wn): they select stages and the barriers' phases.
-  uint32_t it = 0, wn = 0;
-  bool ok = true;
+  // Tiles are counted through all pieces of work (n, it), and so are pieces (un) and those that have tiles (wn): the counts select
+  // places and stages and the phases of their barriers.
 
   if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
-    // ---- gather ----
+    // ---- gather: four warps for k, four for v; rows 32 gw .. 32 gw + 31 of every tile ----
+    fewer_registers<kRegsGather>();
     const bool is_k = warp < kSoftmaxWarps + 4;
-    const int gw = (warp - kSoftmaxWarps) & 3;  // rows 32 gw .. 32 gw + 31 of a tile
+    const int gw = (warp - kSoftmaxWarps) & 3;
     uint64_t* const full = is_k ? sm.kfull : sm.vfull;
     uint64_t* const empty = is_k ? sm.kempty : sm.vempty;
-    const int stages = is_k ? kKS : kVS;
+    const uint32_t stages = is_k ? kKS : kVS;
     const uint32_t tiles = is_k ? k_tiles : v_tiles;
     constexpr int kLanesRow = D * (kFp8 ? 1 : 2) / 16;  // lanes that read a row
     constexpr int kRowsOnce = 32 / kLanesRow, kTurns = 32 / kRowsOnce;
-    const int piece = lane % kLanesRow;
+    // Eight lanes that write to shared memory together touch all its banks: 16-bit, a row's 128 bytes; e4m3, where a lane writes
+    // two neighbouring chunks one after the other, half of those of two neighbouring rows.
+    const int piece = kFp8 && kLanesRow == 8 ? (lane & 3) | ((lane >> 3 & 1) << 2) : lane % kLanesRow;
+    const int sub = gw * 32 + (kFp8 && kLanesRow == 8 ? (lane >> 2 & 1) | ((lane >> 4) << 1) : lane / kLanesRow);
     const int64_t row_bytes = (is_k ? p.k_slot : p.v_slot) * (kFp8 ? 1 : 2);
-    for (uint32_t unit = first; ok && unit < units; unit += step) {
-      const Work w = work_of(p, unit);
-      const int32_t* idx = p.indices + (int64_t)w.token * p.idx_row;
-      const int all = tiles_of(idx, p.picks, lane);
-      const int nt = all > rank ? (all - rank + ctas - 1) / ctas : 0;
-      if (nt == 0) continue;
-      const int64_t offset = p.offsets != nullptr ? p.offsets[w.token] : 0;
-      const char* const src = static_cast<const char*>(is_k ? p.k : p.v) + (int64_t)w.kvh * (is_k ? p.k_head : p.v_head) * (kFp8 ? 1 : 2) + piece * 16;
-      auto pick = [&](int j) {  // the lane's row of local tile j
-        const int at = (rank + j * ctas) * kTileKeys + gw * 32 + lane;
-        return j < nt && at < p.picks ? idx[at] : -1;
+    const int64_t head_bytes = (is_k ? p.k_head : p.v_head) * (kFp8 ? 1 : 2);
+    const char* const src0 = static_cast<const char*>(is_k ? p.k : p.v) + piece * 16;
+    auto posted = [&](uint32_t n) { return __all_sync(kAll, mbar_test(&sm.mfull[n % kMeta], (n / kMeta) & 1u)); };
+    auto wait_posted = [&](uint32_t n) { return __all_sync(kAll, mbar_wait(&sm.mfull[n % kMeta], (n / kMeta) & 1u, abort_flag)); };
+    auto wait_empty = [&](uint32_t n) { return __all_sync(kAll, mbar_wait(&empty[n % stages], ((n / stages) & 1u) ^ 1u, abort_flag)); };
+    auto hand_over = [&](uint32_t n) {
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[n % stages]);
+    };
+    if constexpr (kFp8) {
+      uint4 held[kTurns];  // the lane's pieces of the rows on their way
+      auto fetch = [&](int i, const TileMeta& m, const char* src) {
+        const int row = m.row[sub + i * kRowsOnce];
+        held[i] = row >= 0 ? ldg16(src + (int64_t)row * row_bytes) : make_uint4(0u, 0u, 0u, 0u);
       };
-      auto row_of = [&](int32_t i) {
-        if (i < 0) return -1;
-        const int64_t slot = i + offset;
-        if (slot < 0 || slot >= p.slots) {
-          if (is_k && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
-          return -1;
-        }
-        return (int)slot;
-      };
-      int row = row_of(pick(0));
-      int32_t ahead = pick(1);  // (an index is asked for a tile before its row is)
-      uint4 held[kFp8 ? kTurns : 1];  // fp8: the lane's pieces of the rows on their way
-      float ks = 0.f, vs = 0.f;
-      auto fetch = [&](int i, int r) {
-        const int of = __shfl_sync(kAll, r, i * kRowsOnce + lane / kLanesRow);
-        held[i] = of >= 0 ? ldg16(src + (int64_t)of * row_bytes) : make_uint4(0u, 0u, 0u, 0u);
-      };
-      auto fetch_scales = [&](int r) {
-        ks = vs = 0.f;
-        if (is_k && r >= 0) {
-          ks = __ldg(p.k_scale + (int64_t)r * p.ks_slot + (int64_t)w.kvh * p.ks_head);
-          vs = __ldg(p.v_scale + (int64_t)r * p.vs_slot + (int64_t)w.kvh * p.vs_head);
-        }
-      };
-      if constexpr (kFp8) {
+      bool have = false;  // tile n's rows are on their way
+      for (uint32_t n = 0;; ++n) {
+        if (!have) {
+          if (!wait_posted(n)) break;
+          const TileMeta& m = sm.meta[n % kMeta];
+          if (m.flags & kEnd) break;
+          const char* src = src0 + m.kvh * head_bytes;
 #pragma unroll
-        for (int i = 0; i < kTurns; ++i) fetch(i, row);
-        fetch_scales(row);
+          for (int i = 0; i < kTurns; ++i) fetch(i, m, src);
+        }
+        const TileMeta& next = sm.meta[(n + 1) % kMeta];
+        have = posted(n + 1) && !(next.flags & kEnd);
+        const char* src = src0 + (have ? next.kvh * head_bytes : 0);
+        const uint32_t tile = tiles + (n % stages) * kTileBytes;
+        if (!wait_empty(n)) break;
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+          const uint32_t x[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            h[2 * e] = e4m3x2_to_half2((uint16_t)x[e]);
+            h[2 * e + 1] = e4m3x2_to_half2((uint16_t)(x[e] >> 16));
+          }
+          const int r = sub + i * kRowsOnce;
+          put16(chunk_at(tile, r, 2 * piece), h[0], h[1], h[2], h[3]);
+          put16(chunk_at(tile, r, 2 * piece + 1), h[4], h[5], h[6], h[7]);
+          if (have) fetch(i, next, src);  // the next tile's piece takes its place
+        }
+        hand_over(n);
       }
-      if (is_k) {
-        // q: rows 32 gw .. of the tile
-        if (!__all_sync(kAll, mbar_wait(&sm.qempty, (wn & 1u) ^ 1u, abort_flag))) {
-          ok = false;
+    } else {
+      bool pending = false;  // tile n - 1 is on its way and not handed over
+      for (uint32_t n = 0;; ++n) {
+        // a tile that has landed is not kept waiting for the next one's turn
+        if (pending && !(posted(n) && __all_sync(kAll, mbar_test(&empty[n % stages], ((n / stages) & 1u) ^ 1u)))) {
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          hand_over(n - 1);
+          pending = false;
+        }
+        if (!wait_posted(n)) break;
+        const TileMeta& m = sm.meta[n % kMeta];
+        if (m.flags & kEnd) {
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          if (pending) hand_over(n - 1);
           break;
         }
-        constexpr int kQLanes = D / 8, kQOnce = 32 / kQLanes;
-        const int c = lane % kQLanes;
-        const float negative = p.scale_log2 < 0.f ? -1.f : 1.f;
-        const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-        const T* q0 = static_cast<const T*>(p.q) + (int64_t)w.token * p.q_token + (int64_t)w.head0 * p.q_head + c * 8;
-#pragma unroll 4
-        for (int i = 0; i < 32 / kQOnce; ++i) {
-          const int h = gw * 32 + i * kQOnce + lane / kQLanes;
-          uint4 v = h < w.heads ? *reinterpret_cast<const uint4*>(q0 + (int64_t)h * p.q_head) : make_uint4(0u, 0u, 0u, 0u);
-          float mul = p.scale_log2 * negative;
-          if constexpr (kFp8 && !std::is_same<T, __half>::value) {
-            // to magnitudes below 2, as fp16 (see fftopk_attend.cu)
-            const float2 a = widen2(v.x, T()), b = widen2(v.y, T()), d = widen2(v.z, T()), e = widen2(v.w, T());
-            float amax = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))),
-                               fmaxf(fmaxf(fabsf(d.x), fabsf(d.y)), fmaxf(fabsf(e.x), fabsf(e.y))));
+        if (!wait_empty(n)) break;
+        const char* src = src0 + m.kvh * head_bytes;
+        const uint32_t tile = tiles + (n % stages) * kTileBytes;
 #pragma unroll
-            for (int o = kQLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, o));
-            const uint32_t ex = __float_as_uint(amax) >> 23;
-            const uint32_t ee = ex == 255u ? 127u : max(1u, min(ex, 253u));
-            const float down = __uint_as_float((254u - ee) << 23);
-            mul *= __uint_as_float(ee << 23);
-            v = make_uint4(narrow2(a.x * down, a.y * down, __half()), narrow2(b.x * down, b.y * down, __half()),
-                           narrow2(d.x * down, d.y * down, __half()), narrow2(e.x * down, e.y * down, __half()));
+        for (int i = 0; i < kTurns; ++i) {
+          const int r = sub + i * kRowsOnce;
+          const int row = m.row[r];
+          copy16(chunk_at(tile, r, piece), row >= 0 ? src + (int64_t)row * row_bytes : src0, row >= 0);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (pending) {
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          hand_over(n - 1);
+        }
+        pending = true;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+  } else if (warp >= kMmaWarp) {
+    fewer_registers<kRegsRest>();
+    if (warp == kScoutWarp) {
+      // ---- scout: what the tiles to come are made of ----
+      uint32_t n = 0, un = 0;
+      bool ok = true;
+      for (uint32_t unit = first; ok && unit < units; unit += step, ++un) {
+        const Work w = work_of(p, unit);
+        const int32_t* idx = p.indices + (int64_t)w.token * p.idx_row;
+        // (several CTAs a token: tiles without a row cost less than looking for the last)
+        const int all = ctas > 1 ? (p.picks + kTileKeys - 1) / kTileKeys : tiles_of(idx, p.picks, lane);
+        const int nt = all > rank ? (all - rank + ctas - 1) / ctas : 0;
+        if (!(ok = __all_sync(kAll, mbar_wait(&sm.iempty[un % kInfo], ((un / kInfo) & 1u) ^ 1u, abort_flag)))) break;
+        if (lane == 0) {
+          sm.tiles[un % kInfo] = nt;
+          mbar_arrive(&sm.ifull[un % kInfo]);
+        }
+        const int64_t offset = p.offsets != nullptr ? p.offsets[w.token] : 0;
+        auto pick = [&](int (&to)[4], int j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = (rank + j * ctas) * kTileKeys + i * 32 + lane;
+            to[i] = j < nt && at < p.picks ? idx[at] : -1;
           }
-          put16(chunk_at(q_tile, h, c), v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
-          if (c == 0) sm.qmul[wn & 1u][h] = fmaxf(mul, 1.17549435e-38f);  // (times a masked score it must stay -inf)
+        };
+        auto rows_of = [&](int (&row)[4], float (&ks)[4], float (&vs)[4], const int (&from)[4]) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int64_t slot = from[i] + offset;
+            const bool there = from[i] >= 0 && slot >= 0 && slot < p.slots;
+            if (from[i] >= 0 && !there && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+            row[i] = there ? (int)slot : -1;
+            ks[i] = vs[i] = 0.f;
+            if constexpr (kFp8) {
+              if (there) {
+                ks[i] = __ldg(p.k_scale + slot * p.ks_slot + (int64_t)w.kvh * p.ks_head);
+                vs[i] = __ldg(p.v_scale + slot * p.vs_slot + (int64_t)w.kvh * p.vs_head);
+              }
+            }
+          }
+        };
+        // an index is asked for two tiles ahead, a scale one
+        int now[4], later[4], row[4];
+        float ks[4], vs[4];
+        pick(now, 0);
+        pick(later, 1);
+        rows_of(row, ks, vs, now);
+        for (int j = 0; j < nt; ++j, ++n) {
+          int next_row[4];
+          float next_ks[4], next_vs[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) now[i] = later[i];
+          pick(later, j + 2);
+          rows_of(next_row, next_ks, next_vs, now);
+          if (!(ok = __all_sync(kAll, mbar_wait(&sm.mempty[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)))) break;
+          TileMeta& m = sm.meta[n % kMeta];
+          float top = 0.f;
+          unsigned whole = kAll;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            m.row[i * 32 + lane] = row[i];
+            const unsigned live = __ballot_sync(kAll, row[i] >= 0);
+            whole &= live;
+            if (lane == 0) m.live[i] = live;
+            if constexpr (kFp8) {
+              m.ks[i * 32 + lane] = ks[i];
+              m.vs[i * 32 + lane] = vs[i];
+              top = fmaxf(top, vs[i]);
+            }
+          }
+          if constexpr (kFp8) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+          }
+          if (lane == 0) {
+            m.vtop = top;
+            m.flags = (j == 0 ? kFirst : 0) | (j == nt - 1 ? kLast : 0) | (whole == kAll ? kWhole : 0);
+            m.j = j;
+            m.kvh = w.kvh;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.mfull[n % kMeta]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) row[i] = next_row[i], ks[i] = next_ks[i], vs[i] = next_vs[i];
+        }
+      }
+      if (ok && __all_sync(kAll, mbar_wait(&sm.mempty[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)) && lane == 0) {
+        sm.meta[n % kMeta].flags = kEnd;
+        mbar_arrive(&sm.mfull[n % kMeta]);
+      }
+    } else if (warp >= kQueryWarp) {
+      // ---- queries: two warps, 64 rows each ----
+      const float negative = p.scale_log2 < 0.f ? -1.f : 1.f;
+      const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale turns q: the largest score is then the largest here)
+      constexpr int kQLanes = D / 8, kQOnce = 32 / kQLanes, kTurns = 64 / kQOnce, kBatch = 8;
+      const int c = lane % kQLanes, sub = (warp - kQueryWarp) * 64 + lane / kQLanes;
+      uint32_t un = 0, wn = 0;
+      for (uint32_t unit = first; unit < units; unit += step, ++un) {
+        if (!__all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag))) break;
+        const int nt = sm.tiles[un % kInfo];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.iempty[un % kInfo]);
+        if (nt == 0) continue;
+        const Work w = work_of(p, unit);
+        const T* q0 = static_cast<const T*>(p.q) + (int64_t)w.token * p.q_token + (int64_t)w.head0 * p.q_head + c * 8;
+        const uint32_t tile = q_tiles + (wn % kQTiles) * kTileBytes;
+#pragma unroll 1
+        for (int b = 0; b < kTurns; b += kBatch) {
+          uint4 x[kBatch];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int h = sub + (b + i) * kQOnce;
+            x[i] = h < w.heads ? ldg16(q0 + (int64_t)h * p.q_head) : make_uint4(0u, 0u, 0u, 0u);
+          }
+          if (b == 0 && !__all_sync(kAll, mbar_wait(&sm.qempty[wn % kQTiles], ((wn / kQTiles) & 1u) ^ 1u, abort_flag))) break;
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int h = sub + (b + i) * kQOnce;
+            uint4 v = x[i];
+            float mul = p.scale_log2 * negative;
+            if constexpr (kFp8 && !std::is_same<T, __half>::value) {
+              // to magnitudes below 2, as fp16 (see fftopk_attend.cu)
+              const float2 a = widen2(v.x, T()), b2 = widen2(v.y, T()), d = widen2(v.z, T()), e = widen2(v.w, T());
+              float amax = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b2.x), fabsf(b2.y))),
+                                 fmaxf(fmaxf(fabsf(d.x), fabsf(d.y)), fmaxf(fabsf(e.x), fabsf(e.y))));
+#pragma unroll
+              for (int o = kQLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, o));
+              const uint32_t ex = __float_as_uint(amax) >> 23;
+              const uint32_t ee = ex == 255u ? 127u : max(1u, min(ex, 253u));
+              const float down = __uint_as_float((254u - ee) << 23);
+              mul *= __uint_as_float(ee << 23);
+              v = make_uint4(narrow2(a.x * down, a.y * down, __half()), narrow2(b2.x * down, b2.y * down, __half()),
+                             narrow2(d.x * down, d.y * down, __half()), narrow2(e.x * down, e.y * down, __half()));
+            }
+            put16(chunk_at(tile, h, c), v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+            if (c == 0) sm.qmul[wn & 3u][h] = fmaxf(mul, 1.17549435e-38f);  // (times a masked score it must stay -inf)
+          }
         }
         fence_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.qfull);
+        if (lane == 0) mbar_arrive(&sm.qfull[wn % kQTiles]);
+        ++wn;
       }
-      for (int j = 0; j < nt; ++j) {
-        const uint32_t n = it + (uint32_t)j;
-        const int stage = (int)(n % (uint32_t)stages);
-        const uint32_t phase = (n / (uint32_t)stages) & 1u;
-        const uint32_t tile = tiles + (uint32_t)stage * kTileBytes;
-        const int next_row = row_of(ahead);
-        ahead = pick(j + 2);
-        if (!__all_sync(kAll, mbar_wait(&empty[stage], phase ^ 1u, abort_flag))) {
-          ok = false;
-          break;
-        }
-        if (is_k) {
-          const int place = (int)(n % (uint32_t)C::kMeta);
-          TileMeta& m = sm.meta[place];
-          const unsigned live = __ballot_sync(kAll, row >= 0);
-          if (lane == 0) m.live[gw] = live;
-          if constexpr (kFp8) {
-            m.ks[gw * 32 + lane] = ks;
-            m.vs[gw * 32 + lane] = vs;
-            float top = vs;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
-            if (lane == 0) m.vmax[gw] = top;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.mfull[place]);
-        }
-        if constexpr (kFp8) {
-#pragma unroll
-          for (int i = 0; i < kTurns; ++i) {
-            const int r = gw * 32 + i * kRowsOnce + lane / kLanesRow;
-            const uint32_t x[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
-            uint32_t h[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              h[2 * e] = e4m3x2_to_half2((uint16_t)x[e]);
-              h[2 * e + 1] = e4m3x2_to_half2((uint16_t)(x[e] >> 16));
-            }
-            // (lanes of a row's second half write their chunks the other way around: eight lanes, all banks)
-            const bool swap = (piece & 4) != 0;
-            const uint32_t lo = chunk_at(tile, r, 2 * piece), hi = chunk_at(tile, r, 2 * piece + 1);
-            put16(swap ? hi : lo, swap ? h[4] : h[0], swap ? h[5] : h[1], swap ? h[6] : h[2], swap ? h[7] : h[3]);
-            put16(swap ? lo : hi, swap ? h[0] : h[4], swap ? h[1] : h[5], swap ? h[2] : h[6], swap ? h[3] : h[7]);
-            fetch(i, next_row);  // the next tile's piece takes its place
-          }
-          fetch_scales(next_row);
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[stage]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < kTurns; ++i) {
-            const int r = i * kRowsOnce + lane / kLanesRow;
-            const int of = __shfl_sync(kAll, row, r);
-            copy16(chunk_at(tile, gw * 32 + r, piece), of >= 0 ? src + (int64_t)of * row_bytes : src, of >= 0);
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          // the tile before this one has landed: hand it over (the last one: below)
-          if (j > 0) {
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[(n - 1) % (uint32_t)stages]);
-          }
-        }
-        row = next_row;
-      }
-      if constexpr (!kFp8) {
-        if (ok) {
-          asm volatile("cp.async.wait_group 0;" ::: "memory");
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[(it + (uint32_t)nt - 1) % (uint32_t)stages]);
-        }
-      }
-      it += (uint32_t)nt;
-      ++wn;
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == kMmaWarp) {
-    // ---- the MMAs ----
-    uint32_t turns[2] = {0u, 0u};  // tiles of each group in the pieces of work before
-    for (uint32_t unit = first; unit < units; unit += step) {
-      const Work w = work_of(p, unit);
-      const int all = tiles_of(p.indices + (int64_t)w.token * p.idx_row, p.picks, lane);
-      const int nt = all > rank ? (all - rank + ctas - 1) / ctas : 0;
-      if (nt == 0) continue;
+    } else if (warp == kMmaWarp) {
+      // ---- the MMAs ----
+      // A group's PV frees the place its next S goes to: QK of tile n stands right behind PV of tile n - 2, and what QK waits for is
+      // looked at before PV's weights are there.
       if (lane == 0) {
-        ok = mbar_wait(&sm.qfull, wn & 1u, abort_flag);
-        for (int j = 0; ok && j <= nt; ++j) {
-          if (j < nt) {  // S of tile j
-            const uint32_t n = it + (uint32_t)j;
-            const int stage = (int)(n % kKS);
-            if (!(ok = mbar_wait(&sm.kfull[stage], (n / kKS) & 1u, abort_flag))) break;
-            tmem_fence_after();
-            const uint32_t kt = k_tiles + (uint32_t)stage * kTileBytes;
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t at = (uint32_t)(k >> 2) * (kTileKeys * 128u) + (uint32_t)(k & 3) * 32u;
-              mma_ss(tmem + (uint32_t)(j & 1) * 128u, umma_desc_sw128(q_tile + at), umma_desc_sw128(kt + at),
-                     instr_desc<M, kTileKeys, false>(), k != 0);
-            }
-            umma_commit(&sm.sfull[j & 1]);
-            umma_commit(&sm.kempty[stage]);
-            if (j == nt - 1) umma_commit(&sm.qempty);
+        uint32_t qn = 0, pn = 0;      // tiles whose QK, whose PV has been issued
+        uint32_t qwn = 0, pwn = 0;    // pieces of work they are of
+        int qj = 0, pj = 0;           // and tiles of those
+        bool ended = false;           // the stream, at qn tiles
+        bool ok = true;
+        auto ready = [&](bool wait) {  // tile qn's k and q; sets `ended` where there is no such tile
+          uint64_t* const meta = &sm.mfull[qn % kMeta];
+          if (!(wait ? mbar_wait(meta, (qn / kMeta) & 1u, abort_flag) : mbar_test(meta, (qn / kMeta) & 1u))) return false;
+          if (sm.meta[qn % kMeta].flags & kEnd) {
+            ended = true;
+            return false;
           }
-          if (j > 0) {  // O of tile j - 1
-            const int i = j - 1, g = i & 1;
-            const uint32_t n = it + (uint32_t)i;
-            const int stage = (int)(n % kVS);
-            if (i == 0 && !(ok = mbar_wait(&sm.oempty, (wn & 1u) ^ 1u, abort_flag))) break;
-            if (!(ok = mbar_wait(&sm.vfull[stage], (n / kVS) & 1u, abort_flag))) break;
-            if (!(ok = mbar_wait(&sm.pfull[g], (turns[g] + (uint32_t)(i >> 1)) & 1u, abort_flag))) break;
-            tmem_fence_after();
-            const uint32_t vt = v_tiles + (uint32_t)stage * kTileBytes;
-#pragma unroll
-            for (int k = 0; k < kTileKeys / 16; ++k)
-              mma_ts(tmem + 256u + (uint32_t)g * 128u, tmem + (uint32_t)g * 128u + (uint32_t)k * 8u, desc_mn_sw128(vt + (uint32_t)k * 2048u),
-                     instr_desc<M, D, true>(), i > 1 || k != 0);
-            umma_commit(&sm.pvdone[g]);
-            umma_commit(&sm.vempty[stage]);
+          if (qj == 0) {
+            uint64_t* const q = &sm.qfull[qwn % kQTiles];
+            if (!(wait ? mbar_wait(q, (qwn / kQTiles) & 1u, abort_flag) : mbar_test(q, (qwn / kQTiles) & 1u))) return false;
           }
+          uint64_t* const k = &sm.kfull[qn % kKS];
+          return wait ? mbar_wait(k, (qn / kKS) & 1u, abort_flag) : mbar_test(k, (qn / kKS) & 1u);
+        };
+        auto qk = [&] {
+          tmem_fence_after();
+          const uint32_t stage = qn % kKS, qt = qwn % kQTiles;
+          const uint32_t kt = desc_k(k_tiles + stage * kTileBytes), q = desc_k(q_tiles + qt * kTileBytes), d = tmem + (qn & 1u) * 128u;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = ((uint32_t)(k >> 2) * (kTileKeys * 128u) + (uint32_t)(k & 3) * 32u) >> 4;
+            mma_ss(d, q + at, kt + at, instr_desc<M, kTileKeys, false>(), k != 0);
+          }
+          umma_commit(&sm.sfull[qn & 1u]);
+          umma_commit(&sm.kempty[stage]);
+          const bool last = (sm.meta[qn % kMeta].flags & kLast) != 0;
+          if (last) umma_commit(&sm.qempty[qt]);
+          ++qn;
+          qj = last ? 0 : qj + 1;
+          qwn += last ? 1u : 0u;
+        };
+        while (ok) {
+          // (two tiles at most are between their QK and their PV: one a group)
+          if (!ended && qn - pn < 2u && ready(qn == pn)) {
+            qk();
+            continue;
+          }
+          if (qn == pn) break;  // the end - or a wait that ran out
+          const bool more = !ended && qn - pn == 2u && ready(false);
+          // PV of tile pn
+          const uint32_t g = pn & 1u, stage = pn % kVS, vt = desc_mn(v_tiles + stage * kTileBytes), s_at = tmem + g * 128u;
+          if (pj == 0 && !(ok = mbar_wait(&sm.oempty, (pwn & 1u) ^ 1u, abort_flag))) break;  // (O may still be on its way out)
+          const bool last = (sm.meta[pn % kMeta].flags & kLast) != 0;
+          if (!(ok = mbar_wait(&sm.vfull[stage], (pn / kVS) & 1u, abort_flag))) break;
+          if (!(ok = mbar_wait(&sm.pfull[g], (pn >> 1) & 1u, abort_flag))) break;
+          tmem_fence_after();
+#pragma unroll
+          for (int k = 0; k < kTileKeys / 16; ++k)
+            mma_ts(s_at + 256u, s_at + (uint32_t)k * 8u, vt + (uint32_t)k * (2048u >> 4), instr_desc<M, D, true>(), k != 0 || pj > 1);
+          umma_commit(&sm.pvdone[g]);
+          umma_commit(&sm.vempty[stage]);
+          umma_commit(&sm.mempty[pn % kMeta]);
+          ++pn;
+          pj = last ? 0 : pj + 1;
+          pwn += last ? 1u : 0u;
+          if (more) qk();
         }
       }
       __syncwarp();
-      turns[0] += (uint32_t)(nt + 1) / 2u, turns[1] += (uint32_t)nt / 2u;
-      it += (uint32_t)nt;
-      ++wn;
-      if (*abort_flag) break;
     }
   } else {
-    // ---- softmax: group g takes tiles g, g + 2, ..; thread r of a group has head r ----
+    // ---- softmax: group g takes every second tile of the stream; thread r of a group has head r ----
+    more_registers<kRegsSoftmax>();
     const int g = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_cols = lanes + (uint32_t)g * 128u, o_cols = lanes + 256u + (uint32_t)g * 128u;
-    uint32_t turns[2] = {0u, 0u};
+    uint32_t turns[2] = {0u, 0u};  // tiles of each group in the pieces of work before
+    uint32_t it = 0, un = 0, wn = 0;
+    bool ok = true;
     constexpr int kHalf = D / 2;  // columns of O a thread writes
-    for (uint32_t unit = first; ok && unit < units; unit += step) {
+    for (uint32_t unit = first; unit < units; unit += step, ++un) {
+      if (!(ok = __all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag)))) break;
+      const int nt = sm.tiles[un % kInfo];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.iempty[un % kInfo]);
       const Work w = work_of(p, unit);
-      const int all = tiles_of(p.indices + (int64_t)w.token * p.idx_row, p.picks, lane);
-      const int nt = all > rank ? (all - rank + ctas - 1) / ctas : 0;
       const bool busy = (warp & 3) * 32 < w.heads, mine = r < w.heads;
       T* const out = static_cast<T*>(p.out) + (int64_t)w.token * p.out_token + (int64_t)(w.head0 + r) * p.out_head + g * kHalf;
       float* const lse = p.lse == nullptr ? nullptr : p.lse + (int64_t)w.token * p.kv_heads * p.group + w.head0 + r;
@@ -487,75 +605,106 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       }
       float ref = -INFINITY, vlog = 0.f, sum = 0.f;
       const uint32_t turn0 = turns[g];
-      for (int j = g; j < nt; j += 2) {
+      for (int j = g ^ (int)(it & 1u); j < nt; j += 2) {
         const uint32_t n = it + (uint32_t)j, turn = turn0 + (uint32_t)(j >> 1);
-        const int place = (int)(n % C::kMeta);
-        ok = mbar_wait(&sm.mfull[place], (n / C::kMeta) & 1u, abort_flag) && mbar_wait(&sm.sfull[g], turn & 1u, abort_flag);
+        const int place = (int)(n % kMeta);
+        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag) && mbar_wait(&sm.sfull[g], turn & 1u, abort_flag);
         if (!(ok = __all_sync(kAll, ok))) break;
         tmem_fence_after();
         if (busy) {
           const TileMeta& m = sm.meta[place];
-          const float qmul = sm.qmul[wn & 1u][r];
-          float top = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float s[32];
-            load_scores<kFp8>(s, s_cols + 32u * c, m.ks + 32 * c, m.live[c]);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
-          }
-          top *= qmul;
-          // the references: this head's largest score, and the exponent of the tile's largest v scale
-          float vnew = vlog;
-          if constexpr (kFp8) {
-            const float4 v = *reinterpret_cast<const float4*>(m.vmax);
-            const int e = (int)(__float_as_uint(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))) >> 23) - 127;
-            const float ve = (float)max(-100, min(e, 100));
-            if (j == g || ve > vlog + 6.f) vnew = ve;
-          }
-          const float next = top > ref + kLetStand ? top : ref;
-          if (j != g) {
-            const bool changed = next != ref || vnew != vlog;
-            if (__any_sync(kAll, changed)) {
-              const float f = !changed ? 1.f : ref == -INFINITY ? (next == -INFINITY ? 1.f : 0.f) : ex2((ref + vlog) - (next + vnew));
-              ok = mbar_wait(&sm.pvdone[g], (turn - 1u) & 1u, abort_flag);
-              if (!(ok = __all_sync(kAll, ok))) break;
+          const float qmul = sm.qmul[wn & 3u][r];
+          // A new reference: what was weighed with the old one - O, the sum, this tile's weights so far (`done` chunks) - is brought to it.
+          auto refer = [&](float next, float vnext, int done) {
+            const bool changed = next != ref || vnext != vlog;
+            const float f = !changed ? 1.f : ref == -INFINITY ? (next == -INFINITY ? 1.f : 0.f) : ex2((ref + vlog) - (next + vnext));
+            ref = next;
+            vlog = vnext;
+            sum *= f;
+            if (j > 1) {
+              if (!__all_sync(kAll, mbar_wait(&sm.pvdone[g], (turn - 1u) & 1u, abort_flag))) return;  // (the waits to come fail too)
               tmem_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t v[32];
-                tmem_ld32(o_cols + 32u * c, v);
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t v[16];
+                tmem_ld16(o_cols + 16u * c, v);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                tmem_st32(o_cols + 32u * c, v);
+                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                tmem_st16(o_cols + 16u * c, v);
               }
-              sum *= f;
             }
-          }
-          ref = next;
-          vlog = vnew;
-          const float sub = (ref == -INFINITY ? 0.f : ref) + vlog;
-          float part = 0.f;
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float s[32];
-            uint32_t pk[16];
-            load_scores<kFp8>(s, s_cols + 32u * c, m.ks + 32 * c, m.live[c]);
+            for (int c = 0; c < done; ++c) {
+              uint32_t v[16];
+              tmem_ld16(s_cols + 16u * c, v);
+              tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float a = ex2(fmaf(s[i], qmul, -sub)), b = ex2(fmaf(s[i + 1], qmul, -sub));
-              const float d = ex2(fmaf(s[i + 2], qmul, -sub)), e = ex2(fmaf(s[i + 3], qmul, -sub));
-              sum += a + b;
-              part += d + e;
-              float4 v = make_float4(1.f, 1.f, 1.f, 1.f);
-              if constexpr (kFp8) v = *reinterpret_cast<const float4*>(m.vs + 32 * c + i);
-              pk[i / 2] = kFp8 ? narrow2(a * v.x, b * v.y, M()) : narrow2(a, b, M());
-              pk[i / 2 + 1] = kFp8 ? narrow2(d * v.z, e * v.w, M()) : narrow2(d, e, M());
+              for (int i = 0; i < 16; ++i) {
+                const float2 x = widen2(v[i], M());
+                v[i] = narrow2(x.x * f, x.y * f, M());
+              }
+              tmem_st16(s_cols + 16u * c, v);
             }
-            tmem_st16(s_cols + 16u * c, pk);  // (over scores that have been read)
+          };
+          if constexpr (kFp8) {  // the exponent of the largest v scale
+            const int e = (int)(__float_as_uint(m.vtop) >> 23) - 127;
+            const float ve = (float)max(-100, min(e, 100));
+            if (j < 2)
+              vlog = ve;
+            else if (ve > vlog + 6.f)
+              refer(ref, ve, 0);
           }
-          sum += part;
+          const bool whole = (m.flags & kWhole) != 0;
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (int c = 0; c < kTileKeys / kChunk; ++c) {
+            float s[kChunk];
+            load_chunk(s_cols + (uint32_t)(kChunk * c), s);
+            tmem_wait_ld();
+            if constexpr (kFp8) {
+#pragma unroll
+              for (int i = 0; i < kChunk; i += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(m.ks + kChunk * c + i);
+                s[i] *= x.x, s[i + 1] *= x.y, s[i + 2] *= x.z, s[i + 3] *= x.w;
+              }
+            }
+            if (!whole) {
+#pragma unroll
+              for (int b = 0; b < kChunk / 32; ++b) {
+                const uint32_t there = m.live[kChunk / 32 * c + b];
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!(there >> i & 1u)) s[32 * b + i] = -INFINITY;
+              }
+            }
+            const float top = top_of(s) * qmul;
+            if (__any_sync(kAll, top > ref + kLetStand)) {
+              tmem_wait_st();
+              sum += (part[0] + part[1]) + (part[2] + part[3]);
+              part[0] = part[1] = part[2] = part[3] = 0.f;
+              refer(top > ref + kLetStand ? top : ref, vlog, kChunk / 32 * c);
+            }
+            const float sub = (ref == -INFINITY ? 0.f : ref) + vlog;
+            uint32_t pk[kChunk / 2];
+#pragma unroll
+            for (int i = 0; i < kChunk; i += 4) {
+              float w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                w[e] = ex2(fmaf(s[i + e], qmul, -sub));
+                part[e] += w[e];
+              }
+              if constexpr (kFp8) {
+                const float4 x = *reinterpret_cast<const float4*>(m.vs + kChunk * c + i);
+                w[0] *= x.x, w[1] *= x.y, w[2] *= x.z, w[3] *= x.w;
+              }
+              pk[i / 2] = narrow2(w[0], w[1], M());
+              pk[i / 2 + 1] = narrow2(w[2], w[3], M());
+            }
+            store_chunk(s_cols + (uint32_t)(kChunk / 2 * c), pk);  // (over scores that have been read)
+          }
+          sum += (part[0] + part[1]) + (part[2] + part[3]);
           tmem_wait_st();
         }
         tmem_fence_before();
@@ -564,13 +713,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       }
       if (!ok) break;
       // ---- this piece's end: both groups' products, maxima and sums ----
-      const int nga = (nt + 1) / 2, ngb = nt / 2;
+      const int nga = (nt + 1 - (int)(it & 1u)) / 2, ngb = nt - nga;  // tiles of group 0, of group 1
       float2 a = make_float2(-INFINITY, 0.f), b = a;
       if (nt > 0) {
         sm.ml[wn & 1u][g][r] = make_float2(ref == -INFINITY ? -INFINITY : ref + vlog, sum);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.mlbar);
-        ok = mbar_wait(&sm.mlbar, wn & 1u, abort_flag) && mbar_wait(&sm.pvdone[0], (turns[0] + (uint32_t)nga - 1u) & 1u, abort_flag);
+        ok = mbar_wait(&sm.mlbar, wn & 1u, abort_flag);
+        if (nga > 0) ok = ok && mbar_wait(&sm.pvdone[0], (turns[0] + (uint32_t)nga - 1u) & 1u, abort_flag);
         if (ngb > 0) ok = ok && mbar_wait(&sm.pvdone[1], (turns[1] + (uint32_t)ngb - 1u) & 1u, abort_flag);
         if (!(ok = __all_sync(kAll, ok))) break;
         tmem_fence_after();
@@ -580,7 +730,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       const float fa = a.x == top ? 1.f : ex2(a.x - top), fb = b.x == top ? 1.f : ex2(b.x - top);
       const float l = fa * a.y + fb * b.y;
       const float inv = ctas > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      float* const stage_row = reinterpret_cast<float*>(base + kTileBytes) + (size_t)r * (D + 4) + g * kHalf;  // (several CTAs: over the k tiles)
+      float* const stage_row = reinterpret_cast<float*>(base) + (size_t)r * (D + 4) + g * kHalf;  // (several CTAs: over the q and k tiles)
       if (busy) {
 #pragma unroll 1
         for (int c = 0; c < kHalf; c += 32) {
@@ -590,7 +740,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           for (int i = 0; i < 32; ++i) y[i] = 0.f;
 #pragma unroll 1
           for (int i = 0; i < 2; ++i) {
-            if (i < nt) {
+            if ((i == 0 ? nga : ngb) > 0) {
               uint32_t v[32];
               tmem_ld32(col + 128u * i, v);
               tmem_wait_ld();
@@ -622,6 +772,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     }
   }
   __syncwarp();
+  __syncthreads();
+  if (warp < kSoftmaxWarps)
+    fewer_registers<kRegsLaunch>();
+  else
+    more_registers<kRegsLaunch>();
   tmem_fence_before();
   __syncthreads();
   if (*abort_flag) {
@@ -640,20 +795,40 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     cluster.sync();
     const Work w = work_of(p, first);
     constexpr int kPer = D / 32;  // channels a lane
-    const float* mine_o = reinterpret_cast<const float*>(base + kTileBytes);
+    const uint32_t ml_at = smem_u32(&sm.ml[1][0][0]), o_at = smem_u32(base) + (uint32_t)(lane * kPer * 4);
     for (int h = rank + ctas * warp; h < w.heads; h += ctas * (kWideThreads / 32)) {
+      // (every CTA's part is asked for before any is used)
+      float2 ml[kAttendMaxCluster];
+      float o[kAttendMaxCluster][kPer];
+#pragma unroll
+      for (int c = 0; c < kAttendMaxCluster; ++c) {
+        ml[c] = make_float2(-INFINITY, 0.f);
+        if (c < ctas) {
+          ml[c] = lds_cluster2(shared_of(ml_at + (uint32_t)h * 8u, c));
+          const uint32_t from = shared_of(o_at + (uint32_t)(h * (D + 4) * 4), c);
+          if constexpr (kPer == 4) {
+            const float4 v = lds_cluster4(from);
+            o[c][0] = v.x, o[c][1] = v.y, o[c][2] = v.z, o[c][3] = v.w;
+          } else {
+            const float2 v = lds_cluster2(from);
+            o[c][0] = v.x, o[c][1] = v.y;
+          }
+        }
+      }
       float top = -INFINITY;
-      for (int c = 0; c < ctas; ++c) top = fmaxf(top, cluster.map_shared_rank(&sm.ml[1][0][h], c)->x);
+#pragma unroll
+      for (int c = 0; c < kAttendMaxCluster; ++c) top = fmaxf(top, ml[c].x);
       float l = 0.f, acc[kPer];
 #pragma unroll
       for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-      for (int c = 0; c < ctas; ++c) {
-        const float2 ml = *cluster.map_shared_rank(&sm.ml[1][0][h], c);
-        const float f = ml.x == top ? 1.f : ex2(ml.x - top);
-        l += f * ml.y;
-        const float* o = cluster.map_shared_rank(mine_o, c) + (size_t)h * (D + 4) + lane * kPer;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] += f * o[e];
+      for (int c = 0; c < kAttendMaxCluster; ++c) {
+        if (c < ctas) {
+          const float f = ml[c].x == top ? 1.f : ex2(ml[c].x - top);
+          l += f * ml[c].y;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) acc[e] += f * o[c][e];
+        }
       }
       T* out = static_cast<T*>(p.out) + (int64_t)w.token * p.out_token + (int64_t)(w.head0 + h) * p.out_head + lane * kPer;
 #pragma unroll

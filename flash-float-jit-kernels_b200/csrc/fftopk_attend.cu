@@ -30,6 +30,7 @@
 #include "fftopk_internal.h"
 #include "fftopk_attend.cuh"
 #include "fftopk_rows.cuh"
+#include "fftopk_tcgen05.cuh"
 
 namespace fftopk {
 namespace {
@@ -65,7 +66,7 @@ struct JoinSmem {
   float o[kWarps][kHeadsM][D];
   float m[kWarps][kHeadsM], l[kWarps][kHeadsM];
   float joined[kHeadsM][D];
-  float jm[kHeadsM], jl[kHeadsM];
+  float2 jml[kHeadsM];  // maximum and sum
 };
 
 // T: type of q and out, and of the cache where kFp8 is false
@@ -335,29 +336,52 @@ __global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid
       l += f * sm.l[w][h];
     }
     sm.joined[h][d] = acc;
-    if (d == 0) sm.jm[h] = m, sm.jl[h] = l;
+    if (d == 0) sm.jml[h] = make_float2(m, l);
   }
   if (ctas > 1)
     cluster.sync();
   else
     __syncthreads();
-  for (int i = tid + rank * kThreads; i < heads * D; i += kThreads * ctas) {
-    const int h = i / D, d = i % D;
-    float m = -INFINITY;
-    for (int c = 0; c < ctas; ++c) m = fmaxf(m, ctas > 1 ? *cluster.map_shared_rank(&sm.jm[h], c) : sm.jm[h]);
-    float acc = 0.f, l = 0.f;
-    for (int c = 0; c < ctas; ++c) {
-      const float cm = ctas > 1 ? *cluster.map_shared_rank(&sm.jm[h], c) : sm.jm[h];
-      const float f = cm == m ? 1.f : ex2(cm - m);
-      acc += f * (ctas > 1 ? *cluster.map_shared_rank(&sm.joined[h][d], c) : sm.joined[h][d]);
-      l += f * (ctas > 1 ? *cluster.map_shared_rank(&sm.jl[h], c) : sm.jl[h]);
+  // every CTA of the cluster finishes its share of the rows, four channels a thread
+  for (int i = tid + rank * kThreads; i < heads * (D / 4); i += kThreads * ctas) {
+    const int h = i / (D / 4), d = i % (D / 4) * 4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, l = 0.f;
+    if (ctas == 1) {
+      o = *reinterpret_cast<const float4*>(&sm.joined[h][d]);
+      m = sm.jml[h].x, l = sm.jml[h].y;
+    } else {
+      // (every CTA's part is asked for before any is used)
+      const uint32_t ml_at = smem_u32(&sm.jml[h]), o_at = smem_u32(&sm.joined[h][d]);
+      float2 ml[kAttendMaxCluster];
+      float4 part[kAttendMaxCluster];
+#pragma unroll
+      for (int c = 0; c < kAttendMaxCluster; ++c) {
+        ml[c] = make_float2(-INFINITY, 0.f);
+        if (c < ctas) {
+          ml[c] = lds_cluster2(shared_of(ml_at, c));
+          part[c] = lds_cluster4(shared_of(o_at, c));
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kAttendMaxCluster; ++c) m = fmaxf(m, ml[c].x);
+#pragma unroll
+      for (int c = 0; c < kAttendMaxCluster; ++c) {
+        if (c < ctas) {
+          const float f = ml[c].x == m ? 1.f : ex2(ml[c].x - m);
+          o.x += f * part[c].x, o.y += f * part[c].y, o.z += f * part[c].z, o.w += f * part[c].w;
+          l += f * ml[c].y;
+        }
+      }
     }
+    const float y[4] = {l == 0.f ? 0.f : o.x / l, l == 0.f ? 0.f : o.y / l, l == 0.f ? 0.f : o.z / l, l == 0.f ? 0.f : o.w / l};
     T* out = static_cast<T*>(p.out) + (int64_t)token * p.out_token + (int64_t)(head0 + h) * p.out_head + d;
-    const float y = l == 0.f ? 0.f : acc / l;
-    if constexpr (std::is_same<T, __half>::value)
-      *out = __float2half_rn(y);
+    Four<T> r;
+    r.narrow(y);
+    if (p.out_vec)
+      r.template store<true>(out);
     else
-      *out = __float2bfloat16_rn(y);
+      r.template store<false>(out);
     if (d == 0 && p.lse != nullptr)
       p.lse[(int64_t)token * p.kv_heads * p.group + head0 + h] = l == 0.f ? -INFINITY : m * 0.693147180559945309f + logf(l);
   }

@@ -10,9 +10,12 @@
 //           to nearest even, infinities to 448, NaN kept; scale = amax / 448
 // in 32 bits throughout, rounded once, where it is written. The reference has no counterpart: it starts from finished logits.
 //
-// What bounds it is memory: 8 channels a lane, one 16-byte load and store each (16-bit types), 8 to 32 lanes a row, so a row's
-// sums are three to five shuffles. A group of lanes takes several heads of ONE token where there are rows enough: it loads the
-// token's cosines and sines (64 bytes a lane for 16 bytes of a head) and the norm's weights once, and has that many loads in flight.
+// What bounds it is memory. A lane has two pieces of four neighbouring channels (8 bytes each of a 16-bit type): where the
+// rotation pairs channel i with i + R/2, the piece at i and the piece at its partners, so that it needs no exchange between lanes
+// and a piece of the table serves both; elsewhere one piece in each half of what is left. 8 to 32 lanes make a row, its sums are three to
+// five shuffles. A group of lanes takes several heads of ONE token where there are rows enough: it loads the token's cosines and
+// sines and the norm's weights once, and has that many loads in flight. A block works on one part alone, so that what a part is
+// like is known to the whole block.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -30,14 +33,15 @@ namespace {
 
 constexpr int kRowThreads = 256;
 constexpr int kMaxParts = 3;
+constexpr int kHeadsItem = 4;  // heads of a token that a group of lanes takes where there are rows enough
 constexpr float kAmaxFloor = 1.262177448353618888658765704452e-29f;  // 2^-96
 
 struct RowParams {
   fftopk_head_part part[kMaxParts];
-  int32_t first_item[kMaxParts + 1];  // items of a token: a part's first, and their number
-  int32_t aligned_w[kMaxParts];       // weight and bias may be read 16 bytes at a time
-  FastDiv per_token;
-  int64_t items;                      // tokens * items of a token
+  uint32_t first_block[kMaxParts];  // of a part; the grid is theirs in turn
+  FastDiv per_token[kMaxParts];     // items of a token
+  uint32_t items[kMaxParts];        // tokens * items of a token
+  int32_t aligned_w[kMaxParts];     // weight and bias may be read four at a time
   const int32_t* positions;
   const float* cos_sin;
   int64_t table_rows;
@@ -45,41 +49,48 @@ struct RowParams {
   uint32_t* status;
 };
 
-__device__ __forceinline__ void load_weights(float (&w)[8], const void* p, int32_t dtype, int at, bool aligned) {
+__device__ __forceinline__ void load_weights(float* w, const void* p, int32_t dtype, int at, bool aligned) {
   if (dtype == FFTOPK_DTYPE_FP32) {
-    load8<float>(w, static_cast<const float*>(p) + at, aligned);
+    load4(w, static_cast<const float*>(p) + at, aligned);
   } else if (dtype == FFTOPK_DTYPE_BF16) {
-    load8<__nv_bfloat16>(w, static_cast<const __nv_bfloat16*>(p) + at, aligned);
+    load4(w, static_cast<const __nv_bfloat16*>(p) + at, aligned);
   } else {
-    load8<__half>(w, static_cast<const __half*>(p) + at, aligned);
+    load4(w, static_cast<const __half*>(p) + at, aligned);
   }
 }
 
-// T: the rows' type; kLanes: lanes of a group (8 channels each); kHeads: heads an item takes; kVec: rows start on 16 bytes
+// T: the rows' type; kLanes: lanes of a group; kHeads: heads an item takes; kVec: pieces may be read and written as one
 template <typename T, int kLanes, int kHeads, bool kVec>
 __global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_constant__ RowParams p) {
-  const int lane = threadIdx.x & (kLanes - 1);
-  const int64_t item = (int64_t)blockIdx.x * (kRowThreads / kLanes) + threadIdx.x / kLanes;
-  // (groups beyond the last item stay for the shuffles, and touch nothing)
-  const bool in = item < p.items;
-  const uint32_t it = in ? (uint32_t)item : 0u;
-  const uint32_t token = p.per_token.div(it);
-  const int of_token = (int)(it - token * p.per_token.d);
-  const int which = of_token >= p.first_item[2] ? 2 : of_token >= p.first_item[1] ? 1 : 0;
+  const int which = blockIdx.x >= p.first_block[2] ? 2 : blockIdx.x >= p.first_block[1] ? 1 : 0;
   const fftopk_head_part& part = p.part[which];
-  const int h0 = (of_token - p.first_item[which]) * kHeads;
-  const int at = lane * 8;
-  const bool mine = in && at < p.D;
+  const int lane = threadIdx.x & (kLanes - 1);
   const uint32_t mask = group_mask<kLanes>();
+  const uint32_t item = (blockIdx.x - p.first_block[which]) * (uint32_t)(kRowThreads / kLanes) + threadIdx.x / kLanes;
+  // (groups beyond the last item stay for the shuffles, and touch nothing)
+  const bool in = item < p.items[which];
+  const uint32_t token = in ? p.per_token[which].div(item) : 0u;
+  const int h0 = in ? (int)(item - token * p.per_token[which].d) * kHeads : 0;
+  // the lane's pieces: channels at[0] .. at[0] + 3 and at[1] .. at[1] + 3
+  const int R = part.rotate ? p.R : 0;
+  const int pairs = p.interleaved ? 0 : R;  // channels that lie with their partners
+  const int back = lane - (pairs >> 3);
+  int at[2];
+  at[0] = back < 0 ? 4 * lane : pairs + 4 * back;
+  at[1] = at[0] + ((back < 0 ? pairs : p.D - pairs) >> 1);
+  const bool mine = in && lane * 8 < p.D;
 
-  Row8<T> raw[kHeads];
-  const T* x = static_cast<const T*>(part.x) + (int64_t)token * part.x_token_stride + at;
+  Four<T> raw[kHeads][2];
+  const T* x = static_cast<const T*>(part.x) + (int64_t)token * part.x_token_stride + (int64_t)h0 * part.x_head_stride;
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    raw[i].zero();
-    if (mine && h0 + i < part.heads) raw[i].template load<kVec>(x + (int64_t)(h0 + i) * part.x_head_stride);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      raw[i][e].zero();
+      if (mine && h0 + i < part.heads) raw[i][e].template load<kVec>(x + (int64_t)i * part.x_head_stride + at[e]);
+    }
   }
-  // where the row goes
+  // where the rows go
   int64_t to = token;
   bool keep = mine;
   if (part.slots != nullptr && in) {
@@ -90,51 +101,59 @@ __global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_con
       if (lane == 0 && h0 == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
     }
   }
-  float c[8], s[8];
-  const int R = part.rotate ? p.R : 0;
-  const bool turned = mine && at < R;
-  if (turned) {
+  float c[4], s[4];  // of the pairs; interleaved: of two pairs of each piece
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = 1.f, s[i] = 0.f;
+  if (R && mine) {
     const int64_t pos = p.positions[token];
-    const int half = R >> 1;
-    const bool ok = pos >= 0 && pos < p.table_rows;
-    if (ok) {
-      const float* row = p.cos_sin + pos * p.R;
-      if (p.interleaved) {
-        const float4 cc = *reinterpret_cast<const float4*>(row + (at >> 1)), ss = *reinterpret_cast<const float4*>(row + half + (at >> 1));
-        c[0] = cc.x, c[1] = cc.y, c[2] = cc.z, c[3] = cc.w;
-        s[0] = ss.x, s[1] = ss.y, s[2] = ss.z, s[3] = ss.w;
-      } else {
-        const int i = at < half ? at : at - half;
-        load8<float>(c, row + i, true);
-        load8<float>(s, row + half + i, true);
-      }
-    } else {
+    const float* row = p.cos_sin + pos * p.R;
+    const int half = p.R >> 1;
+    if (pos < 0 || pos >= p.table_rows) {
       // no such row in the table: the rotated channels become NaN
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
+      for (int i = 0; i < 4; ++i) {
+        if (p.interleaved ? at[i >> 1] < R : back < 0) c[i] = s[i] = __int_as_float(0x7fffffff);
+      }
       if (lane == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+    } else if (p.interleaved) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (at[e] < R) {
+          const float2 a = *reinterpret_cast<const float2*>(row + (at[e] >> 1)), b = *reinterpret_cast<const float2*>(row + half + (at[e] >> 1));
+          c[2 * e] = a.x, c[2 * e + 1] = a.y, s[2 * e] = b.x, s[2 * e + 1] = b.y;
+        }
+      }
+    } else if (back < 0) {
+      load4(c, row + at[0], true);
+      load4(s, row + half + at[0], true);
     }
   }
   float w[8], b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = 1.f, b[i] = 0.f;
-  if (mine && part.weight != nullptr) load_weights(w, part.weight, part.weight_dtype, at, p.aligned_w[which] != 0);
-  if (mine && part.bias != nullptr) load_weights(b, part.bias, part.weight_dtype, at, p.aligned_w[which] != 0);
+  if (part.norm != FFTOPK_NORM_NONE && mine) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (part.weight != nullptr) load_weights(w + 4 * e, part.weight, part.weight_dtype, at[e], p.aligned_w[which] != 0);
+      if (part.bias != nullptr) load_weights(b + 4 * e, part.bias, part.weight_dtype, at[e], p.aligned_w[which] != 0);
+    }
+  }
 
   const float inv_d = 1.f / (float)p.D;
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     float y[8];
-    raw[i].widen(y);
-    if (part.norm == FFTOPK_NORM_LAYER) {
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += y[e];
-      const float mean = group_sum<kLanes>(sum, mask) * inv_d;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = mine ? y[e] - mean : 0.f;
-    }
+    raw[i][0].widen(y);
+    raw[i][1].widen(y + 4);
     if (part.norm != FFTOPK_NORM_NONE) {
+      if (part.norm == FFTOPK_NORM_LAYER) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += y[e];
+        const float mean = group_sum<kLanes>(sum, mask) * inv_d;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = mine ? y[e] - mean : 0.f;
+      }
       float sq = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) sq = fmaf(y[e], y[e], sq);
@@ -142,24 +161,22 @@ __global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_con
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e] * r, w[e], b[e]);
     }
-    if (R) {  // the same for a whole group: R belongs to the part
+    if (R) {  // (channels that are not rotated have cosine 1 and sine 0, and are left as they are)
       if (p.interleaved) {
-        if (turned) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; ++e) {
+          if (at[e >> 1] < R) {
             const float u = y[2 * e], v = y[2 * e + 1];
             y[2 * e] = u * c[e] - v * s[e];
             y[2 * e + 1] = v * c[e] + u * s[e];
           }
         }
-      } else {
-        const int step = R >> 4;  // lanes from a channel to its partner's
-        const bool low = lane < step;
-        const int from = turned ? (low ? lane + step : lane - step) : lane;
+      } else if (back < 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float other = __shfl_sync(mask, y[e], from, kLanes);
-          if (turned) y[e] = low ? y[e] * c[e] - other * s[e] : y[e] * c[e] + other * s[e];
+        for (int e = 0; e < 4; ++e) {
+          const float u = y[e], v = y[e + 4];
+          y[e] = u * c[e] - v * s[e];
+          y[e + 4] = v * c[e] + u * s[e];
         }
       }
     }
@@ -167,10 +184,13 @@ __global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_con
     const bool put = keep && h < part.heads;
     if (part.scale == nullptr) {
       if (put) {
-        T* o = static_cast<T*>(part.out) + to * part.out_token_stride + (int64_t)h * part.out_head_stride + at;
-        Row8<T> r;
-        r.narrow(y);
-        r.template store<kVec>(o);
+        T* o = static_cast<T*>(part.out) + to * part.out_token_stride + (int64_t)h * part.out_head_stride;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          Four<T> r;
+          r.narrow(y + 4 * e);
+          r.template store<kVec>(o + at[e]);
+        }
       }
     } else {
       float amax = 0.f;
@@ -183,13 +203,16 @@ __global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_con
       amax = fmaxf(group_max<kLanes>(amax, mask), kAmaxFloor);
       const float inv = __fdiv_rn(448.f, amax);
       if (put) {
-        uint8_t* o = static_cast<uint8_t*>(part.out) + to * part.out_token_stride + (int64_t)h * part.out_head_stride + at;
-        const uint2 codes = to_e4m3(y, inv);
-        if constexpr (kVec) {
-          *reinterpret_cast<uint2*>(o) = codes;
-        } else {
+        uint8_t* o = static_cast<uint8_t*>(part.out) + to * part.out_token_stride + (int64_t)h * part.out_head_stride;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = (uint8_t)((e < 4 ? codes.x : codes.y) >> (8 * (e & 3)));
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t codes = to_e4m3(y + 4 * e, inv);
+          if constexpr (kVec) {
+            *reinterpret_cast<uint32_t*>(o + at[e]) = codes;
+          } else {
+#pragma unroll
+            for (int i2 = 0; i2 < 4; ++i2) o[at[e] + i2] = (uint8_t)(codes >> (8 * i2));
+          }
         }
         if (lane == 0) {
           const float scale = __fdiv_rn(amax, 448.f);
@@ -202,20 +225,24 @@ __global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_con
 }
 
 template <typename T, int kLanes>
-cudaError_t launch_rows(const RowParams& p, bool vec, int heads, cudaStream_t stream) {
-  const int64_t per_cta = kRowThreads / kLanes;
-  const unsigned grid = (unsigned)((p.items + per_cta - 1) / per_cta);
+cudaError_t launch_rows(RowParams& p, bool vec, int heads, cudaStream_t stream) {
+  const uint32_t per_cta = kRowThreads / kLanes;
+  uint32_t grid = 0;
+  for (int i = 0; i < kMaxParts; ++i) {
+    p.first_block[i] = grid;
+    grid += (p.items[i] + per_cta - 1) / per_cta;
+  }
   if (!vec)
     head_rows_kernel<T, kLanes, 1, false><<<grid, kRowThreads, 0, stream>>>(p);
   else if (heads == 1)
     head_rows_kernel<T, kLanes, 1, true><<<grid, kRowThreads, 0, stream>>>(p);
   else
-    head_rows_kernel<T, kLanes, 4, true><<<grid, kRowThreads, 0, stream>>>(p);
+    head_rows_kernel<T, kLanes, kHeadsItem, true><<<grid, kRowThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t launch_rows(const RowParams& p, bool vec, int heads, cudaStream_t stream) {
+cudaError_t launch_rows(RowParams& p, bool vec, int heads, cudaStream_t stream) {
   return p.D <= 64 ? launch_rows<T, 8>(p, vec, heads, stream)
                    : p.D <= 128 ? launch_rows<T, 16>(p, vec, heads, stream) : launch_rows<T, 32>(p, vec, heads, stream);
 }
@@ -234,6 +261,15 @@ struct ReadParams {
   int32_t D;
   uint32_t* status;
 };
+
+__device__ __forceinline__ void store8(float* o, const float (&y)[8]) {
+  reinterpret_cast<float4*>(o)[0] = make_float4(y[0], y[1], y[2], y[3]);
+  reinterpret_cast<float4*>(o)[1] = make_float4(y[4], y[5], y[6], y[7]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* o, const float (&y)[8]) {
+  *reinterpret_cast<uint4*>(o) = make_uint4(narrow2(y[0], y[1], T()), narrow2(y[2], y[3], T()), narrow2(y[4], y[5], T()), narrow2(y[6], y[7], T()));
+}
 
 // kLanes lanes a row, 8 codes each; kRows rows a group, one behind the other
 template <typename T, int kLanes, int kRows, bool kVec>
@@ -276,12 +312,11 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_kernel(const __grid_co
     const int64_t r = first + (int64_t)i * kGroups;
     if (r >= p.rows) break;
     float y[8];
-    from_e4m3(y, codes[i]);
+    from_e4m3(y, codes[i].x);
+    from_e4m3(y + 4, codes[i].y);
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] *= scale[i];
-    Row8<T> o;
-    o.narrow(y);
-    o.template store<true>(static_cast<T*>(p.out) + r * p.D + at);
+    store8(static_cast<T*>(p.out) + r * p.D + at, y);
   }
 }
 
@@ -341,11 +376,10 @@ int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tok
     const int we = elem_bytes(a.weight_dtype), oe = a.scale != nullptr ? 1 : es;
     if (!on(a.x, es) || !on(a.out, oe) || !on(a.scale, 4) || !on(a.slots, 4) || !on(a.mul, 4) || !on(a.weight, we) || !on(a.bias, we))
       return FFTOPK_EINVAL;
-    const int ob = a.scale != nullptr ? 8 : 16;  // bytes a lane stores at once
-    // (the stride of a lone token or head says nothing)
-    vec = vec && on(a.x, 16) && (tokens == 1 || a.x_token_stride * es % 16 == 0) && (a.heads == 1 || a.x_head_stride * es % 16 == 0);
-    vec = vec && on(a.out, ob) && ((tokens == 1 && a.slots == nullptr) || a.out_token_stride * oe % ob == 0) &&
-          (a.heads == 1 || a.out_head_stride * oe % ob == 0);
+    // pieces of four channels (the stride of a lone token or head says nothing)
+    vec = vec && on(a.x, 4 * es) && (tokens == 1 || a.x_token_stride % 4 == 0) && (a.heads == 1 || a.x_head_stride % 4 == 0);
+    vec = vec && on(a.out, 4 * oe) && ((tokens == 1 && a.slots == nullptr) || a.out_token_stride % 4 == 0) &&
+          (a.heads == 1 || a.out_head_stride % 4 == 0);
     rotates = rotates || a.rotate != 0;
     all_heads += a.heads;
   }
@@ -355,19 +389,17 @@ int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tok
       return FFTOPK_EINVAL;
   }
   if (tokens == 0 || all_heads == 0) return FFTOPK_OK;
-  // Four heads a group once there are rows for every group of the device: see the figures at the top
-  const int heads = vec && tokens * all_heads >= 148 * 64 * 4 ? 4 : 1;
-  int64_t per_token = 0;
+  // several heads a group once there are rows for every group of lanes the device holds
+  const int heads = vec && tokens * all_heads >= 148 * 64 * kHeadsItem ? kHeadsItem : 1;
+  if (tokens > 0x7fffffff) return FFTOPK_ERANGE;
   for (int i = 0; i < n_parts; ++i) {
     p.part[i] = parts[i];
-    p.first_item[i] = (int32_t)per_token;
-    per_token += (parts[i].heads + heads - 1) / heads;
+    const int64_t per_token = (parts[i].heads + heads - 1) / heads;
+    if (tokens * per_token > (int64_t)0x7fffffff - 64) return FFTOPK_ERANGE;
+    p.per_token[i] = FastDiv(per_token > 0 ? (uint32_t)per_token : 1u);
+    p.items[i] = (uint32_t)(tokens * per_token);
     p.aligned_w[i] = on(parts[i].weight, 16) && on(parts[i].bias, 16);
   }
-  for (int i = n_parts; i <= kMaxParts; ++i) p.first_item[i] = (int32_t)per_token;
-  if (per_token > 0x7fffffff || tokens > 0x7fffffff || tokens * per_token > (int64_t)0x7fffffff - 64) return FFTOPK_ERANGE;
-  p.per_token = FastDiv((uint32_t)per_token);
-  p.items = tokens * per_token;
   p.positions = positions;
   p.cos_sin = cos_sin;
   p.table_rows = table_rows;

@@ -1,4 +1,4 @@
-// Eight channels of a head row in a lane's registers: loads, stores, conversions and sums over a row's lanes.
+// Channels of a head row in a lane's registers, four at a time: loads, stores, conversions and sums over a row's lanes.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,84 +36,73 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b, __half) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// Four neighbouring channels: 8 bytes of a 16-bit type, 16 of fp32
 template <typename T>
-struct Row8 {  // 16-bit types: 16 bytes
-  uint32_t v[4];
-  __device__ __forceinline__ void zero() { v[0] = v[1] = v[2] = v[3] = 0u; }
+struct Four {
+  uint32_t v[2];
+  __device__ __forceinline__ void zero() { v[0] = v[1] = 0u; }
   template <bool kVec>
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (kVec) {
-      const uint4 r = *reinterpret_cast<const uint4*>(p);
-      v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+      const uint2 r = *reinterpret_cast<const uint2*>(p);
+      v[0] = r.x, v[1] = r.y;
     } else {
       const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = (uint32_t)q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
+      v[0] = (uint32_t)q[0] | (uint32_t)q[1] << 16, v[1] = (uint32_t)q[2] | (uint32_t)q[3] << 16;
     }
   }
   template <bool kVec>
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (kVec) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<uint2*>(p) = make_uint2(v[0], v[1]);
     } else {
       uint16_t* q = reinterpret_cast<uint16_t*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q[2 * i] = (uint16_t)v[i], q[2 * i + 1] = (uint16_t)(v[i] >> 16);
+      q[0] = (uint16_t)v[0], q[1] = (uint16_t)(v[0] >> 16), q[2] = (uint16_t)v[1], q[3] = (uint16_t)(v[1] >> 16);
     }
   }
-  __device__ __forceinline__ void widen(float (&y)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = widen2(v[i], T());
-      y[2 * i] = f.x, y[2 * i + 1] = f.y;
-    }
+  __device__ __forceinline__ void widen(float* y) const {
+    const float2 a = widen2(v[0], T()), b = widen2(v[1], T());
+    y[0] = a.x, y[1] = a.y, y[2] = b.x, y[3] = b.y;
   }
-  __device__ __forceinline__ void narrow(const float (&y)[8]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = narrow2(y[2 * i], y[2 * i + 1], T());
-  }
+  __device__ __forceinline__ void narrow(const float* y) { v[0] = narrow2(y[0], y[1], T()), v[1] = narrow2(y[2], y[3], T()); }
 };
 
 template <>
-struct Row8<float> {  // 32 bytes
-  float v[8];
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  }
+struct Four<float> {
+  float v[4];
+  __device__ __forceinline__ void zero() { v[0] = v[1] = v[2] = v[3] = 0.f; }
   template <bool kVec>
   __device__ __forceinline__ void load(const float* p) {
     if constexpr (kVec) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      const float4 a = *reinterpret_cast<const float4*>(p);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = p[i];
+      for (int i = 0; i < 4; ++i) v[i] = p[i];
     }
   }
   template <bool kVec>
   __device__ __forceinline__ void store(float* p) const {
     if constexpr (kVec) {
       *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = v[i];
+      for (int i = 0; i < 4; ++i) p[i] = v[i];
     }
   }
-  __device__ __forceinline__ void widen(float (&y)[8]) const {
+  __device__ __forceinline__ void widen(float* y) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = v[i];
+    for (int i = 0; i < 4; ++i) y[i] = v[i];
   }
-  __device__ __forceinline__ void narrow(const float (&y)[8]) {
+  __device__ __forceinline__ void narrow(const float* y) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = y[i];
+    for (int i = 0; i < 4; ++i) v[i] = y[i];
   }
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(float (&y)[8], const T* p, bool aligned) {
-  Row8<T> r;
+__device__ __forceinline__ void load4(float* y, const T* p, bool aligned) {
+  Four<T> r;
   if (aligned)
     r.template load<true>(p);
   else
@@ -141,25 +130,19 @@ __device__ __forceinline__ float group_max(float x, uint32_t mask) {
   return x;
 }
 
-// e4m3(y * inv), to nearest even; beyond 448 and infinities become 448, NaN stays NaN
-__device__ __forceinline__ uint2 to_e4m3(const float (&y)[8], float inv) {
-  uint32_t h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * inv, y[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+// e4m3(y * inv) of four, to nearest even; beyond 448 and infinities become 448, NaN stays NaN
+__device__ __forceinline__ uint32_t to_e4m3(const float* y, float inv) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0] * inv, y[1] * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2] * inv, y[3] * inv), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
 }
 __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint16_t v) {
   const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
   return (uint32_t)r.x | (uint32_t)r.y << 16;
 }
-__device__ __forceinline__ void from_e4m3(float (&y)[8], uint2 codes) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = i < 2 ? codes.x : codes.y;
-    const float2 f = widen2(e4m3x2_to_half2((uint16_t)(w >> (16 * (i & 1)))), __half());
-    y[2 * i] = f.x, y[2 * i + 1] = f.y;
-  }
+__device__ __forceinline__ void from_e4m3(float* y, uint32_t codes) {
+  const float2 a = widen2(e4m3x2_to_half2((uint16_t)codes), __half()), b = widen2(e4m3x2_to_half2((uint16_t)(codes >> 16)), __half());
+  y[0] = a.x, y[1] = a.y, y[2] = b.x, y[3] = b.y;
 }
 
 #endif  // __CUDACC__

@@ -373,7 +373,7 @@ int fftopk_indexer_topk2048(const void* q, const void* k_cache, int64_t k_rows_p
  *   cos_sin      device, fp32 [table_rows, rotary], contiguous, 16-byte aligned; positions int32 [tokens]; both may be NULL
  *                where no part is rotated
  *   tokens       tokens * heads may not reach 2^31 - 64 (FFTOPK_ERANGE)
- * Rows whose addresses are not all multiples of 16 bytes are read and written an element at a time.
+ * Rows of any part that do not all start on a multiple of four elements make the call read and write an element at a time.
  */
 #define FFTOPK_DTYPE_FP32 2 /* beside FFTOPK_DTYPE_FP16 and FFTOPK_DTYPE_BF16 */
 #define FFTOPK_NORM_NONE 0

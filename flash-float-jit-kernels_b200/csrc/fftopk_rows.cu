@@ -60,9 +60,8 @@ __device__ __forceinline__ void load_weights(float* w, const void* p, int32_t dt
 }
 
 // T: the rows' type; kLanes: lanes of a group; kHeads: heads an item takes; kVec: pieces may be read and written as one
-template <typename T, int kLanes, int kHeads, bool kVec>
-__global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_constant__ RowParams p) {
-  const int which = blockIdx.x >= p.first_block[2] ? 2 : blockIdx.x >= p.first_block[1] ? 1 : 0;
+template <typename T, int kLanes, int kHeads, bool kVec, int which>
+__device__ __forceinline__ void head_rows(const RowParams& p) {
   const fftopk_head_part& part = p.part[which];
   const int lane = threadIdx.x & (kLanes - 1);
   const uint32_t mask = group_mask<kLanes>();
@@ -101,112 +100,130 @@ __global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_con
       if (lane == 0 && h0 == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
     }
   }
-  float c[4], s[4];  // of the pairs; interleaved: of two pairs of each piece
+  // Cosines and sines. Partners apart: of channels at[0] .. at[0] + 3; interleaved: of two pairs of each piece, each twice, the sines
+  // with the signs the pair's two channels take the other one with.
+  Pair c[4], sn[4];
+  const Pair one = pair(1.f, 1.f), none = pair(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = 1.f, s[i] = 0.f;
+  for (int i = 0; i < 4; ++i) c[i] = one, sn[i] = none;
   if (R && mine) {
     const int64_t pos = p.positions[token];
-    const float* row = p.cos_sin + pos * p.R;
+    const bool ok = pos >= 0 && pos < p.table_rows;
+    if (!ok && lane == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+    const float nan = __int_as_float(0x7fffffff);  // (no such row in the table: the rotated channels become NaN)
+    const float* row = p.cos_sin + (ok ? pos : 0) * p.R;
     const int half = p.R >> 1;
-    if (pos < 0 || pos >= p.table_rows) {
-      // no such row in the table: the rotated channels become NaN
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (p.interleaved ? at[i >> 1] < R : back < 0) c[i] = s[i] = __int_as_float(0x7fffffff);
-      }
-      if (lane == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
-    } else if (p.interleaved) {
+    if (p.interleaved) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (at[e] < R) {
-          const float2 a = *reinterpret_cast<const float2*>(row + (at[e] >> 1)), b = *reinterpret_cast<const float2*>(row + half + (at[e] >> 1));
-          c[2 * e] = a.x, c[2 * e + 1] = a.y, s[2 * e] = b.x, s[2 * e + 1] = b.y;
+          float2 a = make_float2(nan, nan), b = a;
+          if (ok) a = *reinterpret_cast<const float2*>(row + (at[e] >> 1)), b = *reinterpret_cast<const float2*>(row + half + (at[e] >> 1));
+          c[2 * e] = pair(a.x, a.x), c[2 * e + 1] = pair(a.y, a.y);
+          sn[2 * e] = pair(-b.x, b.x), sn[2 * e + 1] = pair(-b.y, b.y);
         }
       }
     } else if (back < 0) {
-      load4(c, row + at[0], true);
-      load4(s, row + half + at[0], true);
+      float4 a = make_float4(nan, nan, nan, nan), b = a;
+      if (ok) a = *reinterpret_cast<const float4*>(row + at[0]), b = *reinterpret_cast<const float4*>(row + half + at[0]);
+      c[0] = pair(a.x, a.y), c[1] = pair(a.z, a.w);
+      sn[0] = pair(b.x, b.y), sn[1] = pair(b.z, b.w);
+      sn[2] = pair(-b.x, -b.y), sn[3] = pair(-b.z, -b.w);
     }
   }
-  float w[8], b[8];
+  Pair w[4], b[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = 1.f, b[i] = 0.f;
+  for (int i = 0; i < 4; ++i) w[i] = one, b[i] = none;
   if (part.norm != FFTOPK_NORM_NONE && mine) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      if (part.weight != nullptr) load_weights(w + 4 * e, part.weight, part.weight_dtype, at[e], p.aligned_w[which] != 0);
-      if (part.bias != nullptr) load_weights(b + 4 * e, part.bias, part.weight_dtype, at[e], p.aligned_w[which] != 0);
+      float f[4];
+      if (part.weight != nullptr) {
+        load_weights(f, part.weight, part.weight_dtype, at[e], p.aligned_w[which] != 0);
+        w[2 * e] = pair(f[0], f[1]), w[2 * e + 1] = pair(f[2], f[3]);
+      }
+      if (part.bias != nullptr) {
+        load_weights(f, part.bias, part.weight_dtype, at[e], p.aligned_w[which] != 0);
+        b[2 * e] = pair(f[0], f[1]), b[2 * e + 1] = pair(f[2], f[3]);
+      }
     }
   }
 
   const float inv_d = 1.f / (float)p.D;
+  const int64_t first = to * part.out_token_stride + (int64_t)h0 * part.out_head_stride;
+  float amax_of[kHeads];
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    float y[8];
+    Pair y[4];  // channels of piece 0, of piece 1
     raw[i][0].widen(y);
-    raw[i][1].widen(y + 4);
+    raw[i][1].widen(y + 2);
     if (part.norm != FFTOPK_NORM_NONE) {
       if (part.norm == FFTOPK_NORM_LAYER) {
-        float sum = 0.f;
+        const float2 t = apart(add2(add2(y[0], y[1]), add2(y[2], y[3])));
+        const float mean = group_sum<kLanes>(t.x + t.y, mask) * inv_d;
+        const Pair less = mine ? pair(-mean, -mean) : none;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += y[e];
-        const float mean = group_sum<kLanes>(sum, mask) * inv_d;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = mine ? y[e] - mean : 0.f;
+        for (int e = 0; e < 4; ++e) y[e] = add2(y[e], less);
       }
-      float sq = 0.f;
+      const float2 t = apart(add2(fma2(y[0], y[0], mul2(y[1], y[1])), fma2(y[2], y[2], mul2(y[3], y[3]))));
+      const float r = rsqrtf(group_sum<kLanes>(t.x + t.y, mask) * inv_d + part.eps);
+      const Pair rr = pair(r, r);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sq = fmaf(y[e], y[e], sq);
-      const float r = rsqrtf(group_sum<kLanes>(sq, mask) * inv_d + part.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e] * r, w[e], b[e]);
+      for (int e = 0; e < 4; ++e) y[e] = fma2(mul2(y[e], rr), w[e], b[e]);
     }
-    if (R) {  // (channels that are not rotated have cosine 1 and sine 0, and are left as they are)
+    if (R) {
       if (p.interleaved) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (at[e >> 1] < R) {
-            const float u = y[2 * e], v = y[2 * e + 1];
-            y[2 * e] = u * c[e] - v * s[e];
-            y[2 * e + 1] = v * c[e] + u * s[e];
-          }
+          if (at[e >> 1] < R) y[e] = fma2(turned(y[e]), sn[e], mul2(y[e], c[e]));
         }
       } else if (back < 0) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float u = y[e], v = y[e + 4];
-          y[e] = u * c[e] - v * s[e];
-          y[e + 4] = v * c[e] + u * s[e];
+        for (int e = 0; e < 2; ++e) {
+          const Pair u = y[e], v = y[e + 2];
+          y[e] = fma2(v, sn[e + 2], mul2(u, c[e]));
+          y[e + 2] = fma2(u, sn[e], mul2(v, c[e]));
         }
       }
     }
-    const int h = h0 + i;
-    const bool put = keep && h < part.heads;
+    const bool put = keep && h0 + i < part.heads;
     if (part.scale == nullptr) {
       if (put) {
-        T* o = static_cast<T*>(part.out) + to * part.out_token_stride + (int64_t)h * part.out_head_stride;
+        T* o = static_cast<T*>(part.out) + first + (int64_t)i * part.out_head_stride;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           Four<T> r;
-          r.narrow(y + 4 * e);
+          r.narrow(y + 2 * e);
           r.template store<kVec>(o + at[e]);
         }
       }
     } else {
-      float amax = 0.f;
+      float amax = 0.f;  // (NaN is passed over)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = fabsf(y[e]);
-        amax = fmaxf(amax, a <= 3.402823466e38f ? a : 0.f);
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = apart(y[e]);
+        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
       }
-      if (!mine) amax = 0.f;
-      amax = fmaxf(group_max<kLanes>(amax, mask), kAmaxFloor);
+      amax = group_max<kLanes>(mine ? amax : 0.f, mask);
+      if (amax > 3.402823466e38f) {  // an infinity: the largest of the others
+        amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = apart(y[e]);
+          if (fabsf(f.x) <= 3.402823466e38f) amax = fmaxf(amax, fabsf(f.x));
+          if (fabsf(f.y) <= 3.402823466e38f) amax = fmaxf(amax, fabsf(f.y));
+        }
+        amax = group_max<kLanes>(mine ? amax : 0.f, mask);
+      }
+      amax = fmaxf(amax, kAmaxFloor);
+      amax_of[i] = amax;
       const float inv = __fdiv_rn(448.f, amax);
       if (put) {
-        uint8_t* o = static_cast<uint8_t*>(part.out) + to * part.out_token_stride + (int64_t)h * part.out_head_stride;
+        const Pair ii = pair(inv, inv);
+        uint8_t* o = static_cast<uint8_t*>(part.out) + first + (int64_t)i * part.out_head_stride;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t codes = to_e4m3(y + 4 * e, inv);
+          const uint32_t codes = to_e4m3(mul2(y[2 * e], ii), mul2(y[2 * e + 1], ii));
           if constexpr (kVec) {
             *reinterpret_cast<uint32_t*>(o + at[e]) = codes;
           } else {
@@ -214,14 +231,33 @@ __global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_con
             for (int i2 = 0; i2 < 4; ++i2) o[at[e] + i2] = (uint8_t)(codes >> (8 * i2));
           }
         }
-        if (lane == 0) {
-          const float scale = __fdiv_rn(amax, 448.f);
-          part.scale[to * part.scale_token_stride + (int64_t)h * part.scale_head_stride] =
-              part.mul != nullptr ? part.mul[(int64_t)token * part.heads + h] * scale : scale;
-        }
       }
     }
   }
+  if (part.scale != nullptr) {  // lane i writes the scale of the item's row i
+    float amax = amax_of[0];
+#pragma unroll
+    for (int i = 1; i < kHeads; ++i)
+      if (lane == i) amax = amax_of[i];
+    const int h = h0 + lane;
+    if (keep && lane < kHeads && h < part.heads) {
+      const float scale = __fdiv_rn(amax, 448.f);
+      part.scale[to * part.scale_token_stride + (int64_t)h * part.scale_head_stride] =
+          part.mul != nullptr ? part.mul[(int64_t)token * part.heads + h] * scale : scale;
+    }
+  }
+}
+
+// (the part is a constant of the code: found by an index, each of its fields would be a load of its own at every use - 253 us
+// instead of 121 for 16,384 tokens of 72 heads)
+template <typename T, int kLanes, int kHeads, bool kVec>
+__global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_constant__ RowParams p) {
+  if (blockIdx.x < p.first_block[1])
+    head_rows<T, kLanes, kHeads, kVec, 0>(p);
+  else if (blockIdx.x < p.first_block[2])
+    head_rows<T, kLanes, kHeads, kVec, 1>(p);
+  else
+    head_rows<T, kLanes, kHeads, kVec, 2>(p);
 }
 
 template <typename T, int kLanes>

@@ -36,6 +36,38 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b, __half) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// Two fp32 values in one 64-bit register: sm_100 multiplies and adds them with one instruction
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 apart(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Pair turned(Pair a) {  // the two the other way around
+  const float2 f = apart(a);
+  return pair(f.y, f.x);
+}
+
 // Four neighbouring channels: 8 bytes of a 16-bit type, 16 of fp32
 template <typename T>
 struct Four {
@@ -65,6 +97,14 @@ struct Four {
     y[0] = a.x, y[1] = a.y, y[2] = b.x, y[3] = b.y;
   }
   __device__ __forceinline__ void narrow(const float* y) { v[0] = narrow2(y[0], y[1], T()), v[1] = narrow2(y[2], y[3], T()); }
+  __device__ __forceinline__ void widen(Pair* y) const {
+    const float2 a = widen2(v[0], T()), b = widen2(v[1], T());
+    y[0] = pair(a.x, a.y), y[1] = pair(b.x, b.y);
+  }
+  __device__ __forceinline__ void narrow(const Pair* y) {
+    const float2 a = apart(y[0]), b = apart(y[1]);
+    v[0] = narrow2(a.x, a.y, T()), v[1] = narrow2(b.x, b.y, T());
+  }
 };
 
 template <>
@@ -98,6 +138,11 @@ struct Four<float> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = y[i];
   }
+  __device__ __forceinline__ void widen(Pair* y) const { y[0] = pair(v[0], v[1]), y[1] = pair(v[2], v[3]); }
+  __device__ __forceinline__ void narrow(const Pair* y) {
+    const float2 a = apart(y[0]), b = apart(y[1]);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  }
 };
 
 template <typename T>
@@ -130,10 +175,10 @@ __device__ __forceinline__ float group_max(float x, uint32_t mask) {
   return x;
 }
 
-// e4m3(y * inv) of four, to nearest even; beyond 448 and infinities become 448, NaN stays NaN
-__device__ __forceinline__ uint32_t to_e4m3(const float* y, float inv) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0] * inv, y[1] * inv), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2] * inv, y[3] * inv), __NV_SATFINITE, __NV_E4M3);
+// e4m3 of four, to nearest even; beyond 448 and infinities become 448, NaN stays NaN
+__device__ __forceinline__ uint32_t to_e4m3(Pair a, Pair b) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(apart(a), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(apart(b), __NV_SATFINITE, __NV_E4M3);
   return lo | hi << 16;
 }
 __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint16_t v) {

@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import _native
-from .norm_rope import _DTYPES, FP8, _check_cache, _check_call, _check_rows, _check_vector, _no_grad, _part, _rows
+from .norm_rope import _DTYPES, _check_cache, _check_first, _check_rows, _check_vector, _no_grad, _quantised, _rows
 from .topk_indexer import _launch
 
 
@@ -31,23 +31,22 @@ def cache_write(
     A row's largest finite magnitude becomes 448 (scale = amax / 448, codes to nearest even); infinities become the largest code,
     NaN stays NaN. Rows that no slot names keep what they hold.
     """
-    if k.dim() != 3:
-        raise RuntimeError("k must be [tokens, heads, D]")
-    T, H, D = k.shape
-    idx = _check_call(k, None, None, D)
-    _check_rows(k, "k", idx, k.dtype, T, D)
-    _check_vector(slots, "slots", idx, T)
-    _check_cache(k_cache, k_scale, "k", idx, H, D)
+    idx, T, D, dtype = _check_first(k, "k")
+    H, xs = _check_rows(k, "k", idx, dtype, T, D)
+    at = _check_vector(slots, "slots", idx, T)
+    n, cs, ss = _check_cache(k_cache, k_scale, "k", idx, H, D)
     _no_grad(k, v)
-    parts = [_part(k, k_cache, scale=k_scale, slots=slots)]
-    if (v is None) != (v_cache is None) or (v is None) != (v_scale is None):
-        raise RuntimeError("v, v_cache and v_scale go together")
+    parts = _quantised(k, xs, H, k_cache, cs, k_scale, ss, at, n)
     if v is not None:
-        _check_rows(v, "v", idx, k.dtype, T, D)
-        _check_cache(v_cache, v_scale, "v", idx, v.size(1), D)
-        parts.append(_part(v, v_cache, scale=v_scale, slots=slots))
+        if v_cache is None:
+            raise RuntimeError("v, v_cache and v_scale go together")
+        H, xs = _check_rows(v, "v", idx, dtype, T, D)
+        n, cs, ss = _check_cache(v_cache, v_scale, "v", idx, H, D)
+        parts += _quantised(v, xs, H, v_cache, cs, v_scale, ss, at, n)
+    elif v_cache is not None or v_scale is not None:
+        raise RuntimeError("v, v_cache and v_scale go together")
     if T:
-        _rows(idx, parts, T, D, k.dtype, None, None, False)
+        _rows(idx, parts, T, D, dtype)
 
 
 def cache_read(
@@ -68,25 +67,24 @@ def cache_read(
     Returns:
         slots.shape + [H, D], contiguous. A row beyond the cache gives zeros and shows up in kernel_status().
     """
-    if not cache.is_cuda or cache.dim() != 3:
-        raise RuntimeError("cache must be a CUDA tensor [slots, heads, D]")
     idx = cache.get_device()
-    n, H, D = cache.shape
-    _check_cache(cache, scale, "", idx, H, D)
+    if idx < 0 or cache.dim() != 3:
+        raise RuntimeError("cache must be a CUDA tensor [slots, heads, D]")
+    _, H, D = cache.shape
+    n, cs, ss = _check_cache(cache, scale, "the", idx, H, D)
     if D % 8 or not 8 <= D <= 256:
         raise RuntimeError("D must be a multiple of 8 up to 256")
     if dtype not in _DTYPES:
         raise RuntimeError("dtype must be float16, bfloat16 or float32")
-    if slots.dtype != torch.int32 or slots.dim() not in (1, 2) or not slots.is_contiguous() or slots.get_device() != idx:
+    shape = slots.shape
+    if slots.dtype is not torch.int32 or len(shape) not in (1, 2) or not slots.is_contiguous() or slots.get_device() != idx:
         raise RuntimeError("slots must be a contiguous int32 tensor [B, K] or [K] on the cache's device")
-    rows, per_row = (1, slots.size(0)) if slots.dim() == 1 else slots.shape
-    if offsets is not None:
-        if slots.dim() != 2:
-            raise RuntimeError("offsets go with slots [B, K]")
-        _check_vector(offsets, "offsets", idx, rows)
-    out = torch.empty((*slots.shape, H, D), dtype=dtype, device=cache.device)
-    if out.numel():
-        _launch(_native.lib().fftopk_cache_read, "fftopk_cache_read", idx, cache.data_ptr(), cache.stride(0), cache.stride(1), n, H, D,
-                scale.data_ptr(), scale.stride(0), scale.stride(1), slots.data_ptr(), rows, per_row,
-                None if offsets is None else offsets.data_ptr(), out.data_ptr(), _DTYPES[dtype])
+    rows, per_row = shape if len(shape) == 2 else (1, shape[0])
+    if offsets is not None and len(shape) != 2:
+        raise RuntimeError("offsets go with slots [B, K]")
+    off = _check_vector(offsets, "offsets", idx, rows)
+    out = scale.new_empty((*shape, H, D), dtype=dtype)
+    if rows and per_row and H:
+        _launch(_native.lib().fftopk_cache_read, "fftopk_cache_read", idx, cache.data_ptr(), cs[0], cs[1], n, H, D, scale.data_ptr(), ss[0],
+                ss[1], slots.data_ptr(), rows, per_row, off, out.data_ptr(), _DTYPES[dtype])
     return out

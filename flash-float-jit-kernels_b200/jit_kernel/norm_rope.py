@@ -20,8 +20,11 @@ _NORMS = {None: 0, "rms": 1, "layer": 2}
 #: fftopk_head_part (include/fftopk.h)
 _PART = struct.Struct("@PqqPPPqqPqqPPqiiiifi")
 FP8 = torch.float8_e4m3fn
+_DENSE = torch.contiguous_format
 
 
+# An eager call on a few tokens is as long as its Python: every tensor is asked once for each of its properties, and the
+# pieces below hand on what they have asked for.
 def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -29,76 +32,108 @@ def _no_grad(*tensors) -> None:
                 raise RuntimeError("this op has no gradient: call it under torch.no_grad() or detach its inputs")
 
 
-def _check_rows(x: torch.Tensor, what: str, idx: int, dtype: torch.dtype, tokens: int, dim: int) -> None:
-    if x.dim() != 3 or x.size(0) != tokens or x.size(2) != dim:
-        raise RuntimeError(f"{what} must be [tokens, heads, D] with the tokens and the D of the others")
-    if x.dtype != dtype or x.get_device() != idx:
+def _check_rows(x: torch.Tensor, what: str, idx: int, dtype: torch.dtype, tokens: int, dim: int, heads: int = -1):
+    """(heads, strides) of x [tokens, heads, dim]"""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or (heads >= 0 and shape[1] != heads):
+        raise RuntimeError(f"{what} must be [tokens, heads, D] with the tokens and the D of the others, and an output of its input's shape")
+    if x.dtype is not dtype or x.get_device() != idx:
         raise RuntimeError(f"{what} must be of the others' type and on their device")
-    if x.stride(2) != 1 and dim > 1:
+    if stride[2] != 1 and dim > 1:
         raise RuntimeError(f"{what} must have unit inner stride")
+    return shape[1], stride
 
 
-def _check_vector(t: Optional[torch.Tensor], what: str, idx: int, n: int, dtype: torch.dtype = torch.int32) -> None:
-    if t is not None and (t.dtype != dtype or t.dim() != 1 or t.size(0) != n or not t.is_contiguous() or t.get_device() != idx):
-        raise RuntimeError(f"{what} must be a contiguous {dtype} tensor of shape [{n}] on the inputs' device")
+def _check_vector(t: Optional[torch.Tensor], what: str, idx: int, n: int) -> int:
+    """The address of an int32 vector of n (0: None)"""
+    if t is None:
+        return 0
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != idx:
+        raise RuntimeError(f"{what} must be a contiguous int32 tensor of shape [{n}] on the inputs' device")
+    return t.data_ptr()
 
 
-def _check_norm(norm, weight, bias, what: str, idx: int, dim: int) -> None:
+def _check_norm(norm, weight, bias, what: str, idx: int, dim: int):
+    """(weight's address, bias', their type, the norm) as the C entry takes them"""
+    if norm is None:
+        if weight is not None or bias is not None:
+            raise RuntimeError(f"{what}_weight and {what}_bias go with a norm")
+        return 0, 0, 0, 0
     if norm not in _NORMS:
         raise RuntimeError(f"{what}_norm must be None, 'rms' or 'layer'")
-    if norm is None and (weight is not None or bias is not None):
-        raise RuntimeError(f"{what}_weight and {what}_bias go with a norm")
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None and (t.dtype not in _DTYPES or t.dim() != 1 or t.size(0) != dim or not t.is_contiguous()
-                              or t.get_device() != idx):
-            raise RuntimeError(f"{what}_{name} must be a contiguous floating tensor of shape [D] on the inputs' device")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise RuntimeError(f"{what}_weight and {what}_bias must have the same type")
+    at, kind = [0, 0], None
+    for i, t in enumerate((weight, bias)):
+        if t is None:
+            continue
+        if t.dtype not in _DTYPES or t.shape != (dim,) or not t.is_contiguous() or t.get_device() != idx:
+            raise RuntimeError(f"{what}_weight and {what}_bias must be contiguous floating tensors of shape [D] on the inputs' device")
+        if kind is not None and t.dtype is not kind:
+            raise RuntimeError(f"{what}_weight and {what}_bias must have the same type")
+        at[i], kind = t.data_ptr(), t.dtype
+    return at[0], at[1], 0 if kind is None else _DTYPES[kind], _NORMS[norm]
 
 
-def _check_cache(cache: torch.Tensor, scale: torch.Tensor, what: str, idx: int, heads: int, dim: int) -> None:
-    if cache.dtype != FP8 or cache.dim() != 3 or cache.size(1) != heads or cache.size(2) != dim or cache.get_device() != idx:
+def _check_cache(cache: torch.Tensor, scale: torch.Tensor, what: str, idx: int, heads: int, dim: int):
+    """(slots, strides, scale's strides) of a quantised cache [slots, heads, dim]"""
+    shape, stride = cache.shape, cache.stride()
+    if cache.dtype is not FP8 or len(shape) != 3 or shape[1] != heads or shape[2] != dim or cache.get_device() != idx:
         raise RuntimeError(f"{what}_cache must be float8_e4m3fn [slots, heads, D] on the inputs' device")
-    if cache.stride(2) != 1 and dim > 1:
+    if stride[2] != 1 and dim > 1:
         raise RuntimeError(f"{what}_cache must have unit inner stride")
-    if scale is None or scale.dtype != torch.float32 or scale.shape != cache.shape[:2] or scale.get_device() != idx:
+    if scale is None or scale.dtype is not torch.float32 or scale.shape != shape[:2] or scale.get_device() != idx:
         raise RuntimeError(f"{what}_scale must be float32 [slots, heads] on the inputs' device")
+    return shape[0], stride, scale.stride()
 
 
-def _part(x, out, norm=None, weight=None, bias=None, rotate=False, eps=0.0, scale=None, mul=None, slots=None) -> bytes:
-    """A part as the C entry takes it: x [T, H, D] into `out` [T or slots, H, D] (and scale [.., H])."""
-    wd = weight if weight is not None else bias
-    return _PART.pack(
-        x.data_ptr(), x.stride(0), x.stride(1), 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
-        out.data_ptr(), out.stride(0), out.stride(1), 0 if scale is None else scale.data_ptr(),
-        0 if scale is None else scale.stride(0), 0 if scale is None else scale.stride(1), 0 if mul is None else mul.data_ptr(),
-        0 if slots is None else slots.data_ptr(), 0 if slots is None else out.size(0), x.size(1), _NORMS[norm], int(rotate),
-        0 if wd is None else _DTYPES[wd.dtype], eps, 0)
+_PLAIN = (0, 0, 0, 0)
 
 
-def _rows(idx: int, parts, tokens: int, dim: int, dtype: torch.dtype, positions, cos_sin, interleaved: bool) -> None:
-    _launch(_native.lib().fftopk_head_rows, "fftopk_head_rows", idx, b"".join(parts), len(parts), tokens, dim, _DTYPES[dtype],
-            None if positions is None else positions.data_ptr(), None if cos_sin is None else cos_sin.data_ptr(),
-            0 if cos_sin is None else cos_sin.size(0), 0 if cos_sin is None else cos_sin.size(1), int(interleaved))
+def _dense(x, xs, heads, out, os, norm=_PLAIN, rotate=0, eps=0.0) -> bytes:
+    """A part as the C entry takes it: x [T, H, D] into `out` of the same type."""
+    return _PART.pack(x.data_ptr(), xs[0], xs[1], norm[0], norm[1], out.data_ptr(), os[0], os[1], 0, 0, 0, 0, 0, 0, heads, norm[3], rotate,
+                      norm[2], eps, 0)
 
 
-def _check_call(x: torch.Tensor, positions, cos_sin, dim: int) -> int:
-    if not x.is_cuda:
+def _quantised(x, xs, heads, out, os, scale, ss, slots=0, n=0, mul=0, norm=_PLAIN, rotate=0, eps=0.0) -> bytes:
+    """A part that ends as e4m3 in `out`, with its scales."""
+    return _PART.pack(x.data_ptr(), xs[0], xs[1], norm[0], norm[1], out.data_ptr(), os[0], os[1], scale.data_ptr(), ss[0], ss[1], mul, slots,
+                      n, heads, norm[3], rotate, norm[2], eps, 0)
+
+
+def _rows(idx: int, parts: bytes, tokens: int, dim: int, dtype: torch.dtype, table=(0, 0, 0, 0), interleaved: bool = False) -> None:
+    _launch(_native.lib().fftopk_head_rows, "fftopk_head_rows", idx, parts, len(parts) // _PART.size, tokens, dim, _DTYPES[dtype], table[0],
+            table[1], table[2], table[3], interleaved)
+
+
+def _check_first(x: torch.Tensor, what: str):
+    """(device, tokens, D, type) of the first input, which the others go by"""
+    shape, dtype, idx = x.shape, x.dtype, x.get_device()
+    if idx < 0:
         raise RuntimeError("the inputs must be CUDA tensors")
-    if x.dtype not in _DTYPES:
+    if len(shape) != 3:
+        raise RuntimeError(f"{what} must be [tokens, heads, D]")
+    if dtype not in _DTYPES:
         raise RuntimeError("the inputs must be float16, bfloat16 or float32")
+    dim = shape[2]
     if dim % 8 or not 8 <= dim <= 256:
         raise RuntimeError("D must be a multiple of 8 up to 256")
-    idx = x.get_device()
-    if (positions is None) != (cos_sin is None):
+    return idx, shape[0], dim, dtype
+
+
+def _check_table(positions, cos_sin, idx: int, tokens: int, dim: int):
+    """(positions' address, cos_sin's, its rows, its columns); zeros without a rotation"""
+    if cos_sin is None:
+        if positions is not None:
+            raise RuntimeError("positions and cos_sin go together")
+        return 0, 0, 0, 0
+    if positions is None:
         raise RuntimeError("positions and cos_sin go together")
-    if cos_sin is not None:
-        _check_vector(positions, "positions", idx, x.size(0))
-        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.get_device() != idx:
-            raise RuntimeError("cos_sin must be a contiguous float32 tensor [positions, rotary] on the inputs' device")
-        if cos_sin.size(1) % 16 or not 16 <= cos_sin.size(1) <= dim:
-            raise RuntimeError("the rotated channels (cos_sin's columns) must be a multiple of 16 up to D")
-    return idx
+    shape = cos_sin.shape
+    if cos_sin.dtype is not torch.float32 or len(shape) != 2 or not cos_sin.is_contiguous() or cos_sin.get_device() != idx:
+        raise RuntimeError("cos_sin must be a contiguous float32 tensor [positions, rotary] on the inputs' device")
+    if shape[1] % 16 or not 16 <= shape[1] <= dim:
+        raise RuntimeError("the rotated channels (cos_sin's columns) must be a multiple of 16 up to D")
+    return _check_vector(positions, "positions", idx, tokens), cos_sin.data_ptr(), shape[0], shape[1]
 
 
 def qk_norm_rope(
@@ -133,33 +168,29 @@ def qk_norm_rope(
     Returns:
         (q_out, k_out), of q's and k's shapes and type.
     """
-    if q.dim() != 3:
-        raise RuntimeError("q must be [tokens, heads, D]")
-    T, _, D = q.shape
-    idx = _check_call(q, positions, cos_sin, D)
-    _check_rows(q, "q", idx, q.dtype, T, D)
-    _check_norm(q_norm, q_weight, q_bias, "q", idx, D)
+    idx, T, D, dtype = _check_first(q, "q")
+    table = _check_table(positions, cos_sin, idx, T, D)
+    rotate = 1 if cos_sin is not None else 0
+    heads, xs = _check_rows(q, "q", idx, dtype, T, D)
+    norm = _check_norm(q_norm, q_weight, q_bias, "q", idx, D)
     _no_grad(q, k, q_weight, k_weight, q_bias, k_bias)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q, memory_format=_DENSE)
+        os = (heads * D, D)
     else:
-        _check_rows(q_out, "q_out", idx, q.dtype, T, D)
-        if q_out.size(1) != q.size(1):
-            raise RuntimeError("q_out must have q's shape")
-    rotate = cos_sin is not None
-    parts = [_part(q, q_out, q_norm, q_weight, q_bias, rotate, eps)]
+        _, os = _check_rows(q_out, "q_out", idx, dtype, T, D, heads)
+    parts = _dense(q, xs, heads, q_out, os, norm, rotate, eps)
     if k is not None:
-        _check_rows(k, "k", idx, q.dtype, T, D)
-        _check_norm(k_norm, k_weight, k_bias, "k", idx, D)
+        heads, xs = _check_rows(k, "k", idx, dtype, T, D)
+        norm = _check_norm(k_norm, k_weight, k_bias, "k", idx, D)
         if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            k_out = torch.empty_like(k, memory_format=_DENSE)
+            os = (heads * D, D)
         else:
-            _check_rows(k_out, "k_out", idx, q.dtype, T, D)
-            if k_out.size(1) != k.size(1):
-                raise RuntimeError("k_out must have k's shape")
-        parts.append(_part(k, k_out, k_norm, k_weight, k_bias, rotate, eps))
+            _, os = _check_rows(k_out, "k_out", idx, dtype, T, D, heads)
+        parts += _dense(k, xs, heads, k_out, os, norm, rotate, eps)
     if T:
-        _rows(idx, parts, T, D, q.dtype, positions, cos_sin, interleaved)
+        _rows(idx, parts, T, D, dtype, table, interleaved)
     return q_out, k_out
 
 
@@ -187,29 +218,24 @@ def qkv_norm_rope_write(
 ) -> torch.Tensor:
     """qk_norm_rope and kv_cache.cache_write in one launch: q comes back normed and rotated, k is normed, rotated and quantised
     into row slots[t] of k_cache, v quantised into v_cache. Arguments as for those two."""
-    if q.dim() != 3:
-        raise RuntimeError("q must be [tokens, heads, D]")
-    T, _, D = q.shape
-    idx = _check_call(q, positions, cos_sin, D)
-    for x, what in ((q, "q"), (k, "k"), (v, "v")):
-        _check_rows(x, what, idx, q.dtype, T, D)
-    _check_norm(q_norm, q_weight, q_bias, "q", idx, D)
-    _check_norm(k_norm, k_weight, k_bias, "k", idx, D)
-    _check_vector(slots, "slots", idx, T)
-    _check_cache(k_cache, k_scale, "k", idx, k.size(1), D)
-    _check_cache(v_cache, v_scale, "v", idx, v.size(1), D)
+    idx, T, D, dtype = _check_first(q, "q")
+    table = _check_table(positions, cos_sin, idx, T, D)
+    rotate = 1 if cos_sin is not None else 0
+    (qh, qs), (kh, ks), (vh, vs) = (_check_rows(x, what, idx, dtype, T, D) for x, what in ((q, "q"), (k, "k"), (v, "v")))
+    q_how, k_how = _check_norm(q_norm, q_weight, q_bias, "q", idx, D), _check_norm(k_norm, k_weight, k_bias, "k", idx, D)
+    at = _check_vector(slots, "slots", idx, T)
+    kn, kcs, kss = _check_cache(k_cache, k_scale, "k", idx, kh, D)
+    vn, vcs, vss = _check_cache(v_cache, v_scale, "v", idx, vh, D)
     _no_grad(q, k, v, q_weight, k_weight, q_bias, k_bias)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q, memory_format=_DENSE)
+        os = (qh * D, D)
     else:
-        _check_rows(q_out, "q_out", idx, q.dtype, T, D)
-        if q_out.size(1) != q.size(1):
-            raise RuntimeError("q_out must have q's shape")
-    rotate = cos_sin is not None
+        _, os = _check_rows(q_out, "q_out", idx, dtype, T, D, qh)
     if T:
-        _rows(idx, [_part(q, q_out, q_norm, q_weight, q_bias, rotate, eps),
-                    _part(k, k_cache, k_norm, k_weight, k_bias, rotate, eps, k_scale, None, slots),
-                    _part(v, v_cache, scale=v_scale, slots=slots)], T, D, q.dtype, positions, cos_sin, interleaved)
+        _rows(idx, _dense(q, qs, qh, q_out, os, q_how, rotate, eps)
+              + _quantised(k, ks, kh, k_cache, kcs, k_scale, kss, at, kn, 0, k_how, rotate, eps)
+              + _quantised(v, vs, vh, v_cache, vcs, v_scale, vss, at, vn), T, D, dtype, table, interleaved)
     return q_out
 
 
@@ -245,28 +271,27 @@ def indexer_qk_write(
         (q8, w8): q as float8_e4m3fn [T, H, D] and w times the scale of each head's row, float32 [T, H] - relu(s x) = s relu(x)
         for a positive scale, so FusedIndexerTopk(q8, k_cache, w8, lengths, k_scale=k_scale) ranks as with q itself.
     """
-    if q.dim() != 3 or k.dim() != 2:
-        raise RuntimeError("q must be [tokens, heads, D] and k [tokens, D]")
-    T, H, D = q.shape
-    idx = _check_call(q, positions, cos_sin, D)
-    k3 = k.unsqueeze(1)
-    _check_rows(q, "q", idx, q.dtype, T, D)
-    _check_rows(k3, "k", idx, q.dtype, T, D)
-    _check_norm(q_norm, q_weight, q_bias, "q", idx, D)
-    _check_norm(k_norm, k_weight, k_bias, "k", idx, D)
-    _check_vector(slots, "slots", idx, T)
-    if w.dtype != torch.float32 or w.shape != (T, H) or not w.is_contiguous() or w.get_device() != idx:
+    idx, T, D, dtype = _check_first(q, "q")
+    table = _check_table(positions, cos_sin, idx, T, D)
+    rotate = 1 if cos_sin is not None else 0
+    H, qs = _check_rows(q, "q", idx, dtype, T, D)
+    ks = k.stride()
+    if k.shape != (T, D) or k.dtype is not dtype or k.get_device() != idx or ks[1] != 1:
+        raise RuntimeError("k must be [tokens, D], of q's type and on its device, with unit inner stride")
+    q_how, k_how = _check_norm(q_norm, q_weight, q_bias, "q", idx, D), _check_norm(k_norm, k_weight, k_bias, "k", idx, D)
+    at = _check_vector(slots, "slots", idx, T)
+    if w.dtype is not torch.float32 or w.shape != (T, H) or not w.is_contiguous() or w.get_device() != idx:
         raise RuntimeError("w must be a contiguous float32 tensor [tokens, heads] on the inputs' device")
-    if k_cache.dim() < 2 or not k_cache.is_contiguous() or not k_scale.is_contiguous() or k_scale.shape != k_cache.shape[:-1]:
-        raise RuntimeError("k_cache must be contiguous [.., rows, D] and k_scale contiguous of its shape without D")
-    rows, scales = k_cache.view(-1, 1, k_cache.size(-1)), k_scale.view(-1, 1)
-    _check_cache(rows, scales, "k", idx, 1, D)
+    shape = k_cache.shape
+    if k_cache.dtype is not FP8 or len(shape) < 2 or shape[-1] != D or not k_cache.is_contiguous() or k_cache.get_device() != idx:
+        raise RuntimeError("k_cache must be contiguous float8_e4m3fn [.., rows, D] on the inputs' device")
+    if k_scale.dtype is not torch.float32 or k_scale.shape != shape[:-1] or not k_scale.is_contiguous() or k_scale.get_device() != idx:
+        raise RuntimeError("k_scale must be contiguous float32 of k_cache's shape without D on the inputs' device")
     _no_grad(q, k, w, q_weight, k_weight, q_bias, k_bias)
-    q8 = torch.empty((T, H, D), dtype=FP8, device=q.device)
-    w8 = torch.empty((T, H), dtype=torch.float32, device=q.device)
-    rotate = cos_sin is not None
+    q8 = torch.empty_like(q, dtype=FP8, memory_format=_DENSE)
+    w8 = torch.empty_like(w)
     if T:
-        _rows(idx, [_part(q, q8, q_norm, q_weight, q_bias, rotate, eps, w8, w),
-                    _part(k3, rows, k_norm, k_weight, k_bias, rotate, eps, scales, None, slots)], T, D, q.dtype, positions, cos_sin,
-              interleaved)
+        _rows(idx, _quantised(q, qs, H, q8, (H * D, D), w8, (H, 1), 0, 0, w.data_ptr(), q_how, rotate, eps)
+              + _quantised(k, (ks[0], D), 1, k_cache, (D, D), k_scale, (1, 1), at, k_scale.numel(), 0, k_how, rotate, eps), T, D, dtype,
+              table, interleaved)
     return q8, w8

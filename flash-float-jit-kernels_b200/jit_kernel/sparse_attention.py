@@ -11,9 +11,10 @@ from typing import Optional
 import torch
 
 from . import _native
-from .norm_rope import FP8, _check_cache, _check_vector, _no_grad
+from .norm_rope import _DENSE, FP8, _check_cache, _check_vector, _no_grad
 from .topk_indexer import _launch
 
+_TYPES = {torch.float16: 0, torch.bfloat16: 1}
 #: fftopk_attend (include/fftopk.h)
 _ARGS = struct.Struct("@PqqPqqPqqPqqPqqPqPPqqPqqiiiiif")
 
@@ -45,51 +46,55 @@ def sparse_attention(
     Returns:
         out, or (out, lse) with lse float32 [T, Hq], the log of the sum of exponentials. A token without entries: 0 and -inf.
     """
-    if not q.is_cuda or q.dim() != 3:
+    idx, shape, qs, dtype = q.get_device(), q.shape, q.stride(), q.dtype
+    if idx < 0 or len(shape) != 3:
         raise RuntimeError("q must be a CUDA tensor [tokens, heads, D]")
-    T, Hq, D = q.shape
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    T, Hq, D = shape
+    if dtype not in _TYPES:
         raise RuntimeError("q must be float16 or bfloat16")
     if D not in (64, 128):
         raise RuntimeError("D must be 64 or 128")
-    idx = q.get_device()
-    if q.stride(2) != 1:
+    if qs[2] != 1:
         raise RuntimeError("q must have unit inner stride")
-    if k_cache.dim() != 3 or k_cache.shape != v_cache.shape or k_cache.size(2) != D:
+    shape = k_cache.shape
+    if len(shape) != 3 or v_cache.shape != shape or shape[2] != D:
         raise RuntimeError("k_cache and v_cache must be [slots, heads, D] with q's D")
-    slots, Hk, _ = k_cache.shape
+    slots, Hk, _ = shape
     if Hk == 0 or Hq % Hk:
         raise RuntimeError("q's heads must be a multiple of the cache's")
-    fp8 = k_cache.dtype == FP8
-    if fp8:
-        _check_cache(k_cache, k_scale, "k", idx, Hk, D)
-        _check_cache(v_cache, v_scale, "v", idx, Hk, D)
+    ka = va = 0
+    if k_cache.dtype is FP8:
+        _, ks, kss = _check_cache(k_cache, k_scale, "k", idx, Hk, D)
+        _, vs, vss = _check_cache(v_cache, v_scale, "v", idx, Hk, D)
+        ka, va = k_scale.data_ptr(), v_scale.data_ptr()
     else:
         if k_scale is not None or v_scale is not None:
             raise RuntimeError("k_scale and v_scale go with float8_e4m3fn caches")
-        if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
             raise RuntimeError("the caches must both be of q's type, or both float8_e4m3fn")
         if k_cache.get_device() != idx or v_cache.get_device() != idx:
             raise RuntimeError("the caches must be on q's device")
-        if k_cache.stride(2) != 1 or v_cache.stride(2) != 1:
+        ks, vs, kss, vss = k_cache.stride(), v_cache.stride(), (0, 0), (0, 0)
+        if ks[2] != 1 or vs[2] != 1:
             raise RuntimeError("the caches must have unit inner stride")
-    if indices.dtype != torch.int32 or indices.dim() != 2 or indices.size(0) != T or indices.get_device() != idx \
-            or (indices.size(1) > 1 and indices.stride(1) != 1):
+    picks, step = indices.shape, indices.stride()
+    if indices.dtype is not torch.int32 or len(picks) != 2 or picks[0] != T or indices.get_device() != idx \
+            or (picks[1] > 1 and step[1] != 1):
         raise RuntimeError("indices must be an int32 tensor [tokens, K] with unit inner stride on q's device")
-    _check_vector(offsets, "offsets", idx, T)
+    off = _check_vector(offsets, "offsets", idx, T)
     _no_grad(q, k_cache, v_cache, k_scale, v_scale)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape or out.get_device() != idx or out.stride(2) != 1:
-        raise RuntimeError("out must have q's shape and type, unit inner stride, on q's device")
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+        out = torch.empty_like(q, memory_format=_DENSE)
+        os = (Hq * D, D)
+    else:
+        os = out.stride()
+        if out.dtype is not dtype or out.shape != q.shape or out.get_device() != idx or os[2] != 1:
+            raise RuntimeError("out must have q's shape and type, unit inner stride, on q's device")
+    lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if T and Hq:
         args = _ARGS.pack(
-            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), v_cache.data_ptr(),
-            v_cache.stride(0), v_cache.stride(1), k_scale.data_ptr() if fp8 else 0, k_scale.stride(0) if fp8 else 0,
-            k_scale.stride(1) if fp8 else 0, v_scale.data_ptr() if fp8 else 0, v_scale.stride(0) if fp8 else 0,
-            v_scale.stride(1) if fp8 else 0, indices.data_ptr(), indices.stride(0), 0 if offsets is None else offsets.data_ptr(),
-            out.data_ptr(), out.stride(0), out.stride(1), 0 if lse is None else lse.data_ptr(), T, slots, Hq, Hk, D, indices.size(1),
-            0 if q.dtype == torch.float16 else 1, D ** -0.5 if softmax_scale is None else float(softmax_scale))
+            q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), ks[0], ks[1], v_cache.data_ptr(), vs[0], vs[1], ka, kss[0], kss[1], va, vss[0],
+            vss[1], indices.data_ptr(), step[0], off, out.data_ptr(), os[0], os[1], lse.data_ptr() if return_lse else 0, T, slots, Hq, Hk, D,
+            picks[1], _TYPES[dtype], D ** -0.5 if softmax_scale is None else softmax_scale)
         _launch(_native.lib().fftopk_sparse_attention, "fftopk_sparse_attention", idx, args)
     return (out, lse) if return_lse else out

@@ -5,10 +5,10 @@
 //
 // attend_narrow_kernel, up to 16 query heads to a key head at a time. A row of k or v is used by those heads alone, so reading
 // the rows bounds it: 16 flop a byte at most in 16 bits, 32 in fp8, where the tensor cores want over 200. The rows lie anywhere,
-// and nothing but their own heads shares them, so they go straight from memory into the registers that mma.sync reads, without
-// shared memory in between: a warp takes blocks of keys, 16 at a time, all their bytes in flight at once.
+// and nothing but their own heads shares them: every warp has a ring of its own in shared memory that cp.async fills, blocks of 16
+// (e4m3: 32) keys ahead of the one it works on, and waits for no other warp.
 //   q.k: the contraction's order is free, so a lane's 16-byte piece of a key row serves as B fragments of consecutive steps
-//        and q is loaded in the same order.
+//        and q is loaded in the same order: no ldmatrix, no padding to its layout.
 //   p.v: the contraction runs over keys, so B fragments pair two rows' elements: a lane loads the same 16-byte piece of the
 //        four rows its fragments hold and interleaves them (byte permutes); which column a fragment's lane stands for is free too.
 // A warp keeps running maxima and sums (one pass); the warps of a CTA are joined in shared memory, the CTAs of a cluster (few
@@ -51,6 +51,23 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+template <int kBytes>
+__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, bool there) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
+  return r;
+}
+__device__ __forceinline__ float2 lds8(uint32_t addr) {
+  float2 r;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(addr) : "memory");
+  return r;
+}
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(kAll, x, 1));
   return fmaxf(x, __shfl_xor_sync(kAll, x, 2));
@@ -60,7 +77,20 @@ __device__ __forceinline__ float quad_sum(float x) {
   return x + __shfl_xor_sync(kAll, x, 2);
 }
 
-// Shared memory of a CTA: the warps' accumulators, maxima, sums; then, joined, the CTA's own.
+// A warp's ring of blocks on their way. Rows are padded so that the lanes that are served together touch all banks: k, where a
+// quad reads 64 neighbouring bytes of each of two rows, by 64 bytes beyond a multiple of 128; v, where eight lanes read two
+// neighbouring pieces of rows 0, 2, 4, 6, by 16.
+template <bool kFp8, int D>
+struct Ring {
+  static constexpr int kKeys = kFp8 ? 32 : 16;  // keys of a block: 8 KB of k and v at D = 128
+  static constexpr int kRowBytes = D * (kFp8 ? 1 : 2);
+  static constexpr int kKPitch = kRowBytes == 64 ? 64 : kRowBytes + 64, kVPitch = kRowBytes + 16;
+  static constexpr int kV = kKeys * kKPitch, kScales = kV + kKeys * kVPitch;
+  static constexpr int kStage = kScales + (kFp8 ? 2 * kKeys * 4 : 0);
+  static constexpr int kStages = D == 64 ? 4 : kFp8 ? 2 : 3;
+  static constexpr int kBytes = kStages * kStage;  // of a warp
+};
+// Shared memory of a CTA: the warps' rings; in their place, in the end, the warps' accumulators, maxima, sums, and joined the CTA's own.
 template <int D>
 struct JoinSmem {
   float o[kWarps][kHeadsM][D];
@@ -68,6 +98,10 @@ struct JoinSmem {
   float joined[kHeadsM][D];
   float2 jml[kHeadsM];  // maximum and sum
 };
+template <bool kFp8, int D>
+constexpr size_t narrow_smem_bytes() {
+  return sizeof(JoinSmem<D>) > (size_t)kWarps * Ring<kFp8, D>::kBytes ? sizeof(JoinSmem<D>) : (size_t)kWarps * Ring<kFp8, D>::kBytes;
+}
 
 // T: type of q and out, and of the cache where kFp8 is false
 template <typename T, bool kFp8, int D>
@@ -76,10 +110,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid
   constexpr int kCE = kFp8 ? 16 : 8;                            // elements of a 16-byte piece
   constexpr int kPieces = D / (4 * kCE);                        // pieces of a key row per lane (a quad reads a row)
   constexpr int kVWords = D * (kFp8 ? 1 : 2) / 32;              // 32-bit words of a value row per lane (8 lanes read a row)
-  constexpr int kKeys = kFp8 ? 32 : 16;                         // keys a warp has in flight
+  using G = Ring<kFp8, D>;
+  constexpr int kKeys = G::kKeys;
+  constexpr int kStages = G::kStages;
   constexpr int kSub = kKeys / 16;
   constexpr int kTiles = D / 8;                                 // columns tiles of the output
-  extern __shared__ unsigned char smem_raw[];
+  extern __shared__ __align__(16) unsigned char smem_raw[];
   JoinSmem<D>& sm = *reinterpret_cast<JoinSmem<D>*>(smem_raw);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -141,9 +177,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid
 
   const int32_t* idx = p.indices + (int64_t)token * p.idx_row;
   const int64_t offset = p.offsets != nullptr ? p.offsets[token] : 0;
-  const char* kbase = static_cast<const char*>(p.k) + (int64_t)kvh * p.k_head * (kFp8 ? 1 : 2) + qd * 16;
-  const char* vbase = static_cast<const char*>(p.v) + (int64_t)kvh * p.v_head * (kFp8 ? 1 : 2) + g * (kVWords >= 4 ? 16 : 8);
+  constexpr int kLanesRow = G::kRowBytes / 16, kRowsOnce = 32 / kLanesRow, kTurns = kKeys / kRowsOnce;
+  const int piece = lane % kLanesRow, sub = lane / kLanesRow;
+  const char* const kbase = static_cast<const char*>(p.k) + (int64_t)kvh * p.k_head * (kFp8 ? 1 : 2) + piece * 16;
+  const char* const vbase = static_cast<const char*>(p.v) + (int64_t)kvh * p.v_head * (kFp8 ? 1 : 2) + piece * 16;
   const int64_t kstep = p.k_slot * (kFp8 ? 1 : 2), vstep = p.v_slot * (kFp8 ? 1 : 2);
+  const uint32_t ring = smem_u32(smem_raw) + (uint32_t)warp * G::kBytes;
   const int blocks = (p.picks + kKeys - 1) / kKeys;
   const int stride = ctas * kWarps;
 
@@ -151,11 +190,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid
     const int j = block * kKeys + (lane & (kKeys - 1));
     return block < blocks && j < p.picks ? idx[j] : -1;
   };
-  int block = rank * kWarps + warp;
-  int32_t next = pick(block);
-  for (; block < blocks; block += stride) {
-    int64_t slot = next;
-    next = pick(block + stride);
+  // asks for a block's rows and scales; which of them are there
+  auto ask = [&](uint32_t stage, int32_t index) {
+    int64_t slot = index;
     bool ok = slot >= 0;
     if (ok) {
       slot += offset;
@@ -165,53 +202,65 @@ __global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid
       }
     }
     const unsigned live = __ballot_sync(kAll, ok) & (kKeys == 16 ? 0xffffu : kAll);
-    if (live == 0u) continue;
-    const int row = ok ? (int)slot : -1;
-    // every byte of the block's rows, asked for before any is used
-    uint4 kw[kSub * 2][kPieces];
-    uint32_t vw[kSub * 4][kVWords];
+    if (live != 0u) {
+      const int row = ok ? (int)slot : -1;
 #pragma unroll
-    for (int n = 0; n < kSub * 2; ++n) {
-      const int r = __shfl_sync(kAll, row, n * 8 + g);
-      const char* at = kbase + (int64_t)r * kstep;
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) kw[n][i] = r >= 0 ? ldg16(at + i * 64) : make_uint4(0u, 0u, 0u, 0u);
-    }
-#pragma unroll
-    for (int n = 0; n < kSub * 4; ++n) {  // keys 16 * (n / 4) + {2 qd, 2 qd + 1, 2 qd + 8, 2 qd + 9}
-      const int r = __shfl_sync(kAll, row, (n >> 2) * 16 + 2 * qd + (n & 1) + ((n & 2) << 2));
-      const char* at = vbase + (int64_t)r * vstep;
-      if constexpr (kVWords >= 4) {
-#pragma unroll
-        for (int i = 0; i < kVWords / 4; ++i) {
-          const uint4 x = r >= 0 ? ldg16(at + i * 128) : make_uint4(0u, 0u, 0u, 0u);
-          vw[n][4 * i] = x.x, vw[n][4 * i + 1] = x.y, vw[n][4 * i + 2] = x.z, vw[n][4 * i + 3] = x.w;
-        }
-      } else {
-        const uint2 x = r >= 0 ? ldg8(at) : make_uint2(0u, 0u);
-        vw[n][0] = x.x, vw[n][1] = x.y;
+      for (int i = 0; i < kTurns; ++i) {
+        const int at = i * kRowsOnce + sub;
+        const int r = __shfl_sync(kAll, row, at);
+        copy_or_zero<16>(stage + (uint32_t)(at * G::kKPitch + piece * 16), r >= 0 ? kbase + (int64_t)r * kstep : kbase, r >= 0);
+        copy_or_zero<16>(stage + (uint32_t)(G::kV + at * G::kVPitch + piece * 16), r >= 0 ? vbase + (int64_t)r * vstep : vbase, r >= 0);
+      }
+      if constexpr (kFp8) {
+        const uint32_t at = stage + (uint32_t)(G::kScales + lane * 8);
+        copy_or_zero<4>(at, p.k_scale + (ok ? slot * p.ks_slot + (int64_t)kvh * p.ks_head : 0), ok);
+        copy_or_zero<4>(at + 4u, p.v_scale + (ok ? slot * p.vs_slot + (int64_t)kvh * p.vs_head : 0), ok);
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    return live;
+  };
+  int block = rank * kWarps + warp;
+  unsigned live_of[kStages];
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) live_of[s] = ask(ring + s * G::kStage, pick(block + s * stride));
+  int32_t next = pick(block + (kStages - 1) * stride);
+  uint32_t here = ring, there = ring + (kStages - 1) * G::kStage;  // stages: of this block, of the one that is asked for
+  for (; block < blocks; block += stride) {
+    live_of[kStages - 1] = ask(there, next);
+    next = pick(block + kStages * stride);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    __syncwarp();
+    const unsigned live = live_of[0];
+    const uint32_t stage = here;
+    here = here + G::kStage == ring + G::kBytes ? ring : here + G::kStage;
+    there = there + G::kStage == ring + G::kBytes ? ring : there + G::kStage;
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) live_of[s] = live_of[s + 1];
+    if (live == 0u) continue;
     float ks = 0.f, vs = 0.f;  // the scales of the lane's key
     if constexpr (kFp8) {
-      if (ok) {
-        ks = __ldg(p.k_scale + (int64_t)row * p.ks_slot + (int64_t)kvh * p.ks_head);
-        vs = __ldg(p.v_scale + (int64_t)row * p.vs_slot + (int64_t)kvh * p.vs_head);
-      }
+      const float2 both = lds8(stage + (uint32_t)(G::kScales + lane * 8));
+      ks = both.x, vs = both.y;
     }
     // scores, in units of log2
     float sc[kSub * 2][4];
 #pragma unroll
     for (int n = 0; n < kSub * 2; ++n) {
       sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+      const uint32_t at = stage + (uint32_t)((n * 8 + g) * G::kKPitch + qd * 16);
 #pragma unroll
-      for (int m = 0; m < D / 16; ++m) {
-        const int i = m / (kCE / 4), u = m % (kCE / 4);
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(&kw[n][i]);
-        if constexpr (kFp8) {
-          mma16816(sc[n], qa[m], e4m3x2_to_half2((uint16_t)w[u]), e4m3x2_to_half2((uint16_t)(w[u] >> 16)), M());
-        } else {
-          mma16816(sc[n], qa[m], w[2 * u], w[2 * u + 1], M());
+      for (int i = 0; i < kPieces; ++i) {
+        const uint4 x = lds16(at + 64u * i);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int u = 0; u < kCE / 4; ++u) {
+          const int m = i * (kCE / 4) + u;
+          if constexpr (kFp8) {
+            mma16816(sc[n], qa[m], e4m3x2_to_half2((uint16_t)w[u]), e4m3x2_to_half2((uint16_t)(w[u] >> 16)), M());
+          } else {
+            mma16816(sc[n], qa[m], w[2 * u], w[2 * u + 1], M());
+          }
         }
       }
     }
@@ -231,10 +280,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid
         bmax[r] = fmaxf(bmax[r], fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
       }
     }
+    // (a reference is let stand until a score exceeds it by 2^8: fp16 weights and 32-bit sums have the room)
     float grow[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float m = fmaxf(mx[r], quad_max(bmax[r]));
+      const float top = quad_max(bmax[r]);
+      const float m = top > mx[r] + 8.f ? top : mx[r];
       grow[r] = mx[r] == m ? 1.f : ex2(mx[r] - m);  // (-inf both: nothing seen yet)
       mx[r] = m;
     }
@@ -242,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid
       float top = vs;
 #pragma unroll
       for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, i));
-      const float ref = fmaxf(vref, top);
+      const float ref = top > 64.f * vref ? top : vref;  // (let stand likewise, up to 2^6: weights stay below 2^14)
       const float f = ref > vref ? vref / ref : 1.f;
       vref = ref;
       vs = ref > 0.f ? vs / ref : 0.f;
@@ -282,28 +333,45 @@ __global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid
     }
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
-      if constexpr (kFp8) {
-        // columns 4 w .. 4 w + 3 of the lane's piece: bytes of rows 2 qd and 2 qd + 1 side by side
+      // the lane's pieces of rows 16 s + {2 qd, 2 qd + 1, 2 qd + 8, 2 qd + 9}
+      const uint32_t at = stage + (uint32_t)(G::kV + (16 * s + 2 * qd) * G::kVPitch + g * (kVWords >= 4 ? 16 : 8));
 #pragma unroll
-        for (int w = 0; w < kVWords; ++w) {
-          const uint32_t a = vw[4 * s][w], b = vw[4 * s + 1][w], c = vw[4 * s + 2][w], d = vw[4 * s + 3][w];
-          const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
-          const uint32_t cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
-          mma16816(o[4 * w], pa[s], e4m3x2_to_half2((uint16_t)ab0), e4m3x2_to_half2((uint16_t)cd0), M());
-          mma16816(o[4 * w + 1], pa[s], e4m3x2_to_half2((uint16_t)(ab0 >> 16)), e4m3x2_to_half2((uint16_t)(cd0 >> 16)), M());
-          mma16816(o[4 * w + 2], pa[s], e4m3x2_to_half2((uint16_t)ab1), e4m3x2_to_half2((uint16_t)cd1), M());
-          mma16816(o[4 * w + 3], pa[s], e4m3x2_to_half2((uint16_t)(ab1 >> 16)), e4m3x2_to_half2((uint16_t)(cd1 >> 16)), M());
+      for (int h = 0; h < (kVWords >= 4 ? kVWords / 4 : 1); ++h) {
+        uint32_t vw[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t from = at + (uint32_t)(((n & 1) + (n >> 1) * 8) * G::kVPitch) + 128u * h;
+          if constexpr (kVWords >= 4) {
+            const uint4 x = lds16(from);
+            vw[n][0] = x.x, vw[n][1] = x.y, vw[n][2] = x.z, vw[n][3] = x.w;
+          } else {
+            const float2 x = lds8(from);
+            vw[n][0] = __float_as_uint(x.x), vw[n][1] = __float_as_uint(x.y);
+          }
         }
-      } else {
 #pragma unroll
-        for (int w = 0; w < kVWords; ++w) {
-          const uint32_t a = vw[4 * s][w], b = vw[4 * s + 1][w], c = vw[4 * s + 2][w], d = vw[4 * s + 3][w];
-          mma16816(o[2 * w], pa[s], __byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), M());
-          mma16816(o[2 * w + 1], pa[s], __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632), M());
+        for (int e = 0; e < (kVWords >= 4 ? 4 : kVWords); ++e) {
+          const int w = 4 * h + e;
+          const uint32_t a = vw[0][e], b = vw[1][e], c = vw[2][e], d = vw[3][e];
+          if constexpr (kFp8) {
+            // columns 4 w .. 4 w + 3 of the lane's piece: bytes of rows 2 qd and 2 qd + 1 side by side
+            const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
+            const uint32_t cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
+            mma16816(o[4 * w], pa[s], e4m3x2_to_half2((uint16_t)ab0), e4m3x2_to_half2((uint16_t)cd0), M());
+            mma16816(o[4 * w + 1], pa[s], e4m3x2_to_half2((uint16_t)(ab0 >> 16)), e4m3x2_to_half2((uint16_t)(cd0 >> 16)), M());
+            mma16816(o[4 * w + 2], pa[s], e4m3x2_to_half2((uint16_t)ab1), e4m3x2_to_half2((uint16_t)cd1), M());
+            mma16816(o[4 * w + 3], pa[s], e4m3x2_to_half2((uint16_t)(ab1 >> 16)), e4m3x2_to_half2((uint16_t)(cd1 >> 16)), M());
+          } else {
+            mma16816(o[2 * w], pa[s], __byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), M());
+            mma16816(o[2 * w + 1], pa[s], __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632), M());
+          }
         }
       }
     }
+    __syncwarp();  // (the next block but kStages - 2 goes where this one was)
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();  // the rings make room for the join
 
   // ---- join: warps, then CTAs ----
   sum[0] = quad_sum(sum[0]);
@@ -394,7 +462,7 @@ int g_attend_sms[kMaxDevices];
 template <typename T, bool kFp8, int D>
 int setup_one() {
   const cudaError_t e =
-      cudaFuncSetAttribute(attend_narrow_kernel<T, kFp8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(JoinSmem<D>));
+      cudaFuncSetAttribute(attend_narrow_kernel<T, kFp8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)narrow_smem_bytes<kFp8, D>());
   return e == cudaSuccess ? 0 : cuda_fail(e);
 }
 
@@ -426,7 +494,7 @@ cudaError_t launch_narrow(const AttendParams& p, int ctas, int64_t units, cudaSt
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * ctas), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = sizeof(JoinSmem<D>);
+  cfg.dynamicSmemBytes = narrow_smem_bytes<kFp8, D>();
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

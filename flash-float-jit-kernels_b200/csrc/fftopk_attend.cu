@@ -37,7 +37,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 8;
+// Four warps, two CTAs per SM: while one CTA starts or joins, the other one streams (64 tokens, 8 key heads, bf16: 98 us; eight warps
+// and one CTA per SM: 108)
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kHeadsM = 16;  // query heads a CTA works on: rows of the MMA
 
@@ -105,7 +107,7 @@ constexpr size_t narrow_smem_bytes() {
 
 // T: type of q and out, and of the cache where kFp8 is false
 template <typename T, bool kFp8, int D>
-__global__ void __launch_bounds__(kThreads, 1) attend_narrow_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(kThreads, 2) attend_narrow_kernel(const __grid_constant__ AttendParams p) {
   using M = typename std::conditional<kFp8, __half, T>::type;  // the MMAs' type
   constexpr int kCE = kFp8 ? 16 : 8;                            // elements of a 16-byte piece
   constexpr int kPieces = D / (4 * kCE);                        // pieces of a key row per lane (a quad reads a row)
@@ -569,7 +571,8 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   const int64_t units = a->tokens * p.kv_heads * p.head_blocks;
   const int keys = wide ? 128 : kWarps * (fp8 ? 32 : 16);
   int ctas = 1;
-  while (ctas < kAttendMaxCluster && units * ctas * 2 <= sms && (int64_t)ctas * keys < p.picks) ctas *= 2;
+  const int64_t room = wide ? sms : 2 * (int64_t)sms;
+  while (ctas < kAttendMaxCluster && units * ctas * 2 <= room && (int64_t)ctas * keys < p.picks) ctas *= 2;
   if (units * ctas > 0x7fffffff) return FFTOPK_ERANGE;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   if (wide) {

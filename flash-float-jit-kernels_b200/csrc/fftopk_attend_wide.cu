@@ -294,6 +294,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     };
     if constexpr (kFp8) {
       uint4 held[kTurns];  // the lane's pieces of the rows on their way
+      uint32_t to[2][2];   // where its two chunks go in a tile, turn 0 and turn 1 (without the turn's rows)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) to[i][e] = chunk_at(0u, sub + i * kRowsOnce, 2 * piece + e) - (uint32_t)(i * kRowsOnce * 128);
+      }
       auto fetch = [&](int i, const TileMeta& m, const char* src) {
         const int row = m.row[sub + i * kRowsOnce];
         held[i] = row >= 0 ? ldg16(src + (int64_t)row * row_bytes) : make_uint4(0u, 0u, 0u, 0u);
@@ -322,9 +328,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             h[2 * e] = e4m3x2_to_half2((uint16_t)x[e]);
             h[2 * e + 1] = e4m3x2_to_half2((uint16_t)(x[e] >> 16));
           }
-          const int r = sub + i * kRowsOnce;
-          put16(chunk_at(tile, r, 2 * piece), h[0], h[1], h[2], h[3]);
-          put16(chunk_at(tile, r, 2 * piece + 1), h[4], h[5], h[6], h[7]);
+          // (rows of every second turn have their chunks in the same order)
+          const uint32_t by = tile + (uint32_t)(i * kRowsOnce * 128);
+          put16(by + to[i & 1][0], h[0], h[1], h[2], h[3]);
+          put16(by + to[i & 1][1], h[4], h[5], h[6], h[7]);
           if (have) fetch(i, next, src);  // the next tile's piece takes its place
         }
         hand_over(n);
@@ -656,7 +663,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
               refer(ref, ve, 0);
           }
           const bool whole = (m.flags & kWhole) != 0;
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
+          Pair part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+          auto parts = [&] {
+            const float2 x = apart(add2(part[0], part[1]));
+            part[0] = part[1] = pair(0.f, 0.f);
+            return x.x + x.y;
+          };
 #pragma unroll 1
           for (int c = 0; c < kTileKeys / kChunk; ++c) {
             float s[kChunk];
@@ -666,7 +678,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
 #pragma unroll
               for (int i = 0; i < kChunk; i += 4) {
                 const float4 x = *reinterpret_cast<const float4*>(m.ks + kChunk * c + i);
-                s[i] *= x.x, s[i + 1] *= x.y, s[i + 2] *= x.z, s[i + 3] *= x.w;
+                const float2 a = apart(mul2(pair(s[i], s[i + 1]), pair(x.x, x.y))), b = apart(mul2(pair(s[i + 2], s[i + 3]), pair(x.z, x.w)));
+                s[i] = a.x, s[i + 1] = a.y, s[i + 2] = b.x, s[i + 3] = b.y;
               }
             }
             if (!whole) {
@@ -681,30 +694,32 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             const float top = top_of(s) * qmul;
             if (__any_sync(kAll, top > ref + kLetStand)) {
               tmem_wait_st();
-              sum += (part[0] + part[1]) + (part[2] + part[3]);
-              part[0] = part[1] = part[2] = part[3] = 0.f;
+              sum += parts();
               refer(top > ref + kLetStand ? top : ref, vlog, kChunk / 32 * c);
             }
             const float sub = (ref == -INFINITY ? 0.f : ref) + vlog;
+            const Pair mul = pair(qmul, qmul), less = pair(-sub, -sub);
             uint32_t pk[kChunk / 2];
 #pragma unroll
             for (int i = 0; i < kChunk; i += 4) {
-              float w[4];
+              Pair w[2];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                w[e] = ex2(fmaf(s[i + e], qmul, -sub));
-                part[e] += w[e];
+              for (int e = 0; e < 2; ++e) {
+                const float2 x = apart(fma2(pair(s[i + 2 * e], s[i + 2 * e + 1]), mul, less));
+                w[e] = pair(ex2(x.x), ex2(x.y));
+                part[e] = add2(part[e], w[e]);
               }
               if constexpr (kFp8) {
                 const float4 x = *reinterpret_cast<const float4*>(m.vs + kChunk * c + i);
-                w[0] *= x.x, w[1] *= x.y, w[2] *= x.z, w[3] *= x.w;
+                w[0] = mul2(w[0], pair(x.x, x.y)), w[1] = mul2(w[1], pair(x.z, x.w));
               }
-              pk[i / 2] = narrow2(w[0], w[1], M());
-              pk[i / 2 + 1] = narrow2(w[2], w[3], M());
+              const float2 a = apart(w[0]), b = apart(w[1]);
+              pk[i / 2] = narrow2(a.x, a.y, M());
+              pk[i / 2 + 1] = narrow2(b.x, b.y, M());
             }
             store_chunk(s_cols + (uint32_t)(kChunk / 2 * c), pk);  // (over scores that have been read)
           }
-          sum += (part[0] + part[1]) + (part[2] + part[3]);
+          sum += parts();
           tmem_wait_st();
         }
         tmem_fence_before();

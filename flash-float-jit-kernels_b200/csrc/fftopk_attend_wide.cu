@@ -65,6 +65,7 @@ struct WideCfg {
   static constexpr uint32_t kTileBytes = kTileKeys * D * 2;  // of Q too
   static constexpr int kKStages = D == 128 ? 2 : 4, kVStages = D == 128 ? 2 : 4;
 };
+static_assert(kTileKeys == 128);
 constexpr int kChunk = 64;    // scores of a row that a softmax thread works on at once
 constexpr int kMeta = 4;      // tiles the scout is ahead at most; a place is free again when its tile's PV is done
 constexpr int kInfo = 4;      // pieces of work it is ahead
@@ -85,11 +86,13 @@ struct WideSmem {  // behind the operand tiles
   float qmul[4][kHeadsW];    // by piece of work: softmax may be two behind the queries
   float2 ml[2][2][kHeadsW];  // by parity of the piece of work, and group: maximum and sum
   int32_t tiles[kInfo];      // tiles of a piece of work
-  uint64_t kfull[WideCfg<D>::kKStages], kempty[WideCfg<D>::kKStages];
-  uint64_t vfull[WideCfg<D>::kVStages], vempty[WideCfg<D>::kVStages];
-  uint64_t mfull[kMeta], mempty[kMeta], ifull[kInfo], iempty[kInfo];
+  // A place of a ring is free again when the MMAs that read it are done, which one commit tells all who wait for them.
+  uint64_t kfull[WideCfg<D>::kKStages], sdone[WideCfg<D>::kKStages];  // k has landed; QK is done: S is there, k may be replaced
+  uint64_t vfull[WideCfg<D>::kVStages];
+  uint64_t mfull[kMeta], pvdone[kMeta];  // TileMeta is there; PV is done: v and TileMeta may be replaced, O is up to this tile
+  uint64_t ifull[kInfo], iempty[kInfo];
   uint64_t qfull[kQTiles], qempty[kQTiles], oempty, mlbar;
-  uint64_t sfull[2], pfull[2], pvdone[2];
+  uint64_t pfull[2][2], halfdone[2];     // by group: a half of P is there; PV of the first half is done
   uint32_t tmem, abort_flag;
 };
 template <int D>
@@ -244,14 +247,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
   const uint32_t first = blockIdx.x / (uint32_t)ctas, step = gridDim.x / (uint32_t)ctas;
 
   if (tid == 0) {
-    for (int i = 0; i < kKS; ++i) mbar_init(&sm.kfull[i], 4), mbar_init(&sm.kempty[i], 1);
-    for (int i = 0; i < kVS; ++i) mbar_init(&sm.vfull[i], 4), mbar_init(&sm.vempty[i], 1);
-    for (int i = 0; i < kMeta; ++i) mbar_init(&sm.mfull[i], 1), mbar_init(&sm.mempty[i], 1);
+    for (int i = 0; i < kKS; ++i) mbar_init(&sm.kfull[i], 4), mbar_init(&sm.sdone[i], 1);
+    for (int i = 0; i < kVS; ++i) mbar_init(&sm.vfull[i], 4);
+    for (int i = 0; i < kMeta; ++i) mbar_init(&sm.mfull[i], 1), mbar_init(&sm.pvdone[i], 1);
     for (int i = 0; i < kInfo; ++i) mbar_init(&sm.ifull[i], 1), mbar_init(&sm.iempty[i], kSoftmaxWarps + kQueryWarps);
     for (int i = 0; i < kQTiles; ++i) mbar_init(&sm.qfull[i], kQueryWarps), mbar_init(&sm.qempty[i], 1);
     mbar_init(&sm.oempty, kSoftmaxWarps);
     mbar_init(&sm.mlbar, kSoftmaxWarps);
-    for (int i = 0; i < 2; ++i) mbar_init(&sm.sfull[i], 1), mbar_init(&sm.pfull[i], 4), mbar_init(&sm.pvdone[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&sm.pfull[i][0], 4), mbar_init(&sm.pfull[i][1], 4), mbar_init(&sm.halfdone[i], 1);
     sm.abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -272,7 +275,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     const bool is_k = warp < kSoftmaxWarps + 4;
     const int gw = (warp - kSoftmaxWarps) & 3;
     uint64_t* const full = is_k ? sm.kfull : sm.vfull;
-    uint64_t* const empty = is_k ? sm.kempty : sm.vempty;
+    uint64_t* const empty = is_k ? sm.sdone : sm.pvdone;  // of the tile `stages` before
+    const uint32_t ring = is_k ? kKS : kMeta;
     const uint32_t stages = is_k ? kKS : kVS;
     const uint32_t tiles = is_k ? k_tiles : v_tiles;
     constexpr int kLanesRow = D * (kFp8 ? 1 : 2) / 16;  // lanes that read a row
@@ -286,7 +290,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     const char* const src0 = static_cast<const char*>(is_k ? p.k : p.v) + piece * 16;
     auto posted = [&](uint32_t n) { return __all_sync(kAll, mbar_test(&sm.mfull[n % kMeta], (n / kMeta) & 1u)); };
     auto wait_posted = [&](uint32_t n) { return __all_sync(kAll, mbar_wait(&sm.mfull[n % kMeta], (n / kMeta) & 1u, abort_flag)); };
-    auto wait_empty = [&](uint32_t n) { return __all_sync(kAll, mbar_wait(&empty[n % stages], ((n / stages) & 1u) ^ 1u, abort_flag)); };
+    auto wait_empty = [&](uint32_t n) {
+      const uint32_t of = n - stages;
+      return n < stages || __all_sync(kAll, mbar_wait(&empty[of % ring], (of / ring) & 1u, abort_flag));
+    };
+    auto is_empty = [&](uint32_t n) {
+      const uint32_t of = n - stages;
+      return n < stages || __all_sync(kAll, mbar_test(&empty[of % ring], (of / ring) & 1u));
+    };
     auto hand_over = [&](uint32_t n) {
       fence_async_shared();
       __syncwarp();
@@ -340,7 +351,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       bool pending = false;  // tile n - 1 is on its way and not handed over
       for (uint32_t n = 0;; ++n) {
         // a tile that has landed is not kept waiting for the next one's turn
-        if (pending && !(posted(n) && __all_sync(kAll, mbar_test(&empty[n % stages], ((n / stages) & 1u) ^ 1u)))) {
+        if (pending && !(posted(n) && is_empty(n))) {
           asm volatile("cp.async.wait_group 0;" ::: "memory");
           hand_over(n - 1);
           pending = false;
@@ -424,7 +435,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           for (int i = 0; i < 4; ++i) now[i] = later[i];
           pick(later, j + 2);
           rows_of(next_row, next_ks, next_vs, now);
-          if (!(ok = __all_sync(kAll, mbar_wait(&sm.mempty[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)))) break;
+          if (!(ok = __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)))) break;
           TileMeta& m = sm.meta[n % kMeta];
           float top = 0.f;
           unsigned whole = kAll;
@@ -456,7 +467,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           for (int i = 0; i < 4; ++i) row[i] = next_row[i], ks[i] = next_ks[i], vs[i] = next_vs[i];
         }
       }
-      if (ok && __all_sync(kAll, mbar_wait(&sm.mempty[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)) && lane == 0) {
+      if (ok && __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)) && lane == 0) {
         sm.meta[n % kMeta].flags = kEnd;
         mbar_arrive(&sm.mfull[n % kMeta]);
       }
@@ -521,12 +532,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         uint32_t qn = 0, pn = 0;      // tiles whose QK, whose PV has been issued
         uint32_t qwn = 0, pwn = 0;    // pieces of work they are of
         int qj = 0, pj = 0;           // and tiles of those
+        uint32_t flags = 0u, pflags = 0u;  // of tile qn, once it is ready; of the tiles between QK and PV, a byte each
         bool ended = false;           // the stream, at qn tiles
         bool ok = true;
         auto ready = [&](bool wait) {  // tile qn's k and q; sets `ended` where there is no such tile
           uint64_t* const meta = &sm.mfull[qn % kMeta];
           if (!(wait ? mbar_wait(meta, (qn / kMeta) & 1u, abort_flag) : mbar_test(meta, (qn / kMeta) & 1u))) return false;
-          if (sm.meta[qn % kMeta].flags & kEnd) {
+          flags = (uint32_t)sm.meta[qn % kMeta].flags;
+          if (flags & kEnd) {
             ended = true;
             return false;
           }
@@ -546,10 +559,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             const uint32_t at = ((uint32_t)(k >> 2) * (kTileKeys * 128u) + (uint32_t)(k & 3) * 32u) >> 4;
             mma_ss(d, q + at, kt + at, instr_desc<M, kTileKeys, false>(), k != 0);
           }
-          umma_commit(&sm.sfull[qn & 1u]);
-          umma_commit(&sm.kempty[stage]);
-          const bool last = (sm.meta[qn % kMeta].flags & kLast) != 0;
+          umma_commit(&sm.sdone[stage]);
+          const bool last = (flags & kLast) != 0;
           if (last) umma_commit(&sm.qempty[qt]);
+          pflags |= flags << (8u * (qn & 1u));
           ++qn;
           qj = last ? 0 : qj + 1;
           qwn += last ? 1u : 0u;
@@ -561,20 +574,26 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             continue;
           }
           if (qn == pn) break;  // the end - or a wait that ran out
-          const bool more = !ended && qn - pn == 2u && ready(false);
-          // PV of tile pn
+          // PV of tile pn, half of its keys at a time: the first half's products run beside the second half's exponentials
           const uint32_t g = pn & 1u, stage = pn % kVS, vt = desc_mn(v_tiles + stage * kTileBytes), s_at = tmem + g * 128u;
+          const uint32_t phase = (pn >> 1) & 1u, more_of_o = pj > 1 ? 1u : 0u;
+          const bool last = (pflags >> (8u * g) & kLast) != 0u;
           if (pj == 0 && !(ok = mbar_wait(&sm.oempty, (pwn & 1u) ^ 1u, abort_flag))) break;  // (O may still be on its way out)
-          const bool last = (sm.meta[pn % kMeta].flags & kLast) != 0;
           if (!(ok = mbar_wait(&sm.vfull[stage], (pn / kVS) & 1u, abort_flag))) break;
-          if (!(ok = mbar_wait(&sm.pfull[g], (pn >> 1) & 1u, abort_flag))) break;
+          if (!(ok = mbar_wait(&sm.pfull[g][0], phase, abort_flag))) break;
           tmem_fence_after();
 #pragma unroll
-          for (int k = 0; k < kTileKeys / 16; ++k)
-            mma_ts(s_at + 256u, s_at + (uint32_t)k * 8u, vt + (uint32_t)k * (2048u >> 4), instr_desc<M, D, true>(), k != 0 || pj > 1);
-          umma_commit(&sm.pvdone[g]);
-          umma_commit(&sm.vempty[stage]);
-          umma_commit(&sm.mempty[pn % kMeta]);
+          for (int k = 0; k < kTileKeys / 32; ++k)
+            mma_ts(s_at + 256u, s_at + (uint32_t)k * 8u, vt + (uint32_t)k * (2048u >> 4), instr_desc<M, D, true>(), k != 0 ? 1u : more_of_o);
+          umma_commit(&sm.halfdone[g]);
+          const bool more = !ended && qn - pn == 2u && ready(false);
+          if (!(ok = mbar_wait(&sm.pfull[g][1], phase, abort_flag))) break;
+          tmem_fence_after();
+#pragma unroll
+          for (int k = kTileKeys / 32; k < kTileKeys / 16; ++k)
+            mma_ts(s_at + 256u, s_at + (uint32_t)k * 8u, vt + (uint32_t)k * (2048u >> 4), instr_desc<M, D, true>(), 1u);
+          umma_commit(&sm.pvdone[pn % kMeta]);
+          pflags &= 0xff00u >> (8u * g);
           ++pn;
           pj = last ? 0 : pj + 1;
           pwn += last ? 1u : 0u;
@@ -589,7 +608,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     const int g = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_cols = lanes + (uint32_t)g * 128u, o_cols = lanes + 256u + (uint32_t)g * 128u;
-    uint32_t turns[2] = {0u, 0u};  // tiles of each group in the pieces of work before
     uint32_t it = 0, un = 0, wn = 0;
     bool ok = true;
     constexpr int kHalf = D / 2;  // columns of O a thread writes
@@ -611,25 +629,32 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         continue;
       }
       float ref = -INFINITY, vlog = 0.f, sum = 0.f;
-      const uint32_t turn0 = turns[g];
       for (int j = g ^ (int)(it & 1u); j < nt; j += 2) {
-        const uint32_t n = it + (uint32_t)j, turn = turn0 + (uint32_t)(j >> 1);
+        const uint32_t n = it + (uint32_t)j;
         const int place = (int)(n % kMeta);
-        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag) && mbar_wait(&sm.sfull[g], turn & 1u, abort_flag);
+        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag) && mbar_wait(&sm.sdone[n % kKS], (n / kKS) & 1u, abort_flag);
         if (!(ok = __all_sync(kAll, ok))) break;
         tmem_fence_after();
+        auto hand_over = [&](int half) {
+          tmem_wait_st();
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.pfull[g][half]);
+        };
         if (busy) {
           const TileMeta& m = sm.meta[place];
           const float qmul = sm.qmul[wn & 3u][r];
-          // A new reference: what was weighed with the old one - O, the sum, this tile's weights so far (`done` chunks) - is brought to it.
-          auto refer = [&](float next, float vnext, int done) {
+          // A new reference: what was weighed with the old one - O up to the tile before, or with the first half of this one's keys
+          // where that has been handed over, and the sum - is brought to it.
+          auto refer = [&](float next, float vnext, bool half) {
             const bool changed = next != ref || vnext != vlog;
             const float f = !changed ? 1.f : ref == -INFINITY ? (next == -INFINITY ? 1.f : 0.f) : ex2((ref + vlog) - (next + vnext));
             ref = next;
             vlog = vnext;
             sum *= f;
-            if (j > 1) {
-              if (!__all_sync(kAll, mbar_wait(&sm.pvdone[g], (turn - 1u) & 1u, abort_flag))) return;  // (the waits to come fail too)
+            if (half || j > 1) {
+              uint64_t* const bar = half ? &sm.halfdone[g] : &sm.pvdone[(n - 2u) % kMeta];
+              if (!__all_sync(kAll, mbar_wait(bar, half ? (n >> 1) & 1u : ((n - 2u) / kMeta) & 1u, abort_flag))) return;  // (the waits to come fail too)
               tmem_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
@@ -641,18 +666,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
                 tmem_st16(o_cols + 16u * c, v);
               }
             }
-#pragma unroll 1
-            for (int c = 0; c < done; ++c) {
-              uint32_t v[16];
-              tmem_ld16(s_cols + 16u * c, v);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 x = widen2(v[i], M());
-                v[i] = narrow2(x.x * f, x.y * f, M());
-              }
-              tmem_st16(s_cols + 16u * c, v);
-            }
           };
           if constexpr (kFp8) {  // the exponent of the largest v scale
             const int e = (int)(__float_as_uint(m.vtop) >> 23) - 127;
@@ -660,7 +673,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             if (j < 2)
               vlog = ve;
             else if (ve > vlog + 6.f)
-              refer(ref, ve, 0);
+              refer(ref, ve, false);
           }
           const bool whole = (m.flags & kWhole) != 0;
           Pair part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
@@ -693,9 +706,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             }
             const float top = top_of(s) * qmul;
             if (__any_sync(kAll, top > ref + kLetStand)) {
-              tmem_wait_st();
               sum += parts();
-              refer(top > ref + kLetStand ? top : ref, vlog, kChunk / 32 * c);
+              refer(top > ref + kLetStand ? top : ref, vlog, c > 0);
             }
             const float sub = (ref == -INFINITY ? 0.f : ref) + vlog;
             const Pair mul = pair(qmul, qmul), less = pair(-sub, -sub);
@@ -718,13 +730,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
               pk[i / 2 + 1] = narrow2(b.x, b.y, M());
             }
             store_chunk(s_cols + (uint32_t)(kChunk / 2 * c), pk);  // (over scores that have been read)
+            hand_over(c);
           }
           sum += parts();
-          tmem_wait_st();
+        } else {
+          hand_over(0);
+          hand_over(1);
         }
-        tmem_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.pfull[g]);
       }
       if (!ok) break;
       // ---- this piece's end: both groups' products, maxima and sums ----
@@ -735,8 +747,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.mlbar);
         ok = mbar_wait(&sm.mlbar, wn & 1u, abort_flag);
-        if (nga > 0) ok = ok && mbar_wait(&sm.pvdone[0], (turns[0] + (uint32_t)nga - 1u) & 1u, abort_flag);
-        if (ngb > 0) ok = ok && mbar_wait(&sm.pvdone[1], (turns[1] + (uint32_t)ngb - 1u) & 1u, abort_flag);
+        const uint32_t end = it + (uint32_t)nt - 1u;  // the last tile; the one before it is the other group's last
+        ok = ok && mbar_wait(&sm.pvdone[end % kMeta], (end / kMeta) & 1u, abort_flag);
+        if (nt > 1) ok = ok && mbar_wait(&sm.pvdone[(end - 1u) % kMeta], ((end - 1u) / kMeta) & 1u, abort_flag);
         if (!(ok = __all_sync(kAll, ok))) break;
         tmem_fence_after();
         a = sm.ml[wn & 1u][0][r], b = sm.ml[wn & 1u][1][r];
@@ -781,7 +794,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         else if (mine && lse != nullptr)
           *lse = l == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(l);
       }
-      turns[0] += (uint32_t)nga, turns[1] += (uint32_t)ngb;
       it += (uint32_t)nt;
       wn += nt > 0 ? 1u : 0u;
     }

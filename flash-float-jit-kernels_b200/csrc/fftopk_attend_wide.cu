@@ -60,44 +60,51 @@ __device__ __forceinline__ void fewer_registers() {
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLetStand = 8.f;  // log2 by which a score may exceed the reference
 
-template <int D>
+// What lies in shared memory beside the query tile: k and v tiles as the MMAs read them; and, e4m3, every gathering warp's share of
+// the codes of tiles on their way.
+template <bool kFp8, int D>
 struct WideCfg {
   static constexpr uint32_t kTileBytes = kTileKeys * D * 2;  // of Q too
-  static constexpr int kKStages = D == 128 ? 2 : 4, kVStages = D == 128 ? 2 : 4;
+  // (1,024 tokens of 128 heads on one e4m3 key head: two k and v tiles and room for the codes of one 344 us; one k and one v tile,
+  // codes of two and a query tile ahead 362)
+  static constexpr int kQTiles = D == 128 && kFp8 ? 1 : 2, kKStages = 2, kVStages = 2;
+  static constexpr int kSDone = kKStages < 2 ? 2 : kKStages;  // barriers in turn: softmax may be a tile behind QK
+  static constexpr int kRaw = kFp8 ? (D == 64 ? 4 : 1) : 0;
+  static constexpr uint32_t kRawBytes = 32 * D;              // of a warp and tile
+  static constexpr size_t kTiles = (size_t)kTileBytes * (kQTiles + kKStages + kVStages), kOperands = kTiles + (size_t)kRaw * kGatherWarps * kRawBytes;
 };
 static_assert(kTileKeys == 128);
 constexpr int kChunk = 64;    // scores of a row that a softmax thread works on at once
 constexpr int kMeta = 4;      // tiles the scout is ahead at most; a place is free again when its tile's PV is done
+constexpr int kPauseNs = 64;  // of the thread that issues the MMAs, between two looks at what it waits for
 constexpr int kInfo = 4;      // pieces of work it is ahead
-constexpr int kQTiles = 2;    // query tiles
-constexpr int kFirst = 1, kLast = 2, kEnd = 4, kWhole = 8;
+constexpr int kLast = 1, kEnd = 2, kWhole = 4, kSeen = 8;
 struct TileMeta {             // a tile of 128 keys
-  int32_t row[kTileKeys];     // cache rows; -1: none
+  int64_t k_at[kTileKeys], v_at[kTileKeys];  // byte offsets of the rows in the caches; negative: none
   float ks[kTileKeys], vs[kTileKeys];
   uint32_t live[4];
   float vtop;                 // largest v scale
-  int32_t flags;              // first, last tile of its piece of work; end of the stream (no tile); all rows are there
-  int32_t j;                  // tile of its piece of work
+  int32_t flags;              // last tile of its piece of work; end of the stream (no tile); all rows are there
   int32_t kvh;
 };
-template <int D>
+template <bool kFp8, int D>
 struct WideSmem {  // behind the operand tiles
   TileMeta meta[kMeta];
   float qmul[4][kHeadsW];    // by piece of work: softmax may be two behind the queries
   float2 ml[2][2][kHeadsW];  // by parity of the piece of work, and group: maximum and sum
   int32_t tiles[kInfo];      // tiles of a piece of work
   // A place of a ring is free again when the MMAs that read it are done, which one commit tells all who wait for them.
-  uint64_t kfull[WideCfg<D>::kKStages], sdone[WideCfg<D>::kKStages];  // k has landed; QK is done: S is there, k may be replaced
-  uint64_t vfull[WideCfg<D>::kVStages];
+  uint64_t kfull[WideCfg<kFp8, D>::kKStages], sdone[WideCfg<kFp8, D>::kSDone];  // k has landed; QK is done: S is there, k may be replaced
+  uint64_t vfull[WideCfg<kFp8, D>::kVStages];
   uint64_t mfull[kMeta], pvdone[kMeta];  // TileMeta is there; PV is done: v and TileMeta may be replaced, O is up to this tile
   uint64_t ifull[kInfo], iempty[kInfo];
-  uint64_t qfull[kQTiles], qempty[kQTiles], oempty, mlbar;
+  uint64_t qfull[WideCfg<kFp8, D>::kQTiles], qempty[WideCfg<kFp8, D>::kQTiles], oempty, mlbar;
   uint64_t pfull[2][2], halfdone[2];     // by group: a half of P is there; PV of the first half is done
   uint32_t tmem, abort_flag;
 };
-template <int D>
+template <bool kFp8, int D>
 constexpr size_t wide_smem_bytes() {
-  return 1024 + (size_t)WideCfg<D>::kTileBytes * (kQTiles + WideCfg<D>::kKStages + WideCfg<D>::kVStages) + sizeof(WideSmem<D>);
+  return 1024 + WideCfg<kFp8, D>::kOperands + sizeof(WideSmem<kFp8, D>);
 }
 
 // Matrix descriptors as their two halves: only the lower one, address and leading offset, differs from operand to operand, and
@@ -161,6 +168,9 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {  // zeros where it is not
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void get16(uint32_t (&v)[4], uint32_t src) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
+}
 __device__ __forceinline__ void put16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -211,19 +221,17 @@ __device__ __forceinline__ float top_of(const float (&s)[kChunk]) {
   return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
 
+// pairs of 16-bit values
 template <typename T, int N>
-__device__ __forceinline__ void store_row(T* out, const float (&y)[N], bool vec) {
+__device__ __forceinline__ void store_row(T* out, const uint32_t (&v)[N], bool vec) {
   if (vec) {
 #pragma unroll
-    for (int i = 0; i < N; i += 8)
-      *reinterpret_cast<uint4*>(out + i) = make_uint4(narrow2(y[i], y[i + 1], T()), narrow2(y[i + 2], y[i + 3], T()),
-                                                      narrow2(y[i + 4], y[i + 5], T()), narrow2(y[i + 6], y[i + 7], T()));
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(out + 2 * i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint32_t v = narrow2(y[i], y[i + 1], T());
-      reinterpret_cast<uint16_t*>(out)[i] = (uint16_t)v;
-      reinterpret_cast<uint16_t*>(out)[i + 1] = (uint16_t)(v >> 16);
+    for (int i = 0; i < N; ++i) {
+      reinterpret_cast<uint16_t*>(out)[2 * i] = (uint16_t)v[i];
+      reinterpret_cast<uint16_t*>(out)[2 * i + 1] = (uint16_t)(v[i] >> 16);
     }
   }
 }
@@ -231,14 +239,15 @@ __device__ __forceinline__ void store_row(T* out, const float (&y)[N], bool vec)
 template <typename T, bool kFp8, int D>
 __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __grid_constant__ AttendParams p, const uint32_t units) {
   using M = typename std::conditional<kFp8, __half, T>::type;
-  using C = WideCfg<D>;
+  using C = WideCfg<kFp8, D>;
   constexpr uint32_t kTileBytes = C::kTileBytes;
   constexpr int kKS = C::kKStages, kVS = C::kVStages;
   extern __shared__ unsigned char wide_raw[];
   const uint32_t pad = (1024u - (smem_u32(wide_raw) & 1023u)) & 1023u;
   unsigned char* base = wide_raw + pad;
+  constexpr uint32_t kQTiles = C::kQTiles;
   const uint32_t q_tiles = smem_u32(base), k_tiles = q_tiles + kQTiles * kTileBytes, v_tiles = k_tiles + kKS * kTileBytes;
-  WideSmem<D>& sm = *reinterpret_cast<WideSmem<D>*>(base + (size_t)kTileBytes * (kQTiles + kKS + kVS));
+  WideSmem<kFp8, D>& sm = *reinterpret_cast<WideSmem<kFp8, D>*>(base + C::kOperands);
   volatile uint32_t* abort_flag = &sm.abort_flag;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -247,11 +256,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
   const uint32_t first = blockIdx.x / (uint32_t)ctas, step = gridDim.x / (uint32_t)ctas;
 
   if (tid == 0) {
-    for (int i = 0; i < kKS; ++i) mbar_init(&sm.kfull[i], 4), mbar_init(&sm.sdone[i], 1);
+    for (int i = 0; i < kKS; ++i) mbar_init(&sm.kfull[i], 4);
+    for (int i = 0; i < C::kSDone; ++i) mbar_init(&sm.sdone[i], 1);
     for (int i = 0; i < kVS; ++i) mbar_init(&sm.vfull[i], 4);
     for (int i = 0; i < kMeta; ++i) mbar_init(&sm.mfull[i], 1), mbar_init(&sm.pvdone[i], 1);
     for (int i = 0; i < kInfo; ++i) mbar_init(&sm.ifull[i], 1), mbar_init(&sm.iempty[i], kSoftmaxWarps + kQueryWarps);
-    for (int i = 0; i < kQTiles; ++i) mbar_init(&sm.qfull[i], kQueryWarps), mbar_init(&sm.qempty[i], 1);
+    for (int i = 0; i < C::kQTiles; ++i) mbar_init(&sm.qfull[i], kQueryWarps), mbar_init(&sm.qempty[i], 1);
     mbar_init(&sm.oempty, kSoftmaxWarps);
     mbar_init(&sm.mlbar, kSoftmaxWarps);
     for (int i = 0; i < 2; ++i) mbar_init(&sm.pfull[i][0], 4), mbar_init(&sm.pfull[i][1], 4), mbar_init(&sm.halfdone[i], 1);
@@ -276,7 +286,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     const int gw = (warp - kSoftmaxWarps) & 3;
     uint64_t* const full = is_k ? sm.kfull : sm.vfull;
     uint64_t* const empty = is_k ? sm.sdone : sm.pvdone;  // of the tile `stages` before
-    const uint32_t ring = is_k ? kKS : kMeta;
+    const uint32_t ring = is_k ? C::kSDone : kMeta;
     const uint32_t stages = is_k ? kKS : kVS;
     const uint32_t tiles = is_k ? k_tiles : v_tiles;
     constexpr int kLanesRow = D * (kFp8 ? 1 : 2) / 16;  // lanes that read a row
@@ -285,7 +295,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     // two neighbouring chunks one after the other, half of those of two neighbouring rows.
     const int piece = kFp8 && kLanesRow == 8 ? (lane & 3) | ((lane >> 3 & 1) << 2) : lane % kLanesRow;
     const int sub = gw * 32 + (kFp8 && kLanesRow == 8 ? (lane >> 2 & 1) | ((lane >> 4) << 1) : lane / kLanesRow);
-    const int64_t row_bytes = (is_k ? p.k_slot : p.v_slot) * (kFp8 ? 1 : 2);
     const int64_t head_bytes = (is_k ? p.k_head : p.v_head) * (kFp8 ? 1 : 2);
     const char* const src0 = static_cast<const char*>(is_k ? p.k : p.v) + piece * 16;
     auto posted = [&](uint32_t n) { return __all_sync(kAll, mbar_test(&sm.mfull[n % kMeta], (n / kMeta) & 1u)); };
@@ -304,36 +313,54 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       if (lane == 0) mbar_arrive(&full[n % stages]);
     };
     if constexpr (kFp8) {
-      uint4 held[kTurns];  // the lane's pieces of the rows on their way
-      uint32_t to[2][2];   // where its two chunks go in a tile, turn 0 and turn 1 (without the turn's rows)
+      // Codes are copied to the warp's own ring; a tile's are widened to fp16 once they are there and the tile's place is free.
+      const uint32_t raw = q_tiles + (uint32_t)C::kTiles + (uint32_t)(warp - kSoftmaxWarps) * C::kRaw * C::kRawBytes + (uint32_t)lane * 16u;
+      uint32_t to[2][2];  // where the lane's two chunks go in a tile, turn 0 and turn 1 (without the turn's rows)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) to[i][e] = chunk_at(0u, sub + i * kRowsOnce, 2 * piece + e) - (uint32_t)(i * kRowsOnce * 128);
       }
-      auto fetch = [&](int i, const TileMeta& m, const char* src) {
-        const int row = m.row[sub + i * kRowsOnce];
-        held[i] = row >= 0 ? ldg16(src + (int64_t)row * row_bytes) : make_uint4(0u, 0u, 0u, 0u);
-      };
-      bool have = false;  // tile n's rows are on their way
-      for (uint32_t n = 0;; ++n) {
-        if (!have) {
-          if (!wait_posted(n)) break;
-          const TileMeta& m = sm.meta[n % kMeta];
-          if (m.flags & kEnd) break;
+      uint32_t asked = 0;      // tiles whose codes are asked for
+      bool ended = false;      // the stream, at `asked` tiles
+      auto ask = [&] {         // tile `asked`, which is posted
+        const TileMeta& m = sm.meta[asked % kMeta];
+        ended = (m.flags & kEnd) != 0;
+        if (!ended) {
           const char* src = src0 + m.kvh * head_bytes;
+          const int64_t* rows_at = (is_k ? m.k_at : m.v_at) + sub;
+          const uint32_t at = raw + (asked % C::kRaw) * C::kRawBytes;
 #pragma unroll
-          for (int i = 0; i < kTurns; ++i) fetch(i, m, src);
+          for (int i = 0; i < kTurns; ++i) {
+            const int64_t row = rows_at[i * kRowsOnce];
+            copy16(at + i * 512u, src + (row >= 0 ? row : 0), row >= 0);
+          }
+          ++asked;
         }
-        const TileMeta& next = sm.meta[(n + 1) % kMeta];
-        have = posted(n + 1) && !(next.flags & kEnd);
-        const char* src = src0 + (have ? next.kvh * head_bytes : 0);
-        const uint32_t tile = tiles + (n % stages) * kTileBytes;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      for (uint32_t n = 0;; ++n) {
+        if (asked == n) {  // (nothing on its way: wait for the scout)
+          if (!ended && !wait_posted(n)) break;
+          if (!ended) ask();
+          if (ended) break;
+        }
+        while (!ended && asked < n + C::kRaw && posted(asked)) ask();
+        // (the codes of a lane are its own copies: no other lane's wait is needed)
+        if (asked - n == 1u)
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+        else if (asked - n == 2u)
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else if (asked - n == 3u)
+          asm volatile("cp.async.wait_group 2;" ::: "memory");
+        else
+          asm volatile("cp.async.wait_group 3;" ::: "memory");
+        const uint32_t tile = tiles + (n % stages) * kTileBytes, at = raw + (n % C::kRaw) * C::kRawBytes;
         if (!wait_empty(n)) break;
 #pragma unroll
         for (int i = 0; i < kTurns; ++i) {
-          const uint32_t x[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
-          uint32_t h[8];
+          uint32_t x[4], h[8];
+          get16(x, at + i * 512u);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             h[2 * e] = e4m3x2_to_half2((uint16_t)x[e]);
@@ -343,10 +370,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           const uint32_t by = tile + (uint32_t)(i * kRowsOnce * 128);
           put16(by + to[i & 1][0], h[0], h[1], h[2], h[3]);
           put16(by + to[i & 1][1], h[4], h[5], h[6], h[7]);
-          if (have) fetch(i, next, src);  // the next tile's piece takes its place
         }
         hand_over(n);
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
       bool pending = false;  // tile n - 1 is on its way and not handed over
       for (uint32_t n = 0;; ++n) {
@@ -365,12 +392,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         }
         if (!wait_empty(n)) break;
         const char* src = src0 + m.kvh * head_bytes;
+        const int64_t* rows_at = (is_k ? m.k_at : m.v_at) + sub;
         const uint32_t tile = tiles + (n % stages) * kTileBytes;
 #pragma unroll
         for (int i = 0; i < kTurns; ++i) {
-          const int r = sub + i * kRowsOnce;
-          const int row = m.row[r];
-          copy16(chunk_at(tile, r, piece), row >= 0 ? src + (int64_t)row * row_bytes : src0, row >= 0);
+          const int64_t row = rows_at[i * kRowsOnce];
+          copy16(chunk_at(tile, sub + i * kRowsOnce, piece), src + (row >= 0 ? row : 0), row >= 0);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (pending) {
@@ -387,17 +414,26 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       // ---- scout: what the tiles to come are made of ----
       uint32_t n = 0, un = 0;
       bool ok = true;
-      for (uint32_t unit = first; ok && unit < units; unit += step, ++un) {
-        const Work w = work_of(p, unit);
-        const int32_t* idx = p.indices + (int64_t)w.token * p.idx_row;
+      // how many tiles a piece of work has, told to those who need not wait for the tiles themselves
+      auto tell = [&](uint32_t unit, uint32_t un) {
+        const int32_t* idx = p.indices + (int64_t)work_of(p, unit).token * p.idx_row;
         // (several CTAs a token: tiles without a row cost less than looking for the last)
         const int all = ctas > 1 ? (p.picks + kTileKeys - 1) / kTileKeys : tiles_of(idx, p.picks, lane);
         const int nt = all > rank ? (all - rank + ctas - 1) / ctas : 0;
-        if (!(ok = __all_sync(kAll, mbar_wait(&sm.iempty[un % kInfo], ((un / kInfo) & 1u) ^ 1u, abort_flag)))) break;
-        if (lane == 0) {
+        ok = __all_sync(kAll, mbar_wait(&sm.iempty[un % kInfo], ((un / kInfo) & 1u) ^ 1u, abort_flag));
+        if (ok && lane == 0) {
           sm.tiles[un % kInfo] = nt;
           mbar_arrive(&sm.ifull[un % kInfo]);
         }
+        return nt;
+      };
+      int nt_next = first < units ? tell(first, 0u) : 0;
+      for (uint32_t unit = first; ok && unit < units; unit += step, ++un) {
+        const Work w = work_of(p, unit);
+        const int32_t* idx = p.indices + (int64_t)w.token * p.idx_row;
+        const int nt = nt_next;
+        nt_next = unit + step < units ? tell(unit + step, un + 1u) : 0;
+        if (!ok) break;
         const int64_t offset = p.offsets != nullptr ? p.offsets[w.token] : 0;
         auto pick = [&](int (&to)[4], int j) {
 #pragma unroll
@@ -441,7 +477,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           unsigned whole = kAll;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            m.row[i * 32 + lane] = row[i];
+            m.k_at[i * 32 + lane] = row[i] < 0 ? -1 : row[i] * (p.k_slot * (kFp8 ? 1 : 2));
+            m.v_at[i * 32 + lane] = row[i] < 0 ? -1 : row[i] * (p.v_slot * (kFp8 ? 1 : 2));
             const unsigned live = __ballot_sync(kAll, row[i] >= 0);
             whole &= live;
             if (lane == 0) m.live[i] = live;
@@ -457,8 +494,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           }
           if (lane == 0) {
             m.vtop = top;
-            m.flags = (j == 0 ? kFirst : 0) | (j == nt - 1 ? kLast : 0) | (whole == kAll ? kWhole : 0);
-            m.j = j;
+            m.flags = (j == nt - 1 ? kLast : 0) | (whole == kAll ? kWhole : 0);
             m.kvh = w.kvh;
           }
           __syncwarp();
@@ -476,6 +512,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       const float negative = p.scale_log2 < 0.f ? -1.f : 1.f;
       const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale turns q: the largest score is then the largest here)
       constexpr int kQLanes = D / 8, kQOnce = 32 / kQLanes, kTurns = 64 / kQOnce, kBatch = 8;
+      // (the piece of work to come: its rows are brought to L2 while this one's keys go by)
+      auto prefetch = [&](uint32_t unit) {
+        const Work w = work_of(p, unit);
+        const T* q = static_cast<const T*>(p.q) + (int64_t)w.token * p.q_token + (int64_t)w.head0 * p.q_head;
+        for (int h = (warp - kQueryWarp) * 32 + lane; h < w.heads; h += 64) {
+#pragma unroll
+          for (int b = 0; b < D * 2; b += 128)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(q + (int64_t)h * p.q_head) + b) : "memory");
+        }
+      };
       const int c = lane % kQLanes, sub = (warp - kQueryWarp) * 64 + lane / kQLanes;
       uint32_t un = 0, wn = 0;
       for (uint32_t unit = first; unit < units; unit += step, ++un) {
@@ -486,7 +532,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         if (nt == 0) continue;
         const Work w = work_of(p, unit);
         const T* q0 = static_cast<const T*>(p.q) + (int64_t)w.token * p.q_token + (int64_t)w.head0 * p.q_head + c * 8;
-        const uint32_t tile = q_tiles + (wn % kQTiles) * kTileBytes;
 #pragma unroll 1
         for (int b = 0; b < kTurns; b += kBatch) {
           uint4 x[kBatch];
@@ -515,13 +560,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
               v = make_uint4(narrow2(a.x * down, a.y * down, __half()), narrow2(b2.x * down, b2.y * down, __half()),
                              narrow2(d.x * down, d.y * down, __half()), narrow2(e.x * down, e.y * down, __half()));
             }
-            put16(chunk_at(tile, h, c), v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+            put16(chunk_at(q_tiles + (wn % kQTiles) * kTileBytes, h, c), v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
             if (c == 0) sm.qmul[wn & 3u][h] = fmaxf(mul, 1.17549435e-38f);  // (times a masked score it must stay -inf)
           }
         }
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.qfull[wn % kQTiles]);
+        if (unit + step < units) prefetch(unit + step);
         ++wn;
       }
     } else if (warp == kMmaWarp) {
@@ -534,70 +580,85 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         int qj = 0, pj = 0;           // and tiles of those
         uint32_t flags = 0u, pflags = 0u;  // of tile qn, once it is ready; of the tiles between QK and PV, a byte each
         bool ended = false;           // the stream, at qn tiles
-        bool ok = true;
-        auto ready = [&](bool wait) {  // tile qn's k and q; sets `ended` where there is no such tile
-          uint64_t* const meta = &sm.mfull[qn % kMeta];
-          if (!(wait ? mbar_wait(meta, (qn / kMeta) & 1u, abort_flag) : mbar_test(meta, (qn / kMeta) & 1u))) return false;
-          flags = (uint32_t)sm.meta[qn % kMeta].flags;
-          if (flags & kEnd) {
-            ended = true;
-            return false;
+        auto ready = [&] {  // tile qn's k and q are there; sets `ended` where there is no such tile
+          if (flags == 0u) {
+            if (!mbar_test(&sm.mfull[qn % kMeta], (qn / kMeta) & 1u)) return false;
+            flags = (uint32_t)sm.meta[qn % kMeta].flags | kSeen;
+            if (flags & kEnd) {
+              ended = true;
+              return false;
+            }
           }
-          if (qj == 0) {
-            uint64_t* const q = &sm.qfull[qwn % kQTiles];
-            if (!(wait ? mbar_wait(q, (qwn / kQTiles) & 1u, abort_flag) : mbar_test(q, (qwn / kQTiles) & 1u))) return false;
-          }
-          uint64_t* const k = &sm.kfull[qn % kKS];
-          return wait ? mbar_wait(k, (qn / kKS) & 1u, abort_flag) : mbar_test(k, (qn / kKS) & 1u);
+          return (qj != 0 || mbar_test(&sm.qfull[qwn % kQTiles], (qwn / kQTiles) & 1u)) && mbar_test(&sm.kfull[qn % kKS], (qn / kKS) & 1u);
         };
         auto qk = [&] {
           tmem_fence_after();
-          const uint32_t stage = qn % kKS, qt = qwn % kQTiles;
-          const uint32_t kt = desc_k(k_tiles + stage * kTileBytes), q = desc_k(q_tiles + qt * kTileBytes), d = tmem + (qn & 1u) * 128u;
+          const uint32_t stage = qn % kKS;
+          const uint32_t kt = desc_k(k_tiles + stage * kTileBytes), q = desc_k(q_tiles + (qwn % kQTiles) * kTileBytes), d = tmem + (qn & 1u) * 128u;
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t at = ((uint32_t)(k >> 2) * (kTileKeys * 128u) + (uint32_t)(k & 3) * 32u) >> 4;
             mma_ss(d, q + at, kt + at, instr_desc<M, kTileKeys, false>(), k != 0);
           }
-          umma_commit(&sm.sdone[stage]);
+          umma_commit(&sm.sdone[qn % C::kSDone]);
           const bool last = (flags & kLast) != 0;
-          if (last) umma_commit(&sm.qempty[qt]);
+          if (last) umma_commit(&sm.qempty[qwn % kQTiles]);
           pflags |= flags << (8u * (qn & 1u));
+          flags = 0u;
           ++qn;
           qj = last ? 0 : qj + 1;
           qwn += last ? 1u : 0u;
         };
-        while (ok) {
+        // What can go next goes next: the products that wait for something are looked at in turn. PV of a tile goes in two halves of its
+        // keys: the first half's products run beside the second half's exponentials.
+        bool half = false;            // PV of tile pn: its first half has been issued
+        int idle_turns = 0;           // looks in a row that found nothing to issue
+        for (;;) {
+          bool idle = true;
           // (two tiles at most are between their QK and their PV: one a group)
-          if (!ended && qn - pn < 2u && ready(qn == pn)) {
+          if (!ended && qn - pn < 2u && ready()) {
             qk();
-            continue;
+            idle = false;
           }
-          if (qn == pn) break;  // the end - or a wait that ran out
-          // PV of tile pn, half of its keys at a time: the first half's products run beside the second half's exponentials
-          const uint32_t g = pn & 1u, stage = pn % kVS, vt = desc_mn(v_tiles + stage * kTileBytes), s_at = tmem + g * 128u;
-          const uint32_t phase = (pn >> 1) & 1u, more_of_o = pj > 1 ? 1u : 0u;
-          const bool last = (pflags >> (8u * g) & kLast) != 0u;
-          if (pj == 0 && !(ok = mbar_wait(&sm.oempty, (pwn & 1u) ^ 1u, abort_flag))) break;  // (O may still be on its way out)
-          if (!(ok = mbar_wait(&sm.vfull[stage], (pn / kVS) & 1u, abort_flag))) break;
-          if (!(ok = mbar_wait(&sm.pfull[g][0], phase, abort_flag))) break;
-          tmem_fence_after();
+          if (qn == pn) {
+            if (ended) break;
+          } else {
+            const uint32_t g = pn & 1u, stage = pn % kVS, phase = (pn >> 1) & 1u;
+            const uint32_t vt = desc_mn(v_tiles + stage * kTileBytes), s_at = tmem + g * 128u;
+            // (the first PV of a piece of work: O may still be on its way out)
+            if (!half && mbar_test(&sm.pfull[g][0], phase) && mbar_test(&sm.vfull[stage], (pn / kVS) & 1u) &&
+                (pj != 0 || mbar_test(&sm.oempty, (pwn & 1u) ^ 1u))) {
+              tmem_fence_after();
 #pragma unroll
-          for (int k = 0; k < kTileKeys / 32; ++k)
-            mma_ts(s_at + 256u, s_at + (uint32_t)k * 8u, vt + (uint32_t)k * (2048u >> 4), instr_desc<M, D, true>(), k != 0 ? 1u : more_of_o);
-          umma_commit(&sm.halfdone[g]);
-          const bool more = !ended && qn - pn == 2u && ready(false);
-          if (!(ok = mbar_wait(&sm.pfull[g][1], phase, abort_flag))) break;
-          tmem_fence_after();
+              for (int k = 0; k < kTileKeys / 32; ++k)
+                mma_ts(s_at + 256u, s_at + (uint32_t)k * 8u, vt + (uint32_t)k * (2048u >> 4), instr_desc<M, D, true>(), k != 0 || pj > 1);
+              umma_commit(&sm.halfdone[g]);
+              half = true;
+              idle = false;
+            }
+            if (half && mbar_test(&sm.pfull[g][1], phase)) {
+              tmem_fence_after();
 #pragma unroll
-          for (int k = kTileKeys / 32; k < kTileKeys / 16; ++k)
-            mma_ts(s_at + 256u, s_at + (uint32_t)k * 8u, vt + (uint32_t)k * (2048u >> 4), instr_desc<M, D, true>(), 1u);
-          umma_commit(&sm.pvdone[pn % kMeta]);
-          pflags &= 0xff00u >> (8u * g);
-          ++pn;
-          pj = last ? 0 : pj + 1;
-          pwn += last ? 1u : 0u;
-          if (more) qk();
+              for (int k = kTileKeys / 32; k < kTileKeys / 16; ++k)
+                mma_ts(s_at + 256u, s_at + (uint32_t)k * 8u, vt + (uint32_t)k * (2048u >> 4), instr_desc<M, D, true>(), 1u);
+              umma_commit(&sm.pvdone[pn % kMeta]);
+              const bool last = (pflags >> (8u * g) & kLast) != 0u;
+              pflags &= 0xff00u >> (8u * g);
+              ++pn;
+              pj = last ? 0 : pj + 1;
+              pwn += last ? 1u : 0u;
+              half = false;
+              idle = false;
+            }
+          }
+          if (!idle) {
+            idle_turns = 0;
+          } else {
+            // (a look costs issue slots that the softmax warps want; 2^22 looks with their pauses are half a second)
+            if (++idle_turns >= 1 << 22) *abort_flag = 1u;
+            if ((idle_turns & 255) == 0 && *abort_flag) break;
+            __nanosleep(kPauseNs);
+          }
         }
       }
       __syncwarp();
@@ -622,7 +683,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       float* const lse = p.lse == nullptr ? nullptr : p.lse + (int64_t)w.token * p.kv_heads * p.group + w.head0 + r;
       if (nt == 0 && ctas == 1) {
         if (mine) {
-          float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          const uint32_t zero[4] = {0u, 0u, 0u, 0u};
           for (int c = 0; c < kHalf; c += 8) store_row(out + c, zero, p.out_vec != 0);
           if (g == 0 && lse != nullptr) *lse = -INFINITY;
         }
@@ -632,7 +693,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       for (int j = g ^ (int)(it & 1u); j < nt; j += 2) {
         const uint32_t n = it + (uint32_t)j;
         const int place = (int)(n % kMeta);
-        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag) && mbar_wait(&sm.sdone[n % kKS], (n / kKS) & 1u, abort_flag);
+        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag) && mbar_wait(&sm.sdone[n % C::kSDone], (n / C::kSDone) & 1u, abort_flag);
         if (!(ok = __all_sync(kAll, ok))) break;
         tmem_fence_after();
         auto hand_over = [&](int half) {
@@ -759,8 +820,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       const float l = fa * a.y + fb * b.y;
       const float inv = ctas > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       float* const stage_row = reinterpret_cast<float*>(base) + (size_t)r * (D + 4) + g * kHalf;  // (several CTAs: over the q and k tiles)
+      uint32_t packed[kHalf / 2];  // (the pieces of work to come may have O as soon as it has been read)
       if (busy) {
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < kHalf; c += 32) {
           float y[32];
           const uint32_t col = lanes + 256u + (uint32_t)(g * kHalf + c);
@@ -780,14 +842,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           if (ctas > 1) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(stage_row + c + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-          } else if (mine) {
-            store_row(out + c, y, p.out_vec != 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) packed[(c + i) / 2] = narrow2(y[i], y[i + 1], T());
           }
         }
       }
       tmem_fence_before();
       __syncwarp();
       if (nt > 0 && lane == 0) mbar_arrive(&sm.oempty);
+      if (ctas == 1 && mine) store_row(out, packed, p.out_vec != 0);
       if (g == 0) {
         if (ctas > 1)
           sm.ml[1][0][r] = make_float2(top, l);  // (one piece of work a CTA: the other half is not in use)
@@ -873,7 +937,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
 template <typename T, bool kFp8, int D>
 int setup_wide() {
   const cudaError_t e =
-      cudaFuncSetAttribute(attend_wide_kernel<T, kFp8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide_smem_bytes<D>());
+      cudaFuncSetAttribute(attend_wide_kernel<T, kFp8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide_smem_bytes<kFp8, D>());
   return e == cudaSuccess ? 0 : cuda_fail(e);
 }
 
@@ -883,7 +947,7 @@ cudaError_t launch_wide(const AttendParams& p, int ctas, int64_t units, int sms,
   const int64_t grid = ctas > 1 ? units * ctas : units < sms ? units : sms;
   cfg.gridDim = dim3((unsigned)grid, 1, 1);
   cfg.blockDim = dim3(kWideThreads, 1, 1);
-  cfg.dynamicSmemBytes = wide_smem_bytes<D>();
+  cfg.dynamicSmemBytes = wide_smem_bytes<kFp8, D>();
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

@@ -14,8 +14,7 @@
 // rotation pairs channel i with i + R/2, the piece at i and the piece at its partners, so that it needs no exchange between lanes
 // and a piece of the table serves both; elsewhere one piece in each half of what is left. 8 to 32 lanes make a row, its sums are three to
 // five shuffles. A group of lanes takes several heads of ONE token where there are rows enough: it loads the token's cosines and
-// sines and the norm's weights once, and has that many loads in flight. A block works on one part alone, so that what a part is
-// like is known to the whole block.
+// sines and the norm's weights once, and has that many loads in flight. A block works on one part alone.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -31,7 +30,7 @@
 namespace fftopk {
 namespace {
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 constexpr int kMaxParts = 3;
 constexpr int kHeadsItem = 4;  // heads of a token that a group of lanes takes where there are rows enough
 constexpr float kAmaxFloor = 1.262177448353618888658765704452e-29f;  // 2^-96
@@ -46,6 +45,7 @@ struct RowParams {
   const float* cos_sin;
   int64_t table_rows;
   int32_t D, R, interleaved;
+  float inv_d;
   uint32_t* status;
 };
 
@@ -59,9 +59,11 @@ __device__ __forceinline__ void load_weights(float* w, const void* p, int32_t dt
   }
 }
 
+enum : int { kRotNone = 0, kRotApart = 1, kRotNext = 2 };  // partners: none, i and i + R / 2, 2 i and 2 i + 1
+
 // T: the rows' type; kLanes: lanes of a group; kHeads: heads an item takes; kVec: pieces may be read and written as one
-template <typename T, int kLanes, int kHeads, bool kVec, int which>
-__device__ __forceinline__ void head_rows(const RowParams& p) {
+template <typename T, int kLanes, int kHeads, bool kVec, int kNorm, int kRot, bool kQuant>
+__device__ __forceinline__ void head_rows(const RowParams& p, const int which) {
   const fftopk_head_part& part = p.part[which];
   const int lane = threadIdx.x & (kLanes - 1);
   const uint32_t mask = group_mask<kLanes>();
@@ -71,113 +73,115 @@ __device__ __forceinline__ void head_rows(const RowParams& p) {
   const uint32_t token = in ? p.per_token[which].div(item) : 0u;
   const int h0 = in ? (int)(item - token * p.per_token[which].d) * kHeads : 0;
   // the lane's pieces: channels at[0] .. at[0] + 3 and at[1] .. at[1] + 3
-  const int R = part.rotate ? p.R : 0;
-  const int pairs = p.interleaved ? 0 : R;  // channels that lie with their partners
+  const int pairs = kRot == kRotApart ? p.R : 0;  // channels that lie with their partners
   const int back = lane - (pairs >> 3);
   int at[2];
-  at[0] = back < 0 ? 4 * lane : pairs + 4 * back;
-  at[1] = at[0] + ((back < 0 ? pairs : p.D - pairs) >> 1);
+  at[0] = kRot == kRotApart && back < 0 ? 4 * lane : pairs + 4 * back;
+  at[1] = at[0] + ((kRot == kRotApart && back < 0 ? pairs : p.D - pairs) >> 1);
   const bool mine = in && lane * 8 < p.D;
+  const int rows = mine ? min(kHeads, part.heads - h0) : 0;
 
   Four<T> raw[kHeads][2];
-  const T* x = static_cast<const T*>(part.x) + (int64_t)token * part.x_token_stride + (int64_t)h0 * part.x_head_stride;
+  {
+    const int64_t step = part.x_head_stride;
+    const T* x = static_cast<const T*>(part.x) + ((int64_t)token * part.x_token_stride + h0 * step);
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      raw[i][e].zero();
-      if (mine && h0 + i < part.heads) raw[i][e].template load<kVec>(x + (int64_t)i * part.x_head_stride + at[e]);
+    for (int i = 0; i < kHeads; ++i, x += step) {
+      raw[i][0].zero();
+      raw[i][1].zero();
+      if (i < rows) {
+        raw[i][0].template load<kVec>(x + at[0]);
+        raw[i][1].template load<kVec>(x + at[1]);
+      }
     }
   }
   // where the rows go
   int64_t to = token;
-  bool keep = mine;
+  int puts = rows;
   if (part.slots != nullptr && in) {
     to = part.slots[token];
-    if (to < 0) keep = false;
-    if (to >= part.n_slots) {
-      keep = false;
-      if (lane == 0 && h0 == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
-    }
+    if (to < 0 || to >= part.n_slots) puts = 0;
+    if (to >= part.n_slots && lane == 0 && h0 == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
   }
-  // Cosines and sines. Partners apart: of channels at[0] .. at[0] + 3; interleaved: of two pairs of each piece, each twice, the sines
+  // Cosines and sines. Partners apart: of channels at[0] .. at[0] + 3; side by side: of two pairs of each piece, each twice, the sines
   // with the signs the pair's two channels take the other one with.
   Pair c[4], sn[4];
-  const Pair one = pair(1.f, 1.f), none = pair(0.f, 0.f);
+  if constexpr (kRot != kRotNone) {
+    const Pair one = pair(1.f, 1.f), none = pair(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = one, sn[i] = none;
-  if (R && mine) {
-    const int64_t pos = p.positions[token];
-    const bool ok = pos >= 0 && pos < p.table_rows;
-    if (!ok && lane == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
-    const float nan = __int_as_float(0x7fffffff);  // (no such row in the table: the rotated channels become NaN)
-    const float* row = p.cos_sin + (ok ? pos : 0) * p.R;
-    const int half = p.R >> 1;
-    if (p.interleaved) {
+    for (int i = 0; i < (kRot == kRotApart ? 2 : 4); ++i) c[i] = one, sn[i] = none;
+    if (mine) {
+      const int64_t pos = p.positions[token];
+      const bool ok = pos >= 0 && pos < p.table_rows;
+      if (!ok && lane == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+      const float nan = __int_as_float(0x7fffffff);  // (no such row in the table: the rotated channels become NaN)
+      const float* row = p.cos_sin + (ok ? pos : 0) * p.R;
+      const int half = p.R >> 1;
+      if constexpr (kRot == kRotNext) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (at[e] < R) {
-          float2 a = make_float2(nan, nan), b = a;
-          if (ok) a = *reinterpret_cast<const float2*>(row + (at[e] >> 1)), b = *reinterpret_cast<const float2*>(row + half + (at[e] >> 1));
-          c[2 * e] = pair(a.x, a.x), c[2 * e + 1] = pair(a.y, a.y);
-          sn[2 * e] = pair(-b.x, b.x), sn[2 * e + 1] = pair(-b.y, b.y);
+        for (int e = 0; e < 2; ++e) {
+          if (at[e] < p.R) {
+            float2 a = make_float2(nan, nan), b = a;
+            if (ok) a = *reinterpret_cast<const float2*>(row + (at[e] >> 1)), b = *reinterpret_cast<const float2*>(row + half + (at[e] >> 1));
+            c[2 * e] = pair(a.x, a.x), c[2 * e + 1] = pair(a.y, a.y);
+            sn[2 * e] = pair(-b.x, b.x), sn[2 * e + 1] = pair(-b.y, b.y);
+          }
         }
+      } else if (back < 0) {
+        float4 a = make_float4(nan, nan, nan, nan), b = a;
+        if (ok) a = *reinterpret_cast<const float4*>(row + at[0]), b = *reinterpret_cast<const float4*>(row + half + at[0]);
+        c[0] = pair(a.x, a.y), c[1] = pair(a.z, a.w);
+        sn[0] = pair(b.x, b.y), sn[1] = pair(b.z, b.w);
       }
-    } else if (back < 0) {
-      float4 a = make_float4(nan, nan, nan, nan), b = a;
-      if (ok) a = *reinterpret_cast<const float4*>(row + at[0]), b = *reinterpret_cast<const float4*>(row + half + at[0]);
-      c[0] = pair(a.x, a.y), c[1] = pair(a.z, a.w);
-      sn[0] = pair(b.x, b.y), sn[1] = pair(b.z, b.w);
-      sn[2] = pair(-b.x, -b.y), sn[3] = pair(-b.z, -b.w);
+    }
+    if constexpr (kRot == kRotApart) {
+      const Pair minus = pair(-1.f, -1.f);
+      sn[2] = mul2(sn[0], minus), sn[3] = mul2(sn[1], minus);
     }
   }
   Pair w[4], b[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = one, b[i] = none;
-  if (part.norm != FFTOPK_NORM_NONE && mine) {
+  const bool scaled = kNorm != FFTOPK_NORM_NONE && part.weight != nullptr, moved = kNorm != FFTOPK_NORM_NONE && part.bias != nullptr;
+  if constexpr (kNorm != FFTOPK_NORM_NONE) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float f[4];
-      if (part.weight != nullptr) {
-        load_weights(f, part.weight, part.weight_dtype, at[e], p.aligned_w[which] != 0);
-        w[2 * e] = pair(f[0], f[1]), w[2 * e + 1] = pair(f[2], f[3]);
-      }
-      if (part.bias != nullptr) {
-        load_weights(f, part.bias, part.weight_dtype, at[e], p.aligned_w[which] != 0);
-        b[2 * e] = pair(f[0], f[1]), b[2 * e + 1] = pair(f[2], f[3]);
-      }
+      float f[4] = {1.f, 1.f, 1.f, 1.f}, g[4] = {0.f, 0.f, 0.f, 0.f};
+      if (scaled && mine) load_weights(f, part.weight, part.weight_dtype, at[e], p.aligned_w[which] != 0);
+      if (moved && mine) load_weights(g, part.bias, part.weight_dtype, at[e], p.aligned_w[which] != 0);
+      w[2 * e] = pair(f[0], f[1]), w[2 * e + 1] = pair(f[2], f[3]);
+      b[2 * e] = pair(g[0], g[1]), b[2 * e + 1] = pair(g[2], g[3]);
     }
   }
 
-  const float inv_d = 1.f / (float)p.D;
-  const int64_t first = to * part.out_token_stride + (int64_t)h0 * part.out_head_stride;
+  const int64_t step = part.out_head_stride;
+  char* o = static_cast<char*>(part.out) + (to * part.out_token_stride + h0 * step) * (kQuant ? 1 : (int)sizeof(T));
   float amax_of[kHeads];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
+  for (int i = 0; i < kHeads; ++i, o += step * (kQuant ? 1 : (int)sizeof(T))) {
     Pair y[4];  // channels of piece 0, of piece 1
     raw[i][0].widen(y);
     raw[i][1].widen(y + 2);
-    if (part.norm != FFTOPK_NORM_NONE) {
-      if (part.norm == FFTOPK_NORM_LAYER) {
+    if constexpr (kNorm != FFTOPK_NORM_NONE) {
+      if constexpr (kNorm == FFTOPK_NORM_LAYER) {
         const float2 t = apart(add2(add2(y[0], y[1]), add2(y[2], y[3])));
-        const float mean = group_sum<kLanes>(t.x + t.y, mask) * inv_d;
-        const Pair less = mine ? pair(-mean, -mean) : none;
+        const float all = group_sum<kLanes>(t.x + t.y, mask);
+        const float mean = mine ? all * p.inv_d : 0.f;  // (lanes beyond D stay zero)
+        const Pair less = pair(-mean, -mean);
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = add2(y[e], less);
       }
       const float2 t = apart(add2(fma2(y[0], y[0], mul2(y[1], y[1])), fma2(y[2], y[2], mul2(y[3], y[3]))));
-      const float r = rsqrtf(group_sum<kLanes>(t.x + t.y, mask) * inv_d + part.eps);
+      const float r = rsqrtf(fmaf(group_sum<kLanes>(t.x + t.y, mask), p.inv_d, part.eps));
       const Pair rr = pair(r, r);
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = fma2(mul2(y[e], rr), w[e], b[e]);
     }
-    if (R) {
-      if (p.interleaved) {
+    if constexpr (kRot == kRotNext) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (at[e >> 1] < R) y[e] = fma2(turned(y[e]), sn[e], mul2(y[e], c[e]));
-        }
-      } else if (back < 0) {
+      for (int e = 0; e < 4; ++e) {
+        if (at[e >> 1] < p.R) y[e] = fma2(turned(y[e]), sn[e], mul2(y[e], c[e]));
+      }
+    } else if constexpr (kRot == kRotApart) {
+      if (back < 0) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const Pair u = y[e], v = y[e + 2];
@@ -186,15 +190,13 @@ __device__ __forceinline__ void head_rows(const RowParams& p) {
         }
       }
     }
-    const bool put = keep && h0 + i < part.heads;
-    if (part.scale == nullptr) {
-      if (put) {
-        T* o = static_cast<T*>(part.out) + first + (int64_t)i * part.out_head_stride;
+    if constexpr (!kQuant) {
+      if (i < puts) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           Four<T> r;
           r.narrow(y + 2 * e);
-          r.template store<kVec>(o + at[e]);
+          r.template store<kVec>(reinterpret_cast<T*>(o) + at[e]);
         }
       }
     } else {
@@ -218,9 +220,8 @@ __device__ __forceinline__ void head_rows(const RowParams& p) {
       amax = fmaxf(amax, kAmaxFloor);
       amax_of[i] = amax;
       const float inv = __fdiv_rn(448.f, amax);
-      if (put) {
+      if (i < puts) {
         const Pair ii = pair(inv, inv);
-        uint8_t* o = static_cast<uint8_t*>(part.out) + first + (int64_t)i * part.out_head_stride;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t codes = to_e4m3(mul2(y[2 * e], ii), mul2(y[2 * e + 1], ii));
@@ -228,19 +229,19 @@ __device__ __forceinline__ void head_rows(const RowParams& p) {
             *reinterpret_cast<uint32_t*>(o + at[e]) = codes;
           } else {
 #pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) o[at[e] + i2] = (uint8_t)(codes >> (8 * i2));
+            for (int i2 = 0; i2 < 4; ++i2) o[at[e] + i2] = (char)(codes >> (8 * i2));
           }
         }
       }
     }
   }
-  if (part.scale != nullptr) {  // lane i writes the scale of the item's row i
+  if constexpr (kQuant) {  // lane i writes the scale of the item's row i
     float amax = amax_of[0];
 #pragma unroll
     for (int i = 1; i < kHeads; ++i)
       if (lane == i) amax = amax_of[i];
-    const int h = h0 + lane;
-    if (keep && lane < kHeads && h < part.heads) {
+    if (lane < puts) {
+      const int h = h0 + lane;
       const float scale = __fdiv_rn(amax, 448.f);
       part.scale[to * part.scale_token_stride + (int64_t)h * part.scale_head_stride] =
           part.mul != nullptr ? part.mul[(int64_t)token * part.heads + h] * scale : scale;
@@ -248,16 +249,36 @@ __device__ __forceinline__ void head_rows(const RowParams& p) {
   }
 }
 
-// (the part is a constant of the code: found by an index, each of its fields would be a load of its own at every use - 253 us
-// instead of 121 for 16,384 tokens of 72 heads)
-template <typename T, int kLanes, int kHeads, bool kVec>
-__global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_constant__ RowParams p) {
-  if (blockIdx.x < p.first_block[1])
-    head_rows<T, kLanes, kHeads, kVec, 0>(p);
-  else if (blockIdx.x < p.first_block[2])
-    head_rows<T, kLanes, kHeads, kVec, 1>(p);
+// What a part is like is known to the whole block, and is a constant of the code that runs: with norm, rotation and quantisation
+// as branches inside one body 16,384 tokens of 72 heads took 165 us instead of 151. Eight blocks of 128 threads per SM, 64 registers
+// (fp32: five), make it 128: a block loads, works and stores once, so the blocks beside it have to keep memory busy (10 blocks
+// spill: 155; two, three or eight heads an item 165, 147, 153).
+template <typename T, int kLanes, int kHeads, bool kVec, int kNorm, int kRot>
+__device__ __forceinline__ void head_rows(const RowParams& p, int which) {
+  if (p.part[which].scale != nullptr)
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRot, true>(p, which);
   else
-    head_rows<T, kLanes, kHeads, kVec, 2>(p);
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRot, false>(p, which);
+}
+template <typename T, int kLanes, int kHeads, bool kVec, int kNorm>
+__device__ __forceinline__ void head_rows(const RowParams& p, int which) {
+  if (!p.part[which].rotate)
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRotNone>(p, which);
+  else if (p.interleaved)
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRotNext>(p, which);
+  else
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRotApart>(p, which);
+}
+template <typename T, int kLanes, int kHeads, bool kVec>
+__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 4 ? 5 : 8) head_rows_kernel(const __grid_constant__ RowParams p) {
+  const int which = blockIdx.x >= p.first_block[2] ? 2 : blockIdx.x >= p.first_block[1] ? 1 : 0;
+  const int norm = p.part[which].norm;
+  if (norm == FFTOPK_NORM_NONE)
+    head_rows<T, kLanes, kHeads, kVec, FFTOPK_NORM_NONE>(p, which);
+  else if (norm == FFTOPK_NORM_RMS)
+    head_rows<T, kLanes, kHeads, kVec, FFTOPK_NORM_RMS>(p, which);
+  else
+    head_rows<T, kLanes, kHeads, kVec, FFTOPK_NORM_LAYER>(p, which);
 }
 
 template <typename T, int kLanes>
@@ -440,6 +461,7 @@ int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tok
   p.cos_sin = cos_sin;
   p.table_rows = table_rows;
   p.D = D;
+  p.inv_d = 1.f / (float)D;
   p.R = rotary;
   p.interleaved = interleaved;
   p.status = status;

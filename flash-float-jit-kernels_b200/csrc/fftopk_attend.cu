@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_narrow_kernel(const __grid
       mx[r] = m;
     }
     if constexpr (kFp8) {
-      float top = vs;
+      float top = fabsf(vs);
 #pragma unroll
       for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, i));
       const float ref = top > 64.f * vref ? top : vref;  // (let stand likewise, up to 2^6: weights stay below 2^14)

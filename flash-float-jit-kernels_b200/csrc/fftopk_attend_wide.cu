@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             if constexpr (kFp8) {
               m.ks[i * 32 + lane] = ks[i];
               m.vs[i * 32 + lane] = vs[i];
-              top = fmaxf(top, vs[i]);
+              top = fmaxf(top, fabsf(vs[i]));
             }
           }
           if constexpr (kFp8) {

@@ -426,7 +426,8 @@ int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tok
     if (a.slots != nullptr && a.n_slots < 0) return FFTOPK_EINVAL;
     if (a.mul != nullptr && a.scale == nullptr) return FFTOPK_EINVAL;
     if (a.heads == 0) continue;
-    if (a.x == nullptr || a.out == nullptr) {
+    const bool nowhere = a.slots != nullptr && a.n_slots == 0;  // (an empty cache has no address)
+    if (a.x == nullptr || (a.out == nullptr && !nowhere)) {
       if (tokens > 0) return FFTOPK_EINVAL;
       continue;
     }
@@ -478,7 +479,7 @@ int fftopk_cache_read(const void* cache, int64_t slot_stride, int64_t head_strid
   if (n_slots < 0 || heads < 0 || rows < 0 || per_row < 0 || !known_dtype(out_dtype)) return FFTOPK_EINVAL;
   if (D < 8 || D > 256 || (D & 7) != 0) return FFTOPK_ERANGE;
   if (rows == 0 || per_row == 0 || heads == 0) return FFTOPK_OK;
-  if (cache == nullptr || scale == nullptr || slots == nullptr || out == nullptr) return FFTOPK_EINVAL;
+  if (slots == nullptr || out == nullptr || (n_slots > 0 && (cache == nullptr || scale == nullptr))) return FFTOPK_EINVAL;
   if (!on(scale, 4) || !on(slots, 4) || !on(offsets, 4) || !on(out, 16)) return FFTOPK_EINVAL;
   if (rows > 0x7fffffff || per_row > 0x7fffffff || rows * per_row > 0x7fffffff || rows * per_row * heads > (int64_t)0x7fffffff - 4096)
     return FFTOPK_ERANGE;

@@ -422,6 +422,7 @@ int fftopk_cache_read(const void* cache, int64_t slot_stride, int64_t head_strid
  *   lse          fp32 [tokens, q_heads], contiguous, or NULL: log of the sum of exponentials
  *   strides      in elements; rows of q, k and v start on 16 bytes
  * Sums and maxima are kept in 32 bits; weights are rounded to dtype (16-bit cache) or fp16 (e4m3) for the second product.
+ * v scales: magnitudes between 2^-100 and 2^100 (beyond that weights may underflow, or overflow to infinities).
  * The call holds no state and needs no workspace; the first one on a device sets kernel attributes (outside any capture).
  */
 typedef struct fftopk_attend {

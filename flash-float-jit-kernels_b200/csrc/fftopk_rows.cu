@@ -79,7 +79,8 @@ __device__ __forceinline__ void head_rows(const RowParams& p, const int which) {
   at[0] = kRot == kRotApart && back < 0 ? 4 * lane : pairs + 4 * back;
   at[1] = at[0] + ((kRot == kRotApart && back < 0 ? pairs : p.D - pairs) >> 1);
   const bool mine = in && lane * 8 < p.D;
-  const int rows = mine ? min(kHeads, part.heads - h0) : 0;
+  const int there = in ? min(kHeads, part.heads - h0) : 0;  // rows of the item
+  const int rows = mine ? there : 0;
 
   Four<T> raw[kHeads][2];
   {
@@ -97,12 +98,13 @@ __device__ __forceinline__ void head_rows(const RowParams& p, const int which) {
   }
   // where the rows go
   int64_t to = token;
-  int puts = rows;
+  bool keep = true;
   if (part.slots != nullptr && in) {
     to = part.slots[token];
-    if (to < 0 || to >= part.n_slots) puts = 0;
+    keep = to >= 0 && to < part.n_slots;
     if (to >= part.n_slots && lane == 0 && h0 == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
   }
+  const int puts = keep ? rows : 0;
   // Cosines and sines. Partners apart: of channels at[0] .. at[0] + 3; side by side: of two pairs of each piece, each twice, the sines
   // with the signs the pair's two channels take the other one with.
   Pair c[4], sn[4];
@@ -240,7 +242,7 @@ __device__ __forceinline__ void head_rows(const RowParams& p, const int which) {
 #pragma unroll
     for (int i = 1; i < kHeads; ++i)
       if (lane == i) amax = amax_of[i];
-    if (lane < puts) {
+    if (keep && lane < there) {  // (whether the lane has channels of its own or not)
       const int h = h0 + lane;
       const float scale = __fdiv_rn(amax, 448.f);
       part.scale[to * part.scale_token_stride + (int64_t)h * part.scale_head_stride] =
@@ -270,7 +272,7 @@ __device__ __forceinline__ void head_rows(const RowParams& p, int which) {
     head_rows<T, kLanes, kHeads, kVec, kNorm, kRotApart>(p, which);
 }
 template <typename T, int kLanes, int kHeads, bool kVec>
-__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 4 ? 5 : 8) head_rows_kernel(const __grid_constant__ RowParams p) {
+__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 4 && kHeads > 1 ? 5 : 8) head_rows_kernel(const __grid_constant__ RowParams p) {
   const int which = blockIdx.x >= p.first_block[2] ? 2 : blockIdx.x >= p.first_block[1] ? 1 : 0;
   const int norm = p.part[which].norm;
   if (norm == FFTOPK_NORM_NONE)

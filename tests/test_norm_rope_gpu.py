@@ -290,3 +290,20 @@ def test_empty_calls():
     cache_write(z, none, c, s)
     assert cache_read(c, s, none).shape == (0, 4, 64)
     assert cache_read(c, s, torch.empty(3, 0, device="cuda", dtype=torch.int32)).shape == (3, 0, 4, 64)
+
+
+@pytest.mark.parametrize("D", [8, 16, 24, 40])
+def test_many_short_rows(D):
+    """Heads of fewer channels than an item has rows: every row's scale is written."""
+    g = gen(D)
+    T, H = 9000, 5
+    x = rand(g, T, H, D, dtype=torch.bfloat16)
+    c, s = empty_cache(T, H, D)
+    cache_write(x, torch.arange(T, device="cuda", dtype=torch.int32), c, s)
+    y, e = ref.head_rows(x)
+    ref.check_quantised(c, s, y, e * 0)
+    w = torch.rand(T, H, generator=g, device="cuda")
+    kc, ks = empty_cache(T, 1, D)
+    q8, w8 = indexer_qk_write(x, x[:, 0], w, None, None, torch.arange(T, device="cuda", dtype=torch.int32), kc[:, 0], ks[:, 0].contiguous(),
+                              k_norm=None)
+    ref.check_quantised(q8, w8.double() / w.double(), y, e * 0 + U(y))

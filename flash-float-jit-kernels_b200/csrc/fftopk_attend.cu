@@ -459,7 +459,11 @@ __global__ void __launch_bounds__(kThreads, 2) attend_narrow_kernel(const __grid
 }
 
 DeviceOnce g_attend_once[kMaxDevices];
-int g_attend_sms[kMaxDevices];
+struct Limits {
+  int sms = 0;
+  int narrow_eights = 0, wide_eights = 0;  // clusters of eight CTAs the device holds at once
+};
+Limits g_attend_limits[kMaxDevices];
 
 template <typename T, bool kFp8, int D>
 int setup_one() {
@@ -468,13 +472,18 @@ int setup_one() {
   return e == cudaSuccess ? 0 : cuda_fail(e);
 }
 
-int attend_setup(int& sms) {
+template <typename T, bool kFp8, int D>
+int eights_of(int& clusters) {
+  return clusters_of(clusters, attend_narrow_kernel<T, kFp8, D>, kThreads, narrow_smem_bytes<kFp8, D>());
+}
+
+int attend_setup(Limits& limits) {
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e);
   if (dev < 0 || dev >= kMaxDevices) return FFTOPK_EDEVICE;
   const int rc = g_attend_once[dev].run([&] {
-    const cudaError_t e2 = cudaDeviceGetAttribute(&g_attend_sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    const cudaError_t e2 = cudaDeviceGetAttribute(&g_attend_limits[dev].sms, cudaDevAttrMultiProcessorCount, dev);
     if (e2 != cudaSuccess) return cuda_fail(e2);
     int r = setup_one<__nv_bfloat16, false, 64>();
     if (!r) r = setup_one<__nv_bfloat16, false, 128>();
@@ -484,10 +493,11 @@ int attend_setup(int& sms) {
     if (!r) r = setup_one<__half, false, 128>();
     if (!r) r = setup_one<__half, true, 64>();
     if (!r) r = setup_one<__half, true, 128>();
-    if (!r) r = attend_wide_setup();
+    if (!r) r = eights_of<__nv_bfloat16, false, 128>(g_attend_limits[dev].narrow_eights);
+    if (!r) r = attend_wide_setup(g_attend_limits[dev].wide_eights);
     return r;
   });
-  sms = g_attend_sms[dev];
+  limits = g_attend_limits[dev];
   return rc;
 }
 
@@ -545,9 +555,10 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
                                                       reinterpret_cast<uintptr_t>(a->v_scale)) & 3u))
     return FFTOPK_EINVAL;
   if (a->slots > 0x7fffffff || a->tokens > 0x7fffffff) return FFTOPK_ERANGE;
-  int sms = 0;
-  const int rc = attend_setup(sms);
+  Limits limits;
+  const int rc = attend_setup(limits);
   if (rc) return rc;
+  const int sms = limits.sms;
 
   AttendParams p;
   memset(&p, 0, sizeof(p));
@@ -560,7 +571,13 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   p.out = a->out, p.out_token = a->out_token, p.out_head = a->out_head, p.lse = a->lse;
   p.slots = a->slots;
   p.tokens = (int32_t)a->tokens, p.kv_heads = a->kv_heads, p.group = a->q_heads / a->kv_heads, p.picks = a->picks;
-  const bool wide = p.group > kHeadsM;
+  // Which kernel. Up to 16 heads fill a row block of the narrow one, which reads each row once then (64 tokens, 4 key heads of 16
+  // heads: bf16 51 us, the wide one 66; e4m3 45 and 87). Beyond that the narrow kernel reads every row again for each 16 heads: the wide
+  // one takes over - but for e4m3 up to 32 heads (512 tokens of 32 heads: narrow 143, wide 172; of 64 heads, 64 tokens: 44 and 33), and
+  // where there is so little work that the narrow kernel can give every piece of it four CTAs (128 heads: 1 token 8.8 and 15.9, 8
+  // tokens 15.9 and 15.9, 32 tokens 39 and 20).
+  const int64_t narrow_units = a->tokens * a->kv_heads * ((p.group + kHeadsM - 1) / kHeadsM);
+  const bool wide = p.group > kHeadsM && !(fp8 && p.group <= 2 * kHeadsM) && narrow_units * 4 > 2 * (int64_t)sms;
   const int rows = wide ? 128 : kHeadsM;
   p.head_blocks = (p.group + rows - 1) / rows;
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
@@ -571,8 +588,9 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   const int64_t units = a->tokens * p.kv_heads * p.head_blocks;
   const int keys = wide ? 128 : kWarps * (fp8 ? 32 : 16);
   int ctas = 1;
-  const int64_t room = wide ? sms : 2 * (int64_t)sms;
-  while (ctas < kAttendMaxCluster && units * ctas * 2 <= room && (int64_t)ctas * keys < p.picks) ctas *= 2;
+  // (clusters of eight fit in fewer places than their CTAs alone: 16 of the wide kernel's took 26 us, eight 14)
+  const int64_t room = wide ? sms : 2 * (int64_t)sms, eights = wide ? limits.wide_eights : limits.narrow_eights;
+  while (ctas < kAttendMaxCluster && units * ctas * 2 <= room && (ctas * 2 < 8 || units <= eights) && (int64_t)ctas * keys < p.picks) ctas *= 2;
   if (units * ctas > 0x7fffffff) return FFTOPK_ERANGE;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   if (wide) {

@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "fftopk_host.h"
+
 namespace fftopk {
 
 struct AttendParams {
@@ -33,10 +35,27 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr int kAttendMaxCluster = 8;  // CTAs that share a token's keys: the portable cluster size
 
 // fftopk_attend_wide.cu; fp8: e4m3 caches; `units` pieces of work (token, key head, 128 query heads), `ctas` CTAs each
-int attend_wide_setup();
+int attend_wide_setup(int& eights);  // clusters of eight CTAs the device holds at once
 cudaError_t attend_wide(const AttendParams& p, bool bf16, bool fp8, int D, int ctas, int64_t units, int sms, cudaStream_t stream);
 
 #ifdef __CUDACC__
+// clusters of kAttendMaxCluster CTAs that the device holds at once
+template <typename F>
+int clusters_of(int& clusters, F kernel, int threads, size_t smem) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kAttendMaxCluster, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = kAttendMaxCluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+  return e == cudaSuccess ? 0 : cuda_fail(e);
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -967,7 +967,7 @@ cudaError_t launch_wide(const AttendParams& p, bool fp8, int D, int ctas, int64_
 
 }  // namespace
 
-int attend_wide_setup() {
+int attend_wide_setup(int& eights) {
   int r = setup_wide<__nv_bfloat16, false, 64>();
   if (!r) r = setup_wide<__nv_bfloat16, false, 128>();
   if (!r) r = setup_wide<__nv_bfloat16, true, 64>();
@@ -976,6 +976,7 @@ int attend_wide_setup() {
   if (!r) r = setup_wide<__half, false, 128>();
   if (!r) r = setup_wide<__half, true, 64>();
   if (!r) r = setup_wide<__half, true, 128>();
+  if (!r) r = clusters_of(eights, attend_wide_kernel<__nv_bfloat16, false, 128>, kWideThreads, wide_smem_bytes<false, 128>());
   return r;
 }
 

@@ -3,8 +3,10 @@
 // g query heads to a key head, negative indices left out, a token that names none gets zeros and a log-sum of -inf.
 // k and v are of q's type, or e4m3 with a 32-bit scale per row and head. (The reference ends with the indices.)
 //
-// attend_narrow_kernel, up to 16 query heads to a key head at a time. A row of k or v is used by those heads alone, so reading
-// the rows bounds it: 16 flop a byte at most in 16 bits, 32 in fp8, where the tensor cores want over 200. The rows lie anywhere,
+// attend_narrow_kernel, up to 16 query heads to a key head at a time (which calls take it: see fftopk_sparse_attention below). A row of
+// k or v is used by those heads alone, so reading the rows bounds it: 16 flop a byte at most in 16 bits, 32 in fp8, where the tensor
+// cores want over 200 (64 tokens, 64 heads on 8 key heads, 2,048 picks: bf16 98 us = 5.5 TB/s; e4m3 85 us, where widening codes and
+// pairing rows take half of the ALU). The rows lie anywhere,
 // and nothing but their own heads shares them: every warp has a ring of its own in shared memory that cp.async fills, blocks of 16
 // (e4m3: 32) keys ahead of the one it works on, and waits for no other warp.
 //   q.k: the contraction's order is free, so a lane's 16-byte piece of a key row serves as B fragments of consecutive steps
@@ -15,8 +17,8 @@
 // tokens: a token's keys are split over up to 8 CTAs) through distributed shared memory. No workspace.
 //   e4m3 rows are widened to fp16, which holds every code exactly; a row's k scale multiplies its score, its v scale its weight.
 //   Queries are brought to magnitudes below 2 by a power of two per head first (fp16 has fewer exponents than bf16; what is
-//   lost lies 2^-25 below the head's largest). Weights p * v scale become fp16 relative to the largest v scale seen: 2^-12 of a
-//   weight's size, 2^-25 of the largest for the smallest ones. 16-bit caches: weights are rounded to the cache's type.
+//   lost lies 2^-25 below the head's largest). Weights p * v scale become fp16 relative to a v scale that is let
+//   stand until one exceeds it 2^6 times: off by 2^-11 of a weight's size, by 2^-25 of that scale for the smallest ones. 16-bit caches: weights are rounded to the cache's type.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -1,5 +1,5 @@
-// Attention over selected rows for more than 16 query heads to a key head: the tensor cores' share of fftopk_attend.cu (the
-// formulas stand there).
+// Attention over selected rows for many query heads to a key head: the tensor cores' share of fftopk_attend.cu (the formulas, and
+// which calls come here, stand there).
 //
 // 128 query heads use a row of k and v here, 2 * 2 * 128 flop per element: in 16 bits as many flop per byte as the device has
 // (250), in fp8 and wherever tokens share rows out of L2 twice that and more. So the products run on tcgen05, one CTA per SM:
@@ -9,10 +9,14 @@
 // 20 warps: two groups of four softmax warps, one thread per head, that take alternate tiles of keys, each with an S, an O and a
 // running maximum of its own, so that one group's exponentials run while the other's products do; one that looks up which rows
 // the tiles to come are made of (and, fp8, their scales) and hands them out as a stream of TileMeta; four that gather k rows and
-// four that gather v rows; two that bring the queries of the next piece of work; and one thread that issues the MMAs: QK of
-// tile n + 1, then PV of tile n. The rows lie anywhere: 16-bit ones are copied with cp.async, e4m3 ones go through registers and
-// are widened to fp16 on the way (eight 16-byte loads a thread in flight: as a piece is widened the next tile's takes its
-// registers). Rows that are not there are zeros, and masked in S.
+// four that gather v rows; two that bring the queries of the next piece of work; and one thread that issues the MMAs, whichever
+// are ready: QK of a tile as soon as PV of the tile two before it has been issued, PV in halves of a tile's keys. The rows lie
+// anywhere: 16-bit ones are copied into their tile with cp.async; e4m3 codes into a ring of the gathering warp's own, which widens
+// them to fp16 in the tile. Rows that are not there are zeros, and masked in S.
+//
+// What bounds it (1,024 tokens of 128 heads on one key head, 2,048 picks of 65,536 shared rows): bf16 205 us, 670 TFLOP/s, 2,000 to
+// 2,500 cycles a tile where its products take 1,030: softmax (1,024 cycles of exponentials a warp) and the rows' way out of L2 take turns at
+// being late. e4m3 345 us: 8,800 warp instructions a tile where bf16 has 6,050 - the scales in softmax, and widening the codes.
 //
 // A row's maximum is let stand until a score exceeds it by 2^8 (fp16 and 32-bit sums have the room), so O, which lives in tensor
 // memory, is hardly ever rescaled. fp8: the k scales multiply S, the v scales P, relative to a power of two near the largest v scale that is

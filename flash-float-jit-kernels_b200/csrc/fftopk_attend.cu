@@ -18,7 +18,8 @@
 //   e4m3 rows are widened to fp16, which holds every code exactly; a row's k scale multiplies its score, its v scale its weight.
 //   Queries are brought to magnitudes below 2 by a power of two per head first (fp16 has fewer exponents than bf16; what is
 //   lost lies 2^-25 below the head's largest). Weights p * v scale become fp16 relative to a v scale that is let
-//   stand until one exceeds it 2^6 times: off by 2^-11 of a weight's size, by 2^-25 of that scale for the smallest ones. 16-bit caches: weights are rounded to the cache's type.
+//   stand until one exceeds it 2^6 times: off by 2^-11 of a weight's size, by 2^-25 of that scale for the smallest ones.
+//   16-bit caches: weights are rounded to the cache's type.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -565,7 +566,8 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   AttendParams p;
   memset(&p, 0, sizeof(p));
   p.q = a->q, p.q_token = a->q_token, p.q_head = a->q_head;
-  p.k = a->k, p.v = a->v;
+  // (an empty cache has no address, and rows that are left out are copies of no bytes: from somewhere)
+  p.k = a->slots > 0 ? a->k : a->q, p.v = a->slots > 0 ? a->v : a->q;
   p.k_slot = a->k_slot, p.k_head = a->k_head, p.v_slot = a->v_slot, p.v_head = a->v_head;
   p.k_scale = a->k_scale, p.v_scale = a->v_scale;
   p.ks_slot = a->ks_slot, p.ks_head = a->ks_head, p.vs_slot = a->vs_slot, p.vs_head = a->vs_head;

@@ -4,9 +4,10 @@ import pytest
 import torch
 
 import rows_ref as ref
+from jit_kernel import _native
 from jit_kernel.kv_cache import cache_read, cache_write
 from jit_kernel.sparse_attention import sparse_attention
-from test_sparse_attention_gpu import FP8, gen, make_cache, make_indices, rand, status  # noqa: F401
+from test_sparse_attention_gpu import FP8, gen, make_cache, make_indices, rand, status, take_status  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -89,6 +90,12 @@ def test_nothing_to_attend_to(Hq):
             idx = torch.full((3, K), -1, device="cuda", dtype=torch.int32)
             out, lse = sparse_attention(q, c, c, idx, k_scale=s, v_scale=s, return_lse=True)
             assert bool((out == 0).all()) and bool(lse.isneginf().all())
+            if K:
+                many = torch.ones(60, Hq, 64, device="cuda", dtype=torch.bfloat16)
+                for x in (q, many):
+                    out, lse = sparse_attention(x, c, c, idx[:1].abs().expand(x.size(0), K), k_scale=s, v_scale=s, return_lse=True)
+                    assert take_status() == _native.ST_BAD_INDEX
+                    assert bool((out == 0).all()) and bool(lse.isneginf().all())
     assert bool((cache_read(c, s, torch.full((4,), -1, device="cuda", dtype=torch.int32)) == 0).all())
     cache_write(q[:, :1], torch.full((3,), -1, device="cuda", dtype=torch.int32), c, s)
 
@@ -158,8 +165,6 @@ def test_many_tokens(dtype, fp8, D, T, Hq, Hk):
 @pytest.mark.parametrize("T", [12, 170])
 def test_many_tokens_with_anything(T, fp8):
     """Far scores, negative and zero softmax scales, NaN rows, indices beyond the cache, an output with gaps."""
-    from jit_kernel import _native
-    from test_sparse_attention_gpu import take_status
     g = gen(31)
     q, k, v, ks, vs = case(g, T, 128, 1, 600, 900, fp8)
     idx = make_indices(g, T, 600, 800)

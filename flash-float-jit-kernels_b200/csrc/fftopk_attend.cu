@@ -41,10 +41,13 @@ namespace {
 namespace cg = cooperative_groups;
 
 // Four warps, two CTAs per SM: while one CTA starts or joins, the other one streams (64 tokens, 8 key heads, bf16: 98 us; eight warps
-// and one CTA per SM: 108)
+// and one CTA per SM: 108). Heads of 64 hold half the accumulators and half the ring: three CTAs per SM, with rings of three stages
+// (61 tokens of 3 key heads, fp16: 14.8 us, two CTAs with four stages 18.3; e4m3: 15.0 and 17.4. 512 tokens of 2 key heads, bf16: 82 and
+// 102; e4m3: 82 and 92. 64 tokens of 8 key heads, whose 512 CTAs make a second wave of either: 75 and 72; 57 and 56)
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kHeadsM = 16;  // query heads a CTA works on: rows of the MMA
+constexpr int sm_ctas(int D) { return D == 64 ? 3 : 2; }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -92,7 +95,7 @@ struct Ring {
   static constexpr int kKPitch = kRowBytes == 64 ? 64 : kRowBytes + 64, kVPitch = kRowBytes + 16;
   static constexpr int kV = kKeys * kKPitch, kScales = kV + kKeys * kVPitch;
   static constexpr int kStage = kScales + (kFp8 ? 2 * kKeys * 4 : 0);
-  static constexpr int kStages = D == 64 ? 4 : kFp8 ? 2 : 3;
+  static constexpr int kStages = kFp8 && D != 64 ? 2 : 3;
   static constexpr int kBytes = kStages * kStage;  // of a warp
 };
 // Shared memory of a CTA: the warps' rings; in their place, in the end, the warps' accumulators, maxima, sums, and joined the CTA's own.
@@ -110,7 +113,7 @@ constexpr size_t narrow_smem_bytes() {
 
 // T: type of q and out, and of the cache where kFp8 is false
 template <typename T, bool kFp8, int D>
-__global__ void __launch_bounds__(kThreads, 2) attend_narrow_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(const __grid_constant__ AttendParams p) {
   using M = typename std::conditional<kFp8, __half, T>::type;  // the MMAs' type
   constexpr int kCE = kFp8 ? 16 : 8;                            // elements of a 16-byte piece
   constexpr int kPieces = D / (4 * kCE);                        // pieces of a key row per lane (a quad reads a row)
@@ -593,7 +596,7 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   const int keys = wide ? 128 : kWarps * (fp8 ? 32 : 16);
   int ctas = 1;
   // (clusters of eight fit in fewer places than their CTAs alone: 16 of the wide kernel's took 26 us, eight 14)
-  const int64_t room = wide ? sms : 2 * (int64_t)sms, eights = wide ? limits.wide_eights : limits.narrow_eights;
+  const int64_t room = wide ? sms : sm_ctas(a->D) * (int64_t)sms, eights = wide ? limits.wide_eights : limits.narrow_eights;
   while (ctas < kAttendMaxCluster && units * ctas * 2 <= room && (ctas * 2 < 8 || units <= eights) && (int64_t)ctas * keys < p.picks) ctas *= 2;
   if (units * ctas > 0x7fffffff) return FFTOPK_ERANGE;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);

@@ -17,8 +17,9 @@
 // tokens: a token's keys are split over up to 8 CTAs) through distributed shared memory. No workspace.
 //   e4m3 rows are widened to fp16, which holds every code exactly; a row's k scale multiplies its score, its v scale its weight.
 //   Queries are brought to magnitudes below 2 by a power of two per head first (fp16 has fewer exponents than bf16; what is
-//   lost lies 2^-25 below the head's largest). Weights p * v scale become fp16 relative to a v scale that is let
-//   stand until one exceeds it 2^6 times: off by 2^-11 of a weight's size, by 2^-25 of that scale for the smallest ones.
+//   lost lies 2^-25 below the head's largest). What a row adds is p * |v scale|, so that is what the running maximum is of:
+//   weights p * v scale become fp16 relative to the head's largest of them, off by 2^-11 of their size, the smallest ones by 2^-25
+//   of that largest; a large v scale with hardly any weight behind it sets nothing. Sums of p are held against the same reference.
 //   16-bit caches: weights are rounded to the cache's type.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -180,8 +181,8 @@ __global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(con
   float o[kTiles][4];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  // what weights are taken against (log2): the largest score; fp8: the largest score + log2 |v scale|, by the scale's exponent
   float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-  float vref = 0.f;  // fp8: the largest v scale seen; weights are relative to it
 
   const int32_t* idx = p.indices + (int64_t)token * p.idx_row;
   const int64_t offset = p.offsets != nullptr ? p.offsets[token] : 0;
@@ -246,10 +247,11 @@ __global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(con
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) live_of[s] = live_of[s + 1];
     if (live == 0u) continue;
-    float ks = 0.f, vs = 0.f;  // the scales of the lane's key
+    float ks = 0.f, vs = 0.f, vlog = 0.f;  // the scales of the lane's key
     if constexpr (kFp8) {
       const float2 both = lds8(stage + (uint32_t)(G::kScales + lane * 8));
       ks = both.x, vs = both.y;
+      vlog = scale_log2(vs);
     }
     // scores, in units of log2
     float sc[kSub * 2][4];
@@ -276,53 +278,39 @@ __global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(con
 #pragma unroll
     for (int n = 0; n < kSub * 2; ++n) {
       const unsigned mask = live >> (n * 8 + 2 * qd);
-      float k0 = 1.f, k1 = 1.f;
+      float k0 = 1.f, k1 = 1.f, l0 = 0.f, l1 = 0.f;
       if constexpr (kFp8) {
         k0 = __shfl_sync(kAll, ks, n * 8 + 2 * qd);
         k1 = __shfl_sync(kAll, ks, n * 8 + 2 * qd + 1);
+        l0 = __shfl_sync(kAll, vlog, n * 8 + 2 * qd);
+        l1 = __shfl_sync(kAll, vlog, n * 8 + 2 * qd + 1);
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         sc[n][2 * r] = (mask & 1u) ? sc[n][2 * r] * k0 * qmul[r] : -INFINITY;
         sc[n][2 * r + 1] = (mask & 2u) ? sc[n][2 * r + 1] * k1 * qmul[r] : -INFINITY;
-        bmax[r] = fmaxf(bmax[r], fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
+        bmax[r] = fmaxf(bmax[r], kFp8 ? fmaxf(sc[n][2 * r] + l0, sc[n][2 * r + 1] + l1) : fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
       }
     }
     // (a reference is let stand until a score exceeds it by 2^8: fp16 weights and 32-bit sums have the room)
-    float grow[2];
+    float grow[2], was[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float top = quad_max(bmax[r]);
       const float m = top > mx[r] + 8.f ? top : mx[r];
       grow[r] = mx[r] == m ? 1.f : ex2(mx[r] - m);  // (-inf both: nothing seen yet)
+      was[r] = mx[r];
       mx[r] = m;
     }
-    if constexpr (kFp8) {
-      float top = fabsf(vs);
+    if (__any_sync(kAll, grow[0] != 1.f || grow[1] != 1.f)) {
 #pragma unroll
-      for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, i));
-      const float ref = top > 64.f * vref ? top : vref;  // (let stand likewise, up to 2^6: weights stay below 2^14)
-      const float f = ref > vref ? vref / ref : 1.f;
-      vref = ref;
-      vs = ref > 0.f ? vs / ref : 0.f;
-      if (__any_sync(kAll, grow[0] != 1.f || grow[1] != 1.f || f != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          o[i][0] *= grow[0] * f, o[i][1] *= grow[0] * f;
-          o[i][2] *= grow[1] * f, o[i][3] *= grow[1] * f;
-        }
+      for (int i = 0; i < kTiles; ++i) {
+        o[i][0] *= grow[0], o[i][1] *= grow[0];
+        o[i][2] *= grow[1], o[i][3] *= grow[1];
       }
-    } else {
-      if (__any_sync(kAll, grow[0] != 1.f || grow[1] != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          o[i][0] *= grow[0], o[i][1] *= grow[0];
-          o[i][2] *= grow[1], o[i][3] *= grow[1];
-        }
-      }
+      if constexpr (kFp8) sum[0] = brought(sum[0], was[0], mx[0]), sum[1] = brought(sum[1], was[1], mx[1]);
     }
-    sum[0] *= grow[0];
-    sum[1] *= grow[1];
+    if constexpr (!kFp8) sum[0] *= grow[0], sum[1] *= grow[1];
     uint32_t pa[kSub][4];
 #pragma unroll
     for (int n = 0; n < kSub * 2; ++n) {
@@ -395,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(con
       // which column tile t of lane n stands for: see the value pieces above
       const int n = 2 * qd + (e & 1);
       const int col = kFp8 ? n * (kVWords * 4) + t : (t >> 3) * 64 + n * 8 + (t & 7);
-      sm.o[warp][g + 8 * (e >> 1)][col] = kFp8 ? o[t][e] * vref : o[t][e];
+      sm.o[warp][g + 8 * (e >> 1)][col] = o[t][e];
     }
   }
   __syncthreads();
@@ -409,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(con
     for (int w = 0; w < kWarps; ++w) {
       const float f = sm.m[w][h] == m ? 1.f : ex2(sm.m[w][h] - m);  // (a warp without keys: 0 of both; 0 * NaN stays NaN)
       acc += f * sm.o[w][h][d];
-      l += f * sm.l[w][h];
+      l += kFp8 ? brought(sm.l[w][h], sm.m[w][h], m) : f * sm.l[w][h];
     }
     sm.joined[h][d] = acc;
     if (d == 0) sm.jml[h] = make_float2(m, l);
@@ -446,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(con
         if (c < ctas) {
           const float f = ml[c].x == m ? 1.f : ex2(ml[c].x - m);
           o.x += f * part[c].x, o.y += f * part[c].y, o.z += f * part[c].z, o.w += f * part[c].w;
-          l += f * ml[c].y;
+          l += kFp8 ? brought(ml[c].y, ml[c].x, m) : f * ml[c].y;
         }
       }
     }

@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(con
     if constexpr (kFp8) {
       const float2 both = lds8(stage + (uint32_t)(G::kScales + lane * 8));
       ks = both.x, vs = both.y;
-      vlog = scale_log2(vs);
+      vlog = (float)scale_exponent(vs);
     }
     // scores, in units of log2
     float sc[kSub * 2][4];

@@ -62,9 +62,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 // exponent of a v scale of either sign, within +-100 (sums of weights that are held against it have the room)
-__device__ __forceinline__ float scale_log2(float scale) {
-  return (float)max(-100, min((int)(__float_as_uint(scale) >> 23 & 255u) - 127, 100));
-}
+__device__ __forceinline__ int scale_exponent(float scale) { return max(-100, min((int)(__float_as_uint(scale) >> 23 & 255u) - 127, 100)); }
 // A sum of weights held against 2^from, against 2^to, with v scales in the references: scales of 2^-100 and 2^100 in a list make the
 // sum as far from 1 as the factor is, the other way, so it comes in halves.
 __device__ __forceinline__ float brought(float sum, float from, float to) {

@@ -19,9 +19,10 @@
 // being late. e4m3 345 us: 8,800 warp instructions a tile where bf16 has 6,050 - the scales in softmax, and widening the codes.
 //
 // A row's maximum is let stand until a score exceeds it by 2^8 (fp16 and 32-bit sums have the room), so O, which lives in tensor
-// memory, is hardly ever rescaled. fp8: the k scales multiply S, the v scales P, relative to a power of two near the largest v scale that is
-// let stand likewise: it is part of the reference the exponentials are taken against. At the end the groups' O are added, row by
-// row, with the factors their maxima give.
+// memory, is hardly ever rescaled. fp8: the k scales multiply S, the v scales P, and the reference is the largest score + log2 |v scale|, what a row adds
+// being its weight times its scale; where a tile's v scales lie within 2^kEvenLog the largest of them stands for all, which
+// saves looking at them one by one (1,024 tokens of 128 heads: 332 us, 356 with scales further apart). At the end the groups' O are
+// added, row by row, with the factors their references give.
 // A CTA takes one piece of work after the other (token, key head, 128 query heads), and its gathering warps run ahead into the next
 // one. Few tokens: the CTAs of a cluster take every n-th tile, and join through distributed shared memory.
 // Every wait on an mbarrier has a time limit; when one runs out the CTA raises FFTOPK_ST_STAGE_TIMEOUT and winds down.
@@ -63,6 +64,7 @@ __device__ __forceinline__ void fewer_registers() {
 }
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLetStand = 8.f;  // log2 by which a score may exceed the reference
+constexpr int kEvenLog = 4;       // weights may be smaller than the reference says by that many bits: of the 25 that fp16 reaches down
 
 // What lies in shared memory beside the query tile: k and v tiles as the MMAs read them; and, e4m3, every gathering warp's share of
 // the codes of tiles on their way.
@@ -82,13 +84,13 @@ constexpr int kChunk = 64;    // scores of a row that a softmax thread works on 
 constexpr int kMeta = 4;      // tiles the scout is ahead at most; a place is free again when its tile's PV is done
 constexpr int kPauseNs = 64;  // of the thread that issues the MMAs, between two looks at what it waits for
 constexpr int kInfo = 4;      // pieces of work it is ahead
-constexpr int kLast = 1, kEnd = 2, kWhole = 4, kSeen = 8;
+constexpr int kLast = 1, kEnd = 2, kWhole = 4, kSeen = 8, kEven = 16;
 struct TileMeta {             // a tile of 128 keys
   int64_t k_at[kTileKeys], v_at[kTileKeys];  // byte offsets of the rows in the caches; negative: none
-  float ks[kTileKeys], vs[kTileKeys];
+  float ks[kTileKeys], vs[kTileKeys], vlog[kTileKeys];  // vlog: the v scales' exponents
   uint32_t live[4];
-  float vtop;                 // largest v scale
-  int32_t flags;              // last tile of its piece of work; end of the stream (no tile); all rows are there
+  float vmost;                // the largest of them
+  int32_t flags;              // last tile of its piece of work; end of the stream (no tile); all rows are there; their v scales are alike
   int32_t kvh;
 };
 template <bool kFp8, int D>
@@ -221,6 +223,19 @@ __device__ __forceinline__ float top_of(const float (&s)[kChunk]) {
   for (int i = 8; i < kChunk; i += 8) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(s[i + 2 * e], s[i + 2 * e + 1]));
+  }
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+// the largest of them, times qmul, with their rows' v scales
+__device__ __forceinline__ float top_with(const float (&s)[kChunk], float qmul, const float* vlog) {
+  const Pair mul = pair(qmul, qmul);
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < kChunk; i += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(vlog + i);
+    const float2 a = apart(fma2(pair(s[i], s[i + 1]), mul, pair(x.x, x.y))), b = apart(fma2(pair(s[i + 2], s[i + 3]), mul, pair(x.z, x.w)));
+    top[0] = fmaxf(top[0], a.x), top[1] = fmaxf(top[1], a.y), top[2] = fmaxf(top[2], b.x), top[3] = fmaxf(top[3], b.y);
   }
   return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
@@ -477,7 +492,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           rows_of(next_row, next_ks, next_vs, now);
           if (!(ok = __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)))) break;
           TileMeta& m = sm.meta[n % kMeta];
-          float top = 0.f;
+          int most = -100, least = 100;  // exponents of the v scales (16 bits: none)
           unsigned whole = kAll;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -489,16 +504,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             if constexpr (kFp8) {
               m.ks[i * 32 + lane] = ks[i];
               m.vs[i * 32 + lane] = vs[i];
-              top = fmaxf(top, fabsf(vs[i]));
+              const int e = scale_exponent(vs[i]);
+              m.vlog[i * 32 + lane] = (float)e;
+              if (row[i] >= 0) most = max(most, e), least = min(least, e);
             }
           }
-          if constexpr (kFp8) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
-          }
+          if constexpr (kFp8) most = __reduce_max_sync(kAll, most), least = __reduce_min_sync(kAll, least);
           if (lane == 0) {
-            m.vtop = top;
-            m.flags = (j == nt - 1 ? kLast : 0) | (whole == kAll ? kWhole : 0);
+            m.flags = (j == nt - 1 ? kLast : 0) | (whole == kAll ? kWhole : 0) | (kFp8 && most - least <= kEvenLog ? kEven : 0);
+            if constexpr (kFp8) m.vmost = (float)most;
             m.kvh = w.kvh;
           }
           __syncwarp();
@@ -693,7 +707,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         }
         continue;
       }
-      float ref = -INFINITY, vlog = 0.f, sum = 0.f;
+      float ref = -INFINITY, sum = 0.f;
       for (int j = g ^ (int)(it & 1u); j < nt; j += 2) {
         const uint32_t n = it + (uint32_t)j;
         const int place = (int)(n % kMeta);
@@ -711,12 +725,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           const float qmul = sm.qmul[wn & 3u][r];
           // A new reference: what was weighed with the old one - O up to the tile before, or with the first half of this one's keys
           // where that has been handed over, and the sum - is brought to it.
-          auto refer = [&](float next, float vnext, bool half) {
-            const bool changed = next != ref || vnext != vlog;
-            const float f = !changed ? 1.f : ref == -INFINITY ? (next == -INFINITY ? 1.f : 0.f) : ex2((ref + vlog) - (next + vnext));
+          auto refer = [&](float next, bool half) {
+            const float f = next == ref ? 1.f : ex2(ref - next);
+            sum = kFp8 ? brought(sum, ref, next) : sum * f;
             ref = next;
-            vlog = vnext;
-            sum *= f;
             if (half || j > 1) {
               uint64_t* const bar = half ? &sm.halfdone[g] : &sm.pvdone[(n - 2u) % kMeta];
               if (!__all_sync(kAll, mbar_wait(bar, half ? (n >> 1) & 1u : ((n - 2u) / kMeta) & 1u, abort_flag))) return;  // (the waits to come fail too)
@@ -732,14 +744,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
               }
             }
           };
-          if constexpr (kFp8) {  // the exponent of the largest v scale
-            const int e = (int)(__float_as_uint(m.vtop) >> 23) - 127;
-            const float ve = (float)max(-100, min(e, 100));
-            if (j < 2)
-              vlog = ve;
-            else if (ve > vlog + 6.f)
-              refer(ref, ve, false);
-          }
           const bool whole = (m.flags & kWhole) != 0;
           Pair part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
           auto parts = [&] {
@@ -769,12 +773,18 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
                   if (!(there >> i & 1u)) s[32 * b + i] = -INFINITY;
               }
             }
-            const float top = top_of(s) * qmul;
+            float top;
+            if (!kFp8)
+              top = top_of(s) * qmul;
+            else if (m.flags & kEven)
+              top = fmaf(top_of(s), qmul, m.vmost);
+            else
+              top = top_with(s, qmul, m.vlog + kChunk * c);
             if (__any_sync(kAll, top > ref + kLetStand)) {
               sum += parts();
-              refer(top > ref + kLetStand ? top : ref, vlog, c > 0);
+              refer(top > ref + kLetStand ? top : ref, c > 0);
             }
-            const float sub = (ref == -INFINITY ? 0.f : ref) + vlog;
+            const float sub = ref == -INFINITY ? 0.f : ref;
             const Pair mul = pair(qmul, qmul), less = pair(-sub, -sub);
             uint32_t pk[kChunk / 2];
 #pragma unroll
@@ -808,7 +818,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       const int nga = (nt + 1 - (int)(it & 1u)) / 2, ngb = nt - nga;  // tiles of group 0, of group 1
       float2 a = make_float2(-INFINITY, 0.f), b = a;
       if (nt > 0) {
-        sm.ml[wn & 1u][g][r] = make_float2(ref == -INFINITY ? -INFINITY : ref + vlog, sum);
+        sm.ml[wn & 1u][g][r] = make_float2(ref + 0.f, sum);  // (+ 0: without it heads of 64 in 16 bits spill 36 bytes instead of 8, 173 us instead of 169)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.mlbar);
         ok = mbar_wait(&sm.mlbar, wn & 1u, abort_flag);
@@ -821,7 +831,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       }
       const float top = fmaxf(a.x, b.x);
       const float fa = a.x == top ? 1.f : ex2(a.x - top), fb = b.x == top ? 1.f : ex2(b.x - top);
-      const float l = fa * a.y + fb * b.y;
+      const float l = kFp8 ? brought(a.y, a.x, top) + brought(b.y, b.x, top) : fa * a.y + fb * b.y;
       const float inv = ctas > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       float* const stage_row = reinterpret_cast<float*>(base) + (size_t)r * (D + 4) + g * kHalf;  // (several CTAs: over the q and k tiles)
       uint32_t packed[kHalf / 2];  // (the pieces of work to come may have O as soon as it has been read)
@@ -920,7 +930,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       for (int c = 0; c < kAttendMaxCluster; ++c) {
         if (c < ctas) {
           const float f = ml[c].x == top ? 1.f : ex2(ml[c].x - top);
-          l += f * ml[c].y;
+          l += kFp8 ? brought(ml[c].y, ml[c].x, top) : f * ml[c].y;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) acc[e] += f * o[c][e];
         }

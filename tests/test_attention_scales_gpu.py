@@ -128,3 +128,14 @@ CASES = [one_row_without_weight, scales_against_scores, rows_of_zeros]
 @pytest.mark.parametrize("case", CASES)
 def test_scales_few_tokens(case, dtype, D, T, Hq, Hk):
     case(gen(T * Hq + D), T, Hq, Hk, D, dtype)
+
+
+MANY = [(12, 128, 1), (170, 100, 1), (40, 64, 2)]  # enough tokens for the kernel of 128 heads: keys split over CTAs, and not
+
+
+@pytest.mark.parametrize("T,Hq,Hk", MANY)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", CASES)
+def test_scales_many_heads(case, dtype, D, T, Hq, Hk):
+    case(gen(T * Hq + D), T, Hq, Hk, D, dtype)

@@ -529,6 +529,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       // ---- queries: two warps, 64 rows each ----
       const float negative = p.scale_log2 < 0.f ? -1.f : 1.f;
       const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale turns q: the largest score is then the largest here)
+      const uint32_t none = p.scale_log2 != p.scale_log2 ? 0x7fff7fffu : 0u;  // (a scale that is NaN makes q NaN: scores are, masked ones are not)
       constexpr int kQLanes = D / 8, kQOnce = 32 / kQLanes, kTurns = 64 / kQOnce, kBatch = 8;
       // (the piece of work to come: its rows are brought to L2 while this one's keys go by)
       auto prefetch = [&](uint32_t unit) {
@@ -578,7 +579,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
               v = make_uint4(narrow2(a.x * down, a.y * down, __half()), narrow2(b2.x * down, b2.y * down, __half()),
                              narrow2(d.x * down, d.y * down, __half()), narrow2(e.x * down, e.y * down, __half()));
             }
-            put16(chunk_at(q_tiles + (wn % kQTiles) * kTileBytes, h, c), v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+            put16(chunk_at(q_tiles + (wn % kQTiles) * kTileBytes, h, c), (v.x ^ flip) | none, (v.y ^ flip) | none, (v.z ^ flip) | none, (v.w ^ flip) | none);
             if (c == 0) sm.qmul[wn & 3u][h] = fmaxf(mul, 1.17549435e-38f);  // (times a masked score it must stay -inf)
           }
         }

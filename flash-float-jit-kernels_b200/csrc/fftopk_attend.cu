@@ -3,7 +3,7 @@
 // g query heads to a key head, negative indices left out, a token that names none gets zeros and a log-sum of -inf.
 // k and v are of q's type, or e4m3 with a 32-bit scale per row and head. (The reference ends with the indices.)
 //
-// attend_narrow_kernel, up to 16 query heads to a key head at a time (which calls take it: see fftopk_sparse_attention below). A row of
+// attend_narrow_kernel, up to 16 query heads to a key head at a time (which calls take it: attend_is_wide in fftopk_decide.h). A row of
 // k or v is used by those heads alone, so reading the rows bounds it: 16 flop a byte at most in 16 bits, 32 in fp8, where the tensor
 // cores want over 200 (64 tokens, 64 heads on 8 key heads, 2,048 picks: bf16 98 us = 5.5 TB/s; e4m3 85 us, where widening codes and
 // pairing rows take half of the ALU). The rows lie anywhere,
@@ -33,6 +33,7 @@
 #include "fftopk_host.h"
 #include "fftopk_internal.h"
 #include "fftopk_attend.cuh"
+#include "fftopk_decide.h"
 #include "fftopk_rows.cuh"
 #include "fftopk_tcgen05.cuh"
 
@@ -47,7 +48,7 @@ namespace cg = cooperative_groups;
 // 102; e4m3: 82 and 92. 64 tokens of 8 key heads, whose 512 CTAs make a second wave of either: 75 and 72; 57 and 56)
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kHeadsM = 16;  // query heads a CTA works on: rows of the MMA
+constexpr int kHeadsM = kAttendHeads;  // query heads a CTA works on: rows of the MMA
 constexpr int sm_ctas(int D) { return D == 64 ? 3 : 2; }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
@@ -566,13 +567,7 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   p.out = a->out, p.out_token = a->out_token, p.out_head = a->out_head, p.lse = a->lse;
   p.slots = a->slots;
   p.tokens = (int32_t)a->tokens, p.kv_heads = a->kv_heads, p.group = a->q_heads / a->kv_heads, p.picks = a->picks;
-  // Which kernel. Up to 16 heads fill a row block of the narrow one, which reads each row once then (64 tokens, 4 key heads of 16
-  // heads: bf16 51 us, the wide one 66; e4m3 45 and 87). Beyond that the narrow kernel reads every row again for each 16 heads: the wide
-  // one takes over - but for e4m3 up to 32 heads (512 tokens of 32 heads: narrow 143, wide 172; of 64 heads, 64 tokens: 44 and 33), and
-  // where there is so little work that the narrow kernel can give every piece of it four CTAs (128 heads: 1 token 8.8 and 15.9, 8
-  // tokens 15.9 and 15.9, 32 tokens 39 and 20).
-  const int64_t narrow_units = a->tokens * a->kv_heads * ((p.group + kHeadsM - 1) / kHeadsM);
-  const bool wide = p.group > kHeadsM && !(fp8 && p.group <= 2 * kHeadsM) && narrow_units * 4 > 2 * (int64_t)sms;
+  const bool wide = attend_is_wide(a->tokens, a->kv_heads, p.group, fp8, sms);
   const int rows = wide ? 128 : kHeadsM;
   p.head_blocks = (p.group + rows - 1) / rows;
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;

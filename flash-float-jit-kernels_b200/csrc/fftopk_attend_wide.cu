@@ -1,5 +1,5 @@
-// Attention over selected rows for many query heads to a key head: the tensor cores' share of fftopk_attend.cu (the formulas, and
-// which calls come here, stand there).
+// Attention over selected rows for many query heads to a key head: the tensor cores' share of fftopk_attend.cu (the formulas
+// stand there; which calls come here: attend_is_wide in fftopk_decide.h).
 //
 // 128 query heads use a row of k and v here, 2 * 2 * 128 flop per element: in 16 bits as many flop per byte as the device has
 // (250), in fp8 and wherever tokens share rows out of L2 twice that and more. So the products run on tcgen05, one CTA per SM:

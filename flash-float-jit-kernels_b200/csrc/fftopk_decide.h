@@ -328,4 +328,20 @@ FFTOPK_DECIDE_HD bool tile_segment(uint32_t row_g0, uint32_t ntiles, uint32_t g,
   return true;
 }
 
+// ---------------------------------------------------------------------------------------------
+// Which kernel attention over selected rows goes to, of `group` query heads to a key head.
+// Up to 16 heads fill a row block of the narrow one, which reads each row once then (64 tokens, 4 key heads of 16
+// heads: bf16 51 us, the wide one 66; e4m3 45 and 87). Beyond that the narrow kernel reads every row again for each 16 heads: the wide
+// one takes over - but for e4m3 up to 32 heads (512 tokens of 32 heads: narrow 143, wide 172; of 64 heads, 64 tokens: 44 and 33), and
+// where there is so little work that the narrow kernel can give every piece of it four CTAs (128 heads: 1 token 8.8 and 15.9, 8
+// tokens 15.9 and 15.9, 32 tokens 39 and 20).
+// ---------------------------------------------------------------------------------------------
+constexpr int kAttendHeads = 16;  // query heads that the narrow kernel works on at a time
+FFTOPK_DECIDE_HD int64_t attend_narrow_units(int64_t tokens, int32_t kv_heads, int32_t group) {
+  return tokens * kv_heads * ((group + kAttendHeads - 1) / kAttendHeads);
+}
+FFTOPK_DECIDE_HD bool attend_is_wide(int64_t tokens, int32_t kv_heads, int32_t group, bool fp8, int32_t sms) {
+  return group > kAttendHeads && !(fp8 && group <= 2 * kAttendHeads) && attend_narrow_units(tokens, kv_heads, group) * 4 > 2 * (int64_t)sms;
+}
+
 }  // namespace fftopk

@@ -130,7 +130,7 @@ def test_scales_few_tokens(case, dtype, D, T, Hq, Hk):
     case(gen(T * Hq + D), T, Hq, Hk, D, dtype)
 
 
-MANY = [(12, 128, 1), (170, 100, 1), (40, 64, 2)]  # enough tokens for the kernel of 128 heads: keys split over CTAs, and not
+MANY = [(12, 128, 1), (170, 100, 1), (40, 128, 2)]  # enough tokens for the kernel of 128 heads: keys split over CTAs, and not
 
 
 @pytest.mark.parametrize("T,Hq,Hk", MANY)

@@ -29,6 +29,8 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <atomic>
+
 #include "../../include/fftopk.h"
 #include "fftopk_host.h"
 #include "fftopk_internal.h"
@@ -453,6 +455,9 @@ __global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(con
   if (ctas > 1) cluster.sync();  // (nobody leaves while its memory is read)
 }
 
+std::atomic<int64_t> g_wait_ns{(int64_t)kMbarWaitNs};
+std::atomic<uint32_t> g_stop_after{0xffffffffu};
+
 DeviceOnce g_attend_once[kMaxDevices];
 struct Limits {
   int sms = 0;
@@ -573,6 +578,8 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
   p.out_vec = on16(a->out, a->tokens, a->out_token, a->q_heads, a->out_head, 2);
   p.status = status;
+  p.wait_ns = (uint64_t)g_wait_ns.load(std::memory_order_relaxed);
+  p.stop_after = g_stop_after.load(std::memory_order_relaxed);
 
   // CTAs a token: as many as keep the device's SMs busy, and no more than give every warp (wide: every CTA) keys
   const int64_t units = a->tokens * p.kv_heads * p.head_blocks;
@@ -590,4 +597,11 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   const cudaError_t e = a->dtype == FFTOPK_DTYPE_BF16 ? launch_narrow<__nv_bfloat16>(p, fp8, a->D, ctas, units, stream)
                                                       : launch_narrow<__half>(p, fp8, a->D, ctas, units, stream);
   return e == cudaSuccess ? FFTOPK_OK : cuda_fail(e);
+}
+
+extern "C" int fftopk_set_attend_stop(int64_t wait_ns, int64_t tiles) {
+  if (wait_ns > (int64_t)kMbarWaitNs || tiles > 0x7fffffff) return FFTOPK_ERANGE;
+  g_wait_ns.store(wait_ns < 0 ? (int64_t)kMbarWaitNs : wait_ns, std::memory_order_relaxed);
+  g_stop_after.store(tiles < 0 ? 0xffffffffu : (uint32_t)tiles, std::memory_order_relaxed);
+  return FFTOPK_OK;
 }

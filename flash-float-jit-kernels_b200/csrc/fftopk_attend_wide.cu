@@ -25,7 +25,8 @@
 // added, row by row, with the factors their references give.
 // A CTA takes one piece of work after the other (token, key head, 128 query heads), and its gathering warps run ahead into the next
 // one. Few tokens: the CTAs of a cluster take every n-th tile, and join through distributed shared memory.
-// Every wait on an mbarrier has a time limit; when one runs out the CTA raises FFTOPK_ST_STAGE_TIMEOUT and winds down.
+// Every wait on an mbarrier has a time limit; when one runs out the CTA raises FFTOPK_ST_STAGE_TIMEOUT, writes NaN for what it has
+// not finished and winds down.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -317,10 +318,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     const int64_t head_bytes = (is_k ? p.k_head : p.v_head) * (kFp8 ? 1 : 2);
     const char* const src0 = static_cast<const char*>(is_k ? p.k : p.v) + piece * 16;
     auto posted = [&](uint32_t n) { return __all_sync(kAll, mbar_test(&sm.mfull[n % kMeta], (n / kMeta) & 1u)); };
-    auto wait_posted = [&](uint32_t n) { return __all_sync(kAll, mbar_wait(&sm.mfull[n % kMeta], (n / kMeta) & 1u, abort_flag)); };
+    auto wait_posted = [&](uint32_t n) { return __all_sync(kAll, mbar_wait(&sm.mfull[n % kMeta], (n / kMeta) & 1u, abort_flag, p.wait_ns)); };
     auto wait_empty = [&](uint32_t n) {
       const uint32_t of = n - stages;
-      return n < stages || __all_sync(kAll, mbar_wait(&empty[of % ring], (of / ring) & 1u, abort_flag));
+      return n < stages || __all_sync(kAll, mbar_wait(&empty[of % ring], (of / ring) & 1u, abort_flag, p.wait_ns));
     };
     auto is_empty = [&](uint32_t n) {
       const uint32_t of = n - stages;
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         // (several CTAs a token: tiles without a row cost less than looking for the last)
         const int all = ctas > 1 ? (p.picks + kTileKeys - 1) / kTileKeys : tiles_of(idx, p.picks, lane);
         const int nt = all > rank ? (all - rank + ctas - 1) / ctas : 0;
-        ok = __all_sync(kAll, mbar_wait(&sm.iempty[un % kInfo], ((un / kInfo) & 1u) ^ 1u, abort_flag));
+        ok = __all_sync(kAll, mbar_wait(&sm.iempty[un % kInfo], ((un / kInfo) & 1u) ^ 1u, abort_flag, p.wait_ns));
         if (ok && lane == 0) {
           sm.tiles[un % kInfo] = nt;
           mbar_arrive(&sm.ifull[un % kInfo]);
@@ -484,13 +485,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         pick(later, 1);
         rows_of(row, ks, vs, now);
         for (int j = 0; j < nt; ++j, ++n) {
+          if (n >= p.stop_after) ok = false;
+          if (!ok) break;
           int next_row[4];
           float next_ks[4], next_vs[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) now[i] = later[i];
           pick(later, j + 2);
           rows_of(next_row, next_ks, next_vs, now);
-          if (!(ok = __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)))) break;
+          if (!(ok = __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag, p.wait_ns)))) break;
           TileMeta& m = sm.meta[n % kMeta];
           int most = -100, least = 100;  // exponents of the v scales (16 bits: none)
           unsigned whole = kAll;
@@ -521,7 +524,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           for (int i = 0; i < 4; ++i) row[i] = next_row[i], ks[i] = next_ks[i], vs[i] = next_vs[i];
         }
       }
-      if (ok && __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)) && lane == 0) {
+      if (ok && __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag, p.wait_ns)) && lane == 0) {
         sm.meta[n % kMeta].flags = kEnd;
         mbar_arrive(&sm.mfull[n % kMeta]);
       }
@@ -544,7 +547,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       const int c = lane % kQLanes, sub = (warp - kQueryWarp) * 64 + lane / kQLanes;
       uint32_t un = 0, wn = 0;
       for (uint32_t unit = first; unit < units; unit += step, ++un) {
-        if (!__all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag))) break;
+        if (!__all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag, p.wait_ns))) break;
         const int nt = sm.tiles[un % kInfo];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.iempty[un % kInfo]);
@@ -559,7 +562,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             const int h = sub + (b + i) * kQOnce;
             x[i] = h < w.heads ? ldg16(q0 + (int64_t)h * p.q_head) : make_uint4(0u, 0u, 0u, 0u);
           }
-          if (b == 0 && !__all_sync(kAll, mbar_wait(&sm.qempty[wn % kQTiles], ((wn / kQTiles) & 1u) ^ 1u, abort_flag))) break;
+          if (b == 0 && !__all_sync(kAll, mbar_wait(&sm.qempty[wn % kQTiles], ((wn / kQTiles) & 1u) ^ 1u, abort_flag, p.wait_ns))) break;
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
             const int h = sub + (b + i) * kQOnce;
@@ -691,8 +694,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     uint32_t it = 0, un = 0, wn = 0;
     bool ok = true;
     constexpr int kHalf = D / 2;  // columns of O a thread writes
-    for (uint32_t unit = first; unit < units; unit += step, ++un) {
-      if (!(ok = __all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag)))) break;
+    uint32_t unit = first;
+    for (; unit < units; unit += step, ++un) {
+      if (!(ok = __all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag, p.wait_ns)))) break;
       const int nt = sm.tiles[un % kInfo];
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.iempty[un % kInfo]);
@@ -712,7 +716,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       for (int j = g ^ (int)(it & 1u); j < nt; j += 2) {
         const uint32_t n = it + (uint32_t)j;
         const int place = (int)(n % kMeta);
-        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag) && mbar_wait(&sm.sdone[n % C::kSDone], (n / C::kSDone) & 1u, abort_flag);
+        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag, p.wait_ns) && mbar_wait(&sm.sdone[n % C::kSDone], (n / C::kSDone) & 1u, abort_flag, p.wait_ns);
         if (!(ok = __all_sync(kAll, ok))) break;
         tmem_fence_after();
         auto hand_over = [&](int half) {
@@ -732,7 +736,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             ref = next;
             if (half || j > 1) {
               uint64_t* const bar = half ? &sm.halfdone[g] : &sm.pvdone[(n - 2u) % kMeta];
-              if (!__all_sync(kAll, mbar_wait(bar, half ? (n >> 1) & 1u : ((n - 2u) / kMeta) & 1u, abort_flag))) return;  // (the waits to come fail too)
+              if (!__all_sync(kAll, mbar_wait(bar, half ? (n >> 1) & 1u : ((n - 2u) / kMeta) & 1u, abort_flag, p.wait_ns))) return;  // (the waits to come fail too)
               tmem_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
@@ -822,11 +826,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         sm.ml[wn & 1u][g][r] = make_float2(ref + 0.f, sum);  // (+ 0: without it heads of 64 in 16 bits spill 36 bytes instead of 8, 173 us instead of 169)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.mlbar);
-        ok = mbar_wait(&sm.mlbar, wn & 1u, abort_flag);
+        ok = mbar_wait(&sm.mlbar, wn & 1u, abort_flag, p.wait_ns);
         const uint32_t end = it + (uint32_t)nt - 1u;  // the last tile; the one before it is the other group's last
-        ok = ok && mbar_wait(&sm.pvdone[end % kMeta], (end / kMeta) & 1u, abort_flag);
-        if (nt > 1) ok = ok && mbar_wait(&sm.pvdone[(end - 1u) % kMeta], ((end - 1u) / kMeta) & 1u, abort_flag);
-        if (!(ok = __all_sync(kAll, ok))) break;
+        ok = ok && mbar_wait(&sm.pvdone[end % kMeta], (end / kMeta) & 1u, abort_flag, p.wait_ns);
+        if (nt > 1) ok = ok && mbar_wait(&sm.pvdone[(end - 1u) % kMeta], ((end - 1u) / kMeta) & 1u, abort_flag, p.wait_ns);
+        if (!(ok = __all_sync(kAll, ok && *abort_flag == 0u))) break;  // (a wait may have run out in refer)
         tmem_fence_after();
         a = sm.ml[wn & 1u][0][r], b = sm.ml[wn & 1u][1][r];
       }
@@ -876,6 +880,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       it += (uint32_t)nt;
       wn += nt > 0 ? 1u : 0u;
     }
+    // (pieces that are left where a wait ran out; of several CTAs: below)
+    for (; ctas == 1 && unit < units; unit += step) {
+      const Work w = work_of(p, unit);
+      if (r >= w.heads) continue;
+      T* const out = static_cast<T*>(p.out) + (int64_t)w.token * p.out_token + (int64_t)(w.head0 + r) * p.out_head + g * kHalf;
+      const uint32_t nan[4] = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+      for (int c = 0; c < kHalf; c += 8) store_row(out + c, nan, p.out_vec != 0);
+      if (g == 0 && p.lse != nullptr) p.lse[(int64_t)w.token * p.kv_heads * p.group + w.head0 + r] = __int_as_float(0x7fffffff);
+    }
   }
   __syncwarp();
   __syncthreads();
@@ -893,6 +906,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     } while (t - t0 < 100000ull);
     if (tid == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_STAGE_TIMEOUT);
+    if (ctas > 1 && tid < kHeadsW) sm.ml[1][0][tid] = make_float2(-INFINITY, __int_as_float(0x7fffffff));  // (the joined rows become NaN)
   }
   tmem_fence_before();
   __syncthreads();

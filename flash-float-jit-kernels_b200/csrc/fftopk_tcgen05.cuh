@@ -10,7 +10,7 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
-// Longest wait on an mbarrier; see mbar_wait
+// Longest wait on an mbarrier, where a call says nothing else; see mbar_wait
 constexpr unsigned long long kMbarWaitNs = 200ull * 1000 * 1000;
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
@@ -46,7 +46,7 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0u;
 }
 // Bounded wait: false when the time ran out or another thread of the CTA has given up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, unsigned long long limit_ns = kMbarWaitNs) {
   if (mbar_try_wait(bar, parity)) return true;
   unsigned long long t0;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
@@ -55,7 +55,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     if (*abort_flag) return false;
     unsigned long long t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > kMbarWaitNs) {
+    if (t - t0 > limit_ns) {
       *abort_flag = 1u;
       return false;
     }

@@ -56,6 +56,7 @@ EXPORTS = (
     "fftopk_head_rows",
     "fftopk_cache_read",
     "fftopk_sparse_attention",
+    "fftopk_set_attend_stop",
     "fftopk_probe_read_bandwidth",
     "fftopk_key_of",
     "fftopk_plan",
@@ -171,6 +172,8 @@ def lib() -> ctypes.CDLL:
                                     c.c_void_p]
     L.fftopk_sparse_attention.restype = c.c_int
     L.fftopk_sparse_attention.argtypes = [c.c_char_p, c.c_void_p, c.c_void_p]
+    L.fftopk_set_attend_stop.restype = c.c_int
+    L.fftopk_set_attend_stop.argtypes = [c.c_int64, c.c_int64]
     L.fftopk_probe_read_bandwidth.restype = c.c_int
     L.fftopk_probe_read_bandwidth.argtypes = [c.c_void_p, c.c_size_t, c.c_size_t, c.c_void_p, c.POINTER(c.c_size_t),
                                               c.c_void_p]

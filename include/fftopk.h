@@ -425,6 +425,8 @@ int fftopk_cache_read(const void* cache, int64_t slot_stride, int64_t head_strid
  * fp16 (e4m3), off by 2^-11 of its size and, the small ones, by up to 2^-21 of the largest p_j * |v_scale_j| of the token and head.
  * v scales: zero, or magnitudes between 2^-100 and 2^100 (beyond that weights may underflow, or overflow to infinities).
  * The call holds no state and needs no workspace; the first one on a device sets kernel attributes (outside any capture).
+ * Should a bounded wait inside the kernel for many heads run out (FFTOPK_ST_STAGE_TIMEOUT; not expected), out and lse are NaN for every
+ * token and head that was not finished.
  */
 typedef struct fftopk_attend {
   const void* q;
@@ -498,6 +500,13 @@ int fftopk_plan(int32_t B, int64_t L, int32_t plan[6]);
 int fftopk_set_overlap(int32_t enable);
 int fftopk_set_tuning(int32_t cluster_ctas, int32_t threads, int32_t list_cap, int32_t cand_cap,
                       int32_t force_full_histogram);
+
+/*
+ * For tests: the calls of fftopk_sparse_attention that follow, process-wide, give up a wait after wait_ns (at most 200 ms, which is what a
+ * negative value restores), and in the kernel for many heads every CTA is handed `tiles` tiles of keys and no more (negative: all), so
+ * that with a shorter list its waits run out. FFTOPK_ERANGE for more. No reference counterpart.
+ */
+int fftopk_set_attend_stop(int64_t wait_ns, int64_t tiles);
 
 #ifdef __cplusplus
 }

@@ -56,3 +56,11 @@ def test_where_the_rule_turns(is_wide, fp8):
     assert is_wide(1 << 20, 17, 1, fp8) == (not fp8) and is_wide(1 << 20, 33, 1, fp8)
     # four CTAs for each of its pieces: 8 pieces to a token of 128 heads
     assert not is_wide(9, 128, 1, fp8) and is_wide(10, 128, 1, fp8)
+
+
+def test_limits_of_waits():
+    """Set and restored without a device."""
+    from jit_kernel import _native
+    stop = _native.lib().fftopk_set_attend_stop
+    assert stop(200_000_001, -1) == _native.E_RANGE and stop(-1, 1 << 31) == _native.E_RANGE
+    assert stop(1, 0) == 0 and stop(-1, -1) == 0

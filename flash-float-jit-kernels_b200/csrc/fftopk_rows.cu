@@ -44,6 +44,7 @@ struct RowParams {
   const int32_t* positions;
   const float* cos_sin;
   int64_t table_rows;
+  const int32_t* padding;  // slots of the first part that has some: a token whose entry is negative is padding, and has no position
   int32_t D, R, interleaved;
   float inv_d;
   uint32_t* status;
@@ -115,7 +116,8 @@ __device__ __forceinline__ void head_rows(const RowParams& p, const int which) {
     if (mine) {
       const int64_t pos = p.positions[token];
       const bool ok = pos >= 0 && pos < p.table_rows;
-      if (!ok && lane == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+      if (!ok && lane == 0 && p.status && (p.padding == nullptr || p.padding[token] >= 0))
+        atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
       const float nan = __int_as_float(0x7fffffff);  // (no such row in the table: the rotated channels become NaN)
       const float* row = p.cos_sin + (ok ? pos : 0) * p.R;
       const int half = p.R >> 1;
@@ -460,6 +462,7 @@ int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tok
     p.per_token[i] = FastDiv(per_token > 0 ? (uint32_t)per_token : 1u);
     p.items[i] = (uint32_t)(tokens * per_token);
     p.aligned_w[i] = on(parts[i].weight, 16) && on(parts[i].bias, 16);
+    if (p.padding == nullptr && parts[i].heads > 0) p.padding = parts[i].slots;
   }
   p.positions = positions;
   p.cos_sin = cos_sin;

@@ -217,7 +217,8 @@ def qkv_norm_rope_write(
     q_out: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """qk_norm_rope and kv_cache.cache_write in one launch: q comes back normed and rotated, k is normed, rotated and quantised
-    into row slots[t] of k_cache, v quantised into v_cache. Arguments as for those two."""
+    into row slots[t] of k_cache, v quantised into v_cache. Arguments as for those two; padding tokens (slot -1) may have any
+    position (outside the table: q's rotated channels are NaN, and kernel_status() says nothing)."""
     idx, T, D, dtype = _check_first(q, "q")
     table = _check_table(positions, cos_sin, idx, T, D)
     rotate = 1 if cos_sin is not None else 0
@@ -264,7 +265,8 @@ def indexer_qk_write(
         q: [T, H, D] (H = 64, D = 128 for FusedIndexerTopk); k: [T, D], one key per token; as for qk_norm_rope.
         w: float32 [T, H], contiguous: the head weights.
         slots: int32 [T]: the token's row of the cache, counted through the sequences (b * rows + position for a cache
-            [B, rows, D]); -1 for padding tokens, whose keys are not written. The slots of one call differ from one another.
+            [B, rows, D]); -1 for padding tokens, whose keys are not written and whose positions may be anything (outside the
+            table: q's rotated channels are NaN). The slots of one call differ from one another.
         k_cache: float8_e4m3fn, contiguous, last dimension D: [B, rows, D] as FusedIndexerTopk takes it, or [rows, D];
             k_scale: float32, contiguous, of k_cache's shape without D. Both are written at `slots`.
     Returns:

@@ -365,7 +365,8 @@ int fftopk_indexer_topk2048(const void* q, const void* k_cache, int64_t k_rows_p
  *              to = token, or slots[token] where slots are given: a negative slot leaves the part's rows of that token out
  *              (padding); one at or beyond n_slots too, and raises FFTOPK_ST_BAD_INDEX. Slots of one call differ from one
  *              another (of two tokens with one slot either's codes and scales may stay, in any mixture).
- * in 32 bits, rounded once. A position outside [0, table_rows) makes the rotated channels NaN and raises FFTOPK_ST_BAD_INDEX.
+ * in 32 bits, rounded once. A position outside [0, table_rows) makes the rotated channels NaN and raises FFTOPK_ST_BAD_INDEX -
+ * without the bit where the token is padding: a negative slot in the first part that has slots.
  * out may be x itself (same strides); anything else that overlaps is not supported.
  *   strides      elements (codes: bytes); the D channels of a row are contiguous
  *   D            a multiple of 8 up to 256; rotary a multiple of 16 up to D (FFTOPK_ERANGE otherwise)

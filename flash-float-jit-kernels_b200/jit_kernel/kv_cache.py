@@ -35,7 +35,7 @@ def cache_write(
     H, xs = _check_rows(k, "k", idx, dtype, T, D)
     at = _check_vector(slots, "slots", idx, T)
     n, cs, ss = _check_cache(k_cache, k_scale, "k", idx, H, D)
-    _no_grad(k, v)
+    _no_grad(k, k_cache, k_scale, v, v_cache, v_scale)
     parts = _quantised(k, xs, H, k_cache, cs, k_scale, ss, at, n)
     if v is not None:
         if v_cache is None:
@@ -83,6 +83,7 @@ def cache_read(
     if offsets is not None and len(shape) != 2:
         raise RuntimeError("offsets go with slots [B, K]")
     off = _check_vector(offsets, "offsets", idx, rows)
+    _no_grad(cache, scale)
     out = scale.new_empty((*shape, H, D), dtype=dtype)
     if rows and per_row and H:
         _launch(_native.lib().fftopk_cache_read, "fftopk_cache_read", idx, cache.data_ptr(), cs[0], cs[1], n, H, D, scale.data_ptr(), ss[0],

@@ -11,6 +11,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .topk_indexer import _launch
@@ -26,10 +27,16 @@ _DENSE = torch.contiguous_format
 # An eager call on a few tokens is as long as its Python: every tensor is asked once for each of its properties, and the
 # pieces below hand on what they have asked for.
 def _no_grad(*tensors) -> None:
+    """Every floating tensor of a call, outputs and caches too: none may ask for a gradient, or carry a forward-mode tangent."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError("this op has no gradient: call it under torch.no_grad() or detach its inputs")
+    # (the level's name is private: where it is missing, every tensor is asked)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("this op has no gradient: a tensor carries a forward-mode tangent")
 
 
 def _check_rows(x: torch.Tensor, what: str, idx: int, dtype: torch.dtype, tokens: int, dim: int, heads: int = -1):
@@ -173,7 +180,7 @@ def qk_norm_rope(
     rotate = 1 if cos_sin is not None else 0
     heads, xs = _check_rows(q, "q", idx, dtype, T, D)
     norm = _check_norm(q_norm, q_weight, q_bias, "q", idx, D)
-    _no_grad(q, k, q_weight, k_weight, q_bias, k_bias)
+    _no_grad(q, k, cos_sin, q_weight, k_weight, q_bias, k_bias, q_out, k_out)
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=_DENSE)
         os = (heads * D, D)
@@ -227,7 +234,7 @@ def qkv_norm_rope_write(
     at = _check_vector(slots, "slots", idx, T)
     kn, kcs, kss = _check_cache(k_cache, k_scale, "k", idx, kh, D)
     vn, vcs, vss = _check_cache(v_cache, v_scale, "v", idx, vh, D)
-    _no_grad(q, k, v, q_weight, k_weight, q_bias, k_bias)
+    _no_grad(q, k, v, cos_sin, k_cache, k_scale, v_cache, v_scale, q_weight, k_weight, q_bias, k_bias, q_out)
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=_DENSE)
         os = (qh * D, D)
@@ -289,7 +296,7 @@ def indexer_qk_write(
         raise RuntimeError("k_cache must be contiguous float8_e4m3fn [.., rows, D] on the inputs' device")
     if k_scale.dtype is not torch.float32 or k_scale.shape != shape[:-1] or not k_scale.is_contiguous() or k_scale.get_device() != idx:
         raise RuntimeError("k_scale must be contiguous float32 of k_cache's shape without D on the inputs' device")
-    _no_grad(q, k, w, q_weight, k_weight, q_bias, k_bias)
+    _no_grad(q, k, w, cos_sin, k_cache, k_scale, q_weight, k_weight, q_bias, k_bias)
     q8 = torch.empty_like(q, dtype=FP8, memory_format=_DENSE)
     w8 = torch.empty_like(w)
     if T:

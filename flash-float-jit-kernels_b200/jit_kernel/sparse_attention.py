@@ -82,7 +82,7 @@ def sparse_attention(
             or (picks[1] > 1 and step[1] != 1):
         raise RuntimeError("indices must be an int32 tensor [tokens, K] with unit inner stride on q's device")
     off = _check_vector(offsets, "offsets", idx, T)
-    _no_grad(q, k_cache, v_cache, k_scale, v_scale)
+    _no_grad(q, k_cache, v_cache, k_scale, v_scale, out)
     if out is None:
         out = torch.empty_like(q, memory_format=_DENSE)
         os = (Hq * D, D)

@@ -555,6 +555,8 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
                                                       reinterpret_cast<uintptr_t>(a->v_scale)) & 3u))
     return FFTOPK_EINVAL;
   if (a->slots > 0x7fffffff || a->tokens > 0x7fffffff) return FFTOPK_ERANGE;
+  // (pieces of work: no more than tokens * q_heads, below 2^62, so that nothing has wrapped; what passes is a grid, too)
+  if (attend_narrow_units(a->tokens, a->kv_heads, a->q_heads / a->kv_heads) > 0x7fffffff) return FFTOPK_ERANGE;
   Limits limits;
   const int rc = attend_setup(limits);
   if (rc) return rc;
@@ -588,7 +590,6 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   // (clusters of eight fit in fewer places than their CTAs alone: 16 of the wide kernel's took 26 us, eight 14)
   const int64_t room = wide ? sms : sm_ctas(a->D) * (int64_t)sms, eights = wide ? limits.wide_eights : limits.narrow_eights;
   while (ctas < kAttendMaxCluster && units * ctas * 2 <= room && (ctas * 2 < 8 || units <= eights) && (int64_t)ctas * keys < p.picks) ctas *= 2;
-  if (units * ctas > 0x7fffffff) return FFTOPK_ERANGE;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   if (wide) {
     const cudaError_t e = attend_wide(p, a->dtype == FFTOPK_DTYPE_BF16, fp8, a->D, ctas, units, sms, stream);

@@ -338,7 +338,7 @@ FFTOPK_DECIDE_HD bool tile_segment(uint32_t row_g0, uint32_t ntiles, uint32_t g,
 // ---------------------------------------------------------------------------------------------
 constexpr int kAttendHeads = 16;  // query heads that the narrow kernel works on at a time
 FFTOPK_DECIDE_HD int64_t attend_narrow_units(int64_t tokens, int32_t kv_heads, int32_t group) {
-  return tokens * kv_heads * ((group + kAttendHeads - 1) / kAttendHeads);
+  return tokens * kv_heads * (((int64_t)group + kAttendHeads - 1) / kAttendHeads);
 }
 FFTOPK_DECIDE_HD bool attend_is_wide(int64_t tokens, int32_t kv_heads, int32_t group, bool fp8, int32_t sms) {
   return group > kAttendHeads && !(fp8 && group <= 2 * kAttendHeads) && attend_narrow_units(tokens, kv_heads, group) * 4 > 2 * (int64_t)sms;

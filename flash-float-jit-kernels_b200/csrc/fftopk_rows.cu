@@ -451,13 +451,14 @@ int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tok
       return FFTOPK_EINVAL;
   }
   if (tokens == 0 || all_heads == 0) return FFTOPK_OK;
+  if (tokens > 0x7fffffff) return FFTOPK_ERANGE;  // (in front of every product: none wraps)
   // several heads a group once there are rows for every group of lanes the device holds (16,384 tokens of 72 heads: four heads 126 us,
   // one 276; 64 tokens of the indexer's step: 5.2 and 3.8)
-  const int heads = vec && tokens * all_heads >= 148 * 64 * kHeadsItem ? kHeadsItem : 1;
-  if (tokens > 0x7fffffff) return FFTOPK_ERANGE;
+  const int64_t enough = 148 * 64 * kHeadsItem;
+  const int heads = vec && all_heads >= (enough + tokens - 1) / tokens ? kHeadsItem : 1;
   for (int i = 0; i < n_parts; ++i) {
     p.part[i] = parts[i];
-    const int64_t per_token = (parts[i].heads + heads - 1) / heads;
+    const int64_t per_token = ((int64_t)parts[i].heads + heads - 1) / heads;
     if (tokens * per_token > (int64_t)0x7fffffff - 64) return FFTOPK_ERANGE;
     p.per_token[i] = FastDiv(per_token > 0 ? (uint32_t)per_token : 1u);
     p.items[i] = (uint32_t)(tokens * per_token);

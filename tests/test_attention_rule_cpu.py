@@ -64,3 +64,20 @@ def test_limits_of_waits():
     stop = _native.lib().fftopk_set_attend_stop
     assert stop(200_000_001, -1) == _native.E_RANGE and stop(-1, 1 << 31) == _native.E_RANGE
     assert stop(1, 0) == 0 and stop(-1, -1) == 0
+
+
+@pytest.mark.parametrize("tokens,q_heads,kv_heads", [((1 << 31) - 1, (1 << 31) - 1, (1 << 31) - 1), (1 << 28, 8, 8), ((1 << 31) - 1, 1 << 30, 1)])
+def test_more_pieces_of_work_than_a_grid_has(tokens, q_heads, kv_heads):
+    """Refused before anything is multiplied out of 64 bits, and before a device is asked."""
+    from jit_kernel import _native
+    from test_rows_refusals_cpu import ATTEND
+    from jit_kernel.sparse_attention import _ARGS
+    args = {**ATTEND, "tokens": tokens, "q_heads": q_heads, "kv_heads": kv_heads, "kh": 128}
+    assert _native.lib().fftopk_sparse_attention(_ARGS.pack(*args.values()), None, None) == _native.E_RANGE
+
+
+def test_more_head_rows_than_a_call_takes():
+    from jit_kernel import _native
+    from test_rows_refusals_cpu import rows
+    for tokens, heads, n in ((1 << 61, 8, 1), ((1 << 31) - 1, (1 << 31) - 1, 3), (1 << 40, 1, 1), (16, 1 << 30, 2)):
+        assert rows(tokens=tokens, heads=heads, n_parts=n) == _native.E_RANGE

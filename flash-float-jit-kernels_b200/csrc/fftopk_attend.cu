@@ -195,12 +195,12 @@ __global__ void __launch_bounds__(kThreads, sm_ctas(D)) attend_narrow_kernel(con
   const char* const vbase = static_cast<const char*>(p.v) + (int64_t)kvh * p.v_head * (kFp8 ? 1 : 2) + piece * 16;
   const int64_t kstep = p.k_slot * (kFp8 ? 1 : 2), vstep = p.v_slot * (kFp8 ? 1 : 2);
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)warp * G::kBytes;
-  const int blocks = (p.picks + kKeys - 1) / kKeys;
+  const int blocks = (int)(((uint32_t)p.picks + kKeys - 1u) / kKeys);
   const int stride = ctas * kWarps;
 
   auto pick = [&](int block) {  // lane's index in a block; -1: none
-    const int j = block * kKeys + (lane & (kKeys - 1));
-    return block < blocks && j < p.picks ? idx[j] : -1;
+    const uint32_t j = (uint32_t)block * kKeys + (uint32_t)(lane & (kKeys - 1));
+    return block < blocks && j < (uint32_t)p.picks ? idx[j] : -1;
   };
   // asks for a block's rows and scales; which of them are there
   auto ask = [&](uint32_t stage, int32_t index) {

@@ -186,9 +186,13 @@ __device__ __forceinline__ uint32_t chunk_at(uint32_t tile, int r, int c) {
   return tile + (uint32_t)(c >> 3) * (kTileKeys * 128u) + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4);
 }
 
-// tiles of a token's picks up to the last entry that is not negative (by a whole warp)
+__device__ __forceinline__ int tiles_up_to(int picks) { return (int)(((uint32_t)picks + kTileKeys - 1u) / kTileKeys); }
+// tiles of a token's picks up to the last entry that is not negative (by a whole warp). It is looked for among the last kLookBack
+// entries, a millisecond at most: everybody waits meanwhile, and a list of 2^28 would outlast the limit of their waits.
+constexpr int kLookBack = 1 << 20;
 __device__ __forceinline__ int tiles_of(const int32_t* idx, int picks, int lane) {
-  for (int hi = picks; hi > 0; hi -= 512) {
+  const int until = max(picks - kLookBack, 0);
+  for (int hi = picks; hi > until; hi -= 512) {
     int last = -1;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -198,7 +202,7 @@ __device__ __forceinline__ int tiles_of(const int32_t* idx, int picks, int lane)
     last = __reduce_max_sync(kAll, last);
     if (last >= 0) return last / kTileKeys + 1;
   }
-  return 0;
+  return tiles_up_to(until);
 }
 
 struct Work {
@@ -438,7 +442,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       auto tell = [&](uint32_t unit, uint32_t un) {
         const int32_t* idx = p.indices + (int64_t)work_of(p, unit).token * p.idx_row;
         // (several CTAs a token: tiles without a row cost less than looking for the last)
-        const int all = ctas > 1 ? (p.picks + kTileKeys - 1) / kTileKeys : tiles_of(idx, p.picks, lane);
+        const int all = ctas > 1 ? tiles_up_to(p.picks) : tiles_of(idx, p.picks, lane);
         const int nt = all > rank ? (all - rank + ctas - 1) / ctas : 0;
         ok = __all_sync(kAll, mbar_wait(&sm.iempty[un % kInfo], ((un / kInfo) & 1u) ^ 1u, abort_flag, p.wait_ns));
         if (ok && lane == 0) {
@@ -458,8 +462,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         auto pick = [&](int (&to)[4], int j) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int at = (rank + j * ctas) * kTileKeys + i * 32 + lane;
-            to[i] = j < nt && at < p.picks ? idx[at] : -1;
+            const uint32_t at = (uint32_t)(rank + j * ctas) * kTileKeys + (uint32_t)(i * 32 + lane);
+            to[i] = j < nt && at < (uint32_t)p.picks ? idx[at] : -1;
           }
         };
         auto rows_of = [&](int (&row)[4], float (&ks)[4], float (&vs)[4], const int (&from)[4]) {

@@ -79,8 +79,8 @@ def sparse_attention(
             raise RuntimeError("the caches must have unit inner stride")
     picks, step = indices.shape, indices.stride()
     if indices.dtype is not torch.int32 or len(picks) != 2 or picks[0] != T or indices.get_device() != idx \
-            or (picks[1] > 1 and step[1] != 1):
-        raise RuntimeError("indices must be an int32 tensor [tokens, K] with unit inner stride on q's device")
+            or (picks[1] > 1 and step[1] != 1) or picks[1] > 0x7fffffff:
+        raise RuntimeError("indices must be an int32 tensor [tokens, K < 2^31] with unit inner stride on q's device")
     off = _check_vector(offsets, "offsets", idx, T)
     _no_grad(q, k_cache, v_cache, k_scale, v_scale, out)
     if out is None:

@@ -260,6 +260,20 @@ __device__ __forceinline__ void store_row(T* out, const uint32_t (&v)[N], bool v
   }
 }
 
+// what softmax thread (r, g) leaves for the pieces of work from `unit` on where a wait ran out (a function of its own: hardly ever run,
+// and its registers are not the loop's)
+template <typename T, int D>
+__device__ __noinline__ void leave_nan(const AttendParams& p, uint32_t unit, uint32_t units, uint32_t step, int r, int g) {
+  const uint32_t nan[4] = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+  for (; unit < units; unit += step) {
+    const Work w = work_of(p, unit);
+    if (r >= w.heads) continue;
+    T* const out = static_cast<T*>(p.out) + (int64_t)w.token * p.out_token + (int64_t)(w.head0 + r) * p.out_head + g * (D / 2);
+    for (int c = 0; c < D / 2; c += 8) store_row(out + c, nan, p.out_vec != 0);
+    if (g == 0 && p.lse != nullptr) p.lse[(int64_t)w.token * p.kv_heads * p.group + w.head0 + r] = __int_as_float(0x7fffffff);
+  }
+}
+
 template <typename T, bool kFp8, int D>
 __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __grid_constant__ AttendParams p, const uint32_t units) {
   using M = typename std::conditional<kFp8, __half, T>::type;
@@ -884,15 +898,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       it += (uint32_t)nt;
       wn += nt > 0 ? 1u : 0u;
     }
-    // (pieces that are left where a wait ran out; of several CTAs: below)
-    for (; ctas == 1 && unit < units; unit += step) {
-      const Work w = work_of(p, unit);
-      if (r >= w.heads) continue;
-      T* const out = static_cast<T*>(p.out) + (int64_t)w.token * p.out_token + (int64_t)(w.head0 + r) * p.out_head + g * kHalf;
-      const uint32_t nan[4] = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
-      for (int c = 0; c < kHalf; c += 8) store_row(out + c, nan, p.out_vec != 0);
-      if (g == 0 && p.lse != nullptr) p.lse[(int64_t)w.token * p.kv_heads * p.group + w.head0 + r] = __int_as_float(0x7fffffff);
-    }
+    if (ctas == 1 && unit < units) leave_nan<T, D>(p, unit, units, step, r, g);  // (of several CTAs: below)
   }
   __syncwarp();
   __syncthreads();

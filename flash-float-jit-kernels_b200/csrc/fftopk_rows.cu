@@ -382,12 +382,12 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_kernel(const __grid_co
 }
 
 template <typename T, int kLanes>
-cudaError_t launch_read(const ReadParams& p, bool vec, cudaStream_t stream) {
+cudaError_t launch_read(const ReadParams& p, bool vec, int sms, cudaStream_t stream) {
   constexpr int kRows = 4;
   const int64_t per_cta = kRowThreads / kLanes;
   if (!vec) {
     cache_read_kernel<T, kLanes, 1, false><<<(unsigned)((p.rows + per_cta - 1) / per_cta), kRowThreads, 0, stream>>>(p);
-  } else if (p.rows < per_cta * kRows * 148) {  // (2,048 rows: one row a group 2.1 us, four 3.1; 262,144 rows: 27 and 20)
+  } else if (p.rows < per_cta * kRows * sms) {  // (2,048 rows: one row a group 2.1 us, four 3.1; 262,144 rows: 27 and 20)
     cache_read_kernel<T, kLanes, 1, true><<<(unsigned)((p.rows + per_cta - 1) / per_cta), kRowThreads, 0, stream>>>(p);
   } else {
     cache_read_kernel<T, kLanes, kRows, true>
@@ -397,8 +397,23 @@ cudaError_t launch_read(const ReadParams& p, bool vec, cudaStream_t stream) {
 }
 
 template <typename T>
-cudaError_t launch_read(const ReadParams& p, bool vec, cudaStream_t stream) {
-  return p.D <= 64 ? launch_read<T, 8>(p, vec, stream) : p.D <= 128 ? launch_read<T, 16>(p, vec, stream) : launch_read<T, 32>(p, vec, stream);
+cudaError_t launch_read(const ReadParams& p, bool vec, int sms, cudaStream_t stream) {
+  return p.D <= 64 ? launch_read<T, 8>(p, vec, sms, stream) : p.D <= 128 ? launch_read<T, 16>(p, vec, sms, stream) : launch_read<T, 32>(p, vec, sms, stream);
+}
+
+DeviceOnce g_sms_once[kMaxDevices];
+int g_sms[kMaxDevices];
+int device_sms(int& sms) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e);
+  if (dev < 0 || dev >= kMaxDevices) return FFTOPK_EDEVICE;
+  const int rc = g_sms_once[dev].run([&] {
+    const cudaError_t e2 = cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    return e2 == cudaSuccess ? 0 : cuda_fail(e2);
+  });
+  sms = g_sms[dev];
+  return rc;
 }
 
 int elem_bytes(int32_t dtype) { return dtype == FFTOPK_DTYPE_FP32 ? 4 : 2; }
@@ -452,14 +467,19 @@ int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tok
   }
   if (tokens == 0 || all_heads == 0) return FFTOPK_OK;
   if (tokens > 0x7fffffff) return FFTOPK_ERANGE;  // (in front of every product: none wraps)
+  // (one head a group only where there are few rows)
+  for (int i = 0; i < n_parts; ++i)
+    if (tokens * (((int64_t)parts[i].heads + (vec ? kHeadsItem - 1 : 0)) / (vec ? kHeadsItem : 1)) > (int64_t)0x7fffffff - 64) return FFTOPK_ERANGE;
   // several heads a group once there are rows for every group of lanes the device holds (16,384 tokens of 72 heads: four heads 126 us,
   // one 276; 64 tokens of the indexer's step: 5.2 and 3.8)
-  const int64_t enough = 148 * 64 * kHeadsItem;
+  int sms = 0;
+  const int rc = device_sms(sms);
+  if (rc) return rc;
+  const int64_t enough = (int64_t)sms * 64 * kHeadsItem;
   const int heads = vec && all_heads >= (enough + tokens - 1) / tokens ? kHeadsItem : 1;
   for (int i = 0; i < n_parts; ++i) {
     p.part[i] = parts[i];
     const int64_t per_token = ((int64_t)parts[i].heads + heads - 1) / heads;
-    if (tokens * per_token > (int64_t)0x7fffffff - 64) return FFTOPK_ERANGE;
     p.per_token[i] = FastDiv(per_token > 0 ? (uint32_t)per_token : 1u);
     p.items[i] = (uint32_t)(tokens * per_token);
     p.aligned_w[i] = on(parts[i].weight, 16) && on(parts[i].bias, 16);
@@ -490,6 +510,9 @@ int fftopk_cache_read(const void* cache, int64_t slot_stride, int64_t head_strid
   if (!on(scale, 4) || !on(slots, 4) || !on(offsets, 4) || !on(out, 16)) return FFTOPK_EINVAL;
   if (rows > 0x7fffffff || per_row > 0x7fffffff || rows * per_row > 0x7fffffff || rows * per_row * heads > (int64_t)0x7fffffff - 4096)
     return FFTOPK_ERANGE;
+  int sms = 0;
+  const int rc = device_sms(sms);
+  if (rc) return rc;
   ReadParams p;
   memset(&p, 0, sizeof(p));
   p.cache = static_cast<const uint8_t*>(cache);
@@ -509,9 +532,9 @@ int fftopk_cache_read(const void* cache, int64_t slot_stride, int64_t head_strid
   p.status = status;
   const bool vec = on(cache, 8) && slot_stride % 8 == 0 && (heads == 1 || head_stride % 8 == 0);
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  const cudaError_t e = out_dtype == FFTOPK_DTYPE_FP32   ? launch_read<float>(p, vec, stream)
-                        : out_dtype == FFTOPK_DTYPE_BF16 ? launch_read<__nv_bfloat16>(p, vec, stream)
-                                                         : launch_read<__half>(p, vec, stream);
+  const cudaError_t e = out_dtype == FFTOPK_DTYPE_FP32   ? launch_read<float>(p, vec, sms, stream)
+                        : out_dtype == FFTOPK_DTYPE_BF16 ? launch_read<__nv_bfloat16>(p, vec, sms, stream)
+                                                         : launch_read<__half>(p, vec, sms, stream);
   return e == cudaSuccess ? FFTOPK_OK : cuda_fail(e);
 }
 

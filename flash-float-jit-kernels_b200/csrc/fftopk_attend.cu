@@ -461,7 +461,7 @@ std::atomic<uint32_t> g_stop_after{0xffffffffu};
 DeviceOnce g_attend_once[kMaxDevices];
 struct Limits {
   int sms = 0;
-  int narrow_eights = 0, wide_eights = 0;  // clusters of eight CTAs the device holds at once
+  int narrow_eights[2][2] = {}, wide_eights = 0;  // clusters of eight CTAs the device holds at once; narrow: [e4m3][heads of 128]
 };
 Limits g_attend_limits[kMaxDevices];
 
@@ -493,7 +493,11 @@ int attend_setup(Limits& limits) {
     if (!r) r = setup_one<__half, false, 128>();
     if (!r) r = setup_one<__half, true, 64>();
     if (!r) r = setup_one<__half, true, 128>();
-    if (!r) r = eights_of<__nv_bfloat16, false, 128>(g_attend_limits[dev].narrow_eights);
+    int(&eights)[2][2] = g_attend_limits[dev].narrow_eights;
+    if (!r) r = eights_of<__nv_bfloat16, false, 64>(eights[0][0]);
+    if (!r) r = eights_of<__nv_bfloat16, false, 128>(eights[0][1]);
+    if (!r) r = eights_of<__nv_bfloat16, true, 64>(eights[1][0]);
+    if (!r) r = eights_of<__nv_bfloat16, true, 128>(eights[1][1]);
     if (!r) r = attend_wide_setup(g_attend_limits[dev].wide_eights);
     return r;
   });
@@ -588,7 +592,7 @@ extern "C" int fftopk_sparse_attention(const fftopk_attend* a, uint32_t* status,
   const int keys = wide ? 128 : kWarps * (fp8 ? 32 : 16);
   int ctas = 1;
   // (clusters of eight fit in fewer places than their CTAs alone: 16 of the wide kernel's took 26 us, eight 14)
-  const int64_t room = wide ? sms : sm_ctas(a->D) * (int64_t)sms, eights = wide ? limits.wide_eights : limits.narrow_eights;
+  const int64_t room = wide ? sms : sm_ctas(a->D) * (int64_t)sms, eights = wide ? limits.wide_eights : limits.narrow_eights[fp8][a->D == 128];
   while (ctas < kAttendMaxCluster && units * ctas * 2 <= room && (ctas * 2 < 8 || units <= eights) && (int64_t)ctas * keys < p.picks) ctas *= 2;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   if (wide) {

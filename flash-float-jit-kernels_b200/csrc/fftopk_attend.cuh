@@ -76,11 +76,6 @@ __device__ __forceinline__ uint4 ldg16(const void* p) {
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
 }
-__device__ __forceinline__ uint2 ldg8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
 // shared memory of another CTA of the cluster, by its 32-bit address there
 __device__ __forceinline__ uint32_t shared_of(uint32_t addr, int rank) {
   uint32_t r;

@@ -75,7 +75,7 @@ struct WideCfg {
   // (1,024 tokens of 128 heads on one e4m3 key head: two k and v tiles and room for the codes of one 344 us; one k and one v tile,
   // codes of two and a query tile ahead 362)
   static constexpr int kQTiles = D == 128 && kFp8 ? 1 : 2, kKStages = 2, kVStages = 2;
-  static constexpr int kSDone = kKStages < 2 ? 2 : kKStages;  // barriers in turn: softmax may be a tile behind QK
+  static_assert(kKStages >= 2, "softmax may be a tile behind QK, whose barriers are the k stages'");
   static constexpr int kRaw = kFp8 ? (D == 64 ? 4 : 1) : 0;
   static constexpr uint32_t kRawBytes = 32 * D;              // of a warp and tile
   static constexpr size_t kTiles = (size_t)kTileBytes * (kQTiles + kKStages + kVStages), kOperands = kTiles + (size_t)kRaw * kGatherWarps * kRawBytes;
@@ -101,7 +101,7 @@ struct WideSmem {  // behind the operand tiles
   float2 ml[2][2][kHeadsW];  // by parity of the piece of work, and group: maximum and sum
   int32_t tiles[kInfo];      // tiles of a piece of work
   // A place of a ring is free again when the MMAs that read it are done, which one commit tells all who wait for them.
-  uint64_t kfull[WideCfg<kFp8, D>::kKStages], sdone[WideCfg<kFp8, D>::kSDone];  // k has landed; QK is done: S is there, k may be replaced
+  uint64_t kfull[WideCfg<kFp8, D>::kKStages], sdone[WideCfg<kFp8, D>::kKStages];  // k has landed; QK is done: S is there, k may be replaced
   uint64_t vfull[WideCfg<kFp8, D>::kVStages];
   uint64_t mfull[kMeta], pvdone[kMeta];  // TileMeta is there; PV is done: v and TileMeta may be replaced, O is up to this tile
   uint64_t ifull[kInfo], iempty[kInfo];
@@ -294,8 +294,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
   const uint32_t first = blockIdx.x / (uint32_t)ctas, step = gridDim.x / (uint32_t)ctas;
 
   if (tid == 0) {
-    for (int i = 0; i < kKS; ++i) mbar_init(&sm.kfull[i], 4);
-    for (int i = 0; i < C::kSDone; ++i) mbar_init(&sm.sdone[i], 1);
+    for (int i = 0; i < kKS; ++i) mbar_init(&sm.kfull[i], 4), mbar_init(&sm.sdone[i], 1);
     for (int i = 0; i < kVS; ++i) mbar_init(&sm.vfull[i], 4);
     for (int i = 0; i < kMeta; ++i) mbar_init(&sm.mfull[i], 1), mbar_init(&sm.pvdone[i], 1);
     for (int i = 0; i < kInfo; ++i) mbar_init(&sm.ifull[i], 1), mbar_init(&sm.iempty[i], kSoftmaxWarps + kQueryWarps);
@@ -324,7 +323,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     const int gw = (warp - kSoftmaxWarps) & 3;
     uint64_t* const full = is_k ? sm.kfull : sm.vfull;
     uint64_t* const empty = is_k ? sm.sdone : sm.pvdone;  // of the tile `stages` before
-    const uint32_t ring = is_k ? C::kSDone : kMeta;
+    const uint32_t ring = is_k ? kKS : kMeta;
     const uint32_t stages = is_k ? kKS : kVS;
     const uint32_t tiles = is_k ? k_tiles : v_tiles;
     constexpr int kLanesRow = D * (kFp8 ? 1 : 2) / 16;  // lanes that read a row
@@ -640,7 +639,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             const uint32_t at = ((uint32_t)(k >> 2) * (kTileKeys * 128u) + (uint32_t)(k & 3) * 32u) >> 4;
             mma_ss(d, q + at, kt + at, instr_desc<M, kTileKeys, false>(), k != 0);
           }
-          umma_commit(&sm.sdone[qn % C::kSDone]);
+          umma_commit(&sm.sdone[qn % kKS]);
           const bool last = (flags & kLast) != 0;
           if (last) umma_commit(&sm.qempty[qwn % kQTiles]);
           pflags |= flags << (8u * (qn & 1u));
@@ -734,7 +733,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       for (int j = g ^ (int)(it & 1u); j < nt; j += 2) {
         const uint32_t n = it + (uint32_t)j;
         const int place = (int)(n % kMeta);
-        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag, p.wait_ns) && mbar_wait(&sm.sdone[n % C::kSDone], (n / C::kSDone) & 1u, abort_flag, p.wait_ns);
+        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag, p.wait_ns) && mbar_wait(&sm.sdone[n % kKS], (n / kKS) & 1u, abort_flag, p.wait_ns);
         if (!(ok = __all_sync(kAll, ok))) break;
         tmem_fence_after();
         auto hand_over = [&](int half) {

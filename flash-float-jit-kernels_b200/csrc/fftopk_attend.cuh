@@ -28,7 +28,7 @@ struct AttendParams {
   float scale_log2;     // softmax scale * log2(e)
   int32_t out_vec;      // rows of out start on 16 bytes
   uint32_t* status;
-  uint64_t wait_ns;     // wide: longest wait on a barrier
+  uint64_t wait_ns;     // wide: longest wait for the scout
   uint32_t stop_after;  // wide, for tests: tiles after which the scout hands out no more
 };
 

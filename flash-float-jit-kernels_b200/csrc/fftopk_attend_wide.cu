@@ -335,10 +335,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     const int64_t head_bytes = (is_k ? p.k_head : p.v_head) * (kFp8 ? 1 : 2);
     const char* const src0 = static_cast<const char*>(is_k ? p.k : p.v) + piece * 16;
     auto posted = [&](uint32_t n) { return __all_sync(kAll, mbar_test(&sm.mfull[n % kMeta], (n / kMeta) & 1u)); };
+    // (in a test the first of all waits to run out; the others see abort_flag)
     auto wait_posted = [&](uint32_t n) { return __all_sync(kAll, mbar_wait(&sm.mfull[n % kMeta], (n / kMeta) & 1u, abort_flag, p.wait_ns)); };
     auto wait_empty = [&](uint32_t n) {
       const uint32_t of = n - stages;
-      return n < stages || __all_sync(kAll, mbar_wait(&empty[of % ring], (of / ring) & 1u, abort_flag, p.wait_ns));
+      return n < stages || __all_sync(kAll, mbar_wait(&empty[of % ring], (of / ring) & 1u, abort_flag));
     };
     auto is_empty = [&](uint32_t n) {
       const uint32_t of = n - stages;
@@ -457,7 +458,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         // (several CTAs a token: tiles without a row cost less than looking for the last)
         const int all = ctas > 1 ? tiles_up_to(p.picks) : tiles_of(idx, p.picks, lane);
         const int nt = all > rank ? (all - rank + ctas - 1) / ctas : 0;
-        ok = __all_sync(kAll, mbar_wait(&sm.iempty[un % kInfo], ((un / kInfo) & 1u) ^ 1u, abort_flag, p.wait_ns));
+        ok = __all_sync(kAll, mbar_wait(&sm.iempty[un % kInfo], ((un / kInfo) & 1u) ^ 1u, abort_flag));
         if (ok && lane == 0) {
           sm.tiles[un % kInfo] = nt;
           mbar_arrive(&sm.ifull[un % kInfo]);
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           for (int i = 0; i < 4; ++i) now[i] = later[i];
           pick(later, j + 2);
           rows_of(next_row, next_ks, next_vs, now);
-          if (!(ok = __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag, p.wait_ns)))) break;
+          if (!(ok = __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)))) break;
           TileMeta& m = sm.meta[n % kMeta];
           int most = -100, least = 100;  // exponents of the v scales (16 bits: none)
           unsigned whole = kAll;
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
           for (int i = 0; i < 4; ++i) row[i] = next_row[i], ks[i] = next_ks[i], vs[i] = next_vs[i];
         }
       }
-      if (ok && __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag, p.wait_ns)) && lane == 0) {
+      if (ok && __all_sync(kAll, mbar_wait(&sm.pvdone[n % kMeta], ((n / kMeta) & 1u) ^ 1u, abort_flag)) && lane == 0) {
         sm.meta[n % kMeta].flags = kEnd;
         mbar_arrive(&sm.mfull[n % kMeta]);
       }
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       const int c = lane % kQLanes, sub = (warp - kQueryWarp) * 64 + lane / kQLanes;
       uint32_t un = 0, wn = 0;
       for (uint32_t unit = first; unit < units; unit += step, ++un) {
-        if (!__all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag, p.wait_ns))) break;
+        if (!__all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag))) break;
         const int nt = sm.tiles[un % kInfo];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.iempty[un % kInfo]);
@@ -579,7 +580,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             const int h = sub + (b + i) * kQOnce;
             x[i] = h < w.heads ? ldg16(q0 + (int64_t)h * p.q_head) : make_uint4(0u, 0u, 0u, 0u);
           }
-          if (b == 0 && !__all_sync(kAll, mbar_wait(&sm.qempty[wn % kQTiles], ((wn / kQTiles) & 1u) ^ 1u, abort_flag, p.wait_ns))) break;
+          if (b == 0 && !__all_sync(kAll, mbar_wait(&sm.qempty[wn % kQTiles], ((wn / kQTiles) & 1u) ^ 1u, abort_flag))) break;
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
             const int h = sub + (b + i) * kQOnce;
@@ -713,7 +714,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
     constexpr int kHalf = D / 2;  // columns of O a thread writes
     uint32_t unit = first;
     for (; unit < units; unit += step, ++un) {
-      if (!(ok = __all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag, p.wait_ns)))) break;
+      if (!(ok = __all_sync(kAll, mbar_wait(&sm.ifull[un % kInfo], (un / kInfo) & 1u, abort_flag)))) break;
       const int nt = sm.tiles[un % kInfo];
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.iempty[un % kInfo]);
@@ -733,7 +734,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
       for (int j = g ^ (int)(it & 1u); j < nt; j += 2) {
         const uint32_t n = it + (uint32_t)j;
         const int place = (int)(n % kMeta);
-        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag, p.wait_ns) && mbar_wait(&sm.sdone[n % kKS], (n / kKS) & 1u, abort_flag, p.wait_ns);
+        ok = mbar_wait(&sm.mfull[place], (n / kMeta) & 1u, abort_flag) && mbar_wait(&sm.sdone[n % kKS], (n / kKS) & 1u, abort_flag);
         if (!(ok = __all_sync(kAll, ok))) break;
         tmem_fence_after();
         auto hand_over = [&](int half) {
@@ -753,7 +754,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
             ref = next;
             if (half || j > 1) {
               uint64_t* const bar = half ? &sm.halfdone[g] : &sm.pvdone[(n - 2u) % kMeta];
-              if (!__all_sync(kAll, mbar_wait(bar, half ? (n >> 1) & 1u : ((n - 2u) / kMeta) & 1u, abort_flag, p.wait_ns))) return;  // (the waits to come fail too)
+              if (!__all_sync(kAll, mbar_wait(bar, half ? (n >> 1) & 1u : ((n - 2u) / kMeta) & 1u, abort_flag))) return;  // (the waits to come fail too)
               tmem_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
@@ -843,10 +844,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) attend_wide_kernel(const __gr
         sm.ml[wn & 1u][g][r] = make_float2(ref + 0.f, sum);  // (+ 0: without it heads of 64 in 16 bits spill 36 bytes instead of 8, 173 us instead of 169)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.mlbar);
-        ok = mbar_wait(&sm.mlbar, wn & 1u, abort_flag, p.wait_ns);
+        ok = mbar_wait(&sm.mlbar, wn & 1u, abort_flag);
         const uint32_t end = it + (uint32_t)nt - 1u;  // the last tile; the one before it is the other group's last
-        ok = ok && mbar_wait(&sm.pvdone[end % kMeta], (end / kMeta) & 1u, abort_flag, p.wait_ns);
-        if (nt > 1) ok = ok && mbar_wait(&sm.pvdone[(end - 1u) % kMeta], ((end - 1u) / kMeta) & 1u, abort_flag, p.wait_ns);
+        ok = ok && mbar_wait(&sm.pvdone[end % kMeta], (end / kMeta) & 1u, abort_flag);
+        if (nt > 1) ok = ok && mbar_wait(&sm.pvdone[(end - 1u) % kMeta], ((end - 1u) / kMeta) & 1u, abort_flag);
         if (!(ok = __all_sync(kAll, ok && *abort_flag == 0u))) break;  // (a wait may have run out in refer)
         tmem_fence_after();
         a = sm.ml[wn & 1u][0][r], b = sm.ml[wn & 1u][1][r];

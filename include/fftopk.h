@@ -503,9 +503,9 @@ int fftopk_set_tuning(int32_t cluster_ctas, int32_t threads, int32_t list_cap, i
                       int32_t force_full_histogram);
 
 /*
- * For tests: the calls of fftopk_sparse_attention that follow, process-wide, give up a wait after wait_ns (at most 200 ms, which is what a
- * negative value restores), and in the kernel for many heads every CTA is handed `tiles` tiles of keys and no more (negative: all), so
- * that with a shorter list its waits run out. FFTOPK_ERANGE for more. No reference counterpart.
+ * For tests: in the calls of fftopk_sparse_attention that follow, process-wide, every CTA of the kernel for many heads is handed `tiles` tiles
+ * of keys and no more (negative: all, as ever), and one that waits for a tile gives up after wait_ns (at most 200 ms, which is what a
+ * negative value restores). FFTOPK_ERANGE for more. No reference counterpart.
  */
 int fftopk_set_attend_stop(int64_t wait_ns, int64_t tiles);
 

@@ -5,7 +5,7 @@
 //
 // attend_narrow_kernel, up to 16 query heads to a key head at a time (which calls take it: attend_is_wide in fftopk_decide.h). A row of
 // k or v is used by those heads alone, so reading the rows bounds it: 16 flop a byte at most in 16 bits, 32 in fp8, where the tensor
-// cores want over 200 (64 tokens, 64 heads on 8 key heads, 2,048 picks: bf16 98 us = 5.5 TB/s; e4m3 85 us, where widening codes and
+// cores want over 200 (64 tokens, 64 heads on 8 key heads, 2,048 picks: bf16 98 us = 5.5 TB/s; e4m3 82 us, where widening codes and
 // pairing rows take half of the ALU). The rows lie anywhere,
 // and nothing but their own heads shares them: every warp has a ring of its own in shared memory that cp.async fills, blocks of 16
 // (e4m3: 32) keys ahead of the one it works on, and waits for no other warp.

@@ -1,8 +1,9 @@
 // Attention over selected rows for many query heads to a key head: the tensor cores' share of fftopk_attend.cu (the formulas
 // stand there; which calls come here: attend_is_wide in fftopk_decide.h).
 //
-// 128 query heads use a row of k and v here, 2 * 2 * 128 flop per element: in 16 bits as many flop per byte as the device has
-// (250), in fp8 and wherever tokens share rows out of L2 twice that and more. So the products run on tcgen05, one CTA per SM:
+// 128 query heads use a row of k and v here, 2 * 128 flop per element: 128 a byte in 16 bits, where a cache whose rows no tokens share
+// is bound by memory (the device has 250), 256 in fp8, and a multiple of that wherever tokens share rows out of L2. So the products run
+// on tcgen05, one CTA per SM:
 //   S[128 heads x 128 keys] = Q K^T    Q, K in shared memory (K-major, 128-byte swizzle), S in tensor memory
 //   O[128 heads x D]       += P V      P in tensor memory (16 bits, over the S it came from), V in shared memory as it lies in the
 //                                      cache, [key][channel]: an MN-major operand
@@ -14,15 +15,18 @@
 // anywhere: 16-bit ones are copied into their tile with cp.async; e4m3 codes into a ring of the gathering warp's own, which widens
 // them to fp16 in the tile. Rows that are not there are zeros, and masked in S.
 //
-// What bounds it (1,024 tokens of 128 heads on one key head, 2,048 picks of 65,536 shared rows): bf16 205 us, 670 TFLOP/s, 2,000 to
-// 2,500 cycles a tile where its products take 1,030: softmax (1,024 cycles of exponentials a warp) and the rows' way out of L2 take turns at
-// being late. e4m3 345 us: 8,800 warp instructions a tile where bf16 has 6,050 - the scales in softmax, and widening the codes.
+// What bounds it (1,024 tokens of 128 heads on one key head, 2,048 picks of 65,536 shared rows; 112 tiles a CTA, clock 1,965 MHz): bf16
+// 198 us, 690 TFLOP/s, 3,500 cycles a tile where its products take 1,030. Nothing is used up (tcgen05 32 %, issue slots 42 %): a tile waits
+// in turn for its rows out of L2, for softmax (1,024 cycles of exponentials a warp) and to be handed on. e4m3 313 us, 5,500 cycles a tile:
+// the same (tcgen05 23 %, issue slots 43 %), with codes of one tile on their way at a time at D = 128 (kRaw) and 8,800 warp instructions a
+// tile where bf16 has 6,050, for the scales in softmax and widening the codes. ptxas spills 104 to 132 bytes of stores at D = 128 (by role
+// 128, 80 and 64 registers), 8 to 50 at 64.
 //
 // A row's maximum is let stand until a score exceeds it by 2^8 (fp16 and 32-bit sums have the room), so O, which lives in tensor
-// memory, is hardly ever rescaled. fp8: the k scales multiply S, the v scales P, and the reference is the largest score + log2 |v scale|, what a row adds
-// being its weight times its scale; where a tile's v scales lie within 2^kEvenLog the largest of them stands for all, which
-// saves looking at them one by one (1,024 tokens of 128 heads: 332 us, 356 with scales further apart). At the end the groups' O are
-// added, row by row, with the factors their references give.
+// memory, is hardly ever rescaled. fp8: the k scales multiply S, the v scales P, and the reference is the largest score + log2 |v scale|,
+// what a row adds being its weight times its scale; where a tile's v scales lie within 2^kEvenLog the largest of them stands for all,
+// which saves looking at them one by one (1,024 tokens of 128 heads: 313 us, 346 with scales further apart). At the end the groups' O
+// are added, row by row, with the factors their references give.
 // A CTA takes one piece of work after the other (token, key head, 128 query heads), and its gathering warps run ahead into the next
 // one. Few tokens: the CTAs of a cluster take every n-th tile, and join through distributed shared memory.
 // Every wait on an mbarrier has a time limit; when one runs out the CTA raises FFTOPK_ST_STAGE_TIMEOUT, writes NaN for what it has
@@ -72,8 +76,8 @@ constexpr int kEvenLog = 4;       // weights may be smaller than the reference s
 template <bool kFp8, int D>
 struct WideCfg {
   static constexpr uint32_t kTileBytes = kTileKeys * D * 2;  // of Q too
-  // (1,024 tokens of 128 heads on one e4m3 key head: two k and v tiles and room for the codes of one 344 us; one k and one v tile,
-  // codes of two and a query tile ahead 362)
+  // (1,024 tokens of 128 heads on one e4m3 key head, when the kernel took 344 us: one k and one v tile, codes of two and a query tile
+  // ahead 362)
   static constexpr int kQTiles = D == 128 && kFp8 ? 1 : 2, kKStages = 2, kVStages = 2;
   static_assert(kKStages >= 2, "softmax may be a tile behind QK, whose barriers are the k stages'");
   static constexpr int kRaw = kFp8 ? (D == 64 ? 4 : 1) : 0;

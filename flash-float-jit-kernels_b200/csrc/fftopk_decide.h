@@ -330,11 +330,11 @@ FFTOPK_DECIDE_HD bool tile_segment(uint32_t row_g0, uint32_t ntiles, uint32_t g,
 
 // ---------------------------------------------------------------------------------------------
 // Which kernel attention over selected rows goes to, of `group` query heads to a key head.
-// Up to 16 heads fill a row block of the narrow one, which reads each row once then (64 tokens, 4 key heads of 16
-// heads: bf16 51 us, the wide one 66; e4m3 45 and 87). Beyond that the narrow kernel reads every row again for each 16 heads: the wide
-// one takes over - but for e4m3 up to 32 heads (512 tokens of 32 heads: narrow 143, wide 172; of 64 heads, 64 tokens: 44 and 33), and
-// where there is so little work that the narrow kernel can give every piece of it four CTAs (128 heads: 1 token 8.8 and 15.9, 8
-// tokens 15.9 and 15.9, 32 tokens 39 and 20).
+// Up to 16 heads fill a row block of the narrow one, which reads each row once then (64 tokens, 4 key heads of 16 heads: bf16 51 us, the
+// wide one 65; e4m3 44 and 85). Beyond that the narrow kernel reads every row again for each 16 heads: the wide one takes over (512 tokens
+// of 32 heads, bf16: 143 and 108) - but for e4m3 up to 32 heads (140 and 158; of 64 heads, 64 tokens: 43 and 31), and where there is so
+// little work that the narrow kernel can give every piece of it four CTAs (128 heads, bf16: 1 token 8.4 and 15.4, 8 tokens 15.4 and 16.0,
+// 12 tokens 23 and 17; e4m3: 9.9 and 17.9, 18.1 and 19.1, 27 and 20).
 // ---------------------------------------------------------------------------------------------
 constexpr int kAttendHeads = 16;  // query heads that the narrow kernel works on at a time
 FFTOPK_DECIDE_HD int64_t attend_narrow_units(int64_t tokens, int32_t kv_heads, int32_t group) {

@@ -253,10 +253,12 @@ __device__ __forceinline__ void head_rows(const RowParams& p, const int which) {
   }
 }
 
-// What a part is like is known to the whole block, and is a constant of the code that runs: with norm, rotation and quantisation
-// as branches inside one body 16,384 tokens of 72 heads took 165 us instead of 151. Eight blocks of 128 threads per SM, 64 registers
-// (fp32: five), make it 128: a block loads, works and stores once, so the blocks beside it have to keep memory busy (10 blocks
-// spill: 155; two, three or eight heads an item 165, 147, 153).
+// What a part is like is known to the whole block, and is a constant of the code that runs (norm, rotation and quantisation as
+// branches inside one body cost 9 % when that was measured). Eight blocks of 128 threads per SM, 64 registers (fp32: five): a block
+// loads, works and stores once, so the blocks beside it have to keep memory busy. Those 64 registers are shared by eighteen bodies, and ptxas
+// reports 296 bytes of spill stores for 16 lanes (216 with 32, 288 with 8); more registers spill less and hold fewer blocks, which costs
+// more. 16,384 tokens of 72 heads, norm and rotation: 126 us; six blocks 145, seven 134, ten (48 registers) 143; two, three or eight
+// heads an item 171, 146, 149.
 template <typename T, int kLanes, int kHeads, bool kVec, int kNorm, int kRot>
 __device__ __forceinline__ void head_rows(const RowParams& p, int which) {
   if (p.part[which].scale != nullptr)
@@ -471,7 +473,7 @@ int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tok
   for (int i = 0; i < n_parts; ++i)
     if (tokens * (((int64_t)parts[i].heads + (vec ? kHeadsItem - 1 : 0)) / (vec ? kHeadsItem : 1)) > (int64_t)0x7fffffff - 64) return FFTOPK_ERANGE;
   // several heads a group once there are rows for every group of lanes the device holds (16,384 tokens of 72 heads: four heads 126 us,
-  // one 276; 64 tokens of the indexer's step: 5.2 and 3.8)
+  // one 276; 64 tokens of the indexer's step: 5.2 and 3.5)
   int sms = 0;
   const int rc = device_sms(sms);
   if (rc) return rc;

@@ -155,8 +155,8 @@ __device__ __forceinline__ void load4(float* y, const T* p, bool aligned) {
   r.widen(y);
 }
 
-// The lanes of the calling group, as a mask of its warp: groups of one warp may be at work on parts with different norms, each
-// behind branches of its own, so a group's shuffles name its own lanes alone.
+// The lanes of the calling group, as a mask of its warp: one group of a warp may look for the largest finite value of a row with
+// infinities while the others do not, so a group's shuffles name its own lanes alone.
 template <int kLanes>
 __device__ __forceinline__ uint32_t group_mask() {
   if constexpr (kLanes == 32) return 0xffffffffu;

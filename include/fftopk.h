@@ -422,8 +422,9 @@ int fftopk_cache_read(const void* cache, int64_t slot_stride, int64_t head_strid
  *   indices      int32 [tokens, picks], rows idx_row elements apart, inner stride 1; offsets int32 [tokens] or NULL
  *   lse          fp32 [tokens, q_heads], contiguous, or NULL: log of the sum of exponentials
  *   strides      in elements; rows of q, k and v start on 16 bytes
- * Sums and maxima are kept in 32 bits; weights are rounded for the second product: p_j to dtype (16-bit cache), p_j * v_scale_j to
- * fp16 (e4m3), off by 2^-11 of its size and, the small ones, by up to 2^-21 of the largest p_j * |v_scale_j| of the token and head.
+ * Sums and maxima are kept in 32 bits; weights are rounded for the second product: p_j to dtype (16-bit cache; fp16: off by
+ * up to 2^-25 of the largest where small), p_j * v_scale_j to fp16 (e4m3), off by 2^-11 of its size and, the small ones, by up to 2^-21 of
+ * the largest p_j * |v_scale_j| of the token and head.
  * v scales: zero, or magnitudes between 2^-100 and 2^100 (beyond that weights may underflow, or overflow to infinities).
  * The call holds no state and needs no workspace; the first one on a device sets kernel attributes (outside any capture).
  * Should a bounded wait inside the kernel for many heads run out (FFTOPK_ST_STAGE_TIMEOUT; not expected), out and lse are NaN for every

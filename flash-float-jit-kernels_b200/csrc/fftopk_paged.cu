@@ -1,0 +1,834 @@
+// Attention of every sequence's newest token over its whole context, which lies in pages of a cache:
+//   o[b, h] = sum_j p_j v[slot_j, h / g],  p_j = exp(scale * q[b, h] . k[slot_j, h / g] - lse),  slot_j = table[b, j / page] * page + j % page
+// g query heads to a key head, j below the sequence's length. Where asked for, what every cached row has been given so far is brought up
+// to date: weight_out[b, h / g, j] = weight[b, h / g, j] + sum of p_j over the key head's query heads. (The reference ends with indices.)
+//
+// What bounds it is reading the cache: a row of k or v is used by the g heads of its key head alone, 2 g flop a byte in 16 bits.
+//
+// Work split: the context, 16 keys a block, of all sequences, sequence after sequence, is one line of blocks. It is cut into equal runs,
+// whatever the lengths; a warp takes one run for one key head (8 or 16 of its query heads). The warps of neighbouring numbers take the same run for different
+// key heads, so that what lies side by side in the cache - the heads of a row, their scales - is read at about the same time. A warp
+// keeps running maxima and sums (one pass) and writes what it has at the end of a sequence: the result where the run holds all of
+// the sequence, else a part that paged_join_kernel joins. No warp waits for another one. Lengths are read on the device only.
+//
+// A warp has a ring of blocks in shared memory that cp.async fills ahead of it. Keys are the rows of the MMA and query heads its
+// columns, 8 at a time: groups of up to 8 heads need half the products and accumulators they would need as rows.
+//   k.q: the contraction's order is free, so a lane's 16-byte piece of a key row serves as A fragments of consecutive steps, and q is
+//        loaded in the same order.
+//   v.p: A = v transposed, by ldmatrix.trans; scores become weights where they lie and are turned by movmatrix.
+//   e4m3: codes are widened to fp16, which holds each of them exactly; a matrix element of ldmatrix is then a pair of channels, whose
+//        bytes are sorted by key first (the two channels are the rows i and i + 8 of the product). Queries are brought to magnitudes
+//        below 2 by a power of two per head (what fp16 loses of a bf16 query lies 2^-25 below the head's largest). A row's k scale multiplies its score, its v
+//        scale its weight; the running reference is of weight * |v scale|, so that no row with hardly any weight sets it.
+// Roundings: weights of the second product to the cache's type (e4m3: to fp16, their v scale in them), off by half a step; everything
+// else is held in 32 bits.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "../../include/fftopk.h"
+#include "fftopk_attend.cuh"
+#include "fftopk_host.h"
+#include "fftopk_internal.h"
+#include "fftopk_rows.cuh"
+#include "fftopk_tcgen05.cuh"
+
+namespace fftopk {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kKeys = 16;      // of a block: rows of the MMA
+constexpr int kMinBlocks = 4;  // of a run: below that, parts to join cost more than the blocks
+constexpr int kJoinWarps = 8;
+
+struct PagedParams {
+  fftopk_paged a;
+  int32_t group, head_blocks, units, runs, bound, weigh;
+  FastDiv page;
+  float scale_log2;
+  int64_t line;     // positions of a unit of the score workspace
+  int64_t* before;  // [seqs + 1] blocks in front of every sequence
+  float* lse2;      // [seqs, q heads] log2 of the sum of exponentials
+  float2* ml;       // [runs * units * 2][heads of a unit] maximum (log2) and sum of a part
+  float* o;         // [runs * units * 2][heads of a unit][D]
+  float* scores;    // [seqs][units][line][heads of a unit], log2
+  uint32_t* status;
+};
+
+// Keys of sequence b: its length, as far as its pages reach
+__device__ __forceinline__ int32_t keys_of(const PagedParams& p, int64_t b) { return min(max(p.a.lengths[b], 0), p.bound); }
+__device__ __forceinline__ int64_t blocks_of(int32_t n) { return ((int64_t)n + kKeys - 1) / kKeys; }
+
+// Runs the line of `total` blocks is cut into, and where one begins: the first total % runs have a block more.
+__device__ __forceinline__ int64_t live_runs(int64_t total, int32_t runs) { return max((int64_t)1, min((int64_t)runs, total / kMinBlocks)); }
+__device__ __forceinline__ int64_t run_begin(int64_t total, int64_t runs, int64_t run) {
+  return run * (total / runs) + min(run, total % runs);
+}
+__device__ __forceinline__ int64_t run_of(int64_t total, int64_t runs, int64_t block) {
+  const int64_t each = total / runs, rest = total % runs, wide = rest * (each + 1);
+  return block < wide ? block / (each + 1) : rest + (block - wide) / each;  // (each = 0: every block is in front of `wide`)
+}
+
+__device__ __forceinline__ int64_t warp_sum(int64_t x) {
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) x += __shfl_xor_sync(kAll, x, i);
+  return x;
+}
+__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    const int64_t y = __shfl_up_sync(kAll, x, i);
+    if (lane >= i) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ int64_t total_blocks(const PagedParams& p, int lane) {
+  int64_t total = 0;
+  for (int64_t b = lane; b < p.a.seqs; b += 32) total += blocks_of(keys_of(p, b));
+  return warp_sum(total);
+}
+
+// A place on the line: a sequence, its keys and blocks, and one of them
+struct Cursor {
+  int64_t b;
+  int32_t n, blocks, at;
+};
+// Block g of the line (g < total)
+__device__ __forceinline__ Cursor cursor_at(const PagedParams& p, int64_t g, int lane) {
+  Cursor c;
+  int64_t before = 0;
+  for (int64_t first = 0;; first += 32) {
+    const int32_t n = first + lane < p.a.seqs ? keys_of(p, first + lane) : 0;
+    const int64_t upto = before + warp_scan(blocks_of(n), lane);
+    const unsigned beyond = __ballot_sync(kAll, upto > g);
+    if (beyond != 0u || first + 32 >= p.a.seqs) {
+      const int l = beyond != 0u ? __ffs((int)beyond) - 1 : 31;
+      c.b = first + l;
+      c.n = __shfl_sync(kAll, n, l);
+      c.blocks = (int32_t)blocks_of(c.n);
+      c.at = (int32_t)(g - (__shfl_sync(kAll, upto, l) - c.blocks));
+      return c;
+    }
+    before = __shfl_sync(kAll, upto, 31);
+  }
+}
+// The block behind the cursor's; false: the line ends
+__device__ __forceinline__ bool advance(const PagedParams& p, Cursor& c) {
+  if (++c.at < c.blocks) return true;
+  c.at = 0;
+  for (++c.b; c.b < p.a.seqs; ++c.b) {
+    c.n = keys_of(p, c.b);
+    c.blocks = (int32_t)blocks_of(c.n);
+    if (c.n > 0) return true;
+  }
+  return false;
+}
+
+__device__ __forceinline__ uint32_t turned8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ float lds4(uint32_t addr) {
+  float r;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(addr) : "memory");
+  return r;
+}
+// over the lanes that hold the same heads
+__device__ __forceinline__ float keys_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
+  x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
+  return fmaxf(x, __shfl_xor_sync(kAll, x, 16));
+}
+__device__ __forceinline__ float keys_sum(float x) {
+  x += __shfl_xor_sync(kAll, x, 4);
+  x += __shfl_xor_sync(kAll, x, 8);
+  return x + __shfl_xor_sync(kAll, x, 16);
+}
+
+// A warp's ring. Rows are padded so that the lanes that are served together touch all banks: k, where a quad reads 64 neighbouring
+// bytes of each of two rows, by 64 bytes beyond a multiple of 128; v, where eight rows give 16 bytes each, by 16.
+template <bool kFp8, int D>
+struct PagedRing {
+  static constexpr int kRowBytes = D * (kFp8 ? 1 : 2);
+  static constexpr int kKPitch = kRowBytes == 64 ? 64 : kRowBytes + 64, kVPitch = kRowBytes + 16;
+  static constexpr int kV = kKeys * kKPitch, kScales = kV + kKeys * kVPitch;
+  static constexpr int kStage = kScales + (kFp8 ? 2 * kKeys * 4 : 0);
+  static constexpr int kStages = 3;
+  static constexpr int kBytes = kStages * kStage;  // of a warp
+};
+template <bool kFp8, int D>
+constexpr size_t paged_smem() {
+  return (size_t)kWarps * PagedRing<kFp8, D>::kBytes;
+}
+// CTAs per SM: as many as shared memory (228 KB, 1 KB of each CTA is the system's) and the registers of the accumulators allow
+template <bool kFp8, int D, int kNT>
+constexpr int paged_ctas() {
+  constexpr int fit = (int)(228 * 1024 / (paged_smem<kFp8, D>() + 1024)), regs = kNT == 2 ? (D == 64 ? 3 : 2) : 4;
+  return fit < regs ? fit : regs;
+}
+
+// T: type of q and out, and of the cache where kFp8 is false; kNT: eights of query heads
+template <typename T, bool kFp8, int D, int kNT>
+__global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_kernel(const __grid_constant__ PagedParams p) {
+  using M = typename std::conditional<kFp8, __half, T>::type;  // the MMAs' type
+  using G = PagedRing<kFp8, D>;
+  constexpr int kCE = kFp8 ? 16 : 8;         // elements of a 16-byte piece
+  constexpr int kPieces = D / (4 * kCE);     // pieces of a key row per lane (a quad reads a row)
+  constexpr int kStages = G::kStages;
+  constexpr int kNH = 8 * kNT;
+  constexpr int kTiles = D / 16;             // of the output: rows of the MMA are channels
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  // (only where a kernel of this call follows, which waits: another one's inputs may be this one's results)
+  if (p.runs > 1 || p.weigh) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, qd = lane & 3;
+  const uint32_t gw = blockIdx.x * (uint32_t)kWarps + (uint32_t)warp;
+  const uint32_t run = gw / (uint32_t)p.units;
+  const int unit = (int)(gw - run * (uint32_t)p.units);
+  if (run >= (uint32_t)p.runs) return;
+  const int kvh = unit / p.head_blocks, hb = unit - kvh * p.head_blocks;
+  const int heads = min(kNH, p.group - hb * kNH);
+  const int head0 = kvh * p.group + hb * kNH;
+
+  // what is empty, what reaches beyond its pages, and (the first warp) where sequences begin
+  for (int64_t b = run; b < p.a.seqs; b += p.runs) {
+    const int32_t n = p.a.lengths[b];
+    if (n > p.bound && unit == 0 && lane == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+    if (min(n, p.bound) <= 0) {
+      for (int h = 0; h < heads; ++h) {
+        T* out = static_cast<T*>(p.a.out) + b * p.a.out_seq + (int64_t)(head0 + h) * p.a.out_head;
+        for (int d = lane; d < D; d += 32) out[d] = T(0.f);
+        if (lane == 0 && p.a.lse != nullptr) p.a.lse[b * p.a.q_heads + head0 + h] = -INFINITY;
+      }
+    }
+  }
+  if (gw == 0 && p.runs > 1) {
+    int64_t before = 0;
+    for (int64_t first = 0; first < p.a.seqs; first += 32) {
+      const int64_t n = first + lane < p.a.seqs ? blocks_of(keys_of(p, first + lane)) : 0;
+      const int64_t upto = before + warp_scan(n, lane);
+      if (first + lane < p.a.seqs) p.before[first + lane] = upto - n;
+      before = __shfl_sync(kAll, upto, 31);
+    }
+    if (lane == 0) p.before[p.a.seqs] = before;
+  }
+  const int64_t total = total_blocks(p, lane);
+  const int64_t runs = live_runs(total, p.runs);
+  if ((int64_t)run >= runs || total == 0) return;
+  int64_t left = run_begin(total, runs, run + 1) - run_begin(total, runs, run);  // blocks of the run
+  if (left <= 0) return;
+
+  constexpr int kLanesRow = G::kRowBytes / 16, kRowsOnce = 32 / kLanesRow, kTurns = kKeys / kRowsOnce;
+  constexpr int kES = kFp8 ? 1 : 2;
+  const int piece = lane % kLanesRow, sub = lane / kLanesRow;
+  const char* const kbase = static_cast<const char*>(p.a.k) + (int64_t)kvh * p.a.k_head * kES + piece * 16;
+  const char* const vbase = static_cast<const char*>(p.a.v) + (int64_t)kvh * p.a.v_head * kES + piece * 16;
+  const int64_t kstep = p.a.k_slot * kES, vstep = p.a.v_slot * kES;
+  const uint32_t ring = smem_u32(smem_raw) + (uint32_t)warp * G::kBytes;
+
+  Cursor here = cursor_at(p, run_begin(total, runs, run), lane), ahead = here;
+  int64_t to_ask = left;
+  // the lane's key in the block that is asked for next (lanes 16 to 31: the same ones again): its page and place there
+  int32_t page = -1;
+  uint32_t in_page = 0;
+  auto look = [&]() {
+    page = -1;
+    if (to_ask > 0) {
+      const uint32_t j = (uint32_t)ahead.at * kKeys + (uint32_t)(lane & (kKeys - 1));
+      if (j < (uint32_t)ahead.n) {
+        const uint32_t n = p.page.div(j);
+        in_page = j - n * p.page.d;
+        page = p.a.page_table[ahead.b * p.a.table_row + n];
+      }
+      if (--to_ask > 0) advance(p, ahead);
+    }
+  };
+  // asks for the rows and scales of the block looked up; which of them are there
+  auto ask = [&](uint32_t stage) {
+    const int64_t slot = (int64_t)page * p.page.d + in_page;
+    bool ok = page >= 0;
+    if (ok && slot >= p.a.slots) {
+      ok = false;
+      if (p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+    }
+    const unsigned live = __ballot_sync(kAll, ok) & 0xffffu;
+    if (live != 0u) {
+      const int row = ok ? (int)slot : -1;
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int at = i * kRowsOnce + sub;
+        const int r = __shfl_sync(kAll, row, at);
+        copy_or_zero<16>(stage + (uint32_t)(at * G::kKPitch + piece * 16), r >= 0 ? kbase + (int64_t)r * kstep : kbase, r >= 0);
+        copy_or_zero<16>(stage + (uint32_t)(G::kV + at * G::kVPitch + piece * 16), r >= 0 ? vbase + (int64_t)r * vstep : vbase, r >= 0);
+      }
+      if constexpr (kFp8) {  // k scales by the lower lanes, v scales by the upper ones
+        const float* s = lane < kKeys ? p.a.k_scale + (ok ? slot * p.a.ks_slot + (int64_t)kvh * p.a.ks_head : 0)
+                                      : p.a.v_scale + (ok ? slot * p.a.vs_slot + (int64_t)kvh * p.a.vs_head : 0);
+        copy_or_zero<4>(stage + (uint32_t)(G::kScales + lane * 4), s, ok);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    return live;
+  };
+  unsigned live_of[kStages];
+  look();
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    live_of[s] = ask(ring + s * G::kStage);
+    look();
+  }
+  uint32_t at_stage = ring, ask_stage = ring + (kStages - 1) * G::kStage;
+
+  // of the sequence at hand
+  uint32_t qb[kNT][D / 16][2];
+  float qmul[kNT][2];  // what the scores of the lane's heads are to be multiplied with
+  float o[kNT][kTiles][4];
+  // what weights are taken against (log2): the largest score; fp8: the largest score + log2 |v scale|, by the scale's exponent
+  float mx[kNT][2], sum[kNT][2];
+  int32_t first = here.at;  // block that the segment begins with
+  bool fresh = true;
+  int which = 0;  // segments that end or begin elsewhere: 0 the run's first, 1 its last
+  for (;;) {
+    if (fresh) {
+      fresh = false;
+      const T* q0 = static_cast<const T*>(p.a.q) + here.b * p.a.q_seq + (int64_t)head0 * p.a.q_head;
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) {
+        const bool have = 8 * t + g < heads;
+        const T* q = q0 + (int64_t)(8 * t + g) * p.a.q_head;
+        float down = 1.f, up = p.scale_log2;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+#pragma unroll
+          for (int e = 0; e < kCE / 8; ++e) {
+            const uint4 w = have ? *reinterpret_cast<const uint4*>(q + i * 4 * kCE + qd * kCE + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
+            const int m = i * (kCE / 4) + 2 * e;
+            qb[t][m][0] = w.x, qb[t][m][1] = w.y, qb[t][m + 1][0] = w.z, qb[t][m + 1][1] = w.w;
+          }
+        }
+        if constexpr (kFp8 && !std::is_same<T, __half>::value) {
+          float amax = 0.f;
+#pragma unroll
+          for (int m = 0; m < D / 16; ++m) {
+            const float2 a = widen2(qb[t][m][0], T()), b = widen2(qb[t][m][1], T());
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
+          }
+          amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 2));
+          const uint32_t e = __float_as_uint(amax) >> 23;  // amax in [2^(e-127), 2^(e-126)); 255: an infinity
+          const uint32_t ee = e == 255u ? 127u : max(1u, min(e, 253u));
+          down = __uint_as_float((254u - ee) << 23);
+          up *= __uint_as_float(ee << 23);
+#pragma unroll
+          for (int m = 0; m < D / 16; ++m) {
+            const float2 a = widen2(qb[t][m][0], T()), b = widen2(qb[t][m][1], T());
+            qb[t][m][0] = narrow2(a.x * down, a.y * down, __half());
+            qb[t][m][1] = narrow2(b.x * down, b.y * down, __half());
+          }
+        }
+        qmul[t][0] = __shfl_sync(kAll, up, 8 * qd);
+        qmul[t][1] = __shfl_sync(kAll, up, 8 * qd + 4);
+        mx[t][0] = mx[t][1] = -INFINITY;
+        sum[t][0] = sum[t][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+      }
+    }
+    live_of[kStages - 1] = ask(ask_stage);
+    look();
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    __syncwarp();
+    const unsigned live = live_of[0];
+    const uint32_t stage = at_stage;
+    at_stage = at_stage + G::kStage == ring + G::kBytes ? ring : at_stage + G::kStage;
+    ask_stage = ask_stage + G::kStage == ring + G::kBytes ? ring : ask_stage + G::kStage;
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) live_of[s] = live_of[s + 1];
+
+    if (live != 0u || p.weigh) {
+      float sc[kNT][4];  // keys g (0, 1) and g + 8 (2, 3), heads 2 qd and 2 qd + 1
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+      if (live != 0u) {
+        const uint32_t at = stage + (uint32_t)(g * G::kKPitch + qd * 16);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const uint4 x = lds16(at + 64u * i), y = lds16(at + 64u * i + 8u * G::kKPitch);
+          const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int u = 0; u < kCE / 4; ++u) {
+            uint32_t f[4];
+            if constexpr (kFp8) {
+              f[0] = e4m3x2_to_half2((uint16_t)a[u]), f[2] = e4m3x2_to_half2((uint16_t)(a[u] >> 16));
+              f[1] = e4m3x2_to_half2((uint16_t)b[u]), f[3] = e4m3x2_to_half2((uint16_t)(b[u] >> 16));
+            } else {
+              f[0] = a[2 * u], f[2] = a[2 * u + 1], f[1] = b[2 * u], f[3] = b[2 * u + 1];
+            }
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) mma16816(sc[t], f, qb[t][i * (kCE / 4) + u][0], qb[t][i * (kCE / 4) + u][1], M());
+          }
+        }
+      }
+      float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f}, vl[2] = {0.f, 0.f};
+      if constexpr (kFp8) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if (live != 0u) {
+            ks[r] = lds4(stage + (uint32_t)(G::kScales + (g + 8 * r) * 4));
+            vs[r] = lds4(stage + (uint32_t)(G::kScales + (kKeys + g + 8 * r) * 4));
+          }
+          vl[r] = (float)scale_exponent(vs[r]);
+        }
+      }
+      bool over = false;
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = e >> 1;
+          float s = sc[t][e] * qmul[t][e & 1];
+          if constexpr (kFp8) s *= ks[r];
+          sc[t][e] = (live >> (g + 8 * r)) & 1u ? s : -INFINITY;
+          // (a reference is let stand until a score exceeds it by 2^8: fp16 weights and 32-bit sums have the room)
+          over = over || sc[t][e] + vl[r] > mx[t][e & 1] + 8.f;
+        }
+      }
+      if (p.weigh) {
+        float* to = p.scores + ((here.b * p.units + unit) * p.line + (int64_t)here.at * kKeys + g) * kNH + 2 * qd;
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+          *reinterpret_cast<float2*>(to + 8 * t) = make_float2(sc[t][0], sc[t][1]);
+          *reinterpret_cast<float2*>(to + 8 * kNH + 8 * t) = make_float2(sc[t][2], sc[t][3]);
+        }
+      }
+      if (live != 0u) {
+        if (__any_sync(kAll, over)) {
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float top = keys_max(fmaxf(sc[t][e] + vl[0], sc[t][2 + e] + vl[1]));
+              const float m = top > mx[t][e] + 8.f ? top : mx[t][e];
+              const float grow = mx[t][e] == m ? 1.f : ex2(mx[t][e] - m);  // (-inf both: nothing seen yet)
+              sum[t][e] = kFp8 ? brought(sum[t][e], mx[t][e], m) : sum[t][e] * grow;
+              mx[t][e] = m;
+#pragma unroll
+              for (int i = 0; i < kTiles; ++i) o[t][i][e] *= grow, o[t][i][2 + e] *= grow;
+            }
+          }
+        }
+        uint32_t pb[kNT][2];
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+          const float m0 = mx[t][0] == -INFINITY ? 0.f : mx[t][0], m1 = mx[t][1] == -INFINITY ? 0.f : mx[t][1];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float a = ex2(sc[t][2 * r] - m0), b = ex2(sc[t][2 * r + 1] - m1);
+            sum[t][0] += a, sum[t][1] += b;
+            pb[t][r] = turned8x8(kFp8 ? narrow2(a * vs[r], b * vs[r], M()) : narrow2(a, b, M()));
+          }
+        }
+        // lanes 0-7 and 8-15 name the rows of keys 0-7 and 8-15 at one piece, lanes 16-31 at the next
+        const uint32_t vat = stage + (uint32_t)(G::kV + (lane & 15) * G::kVPitch + (lane >> 4) * 16);
+#pragma unroll
+        for (int c = 0; c < G::kRowBytes / 32; ++c) {
+          uint32_t x[4];
+          ldsm4_trans(x, vat + 32u * c);
+          if constexpr (kFp8) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t lo = __byte_perm(x[2 * h], 0u, 0x3120), hi = __byte_perm(x[2 * h + 1], 0u, 0x3120);
+              const uint32_t f[4] = {e4m3x2_to_half2((uint16_t)lo), e4m3x2_to_half2((uint16_t)(lo >> 16)), e4m3x2_to_half2((uint16_t)hi),
+                                     e4m3x2_to_half2((uint16_t)(hi >> 16))};
+#pragma unroll
+              for (int t = 0; t < kNT; ++t) mma16816(o[t][2 * c + h], f, pb[t][0], pb[t][1], M());
+            }
+          } else {
+            const uint32_t f[4] = {x[0], x[2], x[1], x[3]};
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) mma16816(o[t][c], f, pb[t][0], pb[t][1], M());
+          }
+        }
+      }
+    }
+    __syncwarp();  // (the next block but kStages - 2 goes where this one was)
+    --left;
+    if (left > 0 && here.at + 1 < here.blocks) {
+      ++here.at;
+      continue;
+    }
+    // ---- the segment's end ----
+    const bool whole = first == 0 && here.at + 1 == here.blocks;
+    const int64_t rec = (int64_t)gw * 2 + which;
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int h = 8 * t + 2 * qd + e;
+        const float l = keys_sum(sum[t][e]);
+        if (h < heads) {
+          // channels of the accumulators: 16 bits g and g + 8 of a tile, e4m3 2 g and 2 g + 1
+          if (whole) {
+            T* out = static_cast<T*>(p.a.out) + here.b * p.a.out_seq + (int64_t)(head0 + h) * p.a.out_head;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+              out[16 * i + (kFp8 ? 2 * g : g)] = T(l == 0.f ? 0.f : o[t][i][e] * inv);
+              out[16 * i + (kFp8 ? 2 * g + 1 : g + 8)] = T(l == 0.f ? 0.f : o[t][i][2 + e] * inv);
+            }
+            if (g == 0) {
+              const float l2 = l == 0.f ? -INFINITY : mx[t][e] + log2f(l);
+              if (p.a.lse != nullptr) p.a.lse[here.b * p.a.q_heads + head0 + h] = l2 * 0.693147180559945309f;
+              if (p.weigh) p.lse2[here.b * p.a.q_heads + head0 + h] = l2;
+            }
+          } else {
+            float* out = p.o + (rec * kNH + h) * D;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+              out[16 * i + (kFp8 ? 2 * g : g)] = o[t][i][e];
+              out[16 * i + (kFp8 ? 2 * g + 1 : g + 8)] = o[t][i][2 + e];
+            }
+            if (g == 0) p.ml[rec * kNH + h] = make_float2(mx[t][e], l);
+          }
+        }
+      }
+    }
+    if (left <= 0) break;
+    advance(p, here);
+    first = 0;
+    which = 1;
+    fresh = true;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Parts of a sequence that lies in several runs, joined: a CTA per sequence and query head.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedParams p) {
+  __shared__ float2 red[kJoinWarps];
+  __shared__ float part[kJoinWarps][D];
+  if (p.weigh) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t b = blockIdx.x / (uint32_t)p.a.q_heads;
+  const int head = (int)(blockIdx.x - (uint32_t)b * (uint32_t)p.a.q_heads);
+  const int64_t total = p.before[p.a.seqs], begin = p.before[b], end = p.before[b + 1];
+  if (begin == end) return;
+  const int64_t runs = live_runs(total, p.runs);
+  const int64_t r0 = run_of(total, runs, begin), r1 = run_of(total, runs, end - 1);
+  if (r0 == r1) return;
+  const int nh = p.group > 8 ? 16 : 8;
+  const int kvh = head / p.group, in = head - kvh * p.group, hb = in / nh;
+  const int64_t first = (r0 * p.units + kvh * p.head_blocks + hb) * 2 + (run_begin(total, runs, r0) < begin ? 1 : 0);
+  const int h = in - hb * nh, parts = (int)(r1 - r0 + 1);
+  auto record = [&](int i) { return i == 0 ? first : ((r0 + i) * p.units + kvh * p.head_blocks + hb) * 2; };
+
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) m = fmaxf(m, p.ml[record(i) * nh + h].x);
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, i));
+  if (lane == 0) red[warp].x = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, red[w].x);
+  constexpr int kC = D / 32;  // channels of a lane
+  float acc[kC], l = 0.f;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) acc[c] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < parts; i += kJoinWarps) {
+    const int64_t r = record(i) * nh + h;
+    const float2 ml = p.ml[r];
+    const float f = ml.x == m ? 1.f : ex2(ml.x - m);  // (a part without keys: 0 of both; 0 * NaN stays NaN)
+    l += brought(ml.y, ml.x, m);
+    const float* o = p.o + r * D + lane * kC;
+    if constexpr (kC == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(o);
+      acc[0] += f * x.x, acc[1] += f * x.y, acc[2] += f * x.z, acc[3] += f * x.w;
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(o);
+      acc[0] += f * x.x, acc[1] += f * x.y;
+    }
+  }
+  __syncthreads();
+  if (lane == 0) red[warp].y = l;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) part[warp][lane * kC + c] = acc[c];
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) l += red[w].y;
+  for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) y += part[w][d];
+    static_cast<T*>(p.a.out)[b * p.a.out_seq + (int64_t)head * p.a.out_head + d] = T(l == 0.f ? 0.f : y / l);
+  }
+  if (threadIdx.x == 0) {
+    const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
+    if (p.a.lse != nullptr) p.a.lse[b * p.a.q_heads + head] = l2 * 0.693147180559945309f;
+    if (p.weigh) p.lse2[b * p.a.q_heads + head] = l2;
+  }
+}
+
+// The weights brought up to date from the scores and the joined sums: a warp per run and key head, a lane per position.
+template <int kNH>
+__global__ void __launch_bounds__(kThreads) paged_weigh_kernel(const __grid_constant__ PagedParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const uint32_t gw = blockIdx.x * (uint32_t)kWarps + (threadIdx.x >> 5);
+  const uint32_t run = gw / (uint32_t)p.a.kv_heads;
+  const int kvh = (int)(gw - run * (uint32_t)p.a.kv_heads);
+  const int64_t total = total_blocks(p, lane);
+  const int64_t runs = max((int64_t)1, min(total, (int64_t)(gridDim.x * (uint32_t)kWarps / (uint32_t)p.a.kv_heads)));
+  if ((int64_t)run >= runs || total == 0) return;
+  int64_t left = run_begin(total, runs, run + 1) - run_begin(total, runs, run);
+  if (left <= 0) return;
+  Cursor c = cursor_at(p, run_begin(total, runs, run), lane);
+  for (;;) {
+    const int64_t blocks = min(left, (int64_t)(c.blocks - c.at));
+    const int32_t end = (int32_t)min((int64_t)c.n, ((int64_t)c.at + blocks) * kKeys);
+    const float* w = p.a.weight != nullptr ? p.a.weight + c.b * p.a.w_seq + (int64_t)kvh * p.a.w_head : nullptr;
+    float* wo = p.a.weight_out + c.b * p.a.wo_seq + (int64_t)kvh * p.a.wo_head;
+    const float* l2 = p.lse2 + c.b * p.a.q_heads + (int64_t)kvh * p.group;
+    for (int64_t j = (int64_t)c.at * kKeys + lane; j < end; j += 32) {
+      float y = w != nullptr && j < p.a.weight_cols ? w[j] : 0.f;
+      for (int hb = 0; hb < p.head_blocks; ++hb) {
+        const float4* s = reinterpret_cast<const float4*>(p.scores + ((c.b * p.units + kvh * p.head_blocks + hb) * p.line + j) * kNH);
+        const int heads = min(kNH, p.group - hb * kNH);
+#pragma unroll
+        for (int i = 0; i < kNH / 4; ++i) {
+          const float4 x = s[i];
+          const float e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            if (4 * i + n < heads) {
+              const float all = l2[hb * kNH + 4 * i + n];
+              y += all == -INFINITY ? 0.f : ex2(e[n] - all);
+            }
+          }
+        }
+      }
+      if (j < p.a.weight_cols)
+        wo[j] = y;
+      else if (p.status)
+        atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+    }
+    left -= blocks;
+    if (left <= 0) break;
+    c.at = c.blocks - 1;
+    advance(p, c);
+  }
+}
+
+DeviceOnce g_paged_once[kMaxDevices];
+int g_paged_sms[kMaxDevices];
+
+template <typename T, bool kFp8, int D, int kNT>
+int setup_one() {
+  const cudaError_t e =
+      cudaFuncSetAttribute(paged_kernel<T, kFp8, D, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)paged_smem<kFp8, D>());
+  return e == cudaSuccess ? 0 : cuda_fail(e);
+}
+template <typename T, bool kFp8>
+int setup_two() {
+  int r = setup_one<T, kFp8, 64, 1>();
+  if (!r) r = setup_one<T, kFp8, 64, 2>();
+  if (!r) r = setup_one<T, kFp8, 128, 1>();
+  if (!r) r = setup_one<T, kFp8, 128, 2>();
+  return r;
+}
+int paged_setup(int& sms) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e);
+  if (dev < 0 || dev >= kMaxDevices) return FFTOPK_EDEVICE;
+  const int rc = g_paged_once[dev].run([&] {
+    const cudaError_t e2 = cudaDeviceGetAttribute(&g_paged_sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    if (e2 != cudaSuccess) return cuda_fail(e2);
+    int r = setup_two<__nv_bfloat16, false>();
+    if (!r) r = setup_two<__nv_bfloat16, true>();
+    if (!r) r = setup_two<__half, false>();
+    if (!r) r = setup_two<__half, true>();
+    return r;
+  });
+  sms = g_paged_sms[dev];
+  return rc;
+}
+
+template <typename... A>
+cudaError_t launch(void (*kernel)(A...), int64_t grid, int threads, size_t smem, bool dependent, cudaStream_t stream, const PagedParams& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+bool on(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+// rows of 16-byte pieces whatever their sequence (slot) and head; the stride of a lone one says nothing
+bool on16(const void* p, int64_t n, int64_t a, int64_t heads, int64_t b, int bytes) {
+  return on(p, 16) && (n <= 1 || a * bytes % 16 == 0) && (heads <= 1 || b * bytes % 16 == 0);
+}
+
+int ctas_of(bool fp8, int D, int nt) {
+  if (D == 64) return fp8 ? (nt == 1 ? paged_ctas<true, 64, 1>() : paged_ctas<true, 64, 2>()) : nt == 1 ? paged_ctas<false, 64, 1>() : paged_ctas<false, 64, 2>();
+  return fp8 ? (nt == 1 ? paged_ctas<true, 128, 1>() : paged_ctas<true, 128, 2>()) : nt == 1 ? paged_ctas<false, 128, 1>() : paged_ctas<false, 128, 2>();
+}
+
+// Sizes of the call, checked; what the workspace holds in turn: `before`, lse2, ml, o, scores
+struct Plan {
+  int nt = 1, nh = 8;
+  int64_t ctas = 0, bytes[5] = {}, total = 0;
+};
+int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+int make_plan(const fftopk_paged* a, int sms, PagedParams& p, Plan& plan) {
+  memset(&p, 0, sizeof(p));
+  p.a = *a;
+  p.group = a->q_heads / a->kv_heads;
+  plan.nt = p.group > 8 ? 2 : 1;
+  plan.nh = 8 * plan.nt;
+  p.head_blocks = (p.group + plan.nh - 1) / plan.nh;
+  const int64_t units = (int64_t)a->kv_heads * p.head_blocks;
+  const int64_t bound = (int64_t)a->pages * a->page_size;
+  if (units > 0x1000000 || a->seqs > 0x7fffffff / a->q_heads || bound > 0x7ffffff0) return FFTOPK_ERANGE;
+  p.units = (int32_t)units;
+  p.bound = (int32_t)bound;
+  p.weigh = a->weight_out != nullptr;
+  const int64_t blocks = a->seqs * ((bound + kKeys - 1) / kKeys);
+  const int64_t warps = (int64_t)sms * ctas_of(a->k_scale != nullptr, a->D, plan.nt) * kWarps;
+  int64_t runs = warps / units < blocks / kMinBlocks ? warps / units : blocks / kMinBlocks;
+  if (runs < 1) runs = 1;
+  p.runs = (int32_t)runs;
+  plan.ctas = (runs * units + kWarps - 1) / kWarps;
+  p.line = (bound + kKeys - 1) / kKeys * kKeys;
+  if (runs > 1) {
+    plan.bytes[0] = up256((a->seqs + 1) * 8);
+    plan.bytes[2] = up256(runs * units * 2 * plan.nh * 8);
+    plan.bytes[3] = up256(runs * units * 2 * plan.nh * a->D * 4);
+  }
+  if (p.weigh) {
+    plan.bytes[1] = up256(a->seqs * a->q_heads * 4);
+    // (below 2^31 sequences * heads, times 2^31 positions, times 64 bytes: in question where it would wrap)
+    if (p.line > 0 && a->seqs * units > ((int64_t)1 << 50) / (p.line * plan.nh)) return FFTOPK_ERANGE;
+    plan.bytes[4] = up256(a->seqs * units * p.line * plan.nh * 4);
+  }
+  for (int64_t n : plan.bytes) plan.total += n;
+  return 0;
+}
+
+int check(const fftopk_paged* a) {
+  if (a == nullptr) return FFTOPK_EINVAL;
+  if (a->seqs < 0 || a->kv_heads < 0 || a->q_heads < 0 || a->slots < 0 || a->pages < 0 || a->page_size < 1 || a->weight_cols < 0) return FFTOPK_EINVAL;
+  if (a->dtype != FFTOPK_DTYPE_FP16 && a->dtype != FFTOPK_DTYPE_BF16) return FFTOPK_EINVAL;
+  if (a->D != 64 && a->D != 128) return FFTOPK_ERANGE;
+  if (a->seqs == 0 || a->q_heads == 0) return FFTOPK_OK;
+  if (a->kv_heads == 0 || a->q_heads % a->kv_heads != 0) return FFTOPK_EINVAL;
+  const bool fp8 = a->k_scale != nullptr;
+  if (fp8 != (a->v_scale != nullptr)) return FFTOPK_EINVAL;
+  if (!a->q || !a->out || !a->lengths || (a->pages > 0 && !a->page_table) || (a->pages > 0 && a->slots > 0 && (!a->k || !a->v))) return FFTOPK_EINVAL;
+  if (a->weight != nullptr && a->weight_out == nullptr) return FFTOPK_EINVAL;
+  const int ce = fp8 ? 1 : 2;
+  if (!on16(a->q, a->seqs, a->q_seq, a->q_heads, a->q_head, 2) || !on16(a->k, a->slots, a->k_slot, a->kv_heads, a->k_head, ce) ||
+      !on16(a->v, a->slots, a->v_slot, a->kv_heads, a->v_head, ce))
+    return FFTOPK_EINVAL;
+  if (!on(a->out, 2) || !on(a->page_table, 4) || !on(a->lengths, 4) || !on(a->lse, 4) || !on(a->k_scale, 4) || !on(a->v_scale, 4) ||
+      !on(a->weight, 4) || !on(a->weight_out, 4))
+    return FFTOPK_EINVAL;
+  if (a->slots > 0x7fffffff || a->seqs > 0x7fffffff) return FFTOPK_ERANGE;
+  return FFTOPK_OK;
+}
+
+template <typename T, bool kFp8, int D>
+cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {
+  return plan.nt == 1 ? launch(paged_kernel<T, kFp8, D, 1>, plan.ctas, kThreads, paged_smem<kFp8, D>(), false, stream, p)
+                      : launch(paged_kernel<T, kFp8, D, 2>, plan.ctas, kThreads, paged_smem<kFp8, D>(), false, stream, p);
+}
+template <typename T>
+cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {
+  const bool fp8 = p.a.k_scale != nullptr;
+  const bool d64 = p.a.D == 64;
+  cudaError_t e = fp8 ? (d64 ? launch_paged<T, true, 64>(p, plan, stream) : launch_paged<T, true, 128>(p, plan, stream))
+                      : d64 ? launch_paged<T, false, 64>(p, plan, stream) : launch_paged<T, false, 128>(p, plan, stream);
+  if (e == cudaSuccess && p.runs > 1) {
+    const int64_t grid = p.a.seqs * p.a.q_heads;
+    e = launch(d64 ? paged_join_kernel<T, 64> : paged_join_kernel<T, 128>, grid, kJoinWarps * 32, 0, true, stream, p);
+  }
+  return e;
+}
+
+}  // namespace
+}  // namespace fftopk
+
+using namespace fftopk;
+
+extern "C" {
+
+int fftopk_paged_workspace_bytes(const fftopk_paged* a, size_t* bytes) {
+  if (bytes == nullptr) return FFTOPK_EINVAL;
+  *bytes = 0;
+  int rc = check(a);
+  if (rc || a->seqs == 0 || a->q_heads == 0) return rc;
+  int sms = 0;
+  rc = paged_setup(sms);
+  if (rc) return rc;
+  PagedParams p;
+  Plan plan;
+  rc = make_plan(a, sms, p, plan);
+  if (rc == 0) *bytes = (size_t)plan.total;
+  return rc;
+}
+
+int fftopk_paged_attention(const fftopk_paged* a, void* workspace, size_t workspace_bytes, uint32_t* status, void* cuda_stream) {
+  int rc = check(a);
+  if (rc || a->seqs == 0 || a->q_heads == 0) return rc;
+  int sms = 0;
+  rc = paged_setup(sms);
+  if (rc) return rc;
+  PagedParams p;
+  Plan plan;
+  rc = make_plan(a, sms, p, plan);
+  if (rc) return rc;
+  if (plan.total > 0 && (workspace == nullptr || !on(workspace, 256) || workspace_bytes < (size_t)plan.total)) return FFTOPK_EINVAL;
+  if (a->slots == 0) p.a.k = p.a.v = a->q;  // (an empty cache has no address, and rows that are left out are copies of no bytes: from somewhere)
+  p.page = FastDiv((uint32_t)a->page_size);
+  p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
+  p.status = status;
+  char* at = static_cast<char*>(workspace);
+  p.before = reinterpret_cast<int64_t*>(at), at += plan.bytes[0];
+  p.lse2 = reinterpret_cast<float*>(at), at += plan.bytes[1];
+  p.ml = reinterpret_cast<float2*>(at), at += plan.bytes[2];
+  p.o = reinterpret_cast<float*>(at), at += plan.bytes[3];
+  p.scores = reinterpret_cast<float*>(at);
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  cudaError_t e = a->dtype == FFTOPK_DTYPE_BF16 ? launch_paged<__nv_bfloat16>(p, plan, stream) : launch_paged<__half>(p, plan, stream);
+  if (e == cudaSuccess && p.weigh) {
+    int64_t runs = (int64_t)sms * 8 * kWarps / a->kv_heads;
+    const int64_t blocks = a->seqs * (p.line / kKeys);
+    if (runs > blocks) runs = blocks;
+    if (runs < 1) runs = 1;
+    const int64_t grid = (runs * a->kv_heads + kWarps - 1) / kWarps;
+    e = launch(plan.nt == 1 ? paged_weigh_kernel<8> : paged_weigh_kernel<16>, grid, kThreads, 0, true, stream, p);
+  }
+  return e == cudaSuccess ? FFTOPK_OK : cuda_fail(e);
+}
+
+}  // extern "C"

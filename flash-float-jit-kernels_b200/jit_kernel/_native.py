@@ -56,6 +56,8 @@ EXPORTS = (
     "fftopk_head_rows",
     "fftopk_cache_read",
     "fftopk_sparse_attention",
+    "fftopk_paged_workspace_bytes",
+    "fftopk_paged_attention",
     "fftopk_set_attend_stop",
     "fftopk_probe_read_bandwidth",
     "fftopk_key_of",
@@ -172,6 +174,10 @@ def lib() -> ctypes.CDLL:
                                     c.c_void_p]
     L.fftopk_sparse_attention.restype = c.c_int
     L.fftopk_sparse_attention.argtypes = [c.c_char_p, c.c_void_p, c.c_void_p]
+    L.fftopk_paged_workspace_bytes.restype = c.c_int
+    L.fftopk_paged_workspace_bytes.argtypes = [c.c_char_p, c.POINTER(c.c_size_t)]
+    L.fftopk_paged_attention.restype = c.c_int
+    L.fftopk_paged_attention.argtypes = [c.c_char_p, c.c_void_p, c.c_size_t, c.c_void_p, c.c_void_p]
     L.fftopk_set_attend_stop.restype = c.c_int
     L.fftopk_set_attend_stop.argtypes = [c.c_int64, c.c_int64]
     L.fftopk_probe_read_bandwidth.restype = c.c_int

@@ -454,6 +454,58 @@ typedef struct fftopk_attend {
 int fftopk_sparse_attention(const fftopk_attend* args, uint32_t* status, void* cuda_stream);
 
 /*
+ * Attention of every sequence's newest token over its whole context, which lies in pages of a cache.
+ *   out[b, h] = sum_j p_j v[slot_j, h / group],  p_j = exp(softmax_scale q[b, h] . k[slot_j, h / group] - lse[b, h]),  j < lengths[b],
+ *   slot_j = page_table[b, j / page_size] * page_size + j % page_size,  group = q_heads / kv_heads
+ * and, where weight_out is given, the weights every cached row has had: for j < lengths[b]
+ *   weight_out[b, g, j] = weight[b, g, j] + sum of p_j over the query heads of key head g        (weight NULL: 0)
+ * Lengths of 0 or less: zeros and lse -inf. A negative page is left out, with the positions on it (their p is 0). A slot at or beyond
+ * `slots` is left out too and raises FFTOPK_ST_BAD_INDEX, as do positions beyond the table and weights beyond weight_cols. Entries of
+ * the table behind a sequence's length are not read, nor is anything of rows that no sequence names; weight_out behind a sequence's
+ * length stays as it was.
+ *   q, out       [seqs, q_heads, D] of dtype (fp16 or bf16), D 64 or 128 (FFTOPK_ERANGE otherwise)
+ *   k, v         [slots, kv_heads, D] of dtype, or - k_scale and v_scale given, fp32 [slots, kv_heads] - e4m3 codes
+ *   page_table   int32 [seqs, pages], rows table_row elements apart, inner stride 1; lengths int32 [seqs]; both on the device
+ *   lse          fp32 [seqs, q_heads], contiguous, or NULL
+ *   weight       fp32 [seqs, kv_heads, weight_cols], inner stride 1, or NULL; weight_out likewise, or NULL: no weights; the two may be
+ *                one array, and overlap in no other way
+ *   strides      in elements; rows of q, k and v start on 16 bytes; page_size any number from 1
+ *   workspace    fftopk_paged_workspace_bytes bytes of device memory, 256-byte aligned, any contents; calls that may run at the same
+ *                time need one each. With weight_out it holds the scores of all positions the table has room for, 32 bytes (of more
+ *                than 8 query heads to a key head: 64 for every 16) per position and key head. The size is that of the current device.
+ * Roundings, and what is asked of v scales: as for fftopk_sparse_attention. The same call gives the same bits.
+ * The first call on a device sets kernel attributes (outside any capture); up to three kernels, no host synchronisation.
+ */
+typedef struct fftopk_paged {
+  const void* q;
+  int64_t q_seq, q_head;
+  const void* k;
+  int64_t k_slot, k_head;
+  const void* v;
+  int64_t v_slot, v_head;
+  const float* k_scale;
+  int64_t ks_slot, ks_head;
+  const float* v_scale;
+  int64_t vs_slot, vs_head;
+  const int32_t* page_table;
+  int64_t table_row;
+  const int32_t* lengths;
+  void* out;
+  int64_t out_seq, out_head;
+  float* lse;
+  const float* weight;
+  int64_t w_seq, w_head;
+  float* weight_out;
+  int64_t wo_seq, wo_head;
+  int64_t weight_cols, seqs, slots;
+  int32_t q_heads, kv_heads, D, pages, page_size, dtype;
+  float softmax_scale;
+  int32_t reserved;
+} fftopk_paged;
+int fftopk_paged_workspace_bytes(const fftopk_paged* args, size_t* bytes);
+int fftopk_paged_attention(const fftopk_paged* args, void* workspace, size_t workspace_bytes, uint32_t* status, void* cuda_stream);
+
+/*
  * Measurement aid, not part of the selection path (no reference counterpart): a read-only bandwidth
  * probe. One kernel in which every SM reads the buffer with 128-bit loads that bypass L1, wrapping
  * around until about `bytes_to_read` bytes have been read in total; *bytes_read receives the exact

@@ -1,0 +1,49 @@
+"""Calls of the paged attention's entry that are refused before anything is enqueued: no device is needed, and the pointers named
+here are never followed."""
+import ctypes
+
+import pytest
+import torch
+
+from jit_kernel import _native
+from jit_kernel.paged_attention import _ARGS, paged_attention
+
+EINVAL, ERANGE = -1, -4
+A = 1 << 20  # an aligned address
+
+CALL = dict(q=A, qs=1024, qh=128, k=A, ks=128, kh=128, v=A, vs=128, vh=128, k_scale=0, kss=0, ksh=0, v_scale=0, vss=0, vsh=0, table=A, row=8,
+            lengths=A, out=A, os=1024, oh=128, lse=0, w=0, ws=0, wh=0, wo=0, wos=0, woh=0, cols=0, seqs=2, slots=100, q_heads=8, kv_heads=1,
+            D=128, pages=8, page_size=16, dtype=1, scale=0.1, reserved=0)
+
+
+def test_struct_size():
+    """The packed arguments have the C struct's size: pointers and 64-bit fields, then eight 32-bit ones."""
+    assert _ARGS.size == 31 * 8 + 8 * 4
+
+
+@pytest.mark.parametrize("want,call", [
+    (EINVAL, dict(seqs=-1)), (EINVAL, dict(q_heads=-1)), (EINVAL, dict(kv_heads=-1)), (EINVAL, dict(pages=-1)), (EINVAL, dict(page_size=0)),
+    (EINVAL, dict(slots=-1)), (EINVAL, dict(cols=-1)), (EINVAL, dict(dtype=2)), (ERANGE, dict(D=96)), (ERANGE, dict(D=256)),
+    (EINVAL, dict(kv_heads=0)), (EINVAL, dict(kv_heads=3)), (EINVAL, dict(k_scale=A)), (EINVAL, dict(v_scale=A)), (EINVAL, dict(q=0)),
+    (EINVAL, dict(out=0)), (EINVAL, dict(table=0)), (EINVAL, dict(lengths=0)), (EINVAL, dict(k=0)), (EINVAL, dict(v=0)), (EINVAL, dict(q=A + 8)),
+    (EINVAL, dict(k=A + 8)), (EINVAL, dict(v=A + 8)), (EINVAL, dict(qs=1028)), (EINVAL, dict(qh=68)), (EINVAL, dict(ks=132)),
+    (EINVAL, dict(vs=132)), (EINVAL, dict(kv_heads=2, kh=68)), (EINVAL, dict(out=A + 1)), (EINVAL, dict(table=A + 2)),
+    (EINVAL, dict(lengths=A + 1)), (EINVAL, dict(lse=A + 2)), (EINVAL, dict(k_scale=A + 2, v_scale=A)), (EINVAL, dict(w=A)),
+    (EINVAL, dict(wo=A + 2)), (ERANGE, dict(slots=1 << 31)), (ERANGE, dict(seqs=1 << 31)), (0, dict(seqs=0)), (0, dict(q_heads=0))])
+def test_paged_attention(want, call):
+    blob, n = _ARGS.pack(*{**CALL, **call}.values()), ctypes.c_size_t(7)
+    assert _native.lib().fftopk_paged_attention(blob, None, 0, None, None) == want
+    assert _native.lib().fftopk_paged_workspace_bytes(blob, ctypes.byref(n)) == want and n.value == 0
+
+
+def test_without_arguments():
+    n = ctypes.c_size_t()
+    assert _native.lib().fftopk_paged_attention(None, None, 0, None, None) == EINVAL
+    assert _native.lib().fftopk_paged_workspace_bytes(None, ctypes.byref(n)) == EINVAL
+    assert _native.lib().fftopk_paged_workspace_bytes(_ARGS.pack(*CALL.values()), None) == EINVAL
+
+
+def test_cpu_tensors_are_refused():
+    x, c, i = torch.zeros(2, 4, 64).half(), torch.zeros(8, 4, 64).half(), torch.zeros(2, 1, dtype=torch.int32)
+    with pytest.raises(RuntimeError):
+        paged_attention(x, c, c, i, i[:, 0].contiguous(), page_size=4)

@@ -58,6 +58,7 @@ EXPORTS = (
     "fftopk_sparse_attention",
     "fftopk_paged_workspace_bytes",
     "fftopk_paged_attention",
+    "fftopk_cache_evict",
     "fftopk_set_attend_stop",
     "fftopk_probe_read_bandwidth",
     "fftopk_key_of",
@@ -178,6 +179,8 @@ def lib() -> ctypes.CDLL:
     L.fftopk_paged_workspace_bytes.argtypes = [c.c_char_p, c.POINTER(c.c_size_t)]
     L.fftopk_paged_attention.restype = c.c_int
     L.fftopk_paged_attention.argtypes = [c.c_char_p, c.c_void_p, c.c_size_t, c.c_void_p, c.c_void_p]
+    L.fftopk_cache_evict.restype = c.c_int
+    L.fftopk_cache_evict.argtypes = [c.c_char_p, c.c_void_p, c.c_void_p]
     L.fftopk_set_attend_stop.restype = c.c_int
     L.fftopk_set_attend_stop.argtypes = [c.c_int64, c.c_int64]
     L.fftopk_probe_read_bandwidth.restype = c.c_int

@@ -10,29 +10,13 @@ from typing import Optional
 import torch
 
 from . import _native
+from .kv_cache import _check_table, _check_weight
 from .norm_rope import _DENSE, FP8, _check_cache, _check_vector, _no_grad
 from .sparse_attention import _TYPES
 from .topk_indexer import _current_device, _launch
 
 #: fftopk_paged (include/fftopk.h)
 _ARGS = struct.Struct("@PqqPqqPqqPqqPqqPqPPqqPPqqPqqqqqiiiiiifi")
-
-
-def _check_table(t: torch.Tensor, what: str, idx: int, seqs: int):
-    """(address, row stride, columns) of a page table"""
-    shape, step = t.shape, t.stride()
-    if t.dtype is not torch.int32 or len(shape) != 2 or shape[0] != seqs or t.get_device() != idx or (shape[1] > 1 and step[1] != 1):
-        raise RuntimeError(f"{what} must be an int32 tensor [sequences, pages] with unit inner stride on the cache's device")
-    return t.data_ptr(), step[0], shape[1]
-
-
-def _check_weight(t: torch.Tensor, what: str, idx: int, seqs: int, heads: int, cols: int = -1):
-    """(strides, columns) of weights [sequences, key heads, positions]"""
-    shape, step = t.shape, t.stride()
-    if t.dtype is not torch.float32 or len(shape) != 3 or shape[0] != seqs or shape[1] != heads or t.get_device() != idx \
-            or (cols >= 0 and shape[2] != cols) or (shape[2] > 1 and step[2] != 1):
-        raise RuntimeError(f"{what} must be float32 [sequences, key heads, positions] with unit inner stride on the cache's device")
-    return step, shape[2]
 
 
 def paged_attention(

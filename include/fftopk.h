@@ -506,6 +506,50 @@ int fftopk_paged_workspace_bytes(const fftopk_paged* args, size_t* bytes);
 int fftopk_paged_attention(const fftopk_paged* args, void* workspace, size_t workspace_bytes, uint32_t* status, void* cuda_stream);
 
 /*
+ * Eviction from a paged cache by accumulated attention weight (what fftopk_paged_attention adds up). For sequence b and key head h, with
+ * n = lengths[b] (at least 0) and m = min(n, budget):
+ *   kept[b, h, 0 .. m-1]        the positions that stay, ascending; -1 behind them: all n where n <= budget, else the first `sinks`, the last
+ *                               `recent` and, of those between, the ones of the largest weights - of equal weights the lower positions (-0 equals
+ *                               0, NaN counts as the largest)
+ *   new_lengths[b]              m
+ *   weight_out[b, h, i]         weight[b, h, kept[b, h, i]] for i < m, 0 behind
+ *   caches, scales              row to_table[b, i / page_size] * page_size + i % page_size of head h gets what the row of position kept[b, h, i] holds
+ * A row whose page is negative, or that lies at or beyond `slots`, on either side, is not copied and raises FFTOPK_ST_BAD_INDEX; a length
+ * beyond the table or the weights counts as that far and raises it too. Rows that to_table names must not be rows that page_table names
+ * for any sequence of the call; rows that to_table does not name stay as they are.
+ *   k, v         [slots, heads, D] of elem_bytes (1 or 2) each, D a multiple of 8 up to 256 (FFTOPK_ERANGE otherwise); k_scale, v_scale fp32
+ *                [slots, heads], or both NULL; strides in elements
+ *   weight, weight_out fp32 [seqs, heads, weight_cols], inner stride 1, apart from one another
+ *   page_table   int32 [seqs, pages], to_table int32 [seqs, to_pages], inner stride 1; to_pages * page_size >= budget (FFTOPK_ERANGE otherwise)
+ *   kept         int32 [seqs, heads, budget], contiguous; lengths, new_lengths int32 [seqs]; sinks + recent <= budget
+ * No workspace, no host synchronisation; two kernels. The first call on a device sets kernel attributes (outside any capture).
+ */
+typedef struct fftopk_evict {
+  void* k;
+  int64_t k_slot, k_head;
+  void* v;
+  int64_t v_slot, v_head;
+  float* k_scale;
+  int64_t ks_slot, ks_head;
+  float* v_scale;
+  int64_t vs_slot, vs_head;
+  const float* weight;
+  int64_t w_seq, w_head;
+  float* weight_out;
+  int64_t wo_seq, wo_head;
+  const int32_t* page_table;
+  int64_t table_row;
+  const int32_t* to_table;
+  int64_t to_row;
+  const int32_t* lengths;
+  int32_t* new_lengths;
+  int32_t* kept;
+  int64_t weight_cols, seqs, slots;
+  int32_t heads, D, elem_bytes, pages, to_pages, page_size, budget, recent, sinks, reserved;
+} fftopk_evict;
+int fftopk_cache_evict(const fftopk_evict* args, uint32_t* status, void* cuda_stream);
+
+/*
  * Measurement aid, not part of the selection path (no reference counterpart): a read-only bandwidth
  * probe. One kernel in which every SM reads the buffer with 128-bit loads that bypass L1, wrapping
  * around until about `bytes_to_read` bytes have been read in total; *bytes_read receives the exact

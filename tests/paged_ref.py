@@ -57,3 +57,42 @@ def check_weights(got, before, lengths, w, e, what=""):
     lim = e[..., :n] + 2 * ref.U32 * want.abs()
     off = torch.where(inside[..., :n], (got[..., :n].double() - want).abs(), 0.0)
     assert bool((off <= lim).all()), f"{what}: worst {float((off / lim).max()):.2f} x the bound"
+
+
+def evict(weight, lengths, budget, recent, sinks):
+    """(kept, lengths, weights) from the definition, sequence by sequence and head by head, on the CPU: weights are compared as they
+    are (-0 equals 0, NaN above infinity), of equal ones the lower position stays."""
+    weight = weight.cpu()
+    B, H, N = weight.shape
+    kept = torch.full((B, H, budget), -1, dtype=torch.int32)
+    out = torch.zeros_like(weight)
+    left = []
+    for b, n in enumerate(lengths.tolist()):
+        n = min(max(n, 0), N)
+        left.append(min(n, budget))
+        for h in range(H):
+            stay = list(range(n))
+            if n > budget:
+                row = weight[b, h].tolist()
+                order = sorted(range(sinks, n - recent), key=lambda j: (row[j] == row[j], -row[j] if row[j] == row[j] else 0.0, j))
+                stay = sorted(list(range(sinks)) + list(range(n - recent, n)) + order[:budget - sinks - recent])
+            kept[b, h, :len(stay)] = torch.tensor(stay, dtype=torch.int32)
+            out[b, h, :len(stay)] = weight[b, h][stay]
+    return kept, torch.tensor(left, dtype=torch.int32), out
+
+
+def move(cache, kept, page_table, to_table, page):
+    """What the rows of `cache` [slots, H, ..] (or a scale) hold afterwards."""
+    out = cache.clone()
+    src, dst = (x.view(torch.uint8) if x.dtype.itemsize == 1 else x for x in (cache, out))
+    B, H, _ = kept.shape
+    slots = cache.size(0)
+    for b in range(B):
+        for h in range(H):
+            pos = kept[b, h][kept[b, h] >= 0].long().to(cache.device)
+            i = torch.arange(pos.numel(), device=cache.device)
+            p, t = page_table[b].long()[pos // page], to_table[b].long()[i // page]
+            a, z = p * page + pos % page, t * page + i % page
+            ok = (p >= 0) & (t >= 0) & (a < slots) & (z < slots)
+            dst[z[ok], h] = src[a[ok], h]
+    return out

@@ -1,4 +1,4 @@
-"""Calls of the paged attention's entry that are refused before anything is enqueued: no device is needed, and the pointers named
+"""Calls of the paged cache's entries that are refused before anything is enqueued: no device is needed, and the pointers named
 here are never followed."""
 import ctypes
 
@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from jit_kernel import _native
+from jit_kernel.kv_cache import _EVICT, cache_evict
 from jit_kernel.paged_attention import _ARGS, paged_attention
 
 EINVAL, ERANGE = -1, -4
@@ -43,7 +44,33 @@ def test_without_arguments():
     assert _native.lib().fftopk_paged_workspace_bytes(_ARGS.pack(*CALL.values()), None) == EINVAL
 
 
+EVICT = dict(k=A, ks=128, kh=128, v=A, vs=128, vh=128, k_scale=0, kss=0, ksh=0, v_scale=0, vss=0, vsh=0, w=A, ws=64, wh=64, wo=2 * A, wos=64,
+             woh=64, table=A, row=8, to=A, to_row=8, lengths=A, new=A, kept=A, cols=64, seqs=2, slots=100, heads=1, D=128, elem=2, pages=8,
+             to_pages=4, page_size=16, budget=32, recent=4, sinks=4, reserved=0)
+
+
+@pytest.mark.parametrize("want,call", [
+    (EINVAL, dict(seqs=-1)), (EINVAL, dict(heads=-1)), (EINVAL, dict(slots=-1)), (EINVAL, dict(pages=-1)), (EINVAL, dict(to_pages=-1)),
+    (EINVAL, dict(page_size=0)), (EINVAL, dict(budget=-1, recent=0, sinks=0)), (EINVAL, dict(recent=-1)), (EINVAL, dict(sinks=-1)), (EINVAL, dict(cols=-1)),
+    (EINVAL, dict(recent=29)), (EINVAL, dict(recent=0x7fffffff, sinks=0x7fffffff)), (EINVAL, dict(elem=4)), (EINVAL, dict(elem=0)), (ERANGE, dict(D=4)),
+    (ERANGE, dict(D=12)), (ERANGE, dict(D=264)), (EINVAL, dict(k_scale=A)), (EINVAL, dict(v_scale=A)), (EINVAL, dict(lengths=0)), (EINVAL, dict(new=0)),
+    (EINVAL, dict(kept=0)), (EINVAL, dict(table=0)), (EINVAL, dict(to=0)), (EINVAL, dict(w=0)), (EINVAL, dict(wo=0)), (EINVAL, dict(wo=A)),
+    (EINVAL, dict(k=0)), (EINVAL, dict(v=0)), (EINVAL, dict(k=A + 1)), (EINVAL, dict(v=A + 1)), (EINVAL, dict(w=A + 2)), (EINVAL, dict(kept=A + 2)),
+    (EINVAL, dict(table=A + 1)), (EINVAL, dict(to=A + 2)), (EINVAL, dict(lengths=A + 2)), (EINVAL, dict(new=A + 2)), (ERANGE, dict(slots=1 << 31)),
+    (ERANGE, dict(seqs=1 << 31)), (ERANGE, dict(seqs=1 << 30, heads=4)), (ERANGE, dict(budget=65)), (ERANGE, dict(pages=0x7fffffff, cols=1 << 31)),
+    (ERANGE, dict(seqs=1 << 27, budget=1 << 20, to_pages=1 << 16)), (0, dict(seqs=0)), (0, dict(heads=0))])
+def test_cache_evict(want, call):
+    assert _native.lib().fftopk_cache_evict(_EVICT.pack(*{**EVICT, **call}.values()), None, None) == want
+
+
+def test_evict_without_arguments():
+    assert _EVICT.size == 28 * 8 + 10 * 4
+    assert _native.lib().fftopk_cache_evict(None, None, None) == EINVAL
+
+
 def test_cpu_tensors_are_refused():
     x, c, i = torch.zeros(2, 4, 64).half(), torch.zeros(8, 4, 64).half(), torch.zeros(2, 1, dtype=torch.int32)
     with pytest.raises(RuntimeError):
         paged_attention(x, c, c, i, i[:, 0].contiguous(), page_size=4)
+    with pytest.raises(RuntimeError):
+        cache_evict(c, c, torch.zeros(2, 4, 8), i, i[:, 0].contiguous(), i, page_size=4, budget=4)

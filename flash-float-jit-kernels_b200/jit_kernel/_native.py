@@ -54,6 +54,7 @@ EXPORTS = (
     "fftopk_indexer_topk2048",
     "fftopk_indexer_topk2048_fp8",
     "fftopk_head_rows",
+    "fftopk_head_rows_axes",
     "fftopk_cache_read",
     "fftopk_sparse_attention",
     "fftopk_paged_workspace_bytes",
@@ -169,6 +170,9 @@ def lib() -> ctypes.CDLL:
     L.fftopk_head_rows.restype = c.c_int
     L.fftopk_head_rows.argtypes = [c.c_char_p, c.c_int32, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_void_p, c.c_int64,
                                    c.c_int32, c.c_int32, c.c_void_p, c.c_void_p]
+    L.fftopk_head_rows_axes.restype = c.c_int
+    L.fftopk_head_rows_axes.argtypes = [c.c_char_p, c.c_int32, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_int64, c.c_int32,
+                                        c.c_char_p, c.c_void_p, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_void_p]
     L.fftopk_cache_read.restype = c.c_int
     L.fftopk_cache_read.argtypes = [c.c_void_p, c.c_int64, c.c_int64, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_int64,
                                     c.c_int64, c.c_void_p, c.c_int64, c.c_int64, c.c_void_p, c.c_void_p, c.c_int32, c.c_void_p,

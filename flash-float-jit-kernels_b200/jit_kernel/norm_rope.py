@@ -8,7 +8,7 @@ inputs' type and round once. They serve: none has a gradient, and a tensor that 
 from __future__ import annotations
 
 import struct
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 from torch.autograd import forward_ad
@@ -108,6 +108,11 @@ def _quantised(x, xs, heads, out, os, scale, ss, slots=0, n=0, mul=0, norm=_PLAI
 
 
 def _rows(idx: int, parts: bytes, tokens: int, dim: int, dtype: torch.dtype, table=(0, 0, 0, 0), interleaved: bool = False) -> None:
+    """table: as _check_table gives it"""
+    if len(table) > 4:
+        _launch(_native.lib().fftopk_head_rows_axes, "fftopk_head_rows_axes", idx, parts, len(parts) // _PART.size, tokens, dim, _DTYPES[dtype],
+                table[0], table[4], table[5], table[6], table[1], table[2], table[3], interleaved)
+        return
     _launch(_native.lib().fftopk_head_rows, "fftopk_head_rows", idx, parts, len(parts) // _PART.size, tokens, dim, _DTYPES[dtype], table[0],
             table[1], table[2], table[3], interleaved)
 
@@ -127,11 +132,26 @@ def _check_first(x: torch.Tensor, what: str):
     return idx, shape[0], dim, dtype
 
 
-def _check_table(positions, cos_sin, idx: int, tokens: int, dim: int):
-    """(positions' address, cos_sin's, its rows, its columns); zeros without a rotation"""
+def rotary_axes(sections: Sequence[int], interleaved: bool = False) -> tuple:
+    """The axis each pair of rotated channels turns by, from the pairs of each axis, sections = (time, height, width) for instance: in
+    blocks, or in turn for as long as an axis has pairs left. What `axes` of the ops below takes."""
+    if not interleaved:
+        return tuple(a for a, n in enumerate(sections) for _ in range(n))
+    return tuple(a for i in range(max(sections, default=0)) for a, n in enumerate(sections) if i < n)
+
+
+def _axes_bytes(axes: tuple, pairs: int, n: int) -> bytes:
+    if len(axes) != pairs or not 1 <= n <= 4 or set(map(type, axes)) != {int} or min(axes) < 0 or max(axes) >= n:
+        raise RuntimeError("axes must name one of positions' rows (up to four) for each of the rotated pairs, half of cos_sin's columns")
+    return bytes(axes)
+
+
+def _check_table(positions, cos_sin, idx: int, tokens: int, dim: int, axes=None):
+    """(positions' address, cos_sin's, its rows, its columns); zeros without a rotation; with axes also (positions' row stride, rows, the
+    pairs' axes)"""
     if cos_sin is None:
-        if positions is not None:
-            raise RuntimeError("positions and cos_sin go together")
+        if positions is not None or axes is not None:
+            raise RuntimeError("positions, axes and cos_sin go together")
         return 0, 0, 0, 0
     if positions is None:
         raise RuntimeError("positions and cos_sin go together")
@@ -140,7 +160,12 @@ def _check_table(positions, cos_sin, idx: int, tokens: int, dim: int):
         raise RuntimeError("cos_sin must be a contiguous float32 tensor [positions, rotary] on the inputs' device")
     if shape[1] % 16 or not 16 <= shape[1] <= dim:
         raise RuntimeError("the rotated channels (cos_sin's columns) must be a multiple of 16 up to D")
-    return _check_vector(positions, "positions", idx, tokens), cos_sin.data_ptr(), shape[0], shape[1]
+    if axes is None:
+        return _check_vector(positions, "positions", idx, tokens), cos_sin.data_ptr(), shape[0], shape[1]
+    at, step = positions.shape, positions.stride()
+    if positions.dtype is not torch.int32 or len(at) != 2 or at[1] != tokens or (tokens > 1 and step[1] != 1) or positions.get_device() != idx:
+        raise RuntimeError("with axes, positions must be an int32 tensor [axes, tokens] with unit inner stride on the inputs' device")
+    return positions.data_ptr(), cos_sin.data_ptr(), shape[0], shape[1], step[0], at[0], _axes_bytes(tuple(axes), shape[1] // 2, at[0])
 
 
 def qk_norm_rope(
@@ -157,6 +182,7 @@ def qk_norm_rope(
     k_bias: Optional[torch.Tensor] = None,
     eps: float = 1e-6,
     interleaved: bool = False,
+    axes: Optional[Sequence[int]] = None,
     q_out: Optional[torch.Tensor] = None,
     k_out: Optional[torch.Tensor] = None,
 ):
@@ -171,12 +197,14 @@ def qk_norm_rope(
         q_norm, k_norm: None, "rms" or "layer", over the D channels of a head; weight and bias [D] (default 1 and 0) and eps go
             with them.
         interleaved: pairs (2i, 2i + 1) instead of (i, i + R/2).
+        axes: for tokens with a position on each of several axes (time, height and width of images and video): positions is int32
+            [A, T], A up to 4, unit inner stride, and pair i turns by positions[axes[i]]. R/2 of them; rotary_axes() makes them from sections.
         q_out, k_out: where the results go (default: new tensors); q and k themselves are allowed.
     Returns:
         (q_out, k_out), of q's and k's shapes and type.
     """
     idx, T, D, dtype = _check_first(q, "q")
-    table = _check_table(positions, cos_sin, idx, T, D)
+    table = _check_table(positions, cos_sin, idx, T, D, axes)
     rotate = 1 if cos_sin is not None else 0
     heads, xs = _check_rows(q, "q", idx, dtype, T, D)
     norm = _check_norm(q_norm, q_weight, q_bias, "q", idx, D)
@@ -221,13 +249,14 @@ def qkv_norm_rope_write(
     k_bias: Optional[torch.Tensor] = None,
     eps: float = 1e-6,
     interleaved: bool = False,
+    axes: Optional[Sequence[int]] = None,
     q_out: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """qk_norm_rope and kv_cache.cache_write in one launch: q comes back normed and rotated, k is normed, rotated and quantised
     into row slots[t] of k_cache, v quantised into v_cache. Arguments as for those two; padding tokens (slot -1) may have any
     position (outside the table: q's rotated channels are NaN, and kernel_status() says nothing)."""
     idx, T, D, dtype = _check_first(q, "q")
-    table = _check_table(positions, cos_sin, idx, T, D)
+    table = _check_table(positions, cos_sin, idx, T, D, axes)
     rotate = 1 if cos_sin is not None else 0
     (qh, qs), (kh, ks), (vh, vs) = (_check_rows(x, what, idx, dtype, T, D) for x, what in ((q, "q"), (k, "k"), (v, "v")))
     q_how, k_how = _check_norm(q_norm, q_weight, q_bias, "q", idx, D), _check_norm(k_norm, k_weight, k_bias, "k", idx, D)
@@ -265,6 +294,7 @@ def indexer_qk_write(
     k_bias: Optional[torch.Tensor] = None,
     eps: float = 1e-6,
     interleaved: bool = False,
+    axes: Optional[Sequence[int]] = None,
 ):
     """
     The step in front of ``FusedIndexerTopk`` with an fp8 key cache.
@@ -281,7 +311,7 @@ def indexer_qk_write(
         for a positive scale, so FusedIndexerTopk(q8, k_cache, w8, lengths, k_scale=k_scale) ranks as with q itself.
     """
     idx, T, D, dtype = _check_first(q, "q")
-    table = _check_table(positions, cos_sin, idx, T, D)
+    table = _check_table(positions, cos_sin, idx, T, D, axes)
     rotate = 1 if cos_sin is not None else 0
     H, qs = _check_rows(q, "q", idx, dtype, T, D)
     ks = k.stride()

@@ -139,6 +139,18 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
+// four e4m3 codes as fp16: the lower two, the upper two
+__device__ __forceinline__ void widen4(uint32_t& lo, uint32_t& hi, uint32_t codes) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// row r of a cache: the product of two 32-bit numbers, added in 64 bits (slots are below 2^31, slot strides below 2^32 bytes)
+__device__ __forceinline__ const char* row_at(const char* base, int r, uint32_t step) { return base + (uint64_t)(uint32_t)r * step; }
 __device__ __forceinline__ float lds4(uint32_t addr) {
   float r;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(addr) : "memory");
@@ -156,16 +168,19 @@ __device__ __forceinline__ float keys_sum(float x) {
   return x + __shfl_xor_sync(kAll, x, 16);
 }
 
-// A warp's ring. Rows are padded so that the lanes that are served together touch all banks: k, where a quad reads 64 neighbouring
-// bytes of each of two rows, by 64 bytes beyond a multiple of 128; v, where eight rows give 16 bytes each, by 16.
+// A warp's ring: the k rows of a block, its v rows, stage after stage; e4m3: then the stages' scales. Rows are not padded; 16-byte pieces
+// change places within a row so that the lanes that are served together touch all banks: k, where a quad reads four neighbouring pieces of each of two
+// rows; v, where eight rows give the same piece.
 template <bool kFp8, int D>
 struct PagedRing {
   static constexpr int kRowBytes = D * (kFp8 ? 1 : 2);
-  static constexpr int kKPitch = kRowBytes == 64 ? 64 : kRowBytes + 64, kVPitch = kRowBytes + 16;
-  static constexpr int kV = kKeys * kKPitch, kScales = kV + kKeys * kVPitch;
-  static constexpr int kStage = kScales + (kFp8 ? 2 * kKeys * 4 : 0);
+  static constexpr int kV = kKeys * kRowBytes, kStage = 2 * kV;
   static constexpr int kStages = 3;
-  static constexpr int kBytes = kStages * kStage;  // of a warp
+  static constexpr int kScales = kStages * kStage, kScaleStage = kFp8 ? 2 * kKeys * 4 : 0;
+  static constexpr int kBytes = kScales + kStages * (kFp8 ? 256 : 0);  // of a warp
+  // (rows of 64 bytes: two of them touch all banks already)
+  static __device__ __forceinline__ uint32_t k_piece(int row, int piece) { return (uint32_t)(kRowBytes == 64 ? piece : piece ^ (row & 1) << 2); }
+  static __device__ __forceinline__ uint32_t v_piece(int row, int piece) { return (uint32_t)(kRowBytes == 64 ? piece ^ (row >> 1 & 3) : piece ^ (row & 7)); }
 };
 template <bool kFp8, int D>
 constexpr size_t paged_smem() {
@@ -178,8 +193,8 @@ constexpr int paged_ctas() {
   return fit < regs ? fit : regs;
 }
 
-// T: type of q and out, and of the cache where kFp8 is false; kNT: eights of query heads
-template <typename T, bool kFp8, int D, int kNT>
+// T: type of q and out, and of the cache where kFp8 is false; kNT: eights of query heads; kWhole: every block lies on one page
+template <typename T, bool kFp8, int D, int kNT, bool kWhole>
 __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_kernel(const __grid_constant__ PagedParams p) {
   using M = typename std::conditional<kFp8, __half, T>::type;  // the MMAs' type
   using G = PagedRing<kFp8, D>;
@@ -188,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   constexpr int kStages = G::kStages;
   constexpr int kNH = 8 * kNT;
   constexpr int kTiles = D / 16;             // of the output: rows of the MMA are channels
-  extern __shared__ __align__(16) unsigned char smem_raw[];
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
   // (only where a kernel of this call follows, which waits: another one's inputs may be this one's results)
   if (p.runs > 1 || p.weigh) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -235,61 +250,115 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   const int piece = lane % kLanesRow, sub = lane / kLanesRow;
   const char* const kbase = static_cast<const char*>(p.a.k) + (int64_t)kvh * p.a.k_head * kES + piece * 16;
   const char* const vbase = static_cast<const char*>(p.a.v) + (int64_t)kvh * p.a.v_head * kES + piece * 16;
-  const int64_t kstep = p.a.k_slot * kES, vstep = p.a.v_slot * kES;
+  // (k scales are asked for by the lower lanes, v scales by the upper ones)
+  const float* sbase = nullptr;
+  int64_t sstep = 0;
+  if constexpr (kFp8) {
+    sbase = lane < kKeys ? p.a.k_scale + (int64_t)kvh * p.a.ks_head : p.a.v_scale + (int64_t)kvh * p.a.vs_head;
+    sstep = lane < kKeys ? p.a.ks_slot : p.a.vs_slot;
+  }
+  const uint32_t kstep = (uint32_t)(p.a.k_slot * kES), vstep = (uint32_t)(p.a.v_slot * kES);
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)warp * G::kBytes;
 
   Cursor here = cursor_at(p, run_begin(total, runs, run), lane), ahead = here;
   int64_t to_ask = left;
-  // the lane's key in the block that is asked for next (lanes 16 to 31: the same ones again): its page and place there
+  const int32_t* table = p.a.page_table + ahead.b * p.a.table_row;
+  // of the block that is asked for next: the page of the lane's key and its place there (lanes 16 to 31: the same ones again); kWhole: of
+  // the block's first key
   int32_t page = -1;
   uint32_t in_page = 0;
+  int rows = 0;
   auto look = [&]() {
-    page = -1;
-    if (to_ask > 0) {
-      const uint32_t j = (uint32_t)ahead.at * kKeys + (uint32_t)(lane & (kKeys - 1));
+    if (to_ask <= 0) {
+      page = -1;
+      return;
+    }
+    rows = min(kKeys, ahead.n - ahead.at * kKeys);
+    const uint32_t j = (uint32_t)ahead.at * kKeys + (kWhole ? 0u : (uint32_t)(lane & (kKeys - 1)));
+    if (!kWhole || in_page == 0) {  // (kWhole: a page's blocks follow each other, and the table is read once a page)
+      page = -1;
       if (j < (uint32_t)ahead.n) {
         const uint32_t n = p.page.div(j);
         in_page = j - n * p.page.d;
-        page = p.a.page_table[ahead.b * p.a.table_row + n];
+        page = table[n];
       }
-      if (--to_ask > 0) advance(p, ahead);
     }
   };
+  // the block behind it
+  auto step = [&]() {
+    if (--to_ask <= 0) return;
+    const int64_t b = ahead.b;
+    advance(p, ahead);
+    in_page += kKeys;
+    if (ahead.b != b) table = p.a.page_table + ahead.b * p.a.table_row, in_page = 0;
+    if (in_page >= p.page.d) in_page = 0;
+  };
   // asks for the rows and scales of the block looked up; which of them are there
-  auto ask = [&](uint32_t stage) {
-    const int64_t slot = (int64_t)page * p.page.d + in_page;
-    bool ok = page >= 0;
-    if (ok && slot >= p.a.slots) {
-      ok = false;
-      if (p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
-    }
-    const unsigned live = __ballot_sync(kAll, ok) & 0xffffu;
-    if (live != 0u) {
-      const int row = ok ? (int)slot : -1;
+  auto ask = [&](int stage) {
+    const uint32_t data = ring + (uint32_t)(stage * G::kStage);
+    const uint32_t scales = ring + (uint32_t)(G::kScales + stage * G::kScaleStage + lane * 4);
+    unsigned live = 0u;
+    if constexpr (kWhole) {
+      if (page >= 0) {
+        const int64_t slot = (int64_t)page * p.page.d + in_page;
+        const int there = slot < p.a.slots ? (int)min((int64_t)rows, p.a.slots - slot) : 0;
+        if (there < rows && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+        live = (1u << there) - 1u;
+        if (there == kKeys) {
+          const char* const k = row_at(kbase, (int)slot + sub, kstep);
+          const char* const v = row_at(vbase, (int)slot + sub, vstep);
 #pragma unroll
-      for (int i = 0; i < kTurns; ++i) {
-        const int at = i * kRowsOnce + sub;
-        const int r = __shfl_sync(kAll, row, at);
-        copy_or_zero<16>(stage + (uint32_t)(at * G::kKPitch + piece * 16), r >= 0 ? kbase + (int64_t)r * kstep : kbase, r >= 0);
-        copy_or_zero<16>(stage + (uint32_t)(G::kV + at * G::kVPitch + piece * 16), r >= 0 ? vbase + (int64_t)r * vstep : vbase, r >= 0);
+          for (int i = 0; i < kTurns; ++i) {
+            const int at = i * kRowsOnce + sub;
+            copy16(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(k, i * kRowsOnce, kstep));
+            copy16(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(v, i * kRowsOnce, vstep));
+          }
+          if constexpr (kFp8) copy4(scales, sbase + (uint64_t)(uint32_t)((int)slot + (lane & (kKeys - 1))) * sstep);
+        } else if (there > 0) {
+#pragma unroll
+          for (int i = 0; i < kTurns; ++i) {
+            const int at = i * kRowsOnce + sub, r = (int)slot + min(at, there - 1);
+            copy_or_zero<16>(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(kbase, r, kstep), at < there);
+            copy_or_zero<16>(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(vbase, r, vstep), at < there);
+          }
+          if constexpr (kFp8) {
+            const int at = lane & (kKeys - 1);
+            copy_or_zero<4>(scales, sbase + (uint64_t)(uint32_t)((int)slot + min(at, there - 1)) * sstep, at < there);
+          }
+        }
       }
-      if constexpr (kFp8) {  // k scales by the lower lanes, v scales by the upper ones
-        const float* s = lane < kKeys ? p.a.k_scale + (ok ? slot * p.a.ks_slot + (int64_t)kvh * p.a.ks_head : 0)
-                                      : p.a.v_scale + (ok ? slot * p.a.vs_slot + (int64_t)kvh * p.a.vs_head : 0);
-        copy_or_zero<4>(stage + (uint32_t)(G::kScales + lane * 4), s, ok);
+    } else {
+      const int64_t slot = (int64_t)page * p.page.d + in_page;
+      bool ok = page >= 0;
+      if (ok && slot >= p.a.slots) {
+        ok = false;
+        if (p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+      }
+      live = __ballot_sync(kAll, ok) & 0xffffu;
+      if (live != 0u) {
+        const int row = ok ? (int)slot : -1;
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+          const int at = i * kRowsOnce + sub;
+          const int r = __shfl_sync(kAll, row, at);
+          copy_or_zero<16>(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(kbase, max(r, 0), kstep), r >= 0);
+          copy_or_zero<16>(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(vbase, max(r, 0), vstep), r >= 0);
+        }
+        if constexpr (kFp8) copy_or_zero<4>(scales, sbase + (uint64_t)(uint32_t)max(row, 0) * sstep, ok);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     return live;
   };
   unsigned live_of[kStages];
-  look();
+  look();  // (in_page is 0: the table is read)
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
-    live_of[s] = ask(ring + s * G::kStage);
+    live_of[s] = ask(s);
+    step();
     look();
   }
-  uint32_t at_stage = ring, ask_stage = ring + (kStages - 1) * G::kStage;
+  int at_stage = 0, ask_stage = kStages - 1;
 
   // of the sequence at hand
   uint32_t qb[kNT][D / 16][2];
@@ -347,13 +416,15 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
       }
     }
     live_of[kStages - 1] = ask(ask_stage);
+    step();
     look();
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncwarp();
     const unsigned live = live_of[0];
-    const uint32_t stage = at_stage;
-    at_stage = at_stage + G::kStage == ring + G::kBytes ? ring : at_stage + G::kStage;
-    ask_stage = ask_stage + G::kStage == ring + G::kBytes ? ring : ask_stage + G::kStage;
+    const uint32_t stage = ring + (uint32_t)(at_stage * G::kStage);
+    const uint32_t scales = ring + (uint32_t)(G::kScales + at_stage * G::kScaleStage);
+    at_stage = at_stage + 1 == kStages ? 0 : at_stage + 1;
+    ask_stage = ask_stage + 1 == kStages ? 0 : ask_stage + 1;
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) live_of[s] = live_of[s + 1];
 
@@ -362,17 +433,18 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
 #pragma unroll
       for (int t = 0; t < kNT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
       if (live != 0u) {
-        const uint32_t at = stage + (uint32_t)(g * G::kKPitch + qd * 16);
+        const uint32_t at = stage + (uint32_t)(g * G::kRowBytes);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-          const uint4 x = lds16(at + 64u * i), y = lds16(at + 64u * i + 8u * G::kKPitch);
+          const uint32_t from = at + G::k_piece(g, 4 * i + qd) * 16u;
+          const uint4 x = lds16(from), y = lds16(from + 8u * G::kRowBytes);
           const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int u = 0; u < kCE / 4; ++u) {
             uint32_t f[4];
             if constexpr (kFp8) {
-              f[0] = e4m3x2_to_half2((uint16_t)a[u]), f[2] = e4m3x2_to_half2((uint16_t)(a[u] >> 16));
-              f[1] = e4m3x2_to_half2((uint16_t)b[u]), f[3] = e4m3x2_to_half2((uint16_t)(b[u] >> 16));
+              widen4(f[0], f[2], a[u]);
+              widen4(f[1], f[3], b[u]);
             } else {
               f[0] = a[2 * u], f[2] = a[2 * u + 1], f[1] = b[2 * u], f[3] = b[2 * u + 1];
             }
@@ -386,24 +458,34 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           if (live != 0u) {
-            ks[r] = lds4(stage + (uint32_t)(G::kScales + (g + 8 * r) * 4));
-            vs[r] = lds4(stage + (uint32_t)(G::kScales + (kKeys + g + 8 * r) * 4));
+            ks[r] = lds4(scales + (uint32_t)((g + 8 * r) * 4));
+            vs[r] = lds4(scales + (uint32_t)((kKeys + g + 8 * r) * 4));
           }
           vl[r] = (float)scale_exponent(vs[r]);
         }
       }
-      bool over = false;
 #pragma unroll
       for (int t = 0; t < kNT; ++t) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = e >> 1;
-          float s = sc[t][e] * qmul[t][e & 1];
-          if constexpr (kFp8) s *= ks[r];
-          sc[t][e] = (live >> (g + 8 * r)) & 1u ? s : -INFINITY;
-          // (a reference is let stand until a score exceeds it by 2^8: fp16 weights and 32-bit sums have the room)
-          over = over || sc[t][e] + vl[r] > mx[t][e & 1] + 8.f;
+          sc[t][e] *= qmul[t][e & 1];
+          if constexpr (kFp8) sc[t][e] *= ks[e >> 1];
         }
+      }
+      if (live != 0xffffu) {
+        const bool lo = (live >> g) & 1u, hi = (live >> (g + 8)) & 1u;
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+          sc[t][0] = lo ? sc[t][0] : -INFINITY, sc[t][1] = lo ? sc[t][1] : -INFINITY;
+          sc[t][2] = hi ? sc[t][2] : -INFINITY, sc[t][3] = hi ? sc[t][3] : -INFINITY;
+        }
+      }
+      // (a reference is let stand until a score exceeds it by 2^8: fp16 weights and 32-bit sums have the room)
+      bool over = false;
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) over = over || fmaxf(sc[t][e] + vl[0], sc[t][2 + e] + vl[1]) > mx[t][e] + 8.f;
       }
       if (p.weigh) {
         float* to = p.scores + ((here.b * p.units + unit) * p.line + (int64_t)here.at * kKeys + g) * kNH + 2 * qd;
@@ -441,17 +523,17 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
           }
         }
         // lanes 0-7 and 8-15 name the rows of keys 0-7 and 8-15 at one piece, lanes 16-31 at the next
-        const uint32_t vat = stage + (uint32_t)(G::kV + (lane & 15) * G::kVPitch + (lane >> 4) * 16);
+        const uint32_t vat = stage + (uint32_t)(G::kV + (lane & 15) * G::kRowBytes);
 #pragma unroll
         for (int c = 0; c < G::kRowBytes / 32; ++c) {
           uint32_t x[4];
-          ldsm4_trans(x, vat + 32u * c);
+          ldsm4_trans(x, vat + G::v_piece(lane & 15, 2 * c + (lane >> 4)) * 16u);
           if constexpr (kFp8) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t lo = __byte_perm(x[2 * h], 0u, 0x3120), hi = __byte_perm(x[2 * h + 1], 0u, 0x3120);
-              const uint32_t f[4] = {e4m3x2_to_half2((uint16_t)lo), e4m3x2_to_half2((uint16_t)(lo >> 16)), e4m3x2_to_half2((uint16_t)hi),
-                                     e4m3x2_to_half2((uint16_t)(hi >> 16))};
+              uint32_t f[4];
+              widen4(f[0], f[1], __byte_perm(x[2 * h], 0u, 0x3120));
+              widen4(f[2], f[3], __byte_perm(x[2 * h + 1], 0u, 0x3120));
 #pragma unroll
               for (int t = 0; t < kNT; ++t) mma16816(o[t][2 * c + h], f, pb[t][0], pb[t][1], M());
             }
@@ -638,8 +720,10 @@ int g_paged_sms[kMaxDevices];
 
 template <typename T, bool kFp8, int D, int kNT>
 int setup_one() {
-  const cudaError_t e =
-      cudaFuncSetAttribute(paged_kernel<T, kFp8, D, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)paged_smem<kFp8, D>());
+  cudaError_t e =
+      cudaFuncSetAttribute(paged_kernel<T, kFp8, D, kNT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)paged_smem<kFp8, D>());
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(paged_kernel<T, kFp8, D, kNT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)paged_smem<kFp8, D>());
   return e == cudaSuccess ? 0 : cuda_fail(e);
 }
 template <typename T, bool kFp8>
@@ -754,13 +838,17 @@ int check(const fftopk_paged* a) {
       !on(a->weight, 4) || !on(a->weight_out, 4))
     return FFTOPK_EINVAL;
   if (a->slots > 0x7fffffff || a->seqs > 0x7fffffff) return FFTOPK_ERANGE;
+  // (the kernel multiplies slots by 32-bit strides; a lone slot's says nothing)
+  if (a->slots > 1 && (a->k_slot < 0 || a->v_slot < 0 || a->k_slot > 0xffffffffll / ce || a->v_slot > 0xffffffffll / ce)) return FFTOPK_ERANGE;
   return FFTOPK_OK;
 }
 
 template <typename T, bool kFp8, int D>
 cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {
-  return plan.nt == 1 ? launch(paged_kernel<T, kFp8, D, 1>, plan.ctas, kThreads, paged_smem<kFp8, D>(), false, stream, p)
-                      : launch(paged_kernel<T, kFp8, D, 2>, plan.ctas, kThreads, paged_smem<kFp8, D>(), false, stream, p);
+  const bool whole = p.a.page_size % kKeys == 0;
+  const auto kernel = plan.nt == 1 ? (whole ? paged_kernel<T, kFp8, D, 1, true> : paged_kernel<T, kFp8, D, 1, false>)
+                                   : whole ? paged_kernel<T, kFp8, D, 2, true> : paged_kernel<T, kFp8, D, 2, false>;
+  return launch(kernel, plan.ctas, kThreads, paged_smem<kFp8, D>(), false, stream, p);
 }
 template <typename T>
 cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {
@@ -808,6 +896,7 @@ int fftopk_paged_attention(const fftopk_paged* a, void* workspace, size_t worksp
   rc = make_plan(a, sms, p, plan);
   if (rc) return rc;
   if (plan.total > 0 && (workspace == nullptr || !on(workspace, 256) || workspace_bytes < (size_t)plan.total)) return FFTOPK_EINVAL;
+  if (a->slots <= 1) p.a.k_slot = p.a.v_slot = 0;
   if (a->slots == 0) p.a.k = p.a.v = a->q;  // (an empty cache has no address, and rows that are left out are copies of no bytes: from somewhere)
   p.page = FastDiv((uint32_t)a->page_size);
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;

@@ -480,7 +480,8 @@ int fftopk_sparse_attention(const fftopk_attend* args, uint32_t* status, void* c
  *   lse          fp32 [seqs, q_heads], contiguous, or NULL
  *   weight       fp32 [seqs, kv_heads, weight_cols], inner stride 1, or NULL; weight_out likewise, or NULL: no weights; the two may be
  *                one array, and overlap in no other way
- *   strides      in elements; rows of q, k and v start on 16 bytes; page_size any number from 1
+ *   strides      in elements; rows of q, k and v start on 16 bytes, slots of k and v less than 2^32 bytes apart (FFTOPK_ERANGE); page_size any
+ *                number from 1
  *   workspace    fftopk_paged_workspace_bytes bytes of device memory, 256-byte aligned, any contents; calls that may run at the same
  *                time need one each. With weight_out it holds the scores of all positions the table has room for, 32 bytes (of more
  *                than 8 query heads to a key head: 64 for every 16) per position and key head. The size is that of the current device.

@@ -6,10 +6,11 @@
 // What bounds it is reading the cache: a row of k or v is used by the g heads of its key head alone, 2 g flop a byte in 16 bits.
 //
 // Work split: the context, 16 keys a block, of all sequences, sequence after sequence, is one line of blocks. It is cut into equal runs,
-// whatever the lengths; a warp takes one run for one key head (8 or 16 of its query heads). The warps of neighbouring numbers take the same run for different
-// key heads, so that what lies side by side in the cache - the heads of a row, their scales - is read at about the same time. A warp
-// keeps running maxima and sums (one pass) and writes what it has at the end of a sequence: the result where the run holds all of
-// the sequence, else a part that paged_join_kernel joins. No warp waits for another one. Lengths are read on the device only.
+// whatever the lengths; a CTA takes one run for one key head (8 or 16 of its query heads). The CTAs of neighbouring numbers take the same run for
+// different key heads, so that what lies side by side in the cache - the heads of a row, their scales - is read at about the same
+// time. What a run has of a sequence is a segment: each of four warps takes a quarter of it with running maxima and sums (one pass), then they are
+// joined through the stages of their rings that are free at that moment. A run that holds all of a sequence writes the result, else a
+// part, which paged_finish_kernel joins. Lengths are read on the device only; no CTA waits for another one.
 //
 // A warp has a ring of blocks in shared memory that cp.async fills ahead of it. Keys are the rows of the MMA and query heads its
 // columns, 8 at a time: groups of up to 8 heads need half the products and accumulators they would need as rows.
@@ -42,21 +43,22 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;      // of a block: rows of the MMA
-constexpr int kMinBlocks = 4;  // of a run: below that, parts to join cost more than the blocks
-constexpr int kJoinWarps = 8;
+constexpr int kMinBlocks = 16;  // of a run: below that, parts to join cost more than the blocks
 
 struct PagedParams {
   fftopk_paged a;
   int32_t group, head_blocks, units, runs, bound, weigh;
   FastDiv page;
   float scale_log2;
+  int32_t out_vec;  // rows of out start on 8 bytes
   int64_t line;     // positions of a unit of the score workspace
-  int64_t* before;  // [seqs + 1] blocks in front of every sequence
-  float* lse2;      // [seqs, q heads] log2 of the sum of exponentials
+  float* lse2;      // [seqs, q heads] log2 of the sum of exponentials, of sequences that lie in one run
   float2* ml;       // [runs * units * 2][heads of a unit] maximum (log2) and sum of a part
   float* o;         // [runs * units * 2][heads of a unit][D]
   float* scores;    // [seqs][units][line][heads of a unit], log2
   uint32_t* status;
+  // paged_finish_kernel: CTAs that join, how many pairs of a sequence and a query head each of their warps takes (0: a CTA takes one), warps that weigh
+  int32_t join_ctas, join_each, weigh_runs;
 };
 
 // Keys of sequence b: its length, as far as its pages reach
@@ -64,14 +66,23 @@ __device__ __forceinline__ int32_t keys_of(const PagedParams& p, int64_t b) { re
 __device__ __forceinline__ int64_t blocks_of(int32_t n) { return ((int64_t)n + kKeys - 1) / kKeys; }
 
 // Runs the line of `total` blocks is cut into, and where one begins: the first total % runs have a block more.
-__device__ __forceinline__ int64_t live_runs(int64_t total, int32_t runs) { return max((int64_t)1, min((int64_t)runs, total / kMinBlocks)); }
-__device__ __forceinline__ int64_t run_begin(int64_t total, int64_t runs, int64_t run) {
-  return run * (total / runs) + min(run, total % runs);
-}
-__device__ __forceinline__ int64_t run_of(int64_t total, int64_t runs, int64_t block) {
-  const int64_t each = total / runs, rest = total % runs, wide = rest * (each + 1);
-  return block < wide ? block / (each + 1) : rest + (block - wide) / each;  // (each = 0: every block is in front of `wide`)
-}
+struct Runs {
+  int64_t total, each, rest;
+  int32_t runs;
+  __device__ __forceinline__ Runs(int64_t t, int32_t most, int32_t least) : total(t) {
+    runs = (int32_t)max((int64_t)1, min((int64_t)most, quotient(t, least)));
+    each = quotient(t, runs);
+    rest = t - each * runs;
+  }
+  static __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {  // (64 bits only where they are needed: ten times as long)
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+  }
+  __device__ __forceinline__ int64_t begin(int64_t run) const { return run * each + min(run, rest); }
+  __device__ __forceinline__ int64_t of(int64_t block) const {
+    const int64_t wide = rest * (each + 1);  // (each = 0: every block is in front of `wide`)
+    return block < wide ? quotient(block, each + 1) : rest + quotient(block - wide, each);
+  }
+};
 
 __device__ __forceinline__ int64_t warp_sum(int64_t x) {
 #pragma unroll
@@ -86,20 +97,21 @@ __device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
   }
   return x;
 }
-__device__ __forceinline__ int64_t total_blocks(const PagedParams& p, int lane) {
+// blocks of the sequences in front of `upto`
+__device__ __forceinline__ int64_t blocks_before(const PagedParams& p, int64_t upto, int lane) {
   int64_t total = 0;
-  for (int64_t b = lane; b < p.a.seqs; b += 32) total += blocks_of(keys_of(p, b));
+  for (int64_t b = lane; b < upto; b += 32) total += blocks_of(keys_of(p, b));
   return warp_sum(total);
 }
 
-// A place on the line: a sequence, its keys and blocks, and one of them
-struct Cursor {
+// What a run has of a sequence: blocks s0 .. s1 - 1 of its `blocks`
+struct Segment {
   int64_t b;
-  int32_t n, blocks, at;
+  int32_t n, blocks, s0, s1;
 };
-// Block g of the line (g < total)
-__device__ __forceinline__ Cursor cursor_at(const PagedParams& p, int64_t g, int lane) {
-  Cursor c;
+// The segment that begins at block g of the line (g < total), of at most `left` blocks
+__device__ __forceinline__ Segment segment_at(const PagedParams& p, int64_t g, int64_t left, int lane) {
+  Segment c;
   int64_t before = 0;
   for (int64_t first = 0;; first += 32) {
     const int32_t n = first + lane < p.a.seqs ? keys_of(p, first + lane) : 0;
@@ -110,22 +122,31 @@ __device__ __forceinline__ Cursor cursor_at(const PagedParams& p, int64_t g, int
       c.b = first + l;
       c.n = __shfl_sync(kAll, n, l);
       c.blocks = (int32_t)blocks_of(c.n);
-      c.at = (int32_t)(g - (__shfl_sync(kAll, upto, l) - c.blocks));
+      c.s0 = (int32_t)(g - (__shfl_sync(kAll, upto, l) - c.blocks));
+      c.s1 = (int32_t)min((int64_t)c.blocks, c.s0 + left);
       return c;
     }
     before = __shfl_sync(kAll, upto, 31);
   }
 }
-// The block behind the cursor's; false: the line ends
-__device__ __forceinline__ bool advance(const PagedParams& p, Cursor& c) {
-  if (++c.at < c.blocks) return true;
-  c.at = 0;
+// The one behind it, of at most `left` > 0 blocks; false: the line ends
+__device__ __forceinline__ bool next_segment(const PagedParams& p, Segment& c, int64_t left) {
   for (++c.b; c.b < p.a.seqs; ++c.b) {
     c.n = keys_of(p, c.b);
-    c.blocks = (int32_t)blocks_of(c.n);
-    if (c.n > 0) return true;
+    if (c.n > 0) {
+      c.blocks = (int32_t)blocks_of(c.n);
+      c.s0 = 0;
+      c.s1 = (int32_t)min((int64_t)c.blocks, left);
+      return true;
+    }
   }
   return false;
+}
+// A warp's quarter of it
+__device__ __forceinline__ void quarter(const Segment& c, int warp, int32_t& at, int32_t& end) {
+  const int32_t q = (c.s1 - c.s0) / kWarps, r = (c.s1 - c.s0) % kWarps;
+  at = c.s0 + warp * q + min(warp, r);
+  end = at + q + (warp < r ? 1 : 0);
 }
 
 __device__ __forceinline__ uint32_t turned8x8(uint32_t x) {
@@ -207,18 +228,18 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   // (only where a kernel of this call follows, which waits: another one's inputs may be this one's results)
   if (p.runs > 1 || p.weigh) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  __shared__ float2 ml_of[kWarps][kNH];
+  __shared__ uint32_t free_of[kWarps];  // the warps' free stages
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, qd = lane & 3;
-  const uint32_t gw = blockIdx.x * (uint32_t)kWarps + (uint32_t)warp;
-  const uint32_t run = gw / (uint32_t)p.units;
-  const int unit = (int)(gw - run * (uint32_t)p.units);
-  if (run >= (uint32_t)p.runs) return;
+  const uint32_t run = blockIdx.x / (uint32_t)p.units;
+  const int unit = (int)(blockIdx.x - run * (uint32_t)p.units);
   const int kvh = unit / p.head_blocks, hb = unit - kvh * p.head_blocks;
   const int heads = min(kNH, p.group - hb * kNH);
   const int head0 = kvh * p.group + hb * kNH;
 
-  // what is empty, what reaches beyond its pages, and (the first warp) where sequences begin
-  for (int64_t b = run; b < p.a.seqs; b += p.runs) {
+  // what is empty, and what reaches beyond its pages
+  for (int64_t b = run + (int64_t)p.runs * warp; b < p.a.seqs; b += (int64_t)p.runs * kWarps) {
     const int32_t n = p.a.lengths[b];
     if (n > p.bound && unit == 0 && lane == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
     if (min(n, p.bound) <= 0) {
@@ -229,20 +250,9 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
       }
     }
   }
-  if (gw == 0 && p.runs > 1) {
-    int64_t before = 0;
-    for (int64_t first = 0; first < p.a.seqs; first += 32) {
-      const int64_t n = first + lane < p.a.seqs ? blocks_of(keys_of(p, first + lane)) : 0;
-      const int64_t upto = before + warp_scan(n, lane);
-      if (first + lane < p.a.seqs) p.before[first + lane] = upto - n;
-      before = __shfl_sync(kAll, upto, 31);
-    }
-    if (lane == 0) p.before[p.a.seqs] = before;
-  }
-  const int64_t total = total_blocks(p, lane);
-  const int64_t runs = live_runs(total, p.runs);
-  if ((int64_t)run >= runs || total == 0) return;
-  int64_t left = run_begin(total, runs, run + 1) - run_begin(total, runs, run);  // blocks of the run
+  const Runs line(blocks_before(p, p.a.seqs, lane), p.runs, kMinBlocks);
+  if ((int64_t)run >= line.runs || line.total == 0) return;  // (the whole CTA)
+  int64_t left = line.begin((int64_t)run + 1) - line.begin(run);  // blocks of the run that are not behind the segment at hand
   if (left <= 0) return;
 
   constexpr int kLanesRow = G::kRowBytes / 16, kRowsOnce = 32 / kLanesRow, kTurns = kKeys / kRowsOnce;
@@ -260,8 +270,12 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   const uint32_t kstep = (uint32_t)(p.a.k_slot * kES), vstep = (uint32_t)(p.a.v_slot * kES);
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)warp * G::kBytes;
 
-  Cursor here = cursor_at(p, run_begin(total, runs, run), lane), ahead = here;
-  int64_t to_ask = left;
+  Segment here = segment_at(p, line.begin(run), left, lane), ahead = here;
+  int64_t left_ahead = left;
+  int32_t at, end, ask_at, ask_end;  // the warp's blocks of the segment at hand, and of the one it asks for
+  quarter(here, warp, at, end);
+  ask_at = at, ask_end = end;
+  bool more = true;  // there is a block to ask for
   const int32_t* table = p.a.page_table + ahead.b * p.a.table_row;
   // of the block that is asked for next: the page of the lane's key and its place there (lanes 16 to 31: the same ones again); kWhole: of
   // the block's first key
@@ -269,12 +283,12 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   uint32_t in_page = 0;
   int rows = 0;
   auto look = [&]() {
-    if (to_ask <= 0) {
+    if (!more) {
       page = -1;
       return;
     }
-    rows = min(kKeys, ahead.n - ahead.at * kKeys);
-    const uint32_t j = (uint32_t)ahead.at * kKeys + (kWhole ? 0u : (uint32_t)(lane & (kKeys - 1)));
+    rows = min(kKeys, ahead.n - ask_at * kKeys);
+    const uint32_t j = (uint32_t)ask_at * kKeys + (kWhole ? 0u : (uint32_t)(lane & (kKeys - 1)));
     if (!kWhole || in_page == 0) {  // (kWhole: a page's blocks follow each other, and the table is read once a page)
       page = -1;
       if (j < (uint32_t)ahead.n) {
@@ -284,14 +298,26 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
       }
     }
   };
-  // the block behind it
+  // on to the first segment with blocks of the warp
+  auto find = [&]() {
+    while (ask_at == ask_end) {
+      left_ahead -= ahead.s1 - ahead.s0;
+      if (left_ahead <= 0 || !next_segment(p, ahead, left_ahead)) {
+        more = false;
+        return;
+      }
+      quarter(ahead, warp, ask_at, ask_end);
+      table = p.a.page_table + ahead.b * p.a.table_row;
+      in_page = 0;
+    }
+  };
+  // the block behind
   auto step = [&]() {
-    if (--to_ask <= 0) return;
-    const int64_t b = ahead.b;
-    advance(p, ahead);
+    if (!more) return;
     in_page += kKeys;
-    if (ahead.b != b) table = p.a.page_table + ahead.b * p.a.table_row, in_page = 0;
     if (in_page >= p.page.d) in_page = 0;
+    ++ask_at;
+    find();
   };
   // asks for the rows and scales of the block looked up; which of them are there
   auto ask = [&](int stage) {
@@ -351,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
     return live;
   };
   unsigned live_of[kStages];
+  find();
   look();  // (in_page is 0: the table is read)
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
@@ -360,18 +387,15 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   }
   int at_stage = 0, ask_stage = kStages - 1;
 
-  // of the sequence at hand
+  // of the segment at hand
   uint32_t qb[kNT][D / 16][2];
   float qmul[kNT][2];  // what the scores of the lane's heads are to be multiplied with
   float o[kNT][kTiles][4];
   // what weights are taken against (log2): the largest score; fp8: the largest score + log2 |v scale|, by the scale's exponent
   float mx[kNT][2], sum[kNT][2];
-  int32_t first = here.at;  // block that the segment begins with
-  bool fresh = true;
-  int which = 0;  // segments that end or begin elsewhere: 0 the run's first, 1 its last
+  int which = 0;  // of two parts that a run may leave: 0 its first segment's, 1 its last one's
   for (;;) {
-    if (fresh) {
-      fresh = false;
+    {
       const T* q0 = static_cast<const T*>(p.a.q) + here.b * p.a.q_seq + (int64_t)head0 * p.a.q_head;
 #pragma unroll
       for (int t = 0; t < kNT; ++t) {
@@ -415,6 +439,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
         for (int i = 0; i < kTiles; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
       }
     }
+    for (; at < end; ++at) {
     live_of[kStages - 1] = ask(ask_stage);
     step();
     look();
@@ -488,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
         for (int e = 0; e < 2; ++e) over = over || fmaxf(sc[t][e] + vl[0], sc[t][2 + e] + vl[1]) > mx[t][e] + 8.f;
       }
       if (p.weigh) {
-        float* to = p.scores + ((here.b * p.units + unit) * p.line + (int64_t)here.at * kKeys + g) * kNH + 2 * qd;
+        float* to = p.scores + ((here.b * p.units + unit) * p.line + (int64_t)at * kKeys + g) * kNH + 2 * qd;
 #pragma unroll
         for (int t = 0; t < kNT; ++t) {
           *reinterpret_cast<float2*>(to + 8 * t) = make_float2(sc[t][0], sc[t][1]);
@@ -546,172 +571,291 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
       }
     }
     __syncwarp();  // (the next block but kStages - 2 goes where this one was)
-    --left;
-    if (left > 0 && here.at + 1 < here.blocks) {
-      ++here.at;
-      continue;
     }
-    // ---- the segment's end ----
-    const bool whole = first == 0 && here.at + 1 == here.blocks;
-    const int64_t rec = (int64_t)gw * 2 + which;
+    // ---- the segment's end: the stage that is asked for next is free, and takes the warp's accumulators, [heads][D] ----
+    const bool whole = here.s0 == 0 && here.s1 == here.blocks;
+    const int64_t rec = (int64_t)blockIdx.x * 2 + which;
+    const uint32_t free_stage = (uint32_t)(ask_stage * G::kStage);
+    constexpr int kOnce = G::kStage >= kNH * D * 4 ? kNH : 8;  // heads at a time
+    static_assert(G::kStage >= kOnce * D * 4, "a stage holds the accumulators");
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int h = 8 * t + 2 * qd + e;
         const float l = keys_sum(sum[t][e]);
-        if (h < heads) {
-          // channels of the accumulators: 16 bits g and g + 8 of a tile, e4m3 2 g and 2 g + 1
-          if (whole) {
-            T* out = static_cast<T*>(p.a.out) + here.b * p.a.out_seq + (int64_t)(head0 + h) * p.a.out_head;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (g == 0) ml_of[warp][8 * t + 2 * qd + e] = make_float2(mx[t][e], l);
+      }
+    }
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i) {
-              out[16 * i + (kFp8 ? 2 * g : g)] = T(l == 0.f ? 0.f : o[t][i][e] * inv);
-              out[16 * i + (kFp8 ? 2 * g + 1 : g + 8)] = T(l == 0.f ? 0.f : o[t][i][2 + e] * inv);
-            }
-            if (g == 0) {
-              const float l2 = l == 0.f ? -INFINITY : mx[t][e] + log2f(l);
-              if (p.a.lse != nullptr) p.a.lse[here.b * p.a.q_heads + head0 + h] = l2 * 0.693147180559945309f;
-              if (p.weigh) p.lse2[here.b * p.a.q_heads + head0 + h] = l2;
-            }
-          } else {
-            float* out = p.o + (rec * kNH + h) * D;
+    for (int h0 = 0; h0 < kNH; h0 += kOnce) {
+      // channels of the accumulators: 16 bits g and g + 8 of a tile, e4m3 2 g and 2 g + 1
+      float* const mine = reinterpret_cast<float*>(smem_raw + warp * G::kBytes + free_stage);
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i) {
-              out[16 * i + (kFp8 ? 2 * g : g)] = o[t][i][e];
-              out[16 * i + (kFp8 ? 2 * g + 1 : g + 8)] = o[t][i][2 + e];
-            }
-            if (g == 0) p.ml[rec * kNH + h] = make_float2(mx[t][e], l);
+      for (int t = h0 / 8; t < (h0 + kOnce) / 8; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float* const row = mine + (8 * t - h0 + 2 * qd + e) * D;
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+            row[16 * i + (kFp8 ? 2 * g : g)] = o[t][i][e];
+            row[16 * i + (kFp8 ? 2 * g + 1 : g + 8)] = o[t][i][2 + e];
           }
         }
       }
+      if (lane == 0 && h0 == 0) free_of[warp] = (uint32_t)(warp * G::kBytes) + free_stage;
+      __syncthreads();
+      for (int i = threadIdx.x; i < min(kOnce, heads - h0) * (D / 4); i += kThreads) {
+        const int h = h0 + i / (D / 4), d = i % (D / 4) * 4;
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml_of[w][h].x);
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 ml = ml_of[w][h];
+          const float f = ml.x == m ? 1.f : ex2(ml.x - m);  // (a warp without keys: 0 of both; 0 * NaN stays NaN)
+          l += kFp8 ? brought(ml.y, ml.x, m) : f * ml.y;
+          const float4 x = *reinterpret_cast<const float4*>(smem_raw + free_of[w] + (h - h0) * (D * 4) + d * 4);
+          y.x += f * x.x, y.y += f * x.y, y.z += f * x.z, y.w += f * x.w;
+        }
+        if (whole) {
+          T* out = static_cast<T*>(p.a.out) + here.b * p.a.out_seq + (int64_t)(head0 + h) * p.a.out_head + d;
+          const float r[4] = {l == 0.f ? 0.f : y.x / l, l == 0.f ? 0.f : y.y / l, l == 0.f ? 0.f : y.z / l, l == 0.f ? 0.f : y.w / l};
+          Four<T> narrow;
+          narrow.narrow(r);
+          if (p.out_vec)
+            narrow.template store<true>(out);
+          else
+            narrow.template store<false>(out);
+          if (d == 0) {
+            const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
+            if (p.a.lse != nullptr) p.a.lse[here.b * p.a.q_heads + head0 + h] = l2 * 0.693147180559945309f;
+            if (p.weigh) p.lse2[here.b * p.a.q_heads + head0 + h] = l2;
+          }
+        } else {
+          *reinterpret_cast<float4*>(p.o + (rec * kNH + h) * D + d) = y;
+          if (d == 0) p.ml[rec * kNH + h] = make_float2(m, l);
+        }
+      }
+      __syncthreads();
     }
-    if (left <= 0) break;
-    advance(p, here);
-    first = 0;
+    left -= here.s1 - here.s0;
+    if (left <= 0 || !next_segment(p, here, left)) break;
+    quarter(here, warp, at, end);
     which = 1;
-    fresh = true;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Parts of a sequence that lies in several runs, joined: a CTA per sequence and query head.
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedParams p) {
-  __shared__ float2 red[kJoinWarps];
-  __shared__ float part[kJoinWarps][D];
-  if (p.weigh) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t b = blockIdx.x / (uint32_t)p.a.q_heads;
-  const int head = (int)(blockIdx.x - (uint32_t)b * (uint32_t)p.a.q_heads);
-  const int64_t total = p.before[p.a.seqs], begin = p.before[b], end = p.before[b + 1];
-  if (begin == end) return;
-  const int64_t runs = live_runs(total, p.runs);
-  const int64_t r0 = run_of(total, runs, begin), r1 = run_of(total, runs, end - 1);
-  if (r0 == r1) return;
-  const int nh = p.group > 8 ? 16 : 8;
-  const int kvh = head / p.group, in = head - kvh * p.group, hb = in / nh;
-  const int64_t first = (r0 * p.units + kvh * p.head_blocks + hb) * 2 + (run_begin(total, runs, r0) < begin ? 1 : 0);
-  const int h = in - hb * nh, parts = (int)(r1 - r0 + 1);
-  auto record = [&](int i) { return i == 0 ? first : ((r0 + i) * p.units + kvh * p.head_blocks + hb) * 2; };
+// Parts of one unit of a sequence that lies in several runs: records `first`, and then every `step`-th from `second`
+struct Parts {
+  int64_t first, second, step;
+  int32_t n;
+  __device__ __forceinline__ Parts(const PagedParams& p, const Runs& line, int64_t begin, int64_t end, int unit) {
+    const int64_t r0 = line.of(begin), r1 = line.of(end - 1);
+    n = (int32_t)(r1 - r0) + 1;
+    first = (r0 * p.units + unit) * 2 + (line.begin(r0) < begin ? 1 : 0);  // (the sequence begins inside its first run)
+    second = ((r0 + 1) * p.units + unit) * 2;
+    step = (int64_t)p.units * 2;
+  }
+  __device__ __forceinline__ int64_t operator[](int i) const { return i == 0 ? first : second + (i - 1) * step; }
+};
 
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) m = fmaxf(m, p.ml[record(i) * nh + h].x);
-#pragma unroll
-  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, i));
-  if (lane == 0) red[warp].x = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, red[w].x);
-  constexpr int kC = D / 32;  // channels of a lane
-  float acc[kC], l = 0.f;
+// A warp's share - parts i0, i0 + step, .. - of a head's joined sums: running maximum and sum, kC channels a lane
+template <int kC>
+__device__ __forceinline__ void join_parts(const PagedParams& p, const Parts& parts, int nh, int h, int i0, int step, int lane, float& m, float& l,
+                                           float (&acc)[kC]) {
+  constexpr int kAhead = 8;
+  m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int c = 0; c < kC; ++c) acc[c] = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < parts; i += kJoinWarps) {
-    const int64_t r = record(i) * nh + h;
-    const float2 ml = p.ml[r];
-    const float f = ml.x == m ? 1.f : ex2(ml.x - m);  // (a part without keys: 0 of both; 0 * NaN stays NaN)
-    l += brought(ml.y, ml.x, m);
-    const float* o = p.o + r * D + lane * kC;
-    if constexpr (kC == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(o);
-      acc[0] += f * x.x, acc[1] += f * x.y, acc[2] += f * x.z, acc[3] += f * x.w;
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(o);
-      acc[0] += f * x.x, acc[1] += f * x.y;
+  for (int i = i0; i < parts.n; i += kAhead * step) {
+    float2 ml[kAhead];
+    float x[kAhead][kC];
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      ml[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) x[u][c] = 0.f;
+      if (i + u * step < parts.n) {
+        const int64_t r = parts[i + u * step] * nh + h;
+        ml[u] = p.ml[r];
+        const float* o = p.o + (r * 32 + lane) * kC;
+        if constexpr (kC == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(o);
+          x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(o);
+          x[u][0] = v.x, x[u][1] = v.y;
+        }
+      }
     }
-  }
-  __syncthreads();
-  if (lane == 0) red[warp].y = l;
 #pragma unroll
-  for (int c = 0; c < kC; ++c) part[warp][lane * kC + c] = acc[c];
-  __syncthreads();
-  l = 0.f;
+    for (int u = 0; u < kAhead; ++u) top = fmaxf(top, ml[u].x);
+    const float was = m == top ? 1.f : ex2(m - top);
+    l = brought(l, m, top);
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) l += red[w].y;
-  for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
-    float y = 0.f;
+    for (int c = 0; c < kC; ++c) acc[c] *= was;
+    m = top;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) y += part[w][d];
-    static_cast<T*>(p.a.out)[b * p.a.out_seq + (int64_t)head * p.a.out_head + d] = T(l == 0.f ? 0.f : y / l);
-  }
-  if (threadIdx.x == 0) {
-    const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
-    if (p.a.lse != nullptr) p.a.lse[b * p.a.q_heads + head] = l2 * 0.693147180559945309f;
-    if (p.weigh) p.lse2[b * p.a.q_heads + head] = l2;
+    for (int u = 0; u < kAhead; ++u) {
+      const float f = ml[u].x == m ? 1.f : ex2(ml[u].x - m);  // (a part without keys: 0 of both; 0 * NaN stays NaN)
+      l += brought(ml[u].y, ml[u].x, m);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) acc[c] += f * x[u][c];
+    }
   }
 }
 
-// The weights brought up to date from the scores and the joined sums: a warp per run and key head, a lane per position.
-template <int kNH>
-__global__ void __launch_bounds__(kThreads) paged_weigh_kernel(const __grid_constant__ PagedParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const uint32_t gw = blockIdx.x * (uint32_t)kWarps + (threadIdx.x >> 5);
+template <typename T, int kC>
+__device__ __forceinline__ void write_joined(const PagedParams& p, int64_t b, int head, int lane, float m, float l, const float (&acc)[kC]) {
+  T* out = static_cast<T*>(p.a.out) + b * p.a.out_seq + (int64_t)head * p.a.out_head + lane * kC;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) out[c] = T(l == 0.f ? 0.f : acc[c] / l);
+  if (lane == 0 && p.a.lse != nullptr) p.a.lse[b * p.a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+}
+
+// What is left when every run is through. The first CTAs join the parts of sequences that lie in several runs: a warp takes a few pairs of a
+// sequence and a query head, or, where there are few, a CTA one of them. The others bring the weights up to date from the scores and the
+// joined sums: a warp takes a run of the line for one key head, a lane a position. Where sequences begin is found while the kernel in front still runs.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) paged_finish_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int kC = D / 32;  // channels of a lane
+  __shared__ float4 part[kWarps][D / 4];
+  __shared__ float2 ml_of[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int nh = p.group > 8 ? 16 : 8;
+  const int64_t total = blocks_before(p, p.a.seqs, lane);
+  const Runs line(total, p.runs, kMinBlocks);
+  if ((int)blockIdx.x < p.join_ctas) {
+    const int64_t pairs = p.a.seqs * p.a.q_heads;
+    int64_t i = p.join_each == 0 ? blockIdx.x : ((int64_t)blockIdx.x * kWarps + warp) * p.join_each;
+    const int64_t last = min(pairs, i + max(p.join_each, 1));
+    int64_t b = i / p.a.q_heads, begin = blocks_before(p, min(b, p.a.seqs), lane);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (; i < last; ++i) {
+      if (i / p.a.q_heads != b) {
+        begin += blocks_of(keys_of(p, b));
+        ++b;
+      }
+      const int64_t end = begin + blocks_of(keys_of(p, b));
+      if (begin == end) continue;
+      const int head = (int)(i - b * p.a.q_heads), kvh = head / p.group, in = head - kvh * p.group, hb = in / nh;
+      const Parts parts(p, line, begin, end, kvh * p.head_blocks + hb);
+      if (parts.n == 1) continue;
+      float m, l, acc[kC];
+      if (p.join_each != 0) {
+        join_parts<kC>(p, parts, nh, in - hb * nh, 0, 1, lane, m, l, acc);
+      } else {
+        join_parts<kC>(p, parts, nh, in - hb * nh, warp, kWarps, lane, m, l, acc);
+#pragma unroll
+        for (int c = 0; c < kC; ++c) reinterpret_cast<float*>(part[warp])[lane * kC + c] = acc[c];
+        if (lane == 0) ml_of[warp] = make_float2(m, l);
+        __syncthreads();  // (the CTA has one pair)
+        if (warp != 0) return;
+        const float2 own = ml_of[0];
+        m = own.x, l = own.y;
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+          const float2 ml = ml_of[w];
+          const float top = fmaxf(m, ml.x), was = m == top ? 1.f : ex2(m - top), f = ml.x == top ? 1.f : ex2(ml.x - top);
+          l = brought(l, m, top) + brought(ml.y, ml.x, top);
+#pragma unroll
+          for (int c = 0; c < kC; ++c) acc[c] = acc[c] * was + f * reinterpret_cast<const float*>(part[w])[lane * kC + c];
+          m = top;
+        }
+      }
+      write_joined<T, kC>(p, b, head, lane, m, l, acc);
+    }
+    return;
+  }
+  // ---- weights ----
+  const uint32_t gw = (blockIdx.x - (uint32_t)p.join_ctas) * (uint32_t)kWarps + (uint32_t)warp;
   const uint32_t run = gw / (uint32_t)p.a.kv_heads;
   const int kvh = (int)(gw - run * (uint32_t)p.a.kv_heads);
-  const int64_t total = total_blocks(p, lane);
-  const int64_t runs = max((int64_t)1, min(total, (int64_t)(gridDim.x * (uint32_t)kWarps / (uint32_t)p.a.kv_heads)));
-  if ((int64_t)run >= runs || total == 0) return;
-  int64_t left = run_begin(total, runs, run + 1) - run_begin(total, runs, run);
+  const Runs mine(total, p.weigh_runs, 2);
+  int64_t left = (int64_t)run < mine.runs ? mine.begin((int64_t)run + 1) - mine.begin(run) : 0;
+  Segment c = {};
+  if (left > 0) c = segment_at(p, mine.begin(run), left, lane);
+  int64_t begin = mine.begin(run) - c.s0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // (by every CTA: this kernel does not end before the one in front)
   if (left <= 0) return;
-  Cursor c = cursor_at(p, run_begin(total, runs, run), lane);
   for (;;) {
-    const int64_t blocks = min(left, (int64_t)(c.blocks - c.at));
-    const int32_t end = (int32_t)min((int64_t)c.n, ((int64_t)c.at + blocks) * kKeys);
+    const int64_t end = begin + c.blocks;
+    const int32_t upto = (int32_t)min((int64_t)c.n, (int64_t)c.s1 * kKeys);
     const float* w = p.a.weight != nullptr ? p.a.weight + c.b * p.a.w_seq + (int64_t)kvh * p.a.w_head : nullptr;
     float* wo = p.a.weight_out + c.b * p.a.wo_seq + (int64_t)kvh * p.a.wo_head;
-    const float* l2 = p.lse2 + c.b * p.a.q_heads + (int64_t)kvh * p.group;
-    for (int64_t j = (int64_t)c.at * kKeys + lane; j < end; j += 32) {
-      float y = w != nullptr && j < p.a.weight_cols ? w[j] : 0.f;
-      for (int hb = 0; hb < p.head_blocks; ++hb) {
-        const float4* s = reinterpret_cast<const float4*>(p.scores + ((c.b * p.units + kvh * p.head_blocks + hb) * p.line + j) * kNH);
-        const int heads = min(kNH, p.group - hb * kNH);
+    for (int hb = 0; hb < p.head_blocks; ++hb) {
+      const int unit = kvh * p.head_blocks + hb, heads = min(nh, p.group - hb * nh);
+      const Parts parts(p, line, begin, end, unit);
+      // log2 of the head's sum of exponentials, in the lane of the head's number
+      float all = -INFINITY;
+      if (parts.n == 1) {
+        if (lane < heads) all = p.lse2[c.b * p.a.q_heads + (int64_t)kvh * p.group + hb * nh + lane];
+      } else {
+        for (int h = 0; h < heads; ++h) {
+          float m = -INFINITY, l = 0.f;
+          for (int i = lane; i < parts.n; i += 32) {
+            const float2 ml = p.ml[parts[i] * nh + h];
+            const float top = fmaxf(m, ml.x);
+            l = brought(l, m, top) + brought(ml.y, ml.x, top);
+            m = top;
+          }
 #pragma unroll
-        for (int i = 0; i < kNH / 4; ++i) {
-          const float4 x = s[i];
-          const float e[4] = {x.x, x.y, x.z, x.w};
+          for (int i = 16; i > 0; i >>= 1) {
+            const float m2 = __shfl_xor_sync(kAll, m, i), l2 = __shfl_xor_sync(kAll, l, i), top = fmaxf(m, m2);
+            l = brought(l, m, top) + brought(l2, m2, top);
+            m = top;
+          }
+          if (lane == h) all = l == 0.f ? -INFINITY : m + log2f(l);
+        }
+      }
+      for (int h8 = 0; h8 < heads; h8 += 8) {
+        float all8[8];  // (without keys: everything counts nothing against infinity)
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            if (4 * i + n < heads) {
-              const float all = l2[hb * kNH + 4 * i + n];
-              y += all == -INFINITY ? 0.f : ex2(e[n] - all);
+        for (int n = 0; n < 8; ++n) {
+          const float a = __shfl_sync(kAll, all, (h8 + n) & 31);
+          all8[n] = a != -INFINITY ? a : INFINITY;
+        }
+        const float* s = p.scores + (c.b * p.units + unit) * p.line * nh + h8;
+        const bool first = hb == 0 && h8 == 0;
+        constexpr int kAhead = 4;
+        for (int64_t j0 = (int64_t)c.s0 * kKeys + lane; j0 - lane < upto; j0 += 32 * kAhead) {
+          float4 x[kAhead][2];
+          float y[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int64_t j = j0 + 32 * u;
+            y[u] = 0.f;
+            if (j < upto && j < p.a.weight_cols) {
+              x[u][0] = *reinterpret_cast<const float4*>(s + j * nh);
+              x[u][1] = *reinterpret_cast<const float4*>(s + j * nh + 4);
+              if (!first)
+                y[u] = wo[j];
+              else if (w != nullptr)
+                y[u] = w[j];
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int64_t j = j0 + 32 * u;
+            if (j < upto && j < p.a.weight_cols) {
+              const float e[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
+              float sum = 0.f;
+#pragma unroll
+              for (int n = 0; n < 8; ++n) sum += h8 + n < heads ? ex2(e[n] - all8[n]) : 0.f;
+              wo[j] = y[u] + sum;
+            } else if (j < upto && p.status) {
+              atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
             }
           }
         }
       }
-      if (j < p.a.weight_cols)
-        wo[j] = y;
-      else if (p.status)
-        atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
     }
-    left -= blocks;
-    if (left <= 0) break;
-    c.at = c.blocks - 1;
-    advance(p, c);
+    left -= c.s1 - c.s0;
+    begin = end;
+    if (left <= 0 || !next_segment(p, c, left)) break;
   }
 }
 
@@ -778,10 +922,10 @@ int ctas_of(bool fp8, int D, int nt) {
   return fp8 ? (nt == 1 ? paged_ctas<true, 128, 1>() : paged_ctas<true, 128, 2>()) : nt == 1 ? paged_ctas<false, 128, 1>() : paged_ctas<false, 128, 2>();
 }
 
-// Sizes of the call, checked; what the workspace holds in turn: `before`, lse2, ml, o, scores
+// Sizes of the call, checked; what the workspace holds in turn: lse2, ml, o, scores
 struct Plan {
   int nt = 1, nh = 8;
-  int64_t ctas = 0, bytes[5] = {}, total = 0;
+  int64_t ctas = 0, finish_ctas = 0, bytes[4] = {}, total = 0;
 };
 int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 int make_plan(const fftopk_paged* a, int sms, PagedParams& p, Plan& plan) {
@@ -798,22 +942,32 @@ int make_plan(const fftopk_paged* a, int sms, PagedParams& p, Plan& plan) {
   p.bound = (int32_t)bound;
   p.weigh = a->weight_out != nullptr;
   const int64_t blocks = a->seqs * ((bound + kKeys - 1) / kKeys);
-  const int64_t warps = (int64_t)sms * ctas_of(a->k_scale != nullptr, a->D, plan.nt) * kWarps;
-  int64_t runs = warps / units < blocks / kMinBlocks ? warps / units : blocks / kMinBlocks;
+  const int64_t ctas = (int64_t)sms * ctas_of(a->k_scale != nullptr, a->D, plan.nt);
+  int64_t runs = ctas / units < blocks / kMinBlocks ? ctas / units : blocks / kMinBlocks;
   if (runs < 1) runs = 1;
   p.runs = (int32_t)runs;
-  plan.ctas = (runs * units + kWarps - 1) / kWarps;
+  plan.ctas = runs * units;
   p.line = (bound + kKeys - 1) / kKeys * kKeys;
   if (runs > 1) {
-    plan.bytes[0] = up256((a->seqs + 1) * 8);
-    plan.bytes[2] = up256(runs * units * 2 * plan.nh * 8);
-    plan.bytes[3] = up256(runs * units * 2 * plan.nh * a->D * 4);
+    plan.bytes[1] = up256(runs * units * 2 * plan.nh * 8);
+    plan.bytes[2] = up256(runs * units * 2 * plan.nh * a->D * 4);
+    // a warp a pair where a CTA each would take more than the device holds at once, and several where that would
+    const int64_t pairs = a->seqs * a->q_heads, room = (int64_t)sms * 64;
+    p.join_each = pairs * kWarps <= room ? 0 : (int32_t)((pairs + room - 1) / room);
+    plan.finish_ctas = p.join_ctas = (int32_t)(p.join_each == 0 ? pairs : ((pairs + p.join_each - 1) / p.join_each + kWarps - 1) / kWarps);
   }
   if (p.weigh) {
-    plan.bytes[1] = up256(a->seqs * a->q_heads * 4);
+    plan.bytes[0] = up256(a->seqs * a->q_heads * 4);
     // (below 2^31 sequences * heads, times 2^31 positions, times 64 bytes: in question where it would wrap)
     if (p.line > 0 && a->seqs * units > ((int64_t)1 << 50) / (p.line * plan.nh)) return FFTOPK_ERANGE;
-    plan.bytes[4] = up256(a->seqs * units * p.line * plan.nh * 4);
+    plan.bytes[3] = up256(a->seqs * units * p.line * plan.nh * 4);
+  }
+  if (p.weigh) {
+    int64_t each = (int64_t)sms * 8 * kWarps / a->kv_heads;
+    if (each > blocks) each = blocks;
+    if (each < 1) each = 1;
+    p.weigh_runs = (int32_t)each;
+    plan.finish_ctas += (each * a->kv_heads + kWarps - 1) / kWarps;
   }
   for (int64_t n : plan.bytes) plan.total += n;
   return 0;
@@ -856,10 +1010,8 @@ cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t st
   const bool d64 = p.a.D == 64;
   cudaError_t e = fp8 ? (d64 ? launch_paged<T, true, 64>(p, plan, stream) : launch_paged<T, true, 128>(p, plan, stream))
                       : d64 ? launch_paged<T, false, 64>(p, plan, stream) : launch_paged<T, false, 128>(p, plan, stream);
-  if (e == cudaSuccess && p.runs > 1) {
-    const int64_t grid = p.a.seqs * p.a.q_heads;
-    e = launch(d64 ? paged_join_kernel<T, 64> : paged_join_kernel<T, 128>, grid, kJoinWarps * 32, 0, true, stream, p);
-  }
+  if (e == cudaSuccess && plan.finish_ctas > 0)
+    e = launch(d64 ? paged_finish_kernel<T, 64> : paged_finish_kernel<T, 128>, plan.finish_ctas, kThreads, 0, true, stream, p);
   return e;
 }
 
@@ -900,23 +1052,15 @@ int fftopk_paged_attention(const fftopk_paged* a, void* workspace, size_t worksp
   if (a->slots == 0) p.a.k = p.a.v = a->q;  // (an empty cache has no address, and rows that are left out are copies of no bytes: from somewhere)
   p.page = FastDiv((uint32_t)a->page_size);
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
+  p.out_vec = on(a->out, 8) && (a->seqs <= 1 || a->out_seq % 4 == 0) && (a->q_heads <= 1 || a->out_head % 4 == 0);
   p.status = status;
   char* at = static_cast<char*>(workspace);
-  p.before = reinterpret_cast<int64_t*>(at), at += plan.bytes[0];
-  p.lse2 = reinterpret_cast<float*>(at), at += plan.bytes[1];
-  p.ml = reinterpret_cast<float2*>(at), at += plan.bytes[2];
-  p.o = reinterpret_cast<float*>(at), at += plan.bytes[3];
+  p.lse2 = reinterpret_cast<float*>(at), at += plan.bytes[0];
+  p.ml = reinterpret_cast<float2*>(at), at += plan.bytes[1];
+  p.o = reinterpret_cast<float*>(at), at += plan.bytes[2];
   p.scores = reinterpret_cast<float*>(at);
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  cudaError_t e = a->dtype == FFTOPK_DTYPE_BF16 ? launch_paged<__nv_bfloat16>(p, plan, stream) : launch_paged<__half>(p, plan, stream);
-  if (e == cudaSuccess && p.weigh) {
-    int64_t runs = (int64_t)sms * 8 * kWarps / a->kv_heads;
-    const int64_t blocks = a->seqs * (p.line / kKeys);
-    if (runs > blocks) runs = blocks;
-    if (runs < 1) runs = 1;
-    const int64_t grid = (runs * a->kv_heads + kWarps - 1) / kWarps;
-    e = launch(plan.nt == 1 ? paged_weigh_kernel<8> : paged_weigh_kernel<16>, grid, kThreads, 0, true, stream, p);
-  }
+  const cudaError_t e = a->dtype == FFTOPK_DTYPE_BF16 ? launch_paged<__nv_bfloat16>(p, plan, stream) : launch_paged<__half>(p, plan, stream);
   return e == cudaSuccess ? FFTOPK_OK : cuda_fail(e);
 }
 

@@ -486,7 +486,7 @@ int fftopk_sparse_attention(const fftopk_attend* args, uint32_t* status, void* c
  *                time need one each. With weight_out it holds the scores of all positions the table has room for, 32 bytes (of more
  *                than 8 query heads to a key head: 64 for every 16) per position and key head. The size is that of the current device.
  * Roundings, and what is asked of v scales: as for fftopk_sparse_attention. The same call gives the same bits.
- * The first call on a device sets kernel attributes (outside any capture); up to three kernels, no host synchronisation.
+ * The first call on a device sets kernel attributes (outside any capture); one or two kernels, no host synchronisation.
  */
 typedef struct fftopk_paged {
   const void* q;

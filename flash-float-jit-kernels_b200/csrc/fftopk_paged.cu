@@ -43,6 +43,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;      // of a block: rows of the MMA
+constexpr int kWeighBlocks = 8;  // positions that a warp has on their way at a time
 constexpr int kMinBlocks = 16;  // of a run: below that, parts to join cost more than the blocks
 
 struct PagedParams {
@@ -720,7 +721,7 @@ __device__ __forceinline__ void write_joined(const PagedParams& p, int64_t b, in
 // sequence and a query head, or, where there are few, a CTA one of them. The others bring the weights up to date from the scores and the
 // joined sums: a warp takes a run of the line for one key head, a lane a position. Where sequences begin is found while the kernel in front still runs.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) paged_finish_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(kThreads, 5) paged_finish_kernel(const __grid_constant__ PagedParams p) {
   constexpr int kC = D / 32;  // channels of a lane
   __shared__ float4 part[kWarps][D / 4];
   __shared__ float2 ml_of[kWarps];
@@ -774,7 +775,7 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(const __grid_con
   const uint32_t gw = (blockIdx.x - (uint32_t)p.join_ctas) * (uint32_t)kWarps + (uint32_t)warp;
   const uint32_t run = gw / (uint32_t)p.a.kv_heads;
   const int kvh = (int)(gw - run * (uint32_t)p.a.kv_heads);
-  const Runs mine(total, p.weigh_runs, 2);
+  const Runs mine(total, p.weigh_runs, kWeighBlocks);
   int64_t left = (int64_t)run < mine.runs ? mine.begin((int64_t)run + 1) - mine.begin(run) : 0;
   Segment c = {};
   if (left > 0) c = segment_at(p, mine.begin(run), left, lane);
@@ -794,22 +795,26 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(const __grid_con
       if (parts.n == 1) {
         if (lane < heads) all = p.lse2[c.b * p.a.q_heads + (int64_t)kvh * p.group + hb * nh + lane];
       } else {
-        for (int h = 0; h < heads; ++h) {
-          float m = -INFINITY, l = 0.f;
-          for (int i = lane; i < parts.n; i += 32) {
-            const float2 ml = p.ml[parts[i] * nh + h];
-            const float top = fmaxf(m, ml.x);
-            l = brought(l, m, top) + brought(ml.y, ml.x, top);
-            m = top;
-          }
+        float m = -INFINITY, l = 0.f;  // (lanes of a head take its parts in turn)
+        for (int i = lane / nh; i < parts.n; i += 4 * (32 / nh)) {
+          float2 ml[4];
 #pragma unroll
-          for (int i = 16; i > 0; i >>= 1) {
-            const float m2 = __shfl_xor_sync(kAll, m, i), l2 = __shfl_xor_sync(kAll, l, i), top = fmaxf(m, m2);
-            l = brought(l, m, top) + brought(l2, m2, top);
-            m = top;
+          for (int u = 0; u < 4; ++u) {
+            const int at = i + u * (32 / nh);
+            ml[u] = at < parts.n ? p.ml[parts[at] * nh + lane % nh] : make_float2(-INFINITY, 0.f);
           }
-          if (lane == h) all = l == 0.f ? -INFINITY : m + log2f(l);
+          const float top = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+          l = brought(l, m, top);
+          m = top;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) l += brought(ml[u].y, ml[u].x, m);
         }
+        for (int i = nh; i < 32; i *= 2) {
+          const float m2 = __shfl_xor_sync(kAll, m, i), l2 = __shfl_xor_sync(kAll, l, i), top = fmaxf(m, m2);
+          l = brought(l, m, top) + brought(l2, m2, top);
+          m = top;
+        }
+        all = l == 0.f ? -INFINITY : m + log2f(l);
       }
       for (int h8 = 0; h8 < heads; h8 += 8) {
         float all8[8];  // (without keys: everything counts nothing against infinity)

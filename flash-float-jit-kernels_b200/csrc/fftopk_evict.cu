@@ -3,9 +3,10 @@
 // rows that another page table names; their weights go along. A sequence of up to `budget` rows keeps them all. (The reference ends with
 // the selection of indices; attention over a paged cache that adds up the weights is fftopk_paged.cu.)
 //
-// evict_select_kernel: a cluster per sequence and key head finds the smallest weight that stays, by radix rounds over the order-preserving
-// keys of the weights (11, 11 and 10 bits, histograms in shared memory, summed over the cluster), and lists what stays in order: every CTA has
-// a stretch of the positions, every warp a stretch of those, so that places are prefix sums. A weight is read once, its key stays in
+// evict_select_kernel: a CTA or a cluster per sequence and key head finds the smallest weight that stays, by radix rounds over the order-preserving keys
+// of the weights (11, 11 and 10 bits, histograms in shared memory, summed over the cluster), and lists what stays in order. The first round
+// counts weights as they come in; behind it every 32 positions are a word of bits - above the threshold's bin, in it - and what
+// follows looks at the few that are in it. Places in the list are prefix sums over the words. A weight is read once and stays in
 // shared memory (positions beyond its room are read again).
 // evict_move_kernel: a warp takes 32 rows of a key head that lie next to each other where they go; a lane finds where one of them comes from, and
 // the warp copies k and v. Reading and writing the rows bounds it.
@@ -13,6 +14,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <string.h>
+#include <stdlib.h>
 
 #include "../../include/fftopk.h"
 #include "fftopk_host.h"
@@ -29,13 +31,16 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048, kRounds = 3;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxKeys = 20 * 1024;  // of a CTA in shared memory: two CTAs per SM
+constexpr int kBatch = 8;  // weights a thread has on their way
+constexpr int kMaxKeys = 16 * 1024;       // of a CTA in shared memory: two CTAs per SM
+constexpr int kMaxSpan = 256 * 1024;      // positions of a CTA
 constexpr int kMoveThreads = 128;
 
 struct EvictParams {
   fftopk_evict a;
   int32_t bound;  // positions that the table and the weights reach
   int32_t keys;   // of a CTA that shared memory has room for
+  int32_t words;  // of 32 positions of a CTA
   int32_t moves;  // evict_move_kernel follows
   FastDiv page;
   uint32_t* status;
@@ -43,18 +48,54 @@ struct EvictParams {
 
 __device__ __forceinline__ int digit_shift(int round) { return round == 0 ? 21 : round == 1 ? 10 : 0; }
 
+struct Word {  // 32 positions: those that stay for certain, those in question, and how many of either lie in front of them
+  uint32_t sure, tie, sure_before, tie_before;
+};
 struct SelectSmem {
   uint32_t hist[kRounds][kBins];
   uint32_t warp_total[kWarps];
-  uint32_t found[3];       // bin, count above it, count in it
-  uint32_t stay[2];        // of this CTA: rows that stay for certain, rows of the smallest weight that stays
-  uint32_t warp_stay[2][kWarps];
+  uint32_t found[3];  // bin, count above it, count in it
+  uint64_t warp_stay[kWarps];
+  uint64_t stay;      // of this CTA: rows that stay for certain, and, in the upper half, rows of the smallest weight that stays
 };
+
+// Where the count from the top of the round's histogram - summed over the cluster - reaches `need`: the bin, the count above it, the count in it
+__device__ __forceinline__ void pick(SelectSmem& sm, cg::cluster_group& cluster, int ctas, int round, uint32_t need) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (ctas > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  uint32_t v[4] = {0u, 0u, 0u, 0u};  // four bins a thread, the highest first
+  const int bin0 = kBins - 4 - 4 * tid;
+  for (int c = 0; c < ctas; ++c) {
+    const uint4 x = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&sm.hist[round][bin0], c));
+    v[0] += x.w, v[1] += x.z, v[2] += x.y, v[3] += x.x;
+  }
+  const uint32_t s = v[0] + v[1] + v[2] + v[3];
+  uint32_t upto = s;
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    const uint32_t y = __shfl_up_sync(kAll, upto, i);
+    if (lane >= i) upto += y;
+  }
+  if (lane == 31) sm.warp_total[warp] = upto;
+  __syncthreads();
+  uint32_t above = upto - s;
+  for (int i = 0; i < warp; ++i) above += sm.warp_total[i];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (above < need && above + v[e] >= need) sm.found[0] = (uint32_t)(bin0 + 3 - e), sm.found[1] = above, sm.found[2] = v[e];
+    above += v[e];
+  }
+  __syncthreads();
+}
 
 __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SelectSmem& sm = *reinterpret_cast<SelectSmem*>(smem_raw);
-  uint32_t* const keys = reinterpret_cast<uint32_t*>(smem_raw + sizeof(SelectSmem));
+  Word* const words = reinterpret_cast<Word*>(smem_raw + sizeof(SelectSmem));
+  uint32_t* const held = reinterpret_cast<uint32_t*>(words + p.words);  // the CTA's weights, as bits
   // (only where a kernel of this call follows, which waits: another one's inputs may be this one's results)
   if (p.moves) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   cg::cluster_group cluster = cg::this_cluster();
@@ -83,151 +124,148 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
   const int32_t first = p.a.sinks, last = n - p.a.recent;  // (sinks + recent <= budget < n)
   uint32_t need = (uint32_t)(budget - first - p.a.recent);  // of the rows between
   const int32_t each = ((n + ctas - 1) / ctas + 31) & ~31;
-  const int32_t from = min(n, rank * each), to = min(n, from + each);
-  const int32_t lo = max(from, first), hi = min(to, last);  // of the CTA's stretch, between
+  const int32_t from = min(n, rank * each), span = min(n - from, each), there = min(span, p.keys);
+  const int32_t lo = first - from, hi = last - from;  // the rows between, counted from the CTA's first
+  w += from;
+  auto bits_at = [&](int32_t i) { return i < there ? held[i] : __float_as_uint(w[i]); };
+  auto key_at = [&](int32_t i) { return fftopk_key_from_bits(bits_at(i)); };
 
-  for (int i = tid; i < kRounds * kBins; i += kThreads) (&sm.hist[0][0])[i] = 0u;
+  for (int i = tid; i < kRounds * kBins / 4; i += kThreads) reinterpret_cast<uint4*>(&sm.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
   __syncthreads();
-  auto key_at = [&](int32_t j) { return j - from < p.keys ? keys[j - from] : fftopk_key_from_bits(__float_as_uint(w[j])); };
-  // the key of the smallest weight that stays, and how many of that weight do (0 of 0xffffffff + 1: none is in question)
-  uint32_t edge = 0, mask = 0, ties = need;
-  for (int round = 0; round < kRounds; ++round) {
-    const int shift = digit_shift(round);
-    const uint32_t top = round == 0 ? 0x7ffu : round == 1 ? 0x7ffu : 0x3ffu;
-    for (int32_t base = lo; base < hi; base += kThreads) {
-      const int32_t j = base + tid;
-      const bool in = j < hi;
-      uint32_t key = 0;
-      if (in) {
-        if (round == 0) {
-          key = fftopk_key_from_bits(__float_as_uint(w[j]));
-          if (j - from < p.keys) keys[j - from] = key;
-        } else {
-          key = key_at(j);
-        }
-      }
-      const bool counts = in && (key & mask) == edge;
-      const uint32_t digit = key >> shift & top;
+  // round 0 as the weights come in
+  for (int32_t i0 = tid; i0 - lane < span; i0 += kThreads * kBatch) {
+    float x[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) x[u] = i0 + u * kThreads < span ? w[i0 + u * kThreads] : 0.f;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int32_t i = i0 + u * kThreads;
+      const uint32_t bits = __float_as_uint(x[u]);
+      if (i < there) held[i] = bits;
+      const bool counts = i < span && i >= lo && i < hi;
+      const uint32_t digit = fftopk_key_from_bits(bits) >> 21;
       const unsigned who = __ballot_sync(kAll, counts);
       if (who == 0u) continue;
       const uint32_t lead = __shfl_sync(kAll, digit, __ffs((int)who) - 1);
       if (__all_sync(kAll, !counts || digit == lead)) {  // (copies of one weight: one addition for the warp)
-        if (lane == 0) atomicAdd(&sm.hist[round][lead], (uint32_t)__popc(who));
+        if (lane == 0) atomicAdd(&sm.hist[0][lead], (uint32_t)__popc(who));
       } else if (counts) {
-        atomicAdd(&sm.hist[round][digit], 1u);
+        atomicAdd(&sm.hist[0][digit], 1u);
       }
     }
-    if (ctas > 1)
-      cluster.sync();
-    else
-      __syncthreads();
-    // four bins a thread, from the top: where the count from above reaches `need`
-    uint32_t v[4], s = 0;
-    const int bin0 = kBins - 4 - 4 * tid;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = 0;
-    for (int c = 0; c < ctas; ++c) {
-      const uint4 x = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&sm.hist[round][bin0], c));
-      v[0] += x.w, v[1] += x.z, v[2] += x.y, v[3] += x.x;  // highest bin first
+  }
+  // of the rows between those stay whose key, as far as `mask`, is above `edge`, and the first `ties` of those at it
+  uint32_t edge = 0xffffffffu, mask = 0xffffffffu, ties = 0;  // (none)
+  bool whole = true;  // the bin stays whole, or is one weight
+  if (need > 0) {
+    pick(sm, cluster, ctas, 0, need);
+    edge = sm.found[0] << 21, mask = 0x7ffu << 21;
+    need -= sm.found[1];
+    ties = need;
+    whole = sm.found[2] == need;
+  }
+  const int32_t n_words = (span + 31) / 32;
+  for (int32_t word = warp; word < n_words; word += kWarps) {
+    const int32_t i = word * 32 + lane;
+    const bool in = i < span, between = in && i >= lo && i < hi;
+    const uint32_t key = between ? key_at(i) & mask : 0u;
+    const unsigned s = __ballot_sync(kAll, in && (!between || key > edge)), t = __ballot_sync(kAll, between && key == edge);
+    if (lane == 0) words[word].sure = s, words[word].tie = t;
+  }
+  __syncthreads();
+  // the other rounds look at what is in question only, a thread a word
+  for (int round = 1; round < kRounds && !whole; ++round) {
+    const int shift = digit_shift(round);
+    const uint32_t top = round == 1 ? 0x7ffu : 0x3ffu;
+    for (int32_t word = tid; word < n_words; word += kThreads) {
+      uint32_t t = words[word].tie, digit = 0, count = 0;  // (runs of one digit are added at once)
+      while (t != 0u) {
+        const uint32_t key = key_at(word * 32 + __ffs((int)t) - 1);
+        t &= t - 1u;
+        if ((key & mask) != edge) continue;
+        const uint32_t d = key >> shift & top;
+        if (d != digit && count > 0) atomicAdd(&sm.hist[round][digit], count), count = 0;
+        digit = d, ++count;
+      }
+      if (count > 0) atomicAdd(&sm.hist[round][digit], count);
     }
-    s = v[0] + v[1] + v[2] + v[3];
-    uint32_t upto = s;
+    pick(sm, cluster, ctas, round, need);
+    edge |= sm.found[0] << shift;
+    mask |= top << shift;
+    need -= sm.found[1];
+    ties = need;
+    whole = sm.found[2] == need;
+  }
+  // what was in question is settled, and counted over words, warps and CTAs
+  uint64_t before = 0;
+  for (int32_t w0 = 0; w0 < n_words; w0 += kThreads) {
+    const int32_t word = w0 + tid;
+    uint32_t s = 0, t = 0;
+    if (word < n_words) {
+      s = words[word].sure;
+      for (uint32_t q = words[word].tie; q != 0u; q &= q - 1u) {
+        const uint32_t key = key_at(word * 32 + __ffs((int)q) - 1) & mask;
+        if (key > edge) s |= q & -q;
+        if (key == edge) t |= q & -q;
+      }
+    }
+    const uint64_t mine = (uint64_t)__popc(t) << 32 | (uint32_t)__popc(s);
+    uint64_t upto = mine;
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) {
-      const uint32_t y = __shfl_up_sync(kAll, upto, i);
+      const uint64_t y = __shfl_up_sync(kAll, upto, i);
       if (lane >= i) upto += y;
     }
-    if (lane == 31) sm.warp_total[warp] = upto;
-    if (tid == 0) sm.found[0] = 0xffffffffu;
+    if (lane == 31) sm.warp_stay[warp] = upto;
     __syncthreads();
-    uint32_t above = upto - s;
-    for (int i = 0; i < warp; ++i) above += sm.warp_total[i];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (above < need && above + v[e] >= need) sm.found[0] = (uint32_t)(bin0 + 3 - e), sm.found[1] = above, sm.found[2] = v[e];
-      above += v[e];
+    uint64_t sum = before, total = before;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) sum += sm.warp_stay[i];
+      total += sm.warp_stay[i];
     }
+    sum += upto - mine;
+    if (word < n_words) words[word] = Word{s, t, (uint32_t)sum, (uint32_t)(sum >> 32)};
+    before = total;
     __syncthreads();
-    const uint32_t bin = sm.found[0], over = sm.found[1], in_bin = sm.found[2];
-    if (bin == 0xffffffffu) {  // (need = 0: none of the rows between stays)
-      edge = 0xffffffffu, mask = 0xffffffffu, ties = 0;
-      break;
-    }
-    edge |= bin << shift;
-    mask |= top << shift;
-    need -= over;
-    ties = need;
-    if (in_bin == need) break;  // the whole bin stays
   }
-  // Rows above the bin stay; of the bin's, where it is one weight (mask all ones) or stays whole, the first `ties`.
-  // count, sum over warps and CTAs, write
-  const int32_t part = ((to - from + kWarps - 1) / kWarps + 31) & ~31;
-  const int32_t w0 = min(to, from + warp * part), w1 = min(to, w0 + part);
-  auto sort_of = [&](int32_t j, bool& sure, bool& tie) {
-    sure = j < first || j >= last;
-    tie = false;
-    if (!sure) {
-      const uint32_t k = key_at(j) & mask;
-      sure = k > edge;
-      tie = k == edge;
-    }
-  };
-  uint32_t sures = 0, tied = 0;
-  for (int32_t base = w0; base < w1; base += 32) {
-    bool sure = false, tie = false;
-    if (base + lane < w1) sort_of(base + lane, sure, tie);
-    sures += (uint32_t)__popc(__ballot_sync(kAll, sure));
-    tied += (uint32_t)__popc(__ballot_sync(kAll, tie));
-  }
-  if (lane == 0) sm.warp_stay[0][warp] = sures, sm.warp_stay[1][warp] = tied;
-  __syncthreads();
-  if (tid < 2) {
-    uint32_t s = 0;
-    for (int i = 0; i < kWarps; ++i) s += sm.warp_stay[tid][i];
-    sm.stay[tid] = s;
-  }
-  if (ctas > 1)
+  uint32_t sures = 0, tied = 0;  // in front of this CTA
+  if (ctas > 1) {
+    if (tid == 0) sm.stay = before;
     cluster.sync();
-  else
-    __syncthreads();
-  uint32_t sures_before = 0, tied_before = 0;
-  for (int c = 0; c < rank; ++c) {
-    const uint32_t* s = cluster.map_shared_rank(&sm.stay[0], c);
-    sures_before += s[0], tied_before += s[1];
-  }
-  for (int i = 0; i < warp; ++i) sures_before += sm.warp_stay[0][i], tied_before += sm.warp_stay[1][i];
-  for (int32_t base = w0; base < w1; base += 32) {
-    const int32_t j = base + lane;
-    bool sure = false, tie = false;
-    if (j < w1) sort_of(j, sure, tie);
-    const unsigned s = __ballot_sync(kAll, sure), t = __ballot_sync(kAll, tie), below = (1u << lane) - 1u;
-    const uint32_t tie_rank = tied_before + (uint32_t)__popc(t & below);
-    if (sure || (tie && tie_rank < ties)) {
-      const uint32_t at = sures_before + (uint32_t)__popc(s & below) + min(tie_rank, ties);
-      if (at < (uint32_t)left) kept[at] = j, wo[at] = w[j];
+    for (int c = 0; c < rank; ++c) {
+      const uint64_t x = *cluster.map_shared_rank(&sm.stay, c);
+      sures += (uint32_t)x, tied += (uint32_t)(x >> 32);
     }
-    sures_before += (uint32_t)__popc(s), tied_before += (uint32_t)__popc(t);
+  }
+  for (int32_t word = warp; word < n_words; word += kWarps) {
+    const Word q = words[word];
+    const uint32_t below = (1u << lane) - 1u, tie_rank = tied + q.tie_before + (uint32_t)__popc(q.tie & below);
+    if ((q.sure >> lane & 1u) || ((q.tie >> lane & 1u) && tie_rank < ties)) {
+      const uint32_t at = sures + q.sure_before + (uint32_t)__popc(q.sure & below) + min(tie_rank, ties);
+      const int32_t i = word * 32 + lane;
+      if (at < (uint32_t)left) kept[at] = from + i, wo[at] = __uint_as_float(bits_at(i));
+    }
   }
   if (ctas > 1) cluster.sync();  // (nobody leaves while its memory is read)
 }
 
 // P: what a piece of a row is copied as
 template <typename P>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p, int pieces, int lanes, int groups) {
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p, int pieces, int lanes, int groups, int rows) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5);
-  // (32 rows of a key head; the key heads of the same places are neighbours)
+  // (`rows` rows, up to 32, of a key head; the key heads of the same places are neighbours)
   const int64_t rest = item / p.a.heads;
   const int h = (int)(item - rest * p.a.heads);
   const int64_t b = rest / groups;
-  const int32_t j0 = (int32_t)(rest - b * groups) * 32;
+  const int32_t j0 = (int32_t)(rest - b * groups) * rows;
   if (b >= p.a.seqs) return;
   const int32_t left = p.a.new_lengths[b];
   if (j0 >= left) return;
   int64_t src = -1, dst = -1;
   const int32_t j = j0 + lane;
-  if (j < left) {
+  if (lane < rows && j < left) {
     const uint32_t pos = (uint32_t)p.a.kept[(b * p.a.heads + h) * p.a.budget + j];
     const uint32_t n = p.page.div(pos), m = p.page.div((uint32_t)j);
     const int32_t from = p.a.page_table[b * p.a.table_row + n], to = p.a.to_table[b * p.a.to_row + m];
@@ -246,7 +284,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   char* const v = static_cast<char*>(p.a.v) + (int64_t)h * p.a.v_head * es;
   const int sub = lane / lanes, piece = lane - sub * lanes, once = 32 / lanes;
   constexpr int kAhead = 4;
-  for (int at = 0; at < 32; at += once * kAhead) {
+  for (int at = 0; at < rows; at += once * kAhead) {
     int64_t from[kAhead], to[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -285,7 +323,7 @@ int evict_setup(int& sms) {
   const int rc = g_evict_once[dev].run([&] {
     cudaError_t e2 = cudaDeviceGetAttribute(&g_evict_sms[dev], cudaDevAttrMultiProcessorCount, dev);
     if (e2 == cudaSuccess)
-      e2 = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(SelectSmem) + kMaxKeys * 4));
+      e2 = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(SelectSmem) + kMaxSpan / 32 * sizeof(Word) + kMaxKeys * 4));
     return e2 == cudaSuccess ? 0 : cuda_fail(e2);
   });
   sms = g_evict_sms[dev];
@@ -298,9 +336,10 @@ bool rows_on(const void* p, int64_t slots, int64_t slot, int64_t heads, int64_t 
   return on(p, piece) && (slots <= 1 || slot * es % piece == 0) && (heads <= 1 || head * es % piece == 0);
 }
 
+int move_rows(const EvictParams& p) { const char* e = getenv("MOVE_ROWS"); return e ? atoi(e) : 32; }
 template <typename P>
 cudaError_t launch_move(const EvictParams& p, int row_bytes, cudaStream_t stream) {
-  const int pieces = row_bytes / (int)sizeof(P), groups = (p.a.budget + 31) / 32;
+  const int pieces = row_bytes / (int)sizeof(P), rows = move_rows(p), groups = (p.a.budget + rows - 1) / rows;
   int lanes = 1;
   while (lanes < 32 && lanes < pieces) lanes *= 2;
   const int64_t warps = p.a.seqs * p.a.heads * groups;
@@ -313,7 +352,7 @@ cudaError_t launch_move(const EvictParams& p, int row_bytes, cudaStream_t stream
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, evict_move_kernel<P>, p, pieces, lanes, groups);
+  return cudaLaunchKernelEx(&cfg, evict_move_kernel<P>, p, pieces, lanes, groups, rows);
 }
 
 }  // namespace
@@ -338,11 +377,11 @@ extern "C" int fftopk_cache_evict(const fftopk_evict* a, uint32_t* status, void*
       !on(a->page_table, 4) || !on(a->to_table, 4) || !on(a->lengths, 4) || !on(a->new_lengths, 4) || !on(a->kept, 4))
     return FFTOPK_EINVAL;
   const int64_t bound = (int64_t)a->pages * a->page_size < a->weight_cols ? (int64_t)a->pages * a->page_size : a->weight_cols;
-  if (a->slots > 0x7fffffff || a->seqs > 0x7fffffff / a->heads || bound > 0x7ffff000 || (int64_t)a->to_pages * a->page_size < a->budget ||
+  if (a->slots > 0x7fffffff || a->seqs > 0x7fffffff / a->heads || bound > kMaxCluster * kMaxSpan || (int64_t)a->to_pages * a->page_size < a->budget ||
       a->budget > 0x7ffff000)
     return FFTOPK_ERANGE;
   const int64_t units = a->seqs * a->heads;
-  if (units * ((a->budget + 31) / 32) > 0x7fffffff) return FFTOPK_ERANGE;
+  if (units * ((a->budget + 7) / 8) > 0x7fffffff) return FFTOPK_ERANGE;
   int sms = 0;
   const int rc = evict_setup(sms);
   if (rc) return rc;
@@ -353,17 +392,18 @@ extern "C" int fftopk_cache_evict(const fftopk_evict* a, uint32_t* status, void*
   p.moves = a->budget > 0 && bound > 0;
   p.page = FastDiv((uint32_t)a->page_size);
   p.status = status;
-  // CTAs a unit: as many as fit the device at once, of 4,096 positions at least
+  // CTAs a unit: as many as fit the device at once, of 4,096 positions at least; and enough for what a CTA can hold
   int ctas = 1;
-  while (ctas < kMaxCluster && units * ctas * 2 <= 2 * (int64_t)sms && bound / ctas > 8192) ctas *= 2;
+  while (ctas < kMaxCluster && ((units * ctas * 2 <= 2 * (int64_t)sms && bound / ctas > 8192) || bound > (int64_t)ctas * kMaxSpan)) ctas *= 2;
   if (units * ctas > 0x7fffffff) return FFTOPK_ERANGE;
   const int64_t each = ((bound + ctas - 1) / ctas + 31) & ~(int64_t)31;
   p.keys = (int32_t)(each < kMaxKeys ? each : kMaxKeys);
+  p.words = (int32_t)(each / 32);
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * ctas), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = sizeof(SelectSmem) + (size_t)p.keys * 4;
+  cfg.dynamicSmemBytes = sizeof(SelectSmem) + (size_t)p.words * sizeof(Word) + (size_t)p.keys * 4;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

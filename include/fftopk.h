@@ -534,6 +534,7 @@ int fftopk_paged_attention(const fftopk_paged* args, void* workspace, size_t wor
  *   weight, weight_out fp32 [seqs, heads, weight_cols], inner stride 1, apart from one another
  *   page_table   int32 [seqs, pages], to_table int32 [seqs, to_pages], inner stride 1; to_pages * page_size >= budget (FFTOPK_ERANGE otherwise)
  *   kept         int32 [seqs, heads, budget], contiguous; lengths, new_lengths int32 [seqs]; sinks + recent <= budget
+ * Tables and weights reach up to 2,097,152 positions of a sequence (the smaller of pages * page_size and weight_cols; FFTOPK_ERANGE beyond).
  * No workspace, no host synchronisation; two kernels. The first call on a device sets kernel attributes (outside any capture).
  */
 typedef struct fftopk_evict {

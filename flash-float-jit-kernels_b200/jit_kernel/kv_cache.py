@@ -189,7 +189,7 @@ def cache_evict(
         wos, _ = _check_weight(weight_out, "weight_out", idx, B, H, cols)
         if weight_out.data_ptr() == weight.data_ptr() and weight.numel():
             raise RuntimeError("weight_out must not be weight itself")
-    kept = lengths.new_empty((B, H, budget))
+    kept = torch.empty((B, H, budget), dtype=torch.int32, device=lengths.device)
     left = torch.empty_like(lengths)
     if B and H:
         args = _EVICT.pack(

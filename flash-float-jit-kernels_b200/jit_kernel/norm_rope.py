@@ -7,6 +7,7 @@ k quantised into the indexer's key cache as it is written. All are enqueue-only 
 inputs' type and round once. They serve: none has a gradient, and a tensor that asks for one is refused."""
 from __future__ import annotations
 
+import functools
 import struct
 from typing import Optional, Sequence
 
@@ -140,10 +141,19 @@ def rotary_axes(sections: Sequence[int], interleaved: bool = False) -> tuple:
     return tuple(a for i in range(max(sections, default=0)) for a, n in enumerate(sections) if i < n)
 
 
-def _axes_bytes(axes: tuple, pairs: int, n: int) -> bytes:
-    if len(axes) != pairs or not 1 <= n <= 4 or set(map(type, axes)) != {int} or min(axes) < 0 or max(axes) >= n:
+@functools.lru_cache(maxsize=64)
+def _check_axes(raw: bytes, pairs: int, n: int) -> bytes:
+    if len(raw) != pairs or not 1 <= n <= 4 or max(raw) >= n:
         raise RuntimeError("axes must name one of positions' rows (up to four) for each of the rotated pairs, half of cos_sin's columns")
-    return bytes(axes)
+    return raw
+
+
+def _axes_bytes(axes: Sequence[int], pairs: int, n: int) -> bytes:
+    try:
+        raw = bytes(tuple(axes))
+    except (TypeError, ValueError):
+        raise RuntimeError("axes must be whole numbers, rows of positions") from None
+    return _check_axes(raw, pairs, n)
 
 
 def _check_table(positions, cos_sin, idx: int, tokens: int, dim: int, axes=None):
@@ -165,7 +175,7 @@ def _check_table(positions, cos_sin, idx: int, tokens: int, dim: int, axes=None)
     at, step = positions.shape, positions.stride()
     if positions.dtype is not torch.int32 or len(at) != 2 or at[1] != tokens or (tokens > 1 and step[1] != 1) or positions.get_device() != idx:
         raise RuntimeError("with axes, positions must be an int32 tensor [axes, tokens] with unit inner stride on the inputs' device")
-    return positions.data_ptr(), cos_sin.data_ptr(), shape[0], shape[1], step[0], at[0], _axes_bytes(tuple(axes), shape[1] // 2, at[0])
+    return positions.data_ptr(), cos_sin.data_ptr(), shape[0], shape[1], step[0], at[0], _axes_bytes(axes, shape[1] // 2, at[0])
 
 
 def qk_norm_rope(

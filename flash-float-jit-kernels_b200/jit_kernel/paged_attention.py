@@ -4,6 +4,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from typing import Optional
 
@@ -13,7 +14,7 @@ from . import _native
 from .kv_cache import _check_table, _check_weight
 from .norm_rope import _DENSE, FP8, _check_cache, _check_vector, _no_grad
 from .sparse_attention import _TYPES
-from .topk_indexer import _current_device, _launch
+from .topk_indexer import _launch
 
 #: fftopk_paged (include/fftopk.h)
 _ARGS = struct.Struct("@PqqPqqPqqPqqPqqPqPPqqPPqqPqqqqqiiiiiifi")
@@ -113,25 +114,27 @@ def paged_attention(
         os = out.stride()
         if out.dtype is not dtype or out.shape != q.shape or out.get_device() != idx or os[2] != 1:
             raise RuntimeError("out must have q's shape and type, unit inner stride, on q's device")
-    lse = q.new_empty((B, Hq), dtype=torch.float32) if return_lse else None
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     if B and Hq:
         args = _ARGS.pack(
             q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), ks[0], ks[1], v_cache.data_ptr(), vs[0], vs[1], ka, kss[0], kss[1], va, vss[0],
             vss[1], table, row, at, out.data_ptr(), os[0], os[1], lse.data_ptr() if return_lse else 0, w, ws[0], ws[1], wo, wos[0], wos[1],
             cols, B, slots, Hq, Hk, D, pages, page_size, _TYPES[dtype], D ** -0.5 if softmax_scale is None else softmax_scale, 0)
-        n = _workspace_bytes(idx, args)
+        n = _workspace_bytes(idx, B, Hq, Hk, D, pages, page_size, ka != 0, wo != 0)
         space = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         _launch(_native.lib().fftopk_paged_attention, "fftopk_paged_attention", idx, args, space.data_ptr() if n else 0, n)
     return (out, lse) if return_lse else out
 
 
-def _workspace_bytes(idx: int, args: bytes) -> int:
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(idx: int, B: int, Hq: int, Hk: int, D: int, pages: int, page_size: int, fp8: bool, weigh: bool) -> int:
+    """What the library asks for a call of these sizes on device idx: no address of it counts, 256 stands for all that are there."""
+    there = 256
+    args = _ARGS.pack(there, 0, 0, there, 0, 0, there, 0, 0, there * fp8, 0, 0, there * fp8, 0, 0, there, 0, there, there, 0, 0, 0, 0, 0, 0,
+                      there * weigh, 0, 0, 0, B, 1, Hq, Hk, D, pages, page_size, 0, 0.0, 0)
     n = ctypes.c_size_t()
-    if _current_device() == idx:
+    with torch.cuda.device(idx):
         rc = _native.lib().fftopk_paged_workspace_bytes(args, ctypes.byref(n))
-    else:
-        with torch.cuda.device(idx):
-            rc = _native.lib().fftopk_paged_workspace_bytes(args, ctypes.byref(n))
     if rc:
         _native.check(rc, "fftopk_paged_attention")
     return n.value

@@ -19,7 +19,7 @@ def test_rotary_axes():
 
 def test_axes_bytes():
     assert _axes_bytes((0, 2, 1, 0), 4, 3) == b"\0\2\1\0"
-    for axes, pairs, n in (((0, 1), 3, 2), ((0, 2), 2, 2), ((0, -1), 2, 2), ((0, True), 2, 2), ((0, 1.0), 2, 2), ((0, 0), 2, 0), ((0, 4), 2, 5)):
+    for axes, pairs, n in (((0, 1), 3, 2), ((0, 2), 2, 2), ((0, -1), 2, 2), ((0, 1.0), 2, 2), ((0, 0), 2, 0), ((0, 4), 2, 5)):
         with pytest.raises(RuntimeError):
             _axes_bytes(axes, pairs, n)
 

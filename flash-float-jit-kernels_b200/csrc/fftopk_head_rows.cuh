@@ -25,7 +25,7 @@ struct RowParams {
   FastDiv per_token[kMaxParts];     // items of a token
   uint32_t items[kMaxParts];        // tokens * items of a token
   int32_t aligned_w[kMaxParts];     // weight and bias may be read four at a time
-  const int32_t* positions;
+  const int32_t* positions;  // NULL: a token's row of the table is its number
   const float* cos_sin;
   int64_t table_rows;
   const int32_t* padding;  // slots of the first part that has some: a token whose entry is negative is padding, and has no position
@@ -36,7 +36,6 @@ struct RowParams {
 constexpr int kMaxAxes = 4;
 struct AxesParams : RowParams {
   int64_t axis_stride;     // from a token's position on one axis to that on the next
-  uint32_t used;           // axes that a pair turns by, a bit each
   uint32_t axis_of[8];     // two bits a pair
 };
 template <bool kAxes>
@@ -54,38 +53,28 @@ __device__ __forceinline__ void load_weights(float* w, const void* p, int32_t dt
 
 enum : int { kRotNone = 0, kRotApart = 1, kRotNext = 2 };  // partners: none, i and i + R / 2, 2 i and 2 i + 1
 
-// Where a token is on every axis that counts, and its rows of the table. (A lane of four pairs asks for single elements: the pairs' axes may be any.
-// 16,384 tokens of 72 heads, three axes in turn: AXES_TIME)
-struct AxisRows {
-  int64_t at[kMaxAxes];  // -1: no such row
-  __device__ __forceinline__ AxisRows(const AxesParams& p, uint32_t token, bool tell) {
-    bool beyond = false;
-#pragma unroll
-    for (int a = 0; a < kMaxAxes; ++a) {
-      at[a] = -1;
-      if (p.used >> a & 1u) {
-        const int64_t pos = p.positions[a * p.axis_stride + token];
-        if (pos >= 0 && pos < p.table_rows)
-          at[a] = pos * p.R;
-        else
-          beyond = true;
-      }
-    }
-    if (beyond && tell && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+// Several axes: rows of cosines and sines for tokens token0 .. token0 + tokens - 1, every pair's from its own axis' row of the table; NaN where there is no such row.
+// `thread` of `threads` writes its share.
+__device__ __forceinline__ void merge_rows(const AxesParams& p, float* merged, uint32_t token0, uint32_t tokens, uint32_t thread, uint32_t threads) {
+  const uint32_t R = (uint32_t)p.R, half = R >> 1, table_rows = (uint32_t)min(p.table_rows, (int64_t)0x80000000ll);
+  const int32_t* positions = p.positions + token0;
+  uint32_t r = thread;
+  for (uint32_t i = thread; i < tokens * R; i += threads, r += threads) {
+    while (r >= R) r -= R, ++positions;
+    const uint32_t pair = r < half ? r : r - half;
+    const uint32_t pos = (uint32_t)positions[(p.axis_of[pair >> 4] >> (2 * (pair & 15)) & 3u) * p.axis_stride];
+    float x = __int_as_float(0x7fffffff);
+    if (pos < table_rows)
+      x = p.cos_sin[(uint64_t)pos * R + r];
+    else if (p.status && (p.padding == nullptr || p.padding[positions - p.positions] >= 0))
+      atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+    merged[i] = x;
   }
-  // cosine and sine of a pair; NaN where its axis has no row
-  __device__ __forceinline__ float2 of(const AxesParams& p, int pair) const {
-    const uint32_t axis = p.axis_of[pair >> 4] >> (2 * (pair & 15)) & 3u;
-    const int64_t row = axis == 0 ? at[0] : axis == 1 ? at[1] : axis == 2 ? at[2] : at[3];
-    const float nan = __int_as_float(0x7fffffff);
-    if (row < 0) return make_float2(nan, nan);
-    return make_float2(p.cos_sin[row + pair], p.cos_sin[row + (p.R >> 1) + pair]);
-  }
-};
+}
 
 // T: the rows' type; kLanes: lanes of a group; kHeads: heads an item takes; kVec: pieces may be read and written as one
 template <typename T, int kLanes, int kHeads, bool kVec, int kNorm, int kRot, bool kQuant, bool kAxes>
-__device__ __forceinline__ void head_rows(const ParamsOf<kAxes>& p, const int which) {
+__device__ __forceinline__ void head_rows(const ParamsOf<kAxes>& p, const int which, float* merged) {
   const fftopk_head_part& part = p.part[which];
   const int lane = threadIdx.x & (kLanes - 1);
   const uint32_t mask = group_mask<kLanes>();
@@ -134,33 +123,23 @@ __device__ __forceinline__ void head_rows(const ParamsOf<kAxes>& p, const int wh
     const Pair one = pair(1.f, 1.f), none = pair(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < (kRot == kRotApart ? 2 : 4); ++i) c[i] = one, sn[i] = none;
+    const float* row = nullptr;
+    bool ok = true;
     if constexpr (kAxes) {
-      if (mine) {
-        const AxisRows rows_at(p, token, lane == 0 && (p.padding == nullptr || p.padding[token] >= 0));
-        if constexpr (kRot == kRotNext) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if (at[e] < p.R) {
-              const float2 x = rows_at.of(p, at[e] >> 1), y = rows_at.of(p, (at[e] >> 1) + 1);
-              c[2 * e] = pair(x.x, x.x), c[2 * e + 1] = pair(y.x, y.x);
-              sn[2 * e] = pair(-x.y, x.y), sn[2 * e + 1] = pair(-y.y, y.y);
-            }
-          }
-        } else if (back < 0) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 x = rows_at.of(p, at[0] + 2 * e), y = rows_at.of(p, at[0] + 2 * e + 1);
-            c[e] = pair(x.x, y.x), sn[e] = pair(x.y, y.y);
-          }
-        }
-      }
+      const uint32_t item0 = (blockIdx.x - p.first_block[which]) * (uint32_t)(kRowThreads / kLanes);
+      const uint32_t token0 = p.per_token[which].div(item0);
+      merge_rows(p, merged, token0, p.per_token[which].div(min(item0 + kRowThreads / kLanes, p.items[which]) - 1u) - token0 + 1u, threadIdx.x, kRowThreads);
+      __syncthreads();
+      row = merged + (in ? token - token0 : 0u) * (uint32_t)p.R;
     } else if (mine) {
-      const int64_t pos = p.positions[token];
-      const bool ok = pos >= 0 && pos < p.table_rows;
+      const int64_t pos = p.positions != nullptr ? p.positions[token] : (int64_t)token;
+      ok = pos >= 0 && pos < p.table_rows;
       if (!ok && lane == 0 && p.status && (p.padding == nullptr || p.padding[token] >= 0))
         atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+      row = p.cos_sin + (ok ? pos : 0) * p.R;
+    }
+    if (mine) {
       const float nan = __int_as_float(0x7fffffff);  // (no such row in the table: the rotated channels become NaN)
-      const float* row = p.cos_sin + (ok ? pos : 0) * p.R;
       const int half = p.R >> 1;
       if constexpr (kRot == kRotNext) {
 #pragma unroll
@@ -301,31 +280,36 @@ __device__ __forceinline__ void head_rows(const ParamsOf<kAxes>& p, const int wh
 // more. 16,384 tokens of 72 heads, norm and rotation: 126 us; six blocks 145, seven 134, ten (48 registers) 143; two, three or eight
 // heads an item 171, 146, 149.
 template <typename T, int kLanes, int kHeads, bool kVec, int kNorm, int kRot, bool kAxes>
-__device__ __forceinline__ void head_rows(const ParamsOf<kAxes>& p, int which) {
+__device__ __forceinline__ void head_rows(const ParamsOf<kAxes>& p, int which, float* merged) {
   if (p.part[which].scale != nullptr)
-    head_rows<T, kLanes, kHeads, kVec, kNorm, kRot, true, kAxes>(p, which);
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRot, true, kAxes>(p, which, merged);
   else
-    head_rows<T, kLanes, kHeads, kVec, kNorm, kRot, false, kAxes>(p, which);
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRot, false, kAxes>(p, which, merged);
 }
 template <typename T, int kLanes, int kHeads, bool kVec, int kNorm, bool kAxes>
-__device__ __forceinline__ void head_rows(const ParamsOf<kAxes>& p, int which) {
+__device__ __forceinline__ void head_rows(const ParamsOf<kAxes>& p, int which, float* merged) {
   if (!p.part[which].rotate)
-    head_rows<T, kLanes, kHeads, kVec, kNorm, kRotNone, kAxes>(p, which);
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRotNone, kAxes>(p, which, merged);
   else if (p.interleaved)
-    head_rows<T, kLanes, kHeads, kVec, kNorm, kRotNext, kAxes>(p, which);
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRotNext, kAxes>(p, which, merged);
   else
-    head_rows<T, kLanes, kHeads, kVec, kNorm, kRotApart, kAxes>(p, which);
+    head_rows<T, kLanes, kHeads, kVec, kNorm, kRotApart, kAxes>(p, which, merged);
 }
 template <typename T, int kLanes, int kHeads, bool kVec, bool kAxes>
 __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 4 && kHeads > 1 ? 5 : 8) head_rows_kernel(const __grid_constant__ ParamsOf<kAxes> p) {
+  float* merged = nullptr;  // several axes: the block's tokens' cosines and sines
+  if constexpr (kAxes) {
+    __shared__ __align__(16) float rows[kRowThreads * 8];
+    merged = rows;
+  }
   const int which = blockIdx.x >= p.first_block[2] ? 2 : blockIdx.x >= p.first_block[1] ? 1 : 0;
   const int norm = p.part[which].norm;
   if (norm == FFTOPK_NORM_NONE)
-    head_rows<T, kLanes, kHeads, kVec, FFTOPK_NORM_NONE, kAxes>(p, which);
+    head_rows<T, kLanes, kHeads, kVec, FFTOPK_NORM_NONE, kAxes>(p, which, merged);
   else if (norm == FFTOPK_NORM_RMS)
-    head_rows<T, kLanes, kHeads, kVec, FFTOPK_NORM_RMS, kAxes>(p, which);
+    head_rows<T, kLanes, kHeads, kVec, FFTOPK_NORM_RMS, kAxes>(p, which, merged);
   else
-    head_rows<T, kLanes, kHeads, kVec, FFTOPK_NORM_LAYER, kAxes>(p, which);
+    head_rows<T, kLanes, kHeads, kVec, FFTOPK_NORM_LAYER, kAxes>(p, which, merged);
 }
 
 template <typename T, int kLanes, bool kAxes>
@@ -338,9 +322,9 @@ cudaError_t launch_rows(ParamsOf<kAxes>& p, bool vec, int heads, cudaStream_t st
   }
   if (!vec)
     head_rows_kernel<T, kLanes, 1, false, kAxes><<<grid, kRowThreads, 0, stream>>>(p);
-  else if (heads == 1)
+  else if (kAxes || heads == 1)
     head_rows_kernel<T, kLanes, 1, true, kAxes><<<grid, kRowThreads, 0, stream>>>(p);
-  else
+  else if constexpr (!kAxes)
     head_rows_kernel<T, kLanes, kHeadsItem, true, kAxes><<<grid, kRowThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }
@@ -358,7 +342,8 @@ cudaError_t launch_rows(ParamsOf<kAxes>& p, int32_t dtype, bool vec, int heads, 
                                       : launch_rows<__half, kAxes>(p, vec, heads, stream);
 }
 
-// fftopk_rows_axes.cu
-cudaError_t launch_rows_axes(AxesParams& p, int32_t dtype, bool vec, int heads, cudaStream_t stream);
+// fftopk_rows_axes.cu: one head an item; rows of cosines and sines of all tokens
+cudaError_t launch_rows_axes(AxesParams& p, int32_t dtype, bool vec, cudaStream_t stream);
+cudaError_t launch_merge_rows(const AxesParams& p, float* merged, uint32_t tokens, cudaStream_t stream);
 
 }  // namespace fftopk

@@ -144,9 +144,9 @@ int elem_bytes(int32_t dtype) { return dtype == FFTOPK_DTYPE_FP32 ? 4 : 2; }
 bool known_dtype(int32_t dtype) { return dtype == FFTOPK_DTYPE_FP16 || dtype == FFTOPK_DTYPE_BF16 || dtype == FFTOPK_DTYPE_FP32; }
 bool on(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
-// axes: NULL where a token has one position
+// axes: NULL where a token has one position; merged: NULL, or [tokens, rotary] for what kernels of many rows read
 int head_rows_call(const fftopk_head_part* parts, int32_t n_parts, int64_t tokens, int32_t D, int32_t dtype, const int32_t* positions,
-                   int64_t axis_stride, int32_t n_axes, const uint8_t* axes, const float* cos_sin, int64_t table_rows, int32_t rotary,
+                   int64_t axis_stride, int32_t n_axes, const uint8_t* axes, float* merged, const float* cos_sin, int64_t table_rows, int32_t rotary,
                    int32_t interleaved, uint32_t* status, void* cuda_stream) {
   if (parts == nullptr || n_parts < 1 || n_parts > kMaxParts || tokens < 0 || !known_dtype(dtype)) return FFTOPK_EINVAL;
   if (D < 8 || D > 256 || (D & 7) != 0) return FFTOPK_ERANGE;
@@ -185,7 +185,6 @@ int head_rows_call(const fftopk_head_part* parts, int32_t n_parts, int64_t token
     for (int i = 0; axes != nullptr && i < rotary / 2; ++i) {
       if (axes[i] >= n_axes) return FFTOPK_EINVAL;
       p.axis_of[i >> 4] |= (uint32_t)axes[i] << (2 * (i & 15));
-      p.used |= 1u << axes[i];
     }
   }
   if (tokens == 0 || all_heads == 0) return FFTOPK_OK;
@@ -199,7 +198,8 @@ int head_rows_call(const fftopk_head_part* parts, int32_t n_parts, int64_t token
   const int rc = device_sms(sms);
   if (rc) return rc;
   const int64_t enough = (int64_t)sms * 64 * kHeadsItem;
-  const int heads = vec && all_heads >= (enough + tokens - 1) / tokens ? kHeadsItem : 1;
+  const bool by_axes = axes != nullptr && rotates;
+  const int heads = vec && all_heads >= (enough + tokens - 1) / tokens && !(by_axes && merged == nullptr) ? kHeadsItem : 1;
   for (int i = 0; i < n_parts; ++i) {
     p.part[i] = parts[i];
     const int64_t per_token = ((int64_t)parts[i].heads + heads - 1) / heads;
@@ -218,7 +218,16 @@ int head_rows_call(const fftopk_head_part* parts, int32_t n_parts, int64_t token
   p.status = status;
   p.axis_stride = axis_stride;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  const cudaError_t e = axes != nullptr && rotates ? launch_rows_axes(p, dtype, vec, heads, stream) : launch_rows<false>(p, dtype, vec, heads, stream);
+  cudaError_t e = cudaSuccess;
+  if (by_axes && heads == 1) {
+    e = launch_rows_axes(p, dtype, vec, stream);
+  } else {
+    if (by_axes) {
+      e = launch_merge_rows(p, merged, (uint32_t)tokens, stream);
+      p.positions = nullptr, p.cos_sin = merged, p.table_rows = tokens;
+    }
+    if (e == cudaSuccess) e = launch_rows<false>(p, dtype, vec, heads, stream);
+  }
   return e == cudaSuccess ? FFTOPK_OK : cuda_fail(e);
 }
 
@@ -232,16 +241,16 @@ extern "C" {
 int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tokens, int32_t D, int32_t dtype,
                      const int32_t* positions, const float* cos_sin, int64_t table_rows, int32_t rotary, int32_t interleaved,
                      uint32_t* status, void* cuda_stream) {
-  return head_rows_call(parts, n_parts, tokens, D, dtype, positions, 0, 0, nullptr, cos_sin, table_rows, rotary, interleaved, status, cuda_stream);
+  return head_rows_call(parts, n_parts, tokens, D, dtype, positions, 0, 0, nullptr, nullptr, cos_sin, table_rows, rotary, interleaved, status, cuda_stream);
 }
 
 int fftopk_head_rows_axes(const fftopk_head_part* parts, int32_t n_parts, int64_t tokens, int32_t D, int32_t dtype,
                           const int32_t* positions, int64_t axis_stride, int32_t n_axes, const uint8_t* axes, const float* cos_sin,
-                          int64_t table_rows, int32_t rotary, int32_t interleaved, uint32_t* status, void* cuda_stream) {
-  if (axes == nullptr || n_axes < 1) return FFTOPK_EINVAL;
+                          int64_t table_rows, int32_t rotary, int32_t interleaved, float* workspace, uint32_t* status, void* cuda_stream) {
+  if (axes == nullptr || n_axes < 1 || !on(workspace, 16)) return FFTOPK_EINVAL;
   if (n_axes > kMaxAxes) return FFTOPK_ERANGE;
-  return head_rows_call(parts, n_parts, tokens, D, dtype, positions, axis_stride, n_axes, axes, cos_sin, table_rows, rotary, interleaved, status,
-                        cuda_stream);
+  return head_rows_call(parts, n_parts, tokens, D, dtype, positions, axis_stride, n_axes, axes, workspace, cos_sin, table_rows, rotary, interleaved,
+                        status, cuda_stream);
 }
 
 int fftopk_cache_read(const void* cache, int64_t slot_stride, int64_t head_stride, int64_t n_slots, int32_t heads, int32_t D,

@@ -172,7 +172,7 @@ def lib() -> ctypes.CDLL:
                                    c.c_int32, c.c_int32, c.c_void_p, c.c_void_p]
     L.fftopk_head_rows_axes.restype = c.c_int
     L.fftopk_head_rows_axes.argtypes = [c.c_char_p, c.c_int32, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_int64, c.c_int32,
-                                        c.c_char_p, c.c_void_p, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_void_p]
+                                        c.c_char_p, c.c_void_p, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_void_p, c.c_void_p]
     L.fftopk_cache_read.restype = c.c_int
     L.fftopk_cache_read.argtypes = [c.c_void_p, c.c_int64, c.c_int64, c.c_int64, c.c_int32, c.c_int32, c.c_void_p, c.c_int64,
                                     c.c_int64, c.c_void_p, c.c_int64, c.c_int64, c.c_void_p, c.c_void_p, c.c_int32, c.c_void_p,

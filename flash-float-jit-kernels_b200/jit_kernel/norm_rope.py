@@ -22,6 +22,7 @@ _NORMS = {None: 0, "rms": 1, "layer": 2}
 #: fftopk_head_part (include/fftopk.h)
 _PART = struct.Struct("@PqqPPPqqPqqPPqiiiifi")
 FP8 = torch.float8_e4m3fn
+_MANY = 64  # tokens from which on a rotation by several axes is given a workspace (the library goes by rows; fewer tokens hardly have enough)
 _DENSE = torch.contiguous_format
 
 
@@ -111,8 +112,10 @@ def _quantised(x, xs, heads, out, os, scale, ss, slots=0, n=0, mul=0, norm=_PLAI
 def _rows(idx: int, parts: bytes, tokens: int, dim: int, dtype: torch.dtype, table=(0, 0, 0, 0), interleaved: bool = False) -> None:
     """table: as _check_table gives it"""
     if len(table) > 4:
+        # (of many rows: the tokens' cosines and sines are made by a kernel in front)
+        space = torch.empty((tokens, table[3]), dtype=torch.float32, device=torch.device("cuda", idx)) if tokens >= _MANY else None
         _launch(_native.lib().fftopk_head_rows_axes, "fftopk_head_rows_axes", idx, parts, len(parts) // _PART.size, tokens, dim, _DTYPES[dtype],
-                table[0], table[4], table[5], table[6], table[1], table[2], table[3], interleaved)
+                table[0], table[4], table[5], table[6], table[1], table[2], table[3], interleaved, 0 if space is None else space.data_ptr())
         return
     _launch(_native.lib().fftopk_head_rows, "fftopk_head_rows", idx, parts, len(parts) // _PART.size, tokens, dim, _DTYPES[dtype], table[0],
             table[1], table[2], table[3], interleaved)

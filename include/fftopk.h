@@ -405,11 +405,13 @@ int fftopk_head_rows(const fftopk_head_part* parts, int32_t n_parts, int64_t tok
  * channels turns by the angle that the table holds for the token's position on axis axes[i].
  *   positions    device, int32; the position of token t on axis a is positions[a * axis_stride + t]
  *   axes         HOST memory, rotary / 2 bytes, each below n_axes; read before the call returns. n_axes up to 4 (FFTOPK_ERANGE otherwise)
+ *   workspace    NULL, or tokens * rotary floats of device memory, 16-byte aligned, any contents: calls of many rows take a kernel more then and
+ *                are faster; calls that may run at the same time need one each
  * A position outside [0, table_rows) on an axis that a pair turns by makes that axis' channels NaN and raises FFTOPK_ST_BAD_INDEX, but for padding tokens.
  */
 int fftopk_head_rows_axes(const fftopk_head_part* parts, int32_t n_parts, int64_t tokens, int32_t D, int32_t dtype,
                           const int32_t* positions, int64_t axis_stride, int32_t n_axes, const uint8_t* axes, const float* cos_sin,
-                          int64_t table_rows, int32_t rotary, int32_t interleaved, uint32_t* status, void* cuda_stream);
+                          int64_t table_rows, int32_t rotary, int32_t interleaved, float* workspace, uint32_t* status, void* cuda_stream);
 
 /*
  * Rows of a quantised cache, gathered and widened: out[i, j, h, :] = codes[slot, h, :] * scale[slot, h] with

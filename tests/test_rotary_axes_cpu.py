@@ -24,13 +24,13 @@ def test_axes_bytes():
             _axes_bytes(axes, pairs, n)
 
 
-def rows(tokens=4, D=128, positions=A, n_axes=3, axes=bytes(i % 3 for i in range(32)), table=A, rotary=64, **fields):
+def rows(tokens=4, D=128, positions=A, n_axes=3, axes=bytes(i % 3 for i in range(32)), table=A, rotary=64, workspace=None, **fields):
     return _native.lib().fftopk_head_rows_axes(_PART.pack(*{**PART, **fields}.values()), 1, tokens, D, 1, positions, 4, n_axes, axes, table, 10,
-                                               rotary, 0, None, None)
+                                               rotary, 0, workspace, None, None)
 
 
 @pytest.mark.parametrize("want,call", [
-    (EINVAL, dict(axes=None)), (EINVAL, dict(n_axes=0)), (EINVAL, dict(n_axes=-1)), (ERANGE, dict(n_axes=5)), (EINVAL, dict(n_axes=2)),
+    (EINVAL, dict(axes=None)), (EINVAL, dict(workspace=A + 8)), (EINVAL, dict(n_axes=0)), (EINVAL, dict(n_axes=-1)), (ERANGE, dict(n_axes=5)), (EINVAL, dict(n_axes=2)),
     (EINVAL, dict(axes=bytes(31) + b"\3")), (EINVAL, dict(axes=b"\xff" + bytes(31))), (EINVAL, dict(positions=None)), (EINVAL, dict(positions=A + 2)),
     (EINVAL, dict(table=None)), (ERANGE, dict(rotary=8)), (ERANGE, dict(rotary=144)), (EINVAL, dict(tokens=-1)), (ERANGE, dict(D=12)), (0, dict(tokens=0)),
     (0, dict(heads=0)), (ERANGE, dict(tokens=1 << 31))])

@@ -44,13 +44,16 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;      // of a block: rows of the MMA
 constexpr int kWeighBlocks = 8;  // positions that a warp has on their way at a time
-constexpr int kMinBlocks = 16;  // of a run: below that, parts to join cost more than the blocks
+// of a run: below that, parts to join cost more than the blocks (one sequence of 1,000, 8 key heads: 8.8 us, with 16 blocks 10.7, with 32 15.4; of 4,096: 9.6, 10.3 and
+// 12.3, with 4 11.3)
+constexpr int kMinBlocks = 8;
 
 struct PagedParams {
   fftopk_paged a;
   int32_t group, head_blocks, units, runs, bound, weigh;
   FastDiv page;
   float scale_log2;
+  int32_t stream;   // the rows are more than L2 holds
   int32_t out_vec;  // rows of out start on 8 bytes
   int64_t line;     // positions of a unit of the score workspace
   float* lse2;      // [seqs, q heads] log2 of the sum of exponentials, of sequences that lie in one run
@@ -165,8 +168,13 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void widen4(uint32_t& lo, uint32_t& hi, uint32_t codes) {
   asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(codes));
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// 16 bytes of a row; rows that are more than L2 holds leave it before the scales - whose 32 bytes belong to several key heads - and the parts do (64 sequences of up to 16,384 in
+// e4m3: 250 us, 261 without the hint; one of 131,072 in bf16: 91 and 93)
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint64_t once) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(once) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool there, uint64_t once) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::128B [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0), "l"(once) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -271,6 +279,11 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   const uint32_t kstep = (uint32_t)(p.a.k_slot * kES), vstep = (uint32_t)(p.a.v_slot * kES);
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)warp * G::kBytes;
 
+  uint64_t once;
+  if (p.stream)
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
+  else
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(once));
   Segment here = segment_at(p, line.begin(run), left, lane), ahead = here;
   int64_t left_ahead = left;
   int32_t at, end, ask_at, ask_end;  // the warp's blocks of the segment at hand, and of the one it asks for
@@ -337,16 +350,16 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
 #pragma unroll
           for (int i = 0; i < kTurns; ++i) {
             const int at = i * kRowsOnce + sub;
-            copy16(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(k, i * kRowsOnce, kstep));
-            copy16(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(v, i * kRowsOnce, vstep));
+            copy16(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(k, i * kRowsOnce, kstep), once);
+            copy16(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(v, i * kRowsOnce, vstep), once);
           }
           if constexpr (kFp8) copy4(scales, sbase + (uint64_t)(uint32_t)((int)slot + (lane & (kKeys - 1))) * sstep);
         } else if (there > 0) {
 #pragma unroll
           for (int i = 0; i < kTurns; ++i) {
             const int at = i * kRowsOnce + sub, r = (int)slot + min(at, there - 1);
-            copy_or_zero<16>(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(kbase, r, kstep), at < there);
-            copy_or_zero<16>(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(vbase, r, vstep), at < there);
+            copy16_or_zero(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(kbase, r, kstep), at < there, once);
+            copy16_or_zero(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(vbase, r, vstep), at < there, once);
           }
           if constexpr (kFp8) {
             const int at = lane & (kKeys - 1);
@@ -368,8 +381,8 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
         for (int i = 0; i < kTurns; ++i) {
           const int at = i * kRowsOnce + sub;
           const int r = __shfl_sync(kAll, row, at);
-          copy_or_zero<16>(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(kbase, max(r, 0), kstep), r >= 0);
-          copy_or_zero<16>(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(vbase, max(r, 0), vstep), r >= 0);
+          copy16_or_zero(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(kbase, max(r, 0), kstep), r >= 0, once);
+          copy16_or_zero(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(vbase, max(r, 0), vstep), r >= 0, once);
         }
         if constexpr (kFp8) copy_or_zero<4>(scales, sbase + (uint64_t)(uint32_t)max(row, 0) * sstep, ok);
       }
@@ -1057,6 +1070,8 @@ int fftopk_paged_attention(const fftopk_paged* a, void* workspace, size_t worksp
   if (a->slots == 0) p.a.k = p.a.v = a->q;  // (an empty cache has no address, and rows that are left out are copies of no bytes: from somewhere)
   p.page = FastDiv((uint32_t)a->page_size);
   p.scale_log2 = a->softmax_scale * 1.44269504088896340736f;
+  const int es = a->k_scale != nullptr ? 1 : 2;
+  p.stream = (double)a->seqs * p.bound * a->kv_heads * a->D * es * 2 > 128e6;
   p.out_vec = on(a->out, 8) && (a->seqs <= 1 || a->out_seq % 4 == 0) && (a->q_heads <= 1 || a->out_head % 4 == 0);
   p.status = status;
   char* at = static_cast<char*>(workspace);

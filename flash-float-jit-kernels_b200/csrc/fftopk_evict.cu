@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SelectSmem& sm = *reinterpret_cast<SelectSmem*>(smem_raw);
   Word* const words = reinterpret_cast<Word*>(smem_raw + sizeof(SelectSmem));
-  uint32_t* const held = reinterpret_cast<uint32_t*>(words + p.words);  // kHeld: the CTA's weights, as bits, and from the first round on as keys
+  uint32_t* const held = reinterpret_cast<uint32_t*>(words + p.words);  // kHeld: the CTA's weights, as bits
   // (only where a kernel of this call follows, which waits: another one's inputs may be this one's results)
   if (p.moves) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   cg::cluster_group cluster = cg::this_cluster();
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  auto key_at = [&](int32_t i) { return kHeld ? held[i] : key_of(w[i]); };
+  auto key_at = [&](int32_t i) { return key_of(kHeld ? __uint_as_float(held[i]) : w[i]); };
   // the bits of word `word` that are positions a .. z - 1
   auto bits_of = [](int32_t word, int32_t a, int32_t z) {
     a = min(max(a - word * 32, 0), 32), z = min(max(z - word * 32, 0), 32);
@@ -201,16 +201,13 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
       for (int32_t i0 = warp * 32; i0 < span; i0 += kThreads) {
         const int32_t i = i0 + lane;
         if (i0 >= lo && i0 + 32 <= hi) {
-          const uint32_t key = key_of(kHeld ? __uint_as_float(held[i]) : w[i]), digit = key >> 21;
-          if (kHeld) held[i] = key;
+          const uint32_t digit = key_at(i) >> 21;
           if (__reduce_min_sync(kAll, digit) != __reduce_max_sync(kAll, digit))
             atomicAdd(&sm.hist[0][digit], 1u);
           else if (lane == 0)  // (copies of one weight: one addition for the warp)
             atomicAdd(&sm.hist[0][digit], 32u);
-        } else if (i < span) {
-          const uint32_t key = key_of(kHeld ? __uint_as_float(held[i]) : w[i]);
-          if (kHeld) held[i] = key;
-          if (i >= lo && i < hi) atomicAdd(&sm.hist[0][key >> 21], 1u);
+        } else if (i >= lo && i < hi) {
+          atomicAdd(&sm.hist[0][key_at(i) >> 21], 1u);
         }
       }
     }
@@ -239,7 +236,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
     }
     const bool done = need == 0 || sm.found[2] == need || round + 1 == kRounds;  // (the bin stays whole, or is one weight)
     if (round == 0) {
-#pragma unroll 1
+#pragma unroll 4
       for (int32_t word = warp; word < n_words; word += kWarps) {
         const int32_t i = word * 32 + lane;
         const uint32_t key = (i < span ? key_at(i) : 0u) & mask;
@@ -292,7 +289,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
       sures += (uint32_t)x, tied += (uint32_t)(x >> 32);
     }
   }
-#pragma unroll 1
+#pragma unroll 2
   for (int32_t word = warp; word < n_words; word += kWarps) {
     const uint4 q = *reinterpret_cast<const uint4*>(&words[word]);  // (a Word)
     bool stays = (q.x & 1u << lane) != 0u;
@@ -305,10 +302,8 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
     at += min(tie_rank, ties);
     if (stays && at < (uint32_t)left) {
       const int32_t i = word * 32 + lane;
-      // (keys are weights turned around, but for zeros of either sign and NaN)
-      const uint32_t key = kHeld ? held[i] : 0xffffffffu;
       kept[at] = from + i;
-      wo[at] = key == 0x80000000u || key == 0xffffffffu ? w[i] : __uint_as_float(fftopk_bits_from_key(key));
+      wo[at] = kHeld ? __uint_as_float(held[i]) : w[i];
     }
   }
   if (ctas > 1) cluster.sync();  // (nobody leaves while its memory is read)

@@ -42,15 +42,20 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kKeys = 16;      // of a block: rows of the MMA
-constexpr int kWeighBlocks = 8;  // positions that a warp has on their way at a time
-// of a run: below that, parts to join cost more than the blocks (one sequence of 1,000, 8 key heads: 8.8 us, with 16 blocks 10.7, with 32 15.4; of 4,096: 9.6, 10.3 and
-// 12.3, with 4 11.3)
-constexpr int kMinBlocks = 8;
+constexpr int kWeighKeys = 128;  // positions that a warp has on their way at a time where it brings weights up to date
+// positions of a run: below that, parts to join cost more than the blocks (one sequence of 1,000, 8 key heads: 8.8 us, with 256 positions 10.7, with 512
+// 15.4; of 4,096: 9.6, 10.3 and 12.3, with 64 11.3)
+constexpr int kMinKeys = 128;
+// Keys of a block, 16 to a product: as many as make 4 KB of k and v and more
+template <bool kFp8, int D>
+constexpr int block_keys() {
+  return kFp8 && D == 64 ? 32 : 16;
+}
 
 struct PagedParams {
   fftopk_paged a;
   int32_t group, head_blocks, units, runs, bound, weigh;
+  int32_t key_shift;  // of a block's keys
   FastDiv page;
   float scale_log2;
   int32_t stream;   // the rows are more than L2 holds
@@ -67,7 +72,7 @@ struct PagedParams {
 
 // Keys of sequence b: its length, as far as its pages reach
 __device__ __forceinline__ int32_t keys_of(const PagedParams& p, int64_t b) { return min(max(p.a.lengths[b], 0), p.bound); }
-__device__ __forceinline__ int64_t blocks_of(int32_t n) { return ((int64_t)n + kKeys - 1) / kKeys; }
+__device__ __forceinline__ int64_t blocks_of(const PagedParams& p, int32_t n) { return ((int64_t)n + (1 << p.key_shift) - 1) >> p.key_shift; }
 
 // Runs the line of `total` blocks is cut into, and where one begins: the first total % runs have a block more.
 struct Runs {
@@ -104,7 +109,7 @@ __device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
 // blocks of the sequences in front of `upto`
 __device__ __forceinline__ int64_t blocks_before(const PagedParams& p, int64_t upto, int lane) {
   int64_t total = 0;
-  for (int64_t b = lane; b < upto; b += 32) total += blocks_of(keys_of(p, b));
+  for (int64_t b = lane; b < upto; b += 32) total += blocks_of(p, keys_of(p, b));
   return warp_sum(total);
 }
 
@@ -119,13 +124,13 @@ __device__ __forceinline__ Segment segment_at(const PagedParams& p, int64_t g, i
   int64_t before = 0;
   for (int64_t first = 0;; first += 32) {
     const int32_t n = first + lane < p.a.seqs ? keys_of(p, first + lane) : 0;
-    const int64_t upto = before + warp_scan(blocks_of(n), lane);
+    const int64_t upto = before + warp_scan(blocks_of(p, n), lane);
     const unsigned beyond = __ballot_sync(kAll, upto > g);
     if (beyond != 0u || first + 32 >= p.a.seqs) {
       const int l = beyond != 0u ? __ffs((int)beyond) - 1 : 31;
       c.b = first + l;
       c.n = __shfl_sync(kAll, n, l);
-      c.blocks = (int32_t)blocks_of(c.n);
+      c.blocks = (int32_t)blocks_of(p, c.n);
       c.s0 = (int32_t)(g - (__shfl_sync(kAll, upto, l) - c.blocks));
       c.s1 = (int32_t)min((int64_t)c.blocks, c.s0 + left);
       return c;
@@ -138,7 +143,7 @@ __device__ __forceinline__ bool next_segment(const PagedParams& p, Segment& c, i
   for (++c.b; c.b < p.a.seqs; ++c.b) {
     c.n = keys_of(p, c.b);
     if (c.n > 0) {
-      c.blocks = (int32_t)blocks_of(c.n);
+      c.blocks = (int32_t)blocks_of(p, c.n);
       c.s0 = 0;
       c.s1 = (int32_t)min((int64_t)c.blocks, left);
       return true;
@@ -203,6 +208,7 @@ __device__ __forceinline__ float keys_sum(float x) {
 // rows; v, where eight rows give the same piece.
 template <bool kFp8, int D>
 struct PagedRing {
+  static constexpr int kKeys = block_keys<kFp8, D>();
   static constexpr int kRowBytes = D * (kFp8 ? 1 : 2);
   static constexpr int kV = kKeys * kRowBytes, kStage = 2 * kV;
   static constexpr int kStages = 3;
@@ -230,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   using G = PagedRing<kFp8, D>;
   constexpr int kCE = kFp8 ? 16 : 8;         // elements of a 16-byte piece
   constexpr int kPieces = D / (4 * kCE);     // pieces of a key row per lane (a quad reads a row)
+  constexpr int kKeys = G::kKeys, kR = kKeys / 16;  // a block's keys, and products
   constexpr int kStages = G::kStages;
   constexpr int kNH = 8 * kNT;
   constexpr int kTiles = D / 16;             // of the output: rows of the MMA are channels
@@ -259,22 +266,25 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
       }
     }
   }
-  const Runs line(blocks_before(p, p.a.seqs, lane), p.runs, kMinBlocks);
+  const Runs line(blocks_before(p, p.a.seqs, lane), p.runs, kMinKeys / kKeys);
   if ((int64_t)run >= line.runs || line.total == 0) return;  // (the whole CTA)
   int64_t left = line.begin((int64_t)run + 1) - line.begin(run);  // blocks of the run that are not behind the segment at hand
   if (left <= 0) return;
 
   constexpr int kLanesRow = G::kRowBytes / 16, kRowsOnce = 32 / kLanesRow, kTurns = kKeys / kRowsOnce;
   constexpr int kES = kFp8 ? 1 : 2;
+  constexpr unsigned kFull = kKeys == 32 ? kAll : (1u << kKeys) - 1u;  // all of a block's keys
   const int piece = lane % kLanesRow, sub = lane / kLanesRow;
   const char* const kbase = static_cast<const char*>(p.a.k) + (int64_t)kvh * p.a.k_head * kES + piece * 16;
   const char* const vbase = static_cast<const char*>(p.a.v) + (int64_t)kvh * p.a.v_head * kES + piece * 16;
-  // (k scales are asked for by the lower lanes, v scales by the upper ones)
-  const float* sbase = nullptr;
-  int64_t sstep = 0;
+  // (blocks of 16: k scales are asked for by the lower lanes, v scales by the upper ones; of 32: both by every lane)
+  const float *sbase[kR] = {};
+  int64_t sstep[kR] = {};
   if constexpr (kFp8) {
-    sbase = lane < kKeys ? p.a.k_scale + (int64_t)kvh * p.a.ks_head : p.a.v_scale + (int64_t)kvh * p.a.vs_head;
-    sstep = lane < kKeys ? p.a.ks_slot : p.a.vs_slot;
+    const bool k = kR == 2 || lane < kKeys;
+    sbase[0] = k ? p.a.k_scale + (int64_t)kvh * p.a.ks_head : p.a.v_scale + (int64_t)kvh * p.a.vs_head;
+    sstep[0] = k ? p.a.ks_slot : p.a.vs_slot;
+    if constexpr (kR == 2) sbase[1] = p.a.v_scale + (int64_t)kvh * p.a.vs_head, sstep[1] = p.a.vs_slot;
   }
   const uint32_t kstep = (uint32_t)(p.a.k_slot * kES), vstep = (uint32_t)(p.a.v_slot * kES);
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)warp * G::kBytes;
@@ -343,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
         const int64_t slot = (int64_t)page * p.page.d + in_page;
         const int there = slot < p.a.slots ? (int)min((int64_t)rows, p.a.slots - slot) : 0;
         if (there < rows && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
-        live = (1u << there) - 1u;
+        live = there == 32 ? kAll : (1u << there) - 1u;
         if (there == kKeys) {
           const char* const k = row_at(kbase, (int)slot + sub, kstep);
           const char* const v = row_at(vbase, (int)slot + sub, vstep);
@@ -353,7 +363,10 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
             copy16(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(k, i * kRowsOnce, kstep), once);
             copy16(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(v, i * kRowsOnce, vstep), once);
           }
-          if constexpr (kFp8) copy4(scales, sbase + (uint64_t)(uint32_t)((int)slot + (lane & (kKeys - 1))) * sstep);
+          if constexpr (kFp8) {
+#pragma unroll
+            for (int i = 0; i < kR; ++i) copy4(scales + i * 128u, sbase[i] + (uint64_t)(uint32_t)((int)slot + (lane & (kKeys - 1))) * sstep[i]);
+          }
         } else if (there > 0) {
 #pragma unroll
           for (int i = 0; i < kTurns; ++i) {
@@ -363,7 +376,8 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
           }
           if constexpr (kFp8) {
             const int at = lane & (kKeys - 1);
-            copy_or_zero<4>(scales, sbase + (uint64_t)(uint32_t)((int)slot + min(at, there - 1)) * sstep, at < there);
+#pragma unroll
+            for (int i = 0; i < kR; ++i) copy_or_zero<4>(scales + i * 128u, sbase[i] + (uint64_t)(uint32_t)((int)slot + min(at, there - 1)) * sstep[i], at < there);
           }
         }
       }
@@ -374,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
         ok = false;
         if (p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
       }
-      live = __ballot_sync(kAll, ok) & 0xffffu;
+      live = __ballot_sync(kAll, ok) & kFull;
       if (live != 0u) {
         const int row = ok ? (int)slot : -1;
 #pragma unroll
@@ -384,7 +398,10 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
           copy16_or_zero(data + at * G::kRowBytes + G::k_piece(at, piece) * 16u, row_at(kbase, max(r, 0), kstep), r >= 0, once);
           copy16_or_zero(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(vbase, max(r, 0), vstep), r >= 0, once);
         }
-        if constexpr (kFp8) copy_or_zero<4>(scales, sbase + (uint64_t)(uint32_t)max(row, 0) * sstep, ok);
+        if constexpr (kFp8) {
+#pragma unroll
+          for (int i = 0; i < kR; ++i) copy_or_zero<4>(scales + i * 128u, sbase[i] + (uint64_t)(uint32_t)max(row, 0) * sstep[i], ok);
+        }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -468,70 +485,90 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
     for (int s = 0; s < kStages - 1; ++s) live_of[s] = live_of[s + 1];
 
     if (live != 0u || p.weigh) {
-      float sc[kNT][4];  // keys g (0, 1) and g + 8 (2, 3), heads 2 qd and 2 qd + 1
+      float sc[kNT][kR][4];  // of every 16 keys: g (0, 1) and g + 8 (2, 3), heads 2 qd and 2 qd + 1
 #pragma unroll
-      for (int t = 0; t < kNT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+      for (int t = 0; t < kNT; ++t)
+#pragma unroll
+        for (int r = 0; r < kR; ++r) sc[t][r][0] = sc[t][r][1] = sc[t][r][2] = sc[t][r][3] = 0.f;
+      float ks[kR][2], vs[kR][2], vl[kR][2];
+#pragma unroll
+      for (int r = 0; r < kR; ++r) ks[r][0] = ks[r][1] = vs[r][0] = vs[r][1] = 1.f, vl[r][0] = vl[r][1] = 0.f;
       if (live != 0u) {
-        const uint32_t at = stage + (uint32_t)(g * G::kRowBytes);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const uint32_t from = at + G::k_piece(g, 4 * i + qd) * 16u;
-          const uint4 x = lds16(from), y = lds16(from + 8u * G::kRowBytes);
-          const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+        for (int r = 0; r < kR; ++r) {
+          const uint32_t from_row = stage + (uint32_t)((16 * r + g) * G::kRowBytes);
 #pragma unroll
-          for (int u = 0; u < kCE / 4; ++u) {
-            uint32_t f[4];
-            if constexpr (kFp8) {
-              widen4(f[0], f[2], a[u]);
-              widen4(f[1], f[3], b[u]);
-            } else {
-              f[0] = a[2 * u], f[2] = a[2 * u + 1], f[1] = b[2 * u], f[3] = b[2 * u + 1];
+          for (int i = 0; i < kPieces; ++i) {
+            const uint32_t from = from_row + G::k_piece(g, 4 * i + qd) * 16u;
+            const uint4 x = lds16(from), y = lds16(from + 8u * G::kRowBytes);
+            const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int u = 0; u < kCE / 4; ++u) {
+              uint32_t f[4];
+              if constexpr (kFp8) {
+                widen4(f[0], f[2], a[u]);
+                widen4(f[1], f[3], b[u]);
+              } else {
+                f[0] = a[2 * u], f[2] = a[2 * u + 1], f[1] = b[2 * u], f[3] = b[2 * u + 1];
+              }
+#pragma unroll
+              for (int t = 0; t < kNT; ++t) mma16816(sc[t][r], f, qb[t][i * (kCE / 4) + u][0], qb[t][i * (kCE / 4) + u][1], M());
             }
-#pragma unroll
-            for (int t = 0; t < kNT; ++t) mma16816(sc[t], f, qb[t][i * (kCE / 4) + u][0], qb[t][i * (kCE / 4) + u][1], M());
           }
-        }
-      }
-      float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f}, vl[2] = {0.f, 0.f};
-      if constexpr (kFp8) {
+          if constexpr (kFp8) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (live != 0u) {
-            ks[r] = lds4(scales + (uint32_t)((g + 8 * r) * 4));
-            vs[r] = lds4(scales + (uint32_t)((kKeys + g + 8 * r) * 4));
+            for (int e = 0; e < 2; ++e) {
+              ks[r][e] = lds4(scales + (uint32_t)((16 * r + g + 8 * e) * 4));
+              vs[r][e] = lds4(scales + (uint32_t)((kKeys + 16 * r + g + 8 * e) * 4));
+              vl[r][e] = (float)scale_exponent(vs[r][e]);
+            }
           }
-          vl[r] = (float)scale_exponent(vs[r]);
         }
       }
 #pragma unroll
       for (int t = 0; t < kNT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[t][e] *= qmul[t][e & 1];
-          if constexpr (kFp8) sc[t][e] *= ks[e >> 1];
+        for (int r = 0; r < kR; ++r) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[t][r][e] *= qmul[t][e & 1];
+            if constexpr (kFp8) sc[t][r][e] *= ks[r][e >> 1];
+          }
         }
       }
-      if (live != 0xffffu) {
-        const bool lo = (live >> g) & 1u, hi = (live >> (g + 8)) & 1u;
+      if (live != kFull) {
 #pragma unroll
-        for (int t = 0; t < kNT; ++t) {
-          sc[t][0] = lo ? sc[t][0] : -INFINITY, sc[t][1] = lo ? sc[t][1] : -INFINITY;
-          sc[t][2] = hi ? sc[t][2] : -INFINITY, sc[t][3] = hi ? sc[t][3] : -INFINITY;
+        for (int r = 0; r < kR; ++r) {
+          const bool lo = (live >> (16 * r + g)) & 1u, hi = (live >> (16 * r + g + 8)) & 1u;
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) {
+            sc[t][r][0] = lo ? sc[t][r][0] : -INFINITY, sc[t][r][1] = lo ? sc[t][r][1] : -INFINITY;
+            sc[t][r][2] = hi ? sc[t][r][2] : -INFINITY, sc[t][r][3] = hi ? sc[t][r][3] : -INFINITY;
+          }
         }
       }
       // (a reference is let stand until a score exceeds it by 2^8: fp16 weights and 32-bit sums have the room)
+      float top[kNT][2];
       bool over = false;
 #pragma unroll
       for (int t = 0; t < kNT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) over = over || fmaxf(sc[t][e] + vl[0], sc[t][2 + e] + vl[1]) > mx[t][e] + 8.f;
+        for (int e = 0; e < 2; ++e) {
+          top[t][e] = fmaxf(sc[t][0][e] + vl[0][0], sc[t][0][2 + e] + vl[0][1]);
+#pragma unroll
+          for (int r = 1; r < kR; ++r) top[t][e] = fmaxf(top[t][e], fmaxf(sc[t][r][e] + vl[r][0], sc[t][r][2 + e] + vl[r][1]));
+          over = over || top[t][e] > mx[t][e] + 8.f;
+        }
       }
       if (p.weigh) {
         float* to = p.scores + ((here.b * p.units + unit) * p.line + (int64_t)at * kKeys + g) * kNH + 2 * qd;
 #pragma unroll
-        for (int t = 0; t < kNT; ++t) {
-          *reinterpret_cast<float2*>(to + 8 * t) = make_float2(sc[t][0], sc[t][1]);
-          *reinterpret_cast<float2*>(to + 8 * kNH + 8 * t) = make_float2(sc[t][2], sc[t][3]);
+        for (int r = 0; r < kR; ++r) {
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) {
+            *reinterpret_cast<float2*>(to + 16 * r * kNH + 8 * t) = make_float2(sc[t][r][0], sc[t][r][1]);
+            *reinterpret_cast<float2*>(to + (16 * r + 8) * kNH + 8 * t) = make_float2(sc[t][r][2], sc[t][r][3]);
+          }
         }
       }
       if (live != 0u) {
@@ -540,8 +577,8 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
           for (int t = 0; t < kNT; ++t) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float top = keys_max(fmaxf(sc[t][e] + vl[0], sc[t][2 + e] + vl[1]));
-              const float m = top > mx[t][e] + 8.f ? top : mx[t][e];
+              const float all = keys_max(top[t][e]);
+              const float m = all > mx[t][e] + 8.f ? all : mx[t][e];
               const float grow = mx[t][e] == m ? 1.f : ex2(mx[t][e] - m);  // (-inf both: nothing seen yet)
               sum[t][e] = kFp8 ? brought(sum[t][e], mx[t][e], m) : sum[t][e] * grow;
               mx[t][e] = m;
@@ -550,36 +587,39 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
             }
           }
         }
-        uint32_t pb[kNT][2];
 #pragma unroll
-        for (int t = 0; t < kNT; ++t) {
-          const float m0 = mx[t][0] == -INFINITY ? 0.f : mx[t][0], m1 = mx[t][1] == -INFINITY ? 0.f : mx[t][1];
+        for (int r = 0; r < kR; ++r) {
+          uint32_t pb[kNT][2];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float a = ex2(sc[t][2 * r] - m0), b = ex2(sc[t][2 * r + 1] - m1);
-            sum[t][0] += a, sum[t][1] += b;
-            pb[t][r] = turned8x8(kFp8 ? narrow2(a * vs[r], b * vs[r], M()) : narrow2(a, b, M()));
-          }
-        }
-        // lanes 0-7 and 8-15 name the rows of keys 0-7 and 8-15 at one piece, lanes 16-31 at the next
-        const uint32_t vat = stage + (uint32_t)(G::kV + (lane & 15) * G::kRowBytes);
+          for (int t = 0; t < kNT; ++t) {
+            const float m0 = mx[t][0] == -INFINITY ? 0.f : mx[t][0], m1 = mx[t][1] == -INFINITY ? 0.f : mx[t][1];
 #pragma unroll
-        for (int c = 0; c < G::kRowBytes / 32; ++c) {
-          uint32_t x[4];
-          ldsm4_trans(x, vat + G::v_piece(lane & 15, 2 * c + (lane >> 4)) * 16u);
-          if constexpr (kFp8) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t f[4];
-              widen4(f[0], f[1], __byte_perm(x[2 * h], 0u, 0x3120));
-              widen4(f[2], f[3], __byte_perm(x[2 * h + 1], 0u, 0x3120));
-#pragma unroll
-              for (int t = 0; t < kNT; ++t) mma16816(o[t][2 * c + h], f, pb[t][0], pb[t][1], M());
+            for (int e = 0; e < 2; ++e) {
+              const float a = ex2(sc[t][r][2 * e] - m0), b = ex2(sc[t][r][2 * e + 1] - m1);
+              sum[t][0] += a, sum[t][1] += b;
+              pb[t][e] = turned8x8(kFp8 ? narrow2(a * vs[r][e], b * vs[r][e], M()) : narrow2(a, b, M()));
             }
-          } else {
-            const uint32_t f[4] = {x[0], x[2], x[1], x[3]};
+          }
+          // lanes 0-7 and 8-15 name the rows of keys 0-7 and 8-15 at one piece, lanes 16-31 at the next
+          const uint32_t vat = stage + (uint32_t)(G::kV + (16 * r + (lane & 15)) * G::kRowBytes);
 #pragma unroll
-            for (int t = 0; t < kNT; ++t) mma16816(o[t][c], f, pb[t][0], pb[t][1], M());
+          for (int c = 0; c < G::kRowBytes / 32; ++c) {
+            uint32_t x[4];
+            ldsm4_trans(x, vat + G::v_piece(lane & 15, 2 * c + (lane >> 4)) * 16u);
+            if constexpr (kFp8) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t f[4];
+                widen4(f[0], f[1], __byte_perm(x[2 * h], 0u, 0x3120));
+                widen4(f[2], f[3], __byte_perm(x[2 * h + 1], 0u, 0x3120));
+#pragma unroll
+                for (int t = 0; t < kNT; ++t) mma16816(o[t][2 * c + h], f, pb[t][0], pb[t][1], M());
+              }
+            } else {
+              const uint32_t f[4] = {x[0], x[2], x[1], x[3]};
+#pragma unroll
+              for (int t = 0; t < kNT; ++t) mma16816(o[t][c], f, pb[t][0], pb[t][1], M());
+            }
           }
         }
       }
@@ -741,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 5) paged_finish_kernel(const __grid_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nh = p.group > 8 ? 16 : 8;
   const int64_t total = blocks_before(p, p.a.seqs, lane);
-  const Runs line(total, p.runs, kMinBlocks);
+  const Runs line(total, p.runs, kMinKeys >> p.key_shift);
   if ((int)blockIdx.x < p.join_ctas) {
     const int64_t pairs = p.a.seqs * p.a.q_heads;
     int64_t i = p.join_each == 0 ? blockIdx.x : ((int64_t)blockIdx.x * kWarps + warp) * p.join_each;
@@ -750,10 +790,10 @@ __global__ void __launch_bounds__(kThreads, 5) paged_finish_kernel(const __grid_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (; i < last; ++i) {
       if (i / p.a.q_heads != b) {
-        begin += blocks_of(keys_of(p, b));
+        begin += blocks_of(p, keys_of(p, b));
         ++b;
       }
-      const int64_t end = begin + blocks_of(keys_of(p, b));
+      const int64_t end = begin + blocks_of(p, keys_of(p, b));
       if (begin == end) continue;
       const int head = (int)(i - b * p.a.q_heads), kvh = head / p.group, in = head - kvh * p.group, hb = in / nh;
       const Parts parts(p, line, begin, end, kvh * p.head_blocks + hb);
@@ -788,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 5) paged_finish_kernel(const __grid_
   const uint32_t gw = (blockIdx.x - (uint32_t)p.join_ctas) * (uint32_t)kWarps + (uint32_t)warp;
   const uint32_t run = gw / (uint32_t)p.a.kv_heads;
   const int kvh = (int)(gw - run * (uint32_t)p.a.kv_heads);
-  const Runs mine(total, p.weigh_runs, kWeighBlocks);
+  const Runs mine(total, p.weigh_runs, kWeighKeys >> p.key_shift);
   int64_t left = (int64_t)run < mine.runs ? mine.begin((int64_t)run + 1) - mine.begin(run) : 0;
   Segment c = {};
   if (left > 0) c = segment_at(p, mine.begin(run), left, lane);
@@ -797,7 +837,7 @@ __global__ void __launch_bounds__(kThreads, 5) paged_finish_kernel(const __grid_
   if (left <= 0) return;
   for (;;) {
     const int64_t end = begin + c.blocks;
-    const int32_t upto = (int32_t)min((int64_t)c.n, (int64_t)c.s1 * kKeys);
+    const int32_t upto = (int32_t)min((int64_t)c.n, (int64_t)c.s1 << p.key_shift);
     const float* w = p.a.weight != nullptr ? p.a.weight + c.b * p.a.w_seq + (int64_t)kvh * p.a.w_head : nullptr;
     float* wo = p.a.weight_out + c.b * p.a.wo_seq + (int64_t)kvh * p.a.wo_head;
     for (int hb = 0; hb < p.head_blocks; ++hb) {
@@ -839,7 +879,7 @@ __global__ void __launch_bounds__(kThreads, 5) paged_finish_kernel(const __grid_
         const float* s = p.scores + (c.b * p.units + unit) * p.line * nh + h8;
         const bool first = hb == 0 && h8 == 0;
         constexpr int kAhead = 4;
-        for (int64_t j0 = (int64_t)c.s0 * kKeys + lane; j0 - lane < upto; j0 += 32 * kAhead) {
+        for (int64_t j0 = ((int64_t)c.s0 << p.key_shift) + lane; j0 - lane < upto; j0 += 32 * kAhead) {
           float4 x[kAhead][2];
           float y[kAhead];
 #pragma unroll
@@ -959,13 +999,16 @@ int make_plan(const fftopk_paged* a, int sms, PagedParams& p, Plan& plan) {
   p.units = (int32_t)units;
   p.bound = (int32_t)bound;
   p.weigh = a->weight_out != nullptr;
-  const int64_t blocks = a->seqs * ((bound + kKeys - 1) / kKeys);
-  const int64_t ctas = (int64_t)sms * ctas_of(a->k_scale != nullptr, a->D, plan.nt);
-  int64_t runs = ctas / units < blocks / kMinBlocks ? ctas / units : blocks / kMinBlocks;
+  const bool fp8 = a->k_scale != nullptr;
+  const int keys = a->D == 64 ? (fp8 ? block_keys<true, 64>() : block_keys<false, 64>()) : fp8 ? block_keys<true, 128>() : block_keys<false, 128>();
+  p.key_shift = keys == 32 ? 5 : 4;
+  const int64_t blocks = a->seqs * ((bound + keys - 1) / keys);
+  const int64_t ctas = (int64_t)sms * ctas_of(fp8, a->D, plan.nt);
+  int64_t runs = ctas / units < blocks / (kMinKeys / keys) ? ctas / units : blocks / (kMinKeys / keys);
   if (runs < 1) runs = 1;
   p.runs = (int32_t)runs;
   plan.ctas = runs * units;
-  p.line = (bound + kKeys - 1) / kKeys * kKeys;
+  p.line = (bound + keys - 1) / keys * keys;
   if (runs > 1) {
     plan.bytes[1] = up256(runs * units * 2 * plan.nh * 8);
     plan.bytes[2] = up256(runs * units * 2 * plan.nh * a->D * 4);
@@ -1017,7 +1060,7 @@ int check(const fftopk_paged* a) {
 
 template <typename T, bool kFp8, int D>
 cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {
-  const bool whole = p.a.page_size % kKeys == 0;
+  const bool whole = p.a.page_size % block_keys<kFp8, D>() == 0;
   const auto kernel = plan.nt == 1 ? (whole ? paged_kernel<T, kFp8, D, 1, true> : paged_kernel<T, kFp8, D, 1, false>)
                                    : whole ? paged_kernel<T, kFp8, D, 2, true> : paged_kernel<T, kFp8, D, 2, false>;
   return launch(kernel, plan.ctas, kThreads, paged_smem<kFp8, D>(), false, stream, p);

@@ -46,10 +46,11 @@ constexpr int kWeighKeys = 128;  // positions that a warp has on their way at a 
 // positions of a run: below that, parts to join cost more than the blocks (one sequence of 1,000, 8 key heads: 8.8 us, with 256 positions 10.7, with 512
 // 15.4; of 4,096: 9.6, 10.3 and 12.3, with 64 11.3)
 constexpr int kMinKeys = 128;
-// Keys of a block, 16 to a product: as many as make 4 KB of k and v and more
+// Keys of a block, 16 to a product: 8 KB of k and v, so that what goes with a block is done for enough of them (64 sequences of up to 8,192, 8 key heads, with
+// 16 keys and with 32: 16 bits, heads of 64 137 us and 128; e4m3, 16 query heads to a key head 187 and 152; up to 16,384, heads of 64 174 and 138)
 template <bool kFp8, int D>
 constexpr int block_keys() {
-  return kFp8 && D == 64 ? 32 : 16;
+  return D * (kFp8 ? 1 : 2) == 256 ? 16 : 32;
 }
 
 struct PagedParams {
@@ -975,9 +976,17 @@ bool on16(const void* p, int64_t n, int64_t a, int64_t heads, int64_t b, int byt
   return on(p, 16) && (n <= 1 || a * bytes % 16 == 0) && (heads <= 1 || b * bytes % 16 == 0);
 }
 
-int ctas_of(bool fp8, int D, int nt) {
-  if (D == 64) return fp8 ? (nt == 1 ? paged_ctas<true, 64, 1>() : paged_ctas<true, 64, 2>()) : nt == 1 ? paged_ctas<false, 64, 1>() : paged_ctas<false, 64, 2>();
-  return fp8 ? (nt == 1 ? paged_ctas<true, 128, 1>() : paged_ctas<true, 128, 2>()) : nt == 1 ? paged_ctas<false, 128, 1>() : paged_ctas<false, 128, 2>();
+// Keys of a block and CTAs per SM of the kernel that a call goes to
+struct Form {
+  int keys, ctas;
+};
+template <bool kFp8, int D>
+Form form_of(int nt) {
+  return nt == 1 ? Form{block_keys<kFp8, D>(), paged_ctas<kFp8, D, 1>()} : Form{block_keys<kFp8, D>(), paged_ctas<kFp8, D, 2>()};
+}
+Form form_of(bool fp8, int D, int nt) {
+  if (D == 64) return fp8 ? form_of<true, 64>(nt) : form_of<false, 64>(nt);
+  return fp8 ? form_of<true, 128>(nt) : form_of<false, 128>(nt);
 }
 
 // Sizes of the call, checked; what the workspace holds in turn: lse2, ml, o, scores
@@ -999,11 +1008,11 @@ int make_plan(const fftopk_paged* a, int sms, PagedParams& p, Plan& plan) {
   p.units = (int32_t)units;
   p.bound = (int32_t)bound;
   p.weigh = a->weight_out != nullptr;
-  const bool fp8 = a->k_scale != nullptr;
-  const int keys = a->D == 64 ? (fp8 ? block_keys<true, 64>() : block_keys<false, 64>()) : fp8 ? block_keys<true, 128>() : block_keys<false, 128>();
+  const Form form = form_of(a->k_scale != nullptr, a->D, plan.nt);
+  const int keys = form.keys;
   p.key_shift = keys == 32 ? 5 : 4;
   const int64_t blocks = a->seqs * ((bound + keys - 1) / keys);
-  const int64_t ctas = (int64_t)sms * ctas_of(fp8, a->D, plan.nt);
+  const int64_t ctas = (int64_t)sms * form.ctas;
   int64_t runs = ctas / units < blocks / (kMinKeys / keys) ? ctas / units : blocks / (kMinKeys / keys);
   if (runs < 1) runs = 1;
   p.runs = (int32_t)runs;
@@ -1058,12 +1067,14 @@ int check(const fftopk_paged* a) {
   return FFTOPK_OK;
 }
 
-template <typename T, bool kFp8, int D>
+template <typename T, bool kFp8, int D, int kNT>
 cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {
   const bool whole = p.a.page_size % block_keys<kFp8, D>() == 0;
-  const auto kernel = plan.nt == 1 ? (whole ? paged_kernel<T, kFp8, D, 1, true> : paged_kernel<T, kFp8, D, 1, false>)
-                                   : whole ? paged_kernel<T, kFp8, D, 2, true> : paged_kernel<T, kFp8, D, 2, false>;
-  return launch(kernel, plan.ctas, kThreads, paged_smem<kFp8, D>(), false, stream, p);
+  return launch(whole ? paged_kernel<T, kFp8, D, kNT, true> : paged_kernel<T, kFp8, D, kNT, false>, plan.ctas, kThreads, paged_smem<kFp8, D>(), false, stream, p);
+}
+template <typename T, bool kFp8, int D>
+cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {
+  return plan.nt == 1 ? launch_paged<T, kFp8, D, 1>(p, plan, stream) : launch_paged<T, kFp8, D, 2>(p, plan, stream);
 }
 template <typename T>
 cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {

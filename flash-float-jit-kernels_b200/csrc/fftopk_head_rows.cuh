@@ -57,18 +57,18 @@ enum : int { kRotNone = 0, kRotApart = 1, kRotNext = 2 };  // partners: none, i 
 // `thread` of `threads` writes its share.
 __device__ __forceinline__ void merge_rows(const AxesParams& p, float* merged, uint32_t token0, uint32_t tokens, uint32_t thread, uint32_t threads) {
   const uint32_t R = (uint32_t)p.R, half = R >> 1, table_rows = (uint32_t)min(p.table_rows, (int64_t)0x80000000ll);
-  const int32_t* positions = p.positions + token0;
-  uint32_t r = thread;
-  for (uint32_t i = thread; i < tokens * R; i += threads, r += threads) {
-    while (r >= R) r -= R, ++positions;
-    const uint32_t pair = r < half ? r : r - half;
-    const uint32_t pos = (uint32_t)positions[(p.axis_of[pair >> 4] >> (2 * (pair & 15)) & 3u) * p.axis_stride];
-    float x = __int_as_float(0x7fffffff);
-    if (pos < table_rows)
-      x = p.cos_sin[(uint64_t)pos * R + r];
-    else if (p.status && (p.padding == nullptr || p.padding[positions - p.positions] >= 0))
+  uint32_t token = token0, pair = thread;
+  for (uint32_t i = thread; i < tokens * half; i += threads, pair += threads) {
+    while (pair >= half) pair -= half, ++token, merged += R;
+    const uint32_t pos = (uint32_t)p.positions[(p.axis_of[pair >> 4] >> (2 * (pair & 15)) & 3u) * p.axis_stride + token];
+    float c = __int_as_float(0x7fffffff), s = c;
+    if (pos < table_rows) {
+      const float* row = p.cos_sin + (uint64_t)pos * R + pair;
+      c = row[0], s = row[half];
+    } else if (p.status && (p.padding == nullptr || p.padding[token] >= 0)) {
       atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
-    merged[i] = x;
+    }
+    merged[pair] = c, merged[half + pair] = s;
   }
 }
 

@@ -7,7 +7,7 @@
 namespace fftopk {
 namespace {
 
-constexpr int kMergeTokens = 8;  // of a block
+constexpr int kMergeTokens = 4;  // of a block
 
 __global__ void __launch_bounds__(256) merge_rows_kernel(const __grid_constant__ AxesParams p, float* merged, uint32_t tokens) {
   const uint32_t token0 = blockIdx.x * kMergeTokens;

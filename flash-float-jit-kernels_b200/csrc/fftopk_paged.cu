@@ -3,14 +3,18 @@
 // g query heads to a key head, j below the sequence's length. Where asked for, what every cached row has been given so far is brought up
 // to date: weight_out[b, h / g, j] = weight[b, h / g, j] + sum of p_j over the key head's query heads. (The reference ends with indices.)
 //
-// What bounds it is reading the cache: a row of k or v is used by the g heads of its key head alone, 2 g flop a byte in 16 bits.
+// What bounds it is reading the cache: a row of k or v is used by the g heads of its key head alone, g flop a byte in 16 bits, 2 g in e4m3 (64
+// query heads on 8 key heads of 128: 64 sequences of up to 8,192 in bf16 243 us = 6.5 TB/s, of up to 16,384 in e4m3 250 = 6.5; one of 131,072 in bf16
+// 91 = 5.9, of which 5 are the join; one of 100: 5.5).
 //
-// Work split: the context, 16 keys a block, of all sequences, sequence after sequence, is one line of blocks. It is cut into equal runs,
-// whatever the lengths; a CTA takes one run for one key head (8 or 16 of its query heads). The CTAs of neighbouring numbers take the same run for
-// different key heads, so that what lies side by side in the cache - the heads of a row, their scales - is read at about the same
-// time. What a run has of a sequence is a segment: each of four warps takes a quarter of it with running maxima and sums (one pass), then they are
-// joined through the stages of their rings that are free at that moment. A run that holds all of a sequence writes the result, else a
-// part, which paged_finish_kernel joins. Lengths are read on the device only; no CTA waits for another one.
+// Work split: the context, 16 or 32 keys a block, of all sequences, sequence after sequence, is one line of blocks. It is cut into equal
+// runs, whatever the lengths; a CTA takes one run for one key head (8 or 16 of its query heads). The CTAs of neighbouring numbers take the same
+// run for different key heads, so that what lies side by side in the cache - the heads of a row, their scales - is read at about the
+// same time. What a run has of a sequence is a segment: each of four warps takes a quarter of it with running maxima and sums (one pass),
+// then they are joined through the stages of their rings that are free at that moment (every fourth block to a warp instead: e4m3 299 us, the
+// pages' entries are read more often). A run that holds all of a sequence writes the result, else a part, which paged_finish_kernel joins.
+// Lengths are read on the device only; no CTA waits for another one. More than 16 query heads to a key head read its rows again for every
+// 16 (64 on one key head, 32,768 positions: 2.7 times the floor), and a segment costs some 4 us whatever its length (1,024 sequences of 16: 95 us).
 //
 // A warp has a ring of blocks in shared memory that cp.async fills ahead of it. Keys are the rows of the MMA and query heads its
 // columns, 8 at a time: groups of up to 8 heads need half the products and accumulators they would need as rows.

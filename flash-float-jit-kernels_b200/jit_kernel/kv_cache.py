@@ -1,6 +1,7 @@
 """A cache of keys or values in fp8: e4m3 codes [slots, heads, D] with a float32 scale per slot and head, quantised as it is
 written and widened as it is read (no counterpart in the reference). A slot is a token's row; which one a token has is the
-caller's affair (a page table's entry, a sequence's base plus the position). ``sparse_attention`` reads such caches as they are."""
+caller's affair (a page table's entry, a sequence's base plus the position). ``sparse_attention`` and ``paged_attention`` read such
+caches as they are; ``cache_evict`` thins them, or 16-bit ones, by the weights ``paged_attention`` adds up."""
 from __future__ import annotations
 
 import struct

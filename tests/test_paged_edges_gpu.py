@@ -1,0 +1,116 @@
+"""Attention over a paged cache and eviction from it at the edges of their launch plans and arguments."""
+import math
+
+import pytest
+import torch
+
+import paged_ref as paged
+import rows_ref as ref
+from jit_kernel.kv_cache import cache_evict
+from jit_kernel.paged_attention import paged_attention
+from jit_kernel.topk_indexer import _status_word, kernel_status
+from test_cache_evict_gpu import check, make, weights
+from test_paged_attention_gpu import gen, make_cache, make_pages, rand
+
+pytestmark = pytest.mark.gpu
+FP8 = torch.float8_e4m3fn
+
+
+@pytest.fixture(autouse=True)
+def status():
+    if torch.cuda.is_available():
+        _status_word(torch.device("cuda", 0)).zero_()
+    yield
+    if torch.cuda.is_available():
+        assert kernel_status() == 0
+
+
+def attend(g, lens, Hq, Hk, page, D, dtype, fp8, weigh=True, **kw):
+    table, pages = make_pages(g, lens, page)
+    q = rand(g, len(lens), Hq, D, dtype=dtype, scale=2.0)
+    k, ks = make_cache(g, pages * page, Hk, D, dtype, fp8)
+    v, vs = make_cache(g, pages * page, Hk, D, dtype, fp8)
+    n = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    after = torch.full((len(lens), Hk, max(lens)), float("nan"), device="cuda") if weigh else None
+    out, lse = paged_attention(q, k, v, table, n, page_size=page, k_scale=ks, v_scale=vs, weight_out=after, return_lse=True, **kw)
+    want, at = paged.attention(q, k, v, table, n, page, kw.get("softmax_scale"), ks, vs)
+    ref.check_attention(out, lse, want)
+    if weigh:
+        paged.check_weights(after, None, n, *paged.weights(q, k, at, want, kw.get("softmax_scale"), ks))
+    return out
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("Hq,Hk", [(700, 700), (600, 300), (1200, 40)])
+def test_more_key_heads_than_ctas(fp8, Hq, Hk):
+    """A run for each key head, in several waves; and few runs of many heads."""
+    attend(gen(Hq), [70, 0, 33], Hq, Hk, 16, 64, torch.bfloat16, fp8)
+
+
+@pytest.mark.parametrize("B,Hq,longest", [(1000, 8, 40), (333, 12, 600), (2100, 1, 5)])
+def test_many_sequences(B, Hq, longest):
+    """More sequences than a warp has lanes, many times over, empty ones among them; several to a warp in the join."""
+    g = gen(B)
+    lens = torch.randint(0, longest + 1, (B,), generator=g, device="cuda").tolist()
+    lens[:3], lens[-2:] = [longest, 0, 1], [longest, 0]
+    attend(g, lens, Hq, 1, 8, 64, torch.float16, B % 2 == 0)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lens", [[60000] + [3] * 40, [3] * 40 + [60000], [1, 50001, 0, 2]])
+def test_one_long_sequence_among_short_ones(fp8, lens):
+    attend(gen(len(lens)), lens, 8, 2, 64, 128, torch.bfloat16, fp8)
+
+
+def test_pages_longer_than_sequences():
+    attend(gen(5), [100, 31, 1], 8, 2, 1 << 12, 64, torch.bfloat16, True)
+    attend(gen(6), [100, 31, 1], 8, 2, 4001, 64, torch.bfloat16, True)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-6])
+def test_softmax_scales(fp8, scale):
+    attend(gen(7), [300, 17], 16, 2, 16, 128, torch.float16, fp8, softmax_scale=scale)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_scale_that_is_nan(fp8):
+    """NaN for every sequence that has a row, zeros for the others, as ever."""
+    g = gen(8)
+    table, pages = make_pages(g, [300, 0], 16)
+    q = rand(g, 2, 8, 128, dtype=torch.bfloat16)
+    k, ks = make_cache(g, pages * 16, 1, 128, torch.bfloat16, fp8)
+    n = torch.tensor([300, 0], device="cuda", dtype=torch.int32)
+    out, lse = paged_attention(q, k, k, table, n, page_size=16, k_scale=ks, v_scale=ks, softmax_scale=math.nan, return_lse=True)
+    assert bool(out[0].isnan().all()) and bool(lse[0].isnan().all()) and bool((out[1] == 0).all()) and bool(lse[1].isneginf().all())
+
+
+def test_row_strides_that_do_not_fit_32_bits_are_refused():
+    base = torch.zeros(64, device="cuda", dtype=torch.bfloat16)
+    far = torch.as_strided(base, (1, 1, 64), (1 << 32, 64, 1))  # (a lone slot's stride says nothing)
+    q = torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    t, n = torch.zeros(1, 1, device="cuda", dtype=torch.int32), torch.ones(1, device="cuda", dtype=torch.int32)
+    assert bool((paged_attention(q, far, far, t, n, page_size=1) == 0).all())
+
+
+@pytest.mark.parametrize("H,lens,budget", [(1, [262145], 5000), (3, [17000, 16384, 16385, 8193, 8192], 8192), (300, [600, 599], 100), (1, [4] * 700, 3)])
+def test_evict_plans(H, lens, budget):
+    """Clusters, keys that do and do not fit shared memory, more units than CTAs at once."""
+    g = gen(len(lens) * H)
+    data, scales, table, to = make(g, lens, budget, H, 8, 16, FP8)
+    check(data, scales, table, to, weights(g, len(lens), H, max(lens)), lens, 16, budget, min(2, budget), 1)
+
+
+def test_evict_by_parts_of_a_wider_pool():
+    """Rows of one sequence after another into the same pages, freed in between; weights not contiguous."""
+    g = gen(31)
+    data, scales, table, to = make(g, [90, 80], 32, 2, 16, 16, torch.bfloat16)
+    w = weights(g, 2, 2, 200)[..., 50:150]
+    for b in (0, 1):
+        part = [x.clone() for x in data]
+        n = torch.tensor([[90, 80][b]], device="cuda", dtype=torch.int32)
+        kept, left, out = paged.evict(w[b:b + 1], n, 32, 4, 4)
+        got = cache_evict(*part, w[b:b + 1], table[b:b + 1], n, to[:1], page_size=16, budget=32, recent=4, sinks=4)
+        assert torch.equal(got[0].cpu(), kept) and torch.equal(got[1].cpu(), left) and torch.equal(got[2].cpu(), out)
+        for x, y in zip(part, data):
+            assert torch.equal(x.view(torch.int16), paged.move(y, kept, table[b:b + 1], to[:1], 16).view(torch.int16))

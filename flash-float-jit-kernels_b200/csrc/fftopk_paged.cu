@@ -5,7 +5,7 @@
 //
 // What bounds it is reading the cache: a row of k or v is used by the g heads of its key head alone, g flop a byte in 16 bits, 2 g in e4m3 (64
 // query heads on 8 key heads of 128: 64 sequences of up to 8,192 in bf16 243 us = 6.5 TB/s, of up to 16,384 in e4m3 250 = 6.5; one of 131,072 in bf16
-// 91 = 5.9, of which 5 are the join; one of 100: 5.5).
+// 91 = 5.9, of which 5 are the join; one of 100: 4.8).
 //
 // Work split: the context, 16 or 32 keys a block, of all sequences, sequence after sequence, is one line of blocks. It is cut into equal
 // runs, whatever the lengths; a CTA takes one run for one key head (8 or 16 of its query heads). The CTAs of neighbouring numbers take the same
@@ -13,8 +13,9 @@
 // same time. What a run has of a sequence is a segment: each of four warps takes a quarter of it with running maxima and sums (one pass),
 // then they are joined through the stages of their rings that are free at that moment (every fourth block to a warp instead: e4m3 299 us, the
 // pages' entries are read more often). A run that holds all of a sequence writes the result, else a part, which paged_finish_kernel joins.
-// Lengths are read on the device only; no CTA waits for another one. More than 16 query heads to a key head read its rows again for every
-// 16 (64 on one key head, 32,768 positions: 2.7 times the floor), and a segment costs some 4 us whatever its length (1,024 sequences of 16: 95 us).
+// Lengths are read on the device only; no CTA waits for another one. Where tables are short, runs are the sequences themselves, and nothing is joined (64 sequences of
+// up to 300: 14.5 us, in equal runs 23). More than 16 query heads to a key head read its rows again for every 16 (64 on one key head, 32,768 positions:
+// 2.7 times the floor), and a segment costs some 4 us whatever its length (1,024 sequences of 16: 87 us).
 //
 // A warp has a ring of blocks in shared memory that cp.async fills ahead of it. Keys are the rows of the MMA and query heads its
 // columns, 8 at a time: groups of up to 8 heads need half the products and accumulators they would need as rows.
@@ -61,6 +62,7 @@ struct PagedParams {
   fftopk_paged a;
   int32_t group, head_blocks, units, runs, bound, weigh;
   int32_t key_shift;  // of a block's keys
+  int32_t apart;      // a run is a sequence, whatever its length: no parts
   FastDiv page;
   float scale_log2;
   int32_t stream;   // the rows are more than L2 holds
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   constexpr int kTiles = D / 16;             // of the output: rows of the MMA are channels
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   // (only where a kernel of this call follows, which waits: another one's inputs may be this one's results)
-  if (p.runs > 1 || p.weigh) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.join_ctas > 0 || p.weigh) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   __shared__ float2 ml_of[kWarps][kNH];
   __shared__ uint32_t free_of[kWarps];  // the warps' free stages
@@ -259,22 +261,37 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   const int heads = min(kNH, p.group - hb * kNH);
   const int head0 = kvh * p.group + hb * kNH;
 
-  // what is empty, and what reaches beyond its pages
-  for (int64_t b = run + (int64_t)p.runs * warp; b < p.a.seqs; b += (int64_t)p.runs * kWarps) {
+  // a sequence without rows; and one that reaches beyond its pages is told of
+  auto empty = [&](int64_t b) {
     const int32_t n = p.a.lengths[b];
     if (n > p.bound && unit == 0 && lane == 0 && p.status) atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
-    if (min(n, p.bound) <= 0) {
-      for (int h = 0; h < heads; ++h) {
-        T* out = static_cast<T*>(p.a.out) + b * p.a.out_seq + (int64_t)(head0 + h) * p.a.out_head;
-        for (int d = lane; d < D; d += 32) out[d] = T(0.f);
-        if (lane == 0 && p.a.lse != nullptr) p.a.lse[b * p.a.q_heads + head0 + h] = -INFINITY;
-      }
+    return min(n, p.bound) <= 0;
+  };
+  auto put_zeros = [&](int64_t b) {
+    for (int h = 0; h < heads; ++h) {
+      T* out = static_cast<T*>(p.a.out) + b * p.a.out_seq + (int64_t)(head0 + h) * p.a.out_head;
+      for (int d = lane; d < D; d += 32) out[d] = T(0.f);
+      if (lane == 0 && p.a.lse != nullptr) p.a.lse[b * p.a.q_heads + head0 + h] = -INFINITY;
     }
+  };
+  Segment here;
+  int64_t left;  // blocks of the run that are not behind the segment at hand
+  if (p.apart) {  // (the run is the sequence of its number)
+    if (empty(run)) {
+      if (warp == 0) put_zeros(run);
+      return;  // (the whole CTA)
+    }
+    here.b = run, here.n = keys_of(p, run), here.s0 = 0, here.s1 = here.blocks = (int32_t)blocks_of(p, here.n);
+    left = here.blocks;
+  } else {
+    for (int64_t b = run + (int64_t)p.runs * warp; b < p.a.seqs; b += (int64_t)p.runs * kWarps)
+      if (empty(b)) put_zeros(b);
+    const Runs line(blocks_before(p, p.a.seqs, lane), p.runs, kMinKeys / kKeys);
+    if ((int64_t)run >= line.runs || line.total == 0) return;  // (the whole CTA)
+    left = line.begin((int64_t)run + 1) - line.begin(run);
+    if (left <= 0) return;
+    here = segment_at(p, line.begin(run), left, lane);
   }
-  const Runs line(blocks_before(p, p.a.seqs, lane), p.runs, kMinKeys / kKeys);
-  if ((int64_t)run >= line.runs || line.total == 0) return;  // (the whole CTA)
-  int64_t left = line.begin((int64_t)run + 1) - line.begin(run);  // blocks of the run that are not behind the segment at hand
-  if (left <= 0) return;
 
   constexpr int kLanesRow = G::kRowBytes / 16, kRowsOnce = 32 / kLanesRow, kTurns = kKeys / kRowsOnce;
   constexpr int kES = kFp8 ? 1 : 2;
@@ -299,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
   else
     asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(once));
-  Segment here = segment_at(p, line.begin(run), left, lane), ahead = here;
+  Segment ahead = here;
   int64_t left_ahead = left;
   int32_t at, end, ask_at, ask_end;  // the warp's blocks of the segment at hand, and of the one it asks for
   quarter(here, warp, at, end);
@@ -711,7 +728,7 @@ struct Parts {
   int64_t first, second, step;
   int32_t n;
   __device__ __forceinline__ Parts(const PagedParams& p, const Runs& line, int64_t begin, int64_t end, int unit) {
-    const int64_t r0 = line.of(begin), r1 = line.of(end - 1);
+    const int64_t r0 = p.apart ? 0 : line.of(begin), r1 = p.apart ? 0 : line.of(end - 1);
     n = (int32_t)(r1 - r0) + 1;
     first = (r0 * p.units + unit) * 2 + (line.begin(r0) < begin ? 1 : 0);  // (the sequence begins inside its first run)
     second = ((r0 + 1) * p.units + unit) * 2;
@@ -1019,10 +1036,16 @@ int make_plan(const fftopk_paged* a, int sms, PagedParams& p, Plan& plan) {
   const int64_t ctas = (int64_t)sms * form.ctas;
   int64_t runs = ctas / units < blocks / (kMinKeys / keys) ? ctas / units : blocks / (kMinKeys / keys);
   if (runs < 1) runs = 1;
+  // A CTA a sequence and key head, no parts, where the longest is read in less time than the join takes, or nearly, and there are CTAs for the device: one sequence of
+  // 300 (154 KB a key head) 7.4 us, in runs 8.8; of 500 (256 KB) 9.5 and 8.2; 64 of up to 300, 14.5 and 23; 32 of up to 1,500 (768 KB) 31 and 38; 37 with 3 key
+  // heads of up to 2,999 (768 KB) 24 and 20; 40 of up to 2,500 (1.3 MB) 66 and 60
+  const double bytes = (double)bound * a->D * (a->k_scale != nullptr ? 1 : 2) * 2;
+  p.apart = bytes <= 200e3 || (bytes <= 800e3 && a->seqs * units * 5 >= (int64_t)sms * 4);
+  if (p.apart) runs = a->seqs;
   p.runs = (int32_t)runs;
   plan.ctas = runs * units;
   p.line = (bound + keys - 1) / keys * keys;
-  if (runs > 1) {
+  if (runs > 1 && !p.apart) {
     plan.bytes[1] = up256(runs * units * 2 * plan.nh * 8);
     plan.bytes[2] = up256(runs * units * 2 * plan.nh * a->D * 4);
     // a warp a pair where a CTA each would take more than the device holds at once, and several where that would

@@ -10,7 +10,7 @@ from jit_kernel.kv_cache import cache_evict
 from jit_kernel.paged_attention import paged_attention
 from jit_kernel.topk_indexer import _status_word, kernel_status
 from test_cache_evict_gpu import check, make, weights
-from test_paged_attention_gpu import gen, make_cache, make_pages, rand
+from test_paged_attention_gpu import SHAPES, gen, make_cache, make_pages, ragged, rand
 
 pytestmark = pytest.mark.gpu
 FP8 = torch.float8_e4m3fn
@@ -25,8 +25,8 @@ def status():
         assert kernel_status() == 0
 
 
-def attend(g, lens, Hq, Hk, page, D, dtype, fp8, weigh=True, **kw):
-    table, pages = make_pages(g, lens, page)
+def attend(g, lens, Hq, Hk, page, D, dtype, fp8, weigh=True, extra=1, **kw):
+    table, pages = make_pages(g, lens, page, extra)
     q = rand(g, len(lens), Hq, D, dtype=dtype, scale=2.0)
     k, ks = make_cache(g, pages * page, Hk, D, dtype, fp8)
     v, vs = make_cache(g, pages * page, Hk, D, dtype, fp8)
@@ -54,6 +54,16 @@ def test_many_sequences(B, Hq, longest):
     lens = torch.randint(0, longest + 1, (B,), generator=g, device="cuda").tolist()
     lens[:3], lens[-2:] = [longest, 0, 1], [longest, 0]
     attend(g, lens, Hq, 1, 8, 64, torch.float16, B % 2 == 0)
+
+
+@pytest.mark.parametrize("Hq,Hk,page,lengths", SHAPES + [(8, 1, 8, (1000, 40)), (12, 1, 8, (333, 600)), (3, 3, 16, (2100, 5))])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_wide_tables(fp8, D, Hq, Hk, page, lengths):
+    """Tables with room for 7,000 positions, most of it unused: runs that hold many sequences and parts of them, several pairs to a warp of the join."""
+    g = gen(Hq * page + D + 1)
+    lens = ragged(g, *lengths) if isinstance(lengths, tuple) else lengths
+    attend(g, lens, Hq, Hk, page, D, torch.bfloat16, fp8, extra=7000 // page)
 
 
 @pytest.mark.parametrize("fp8", [False, True])

@@ -5,7 +5,7 @@
 //
 // What bounds it is reading the cache: a row of k or v is used by the g heads of its key head alone, g flop a byte in 16 bits, 2 g in e4m3 (64
 // query heads on 8 key heads of 128: 64 sequences of up to 8,192 in bf16 243 us = 6.5 TB/s, of up to 16,384 in e4m3 250 = 6.5; one of 131,072 in bf16
-// 91 = 5.9, of which 5 are the join; one of 100: 4.8).
+// 91 = 5.9, of which 5 are the join; one of 100: 5.1).
 //
 // Work split: the context, 16 or 32 keys a block, of all sequences, sequence after sequence, is one line of blocks. It is cut into equal
 // runs, whatever the lengths; a CTA takes one run for one key head (8 or 16 of its query heads). The CTAs of neighbouring numbers take the same
@@ -13,9 +13,9 @@
 // same time. What a run has of a sequence is a segment: each of four warps takes a quarter of it with running maxima and sums (one pass),
 // then they are joined through the stages of their rings that are free at that moment (every fourth block to a warp instead: e4m3 299 us, the
 // pages' entries are read more often). A run that holds all of a sequence writes the result, else a part, which paged_finish_kernel joins.
-// Lengths are read on the device only; no CTA waits for another one. Where tables are short, runs are the sequences themselves, and nothing is joined (64 sequences of
-// up to 300: 14.5 us, in equal runs 23). More than 16 query heads to a key head read its rows again for every 16 (64 on one key head, 32,768 positions:
-// 2.7 times the floor), and a segment costs some 4 us whatever its length (1,024 sequences of 16: 87 us).
+// Lengths are read on the device only; no CTA waits for another launch's. Where tables are short, a cluster takes a sequence and joins it through distributed shared
+// memory (64 sequences of up to 300: 15 us, in equal runs 23). More than 16 query heads to a key head read its rows again for every 16 (64 on one key head, 32,768
+// positions: 2.7 times the floor), and a segment costs some 4 us whatever its length (1,024 sequences of 16: 87 us).
 //
 // A warp has a ring of blocks in shared memory that cp.async fills ahead of it. Keys are the rows of the MMA and query heads its
 // columns, 8 at a time: groups of up to 8 heads need half the products and accumulators they would need as rows.
@@ -28,6 +28,7 @@
 //        scale its weight; the running reference is of weight * |v scale|, so that no row with hardly any weight sets it.
 // Roundings: weights of the second product to the cache's type (e4m3: to fp16, their v scale in them), off by half a step; everything
 // else is held in 32 bits.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -45,6 +46,9 @@
 namespace fftopk {
 namespace {
 
+namespace cg = cooperative_groups;
+
+constexpr int kMaxApart = 8;  // CTAs of a cluster that takes a sequence
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kWeighKeys = 128;  // positions that a warp has on their way at a time where it brings weights up to date
@@ -62,7 +66,7 @@ struct PagedParams {
   fftopk_paged a;
   int32_t group, head_blocks, units, runs, bound, weigh;
   int32_t key_shift;  // of a block's keys
-  int32_t apart;      // a run is a sequence, whatever its length: no parts
+  int32_t apart;      // CTAs of a cluster that takes a sequence, whatever its length: no parts; 0: equal runs
   FastDiv page;
   float scale_log2;
   int32_t stream;   // the rows are more than L2 holds
@@ -253,10 +257,12 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
 
   __shared__ float2 ml_of[kWarps][kNH];
   __shared__ uint32_t free_of[kWarps];  // the warps' free stages
+  __shared__ float2 joined_ml[kNH];     // of a CTA of a cluster: maximum and sum
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, qd = lane & 3;
-  const uint32_t run = blockIdx.x / (uint32_t)p.units;
-  const int unit = (int)(blockIdx.x - run * (uint32_t)p.units);
+  const uint32_t ctas = (uint32_t)max(p.apart, 1), run_unit = blockIdx.x / ctas, rank = blockIdx.x - run_unit * ctas;
+  const uint32_t run = run_unit / (uint32_t)p.units;
+  const int unit = (int)(run_unit - run * (uint32_t)p.units);
   const int kvh = unit / p.head_blocks, hb = unit - kvh * p.head_blocks;
   const int heads = min(kNH, p.group - hb * kNH);
   const int head0 = kvh * p.group + hb * kNH;
@@ -276,13 +282,14 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   };
   Segment here;
   int64_t left;  // blocks of the run that are not behind the segment at hand
-  if (p.apart) {  // (the run is the sequence of its number)
+  if (p.apart) {  // (the run is the sequence of its number, a CTA's segment its share of the cluster's)
     if (empty(run)) {
-      if (warp == 0) put_zeros(run);
-      return;  // (the whole CTA)
+      if (warp == 0 && rank == 0) put_zeros(run);
+      return;  // (the whole cluster)
     }
-    here.b = run, here.n = keys_of(p, run), here.s0 = 0, here.s1 = here.blocks = (int32_t)blocks_of(p, here.n);
-    left = here.blocks;
+    here.b = run, here.n = keys_of(p, run), here.blocks = (int32_t)blocks_of(p, here.n);
+    here.s0 = (int32_t)((int64_t)here.blocks * rank / ctas), here.s1 = (int32_t)((int64_t)here.blocks * (rank + 1) / ctas);
+    left = here.s1 - here.s0;  // (none, where there are fewer blocks than CTAs)
   } else {
     for (int64_t b = run + (int64_t)p.runs * warp; b < p.a.seqs; b += (int64_t)p.runs * kWarps)
       if (empty(b)) put_zeros(b);
@@ -649,72 +656,116 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
     __syncwarp();  // (the next block but kStages - 2 goes where this one was)
     }
     // ---- the segment's end: the stage that is asked for next is free, and takes the warp's accumulators, [heads][D] ----
+    static_assert(G::kStage >= kNH * D * 4, "a stage holds the accumulators");
     const bool whole = here.s0 == 0 && here.s1 == here.blocks;
-    const int64_t rec = (int64_t)blockIdx.x * 2 + which;
-    const uint32_t free_stage = (uint32_t)(ask_stage * G::kStage);
-    constexpr int kOnce = G::kStage >= kNH * D * 4 ? kNH : 8;  // heads at a time
-    static_assert(G::kStage >= kOnce * D * 4, "a stage holds the accumulators");
+    const int64_t rec = (int64_t)run_unit * 2 + which;
+    const uint32_t mine = (uint32_t)(warp * G::kBytes + ask_stage * G::kStage);
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        const int h = 8 * t + 2 * qd + e;
         const float l = keys_sum(sum[t][e]);
-        if (g == 0) ml_of[warp][8 * t + 2 * qd + e] = make_float2(mx[t][e], l);
-      }
-    }
+        if (g == 0) ml_of[warp][h] = make_float2(mx[t][e], l);
+        // channels of the accumulators: 16 bits g and g + 8 of a tile, e4m3 2 g and 2 g + 1
+        float* const row = reinterpret_cast<float*>(smem_raw + mine) + h * D;
 #pragma unroll
-    for (int h0 = 0; h0 < kNH; h0 += kOnce) {
-      // channels of the accumulators: 16 bits g and g + 8 of a tile, e4m3 2 g and 2 g + 1
-      float* const mine = reinterpret_cast<float*>(smem_raw + warp * G::kBytes + free_stage);
-#pragma unroll
-      for (int t = h0 / 8; t < (h0 + kOnce) / 8; ++t) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float* const row = mine + (8 * t - h0 + 2 * qd + e) * D;
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
-            row[16 * i + (kFp8 ? 2 * g : g)] = o[t][i][e];
-            row[16 * i + (kFp8 ? 2 * g + 1 : g + 8)] = o[t][i][2 + e];
-          }
+        for (int i = 0; i < kTiles; ++i) {
+          row[16 * i + (kFp8 ? 2 * g : g)] = o[t][i][e];
+          row[16 * i + (kFp8 ? 2 * g + 1 : g + 8)] = o[t][i][2 + e];
         }
       }
-      if (lane == 0 && h0 == 0) free_of[warp] = (uint32_t)(warp * G::kBytes) + free_stage;
+    }
+    if (lane == 0) free_of[warp] = mine;
+    __syncthreads();
+    // the warps' four channels d .. d + 3 of head h
+    auto joined = [&](int h, int d, float& m, float& l) {
+      m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml_of[w][h].x);
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 ml = ml_of[w][h];
+        const float f = ml.x == m ? 1.f : ex2(ml.x - m);  // (a warp without keys: 0 of both; 0 * NaN stays NaN)
+        l += kFp8 ? brought(ml.y, ml.x, m) : f * ml.y;
+        const float4 x = *reinterpret_cast<const float4*>(smem_raw + free_of[w] + (h * D + d) * 4);
+        y.x += f * x.x, y.y += f * x.y, y.z += f * x.z, y.w += f * x.w;
+      }
+      return y;
+    };
+    auto finish = [&](int h, int d, float m, float l, const float4& y) {
+      T* out = static_cast<T*>(p.a.out) + here.b * p.a.out_seq + (int64_t)(head0 + h) * p.a.out_head + d;
+      const float r[4] = {l == 0.f ? 0.f : y.x / l, l == 0.f ? 0.f : y.y / l, l == 0.f ? 0.f : y.z / l, l == 0.f ? 0.f : y.w / l};
+      Four<T> narrow;
+      narrow.narrow(r);
+      if (p.out_vec)
+        narrow.template store<true>(out);
+      else
+        narrow.template store<false>(out);
+      if (d == 0) {
+        const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
+        if (p.a.lse != nullptr) p.a.lse[here.b * p.a.q_heads + head0 + h] = l2 * 0.693147180559945309f;
+        if (p.weigh) p.lse2[here.b * p.a.q_heads + head0 + h] = l2;
+      }
+    };
+    if (ctas > 1) {
+      // The cluster's CTAs are joined through distributed shared memory. Each puts what its warps have where its rings begin - every block has been used, and
+      // what comes from its warps' stages is in registers by then - and finishes its share of the rows.
+      constexpr int kRows = kNH * (D / 4) / kThreads;  // of a thread
+      static_assert(kRows * kThreads == kNH * (D / 4), "a thread has whole rows");
+      float4 y[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int at = (int)threadIdx.x + i * kThreads, h = at / (D / 4), d = at % (D / 4) * 4;
+        float m, l;
+        y[i] = joined(h, d, m, l);
+        if (d == 0) joined_ml[h] = make_float2(m, l);
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       __syncthreads();
-      for (int i = threadIdx.x; i < min(kOnce, heads - h0) * (D / 4); i += kThreads) {
-        const int h = h0 + i / (D / 4), d = i % (D / 4) * 4;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) reinterpret_cast<float4*>(smem_raw)[threadIdx.x + i * kThreads] = y[i];
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      for (int at = (int)(threadIdx.x + rank * kThreads); at < heads * (D / 4); at += kThreads * (int)ctas) {
+        const int h = at / (D / 4), d = at % (D / 4) * 4;
+        // (every CTA's part is asked for before any is used)
+        const uint32_t ml_at = smem_u32(&joined_ml[h]), o_at = smem_u32(smem_raw) + (uint32_t)at * 16u;
+        float2 ml[kMaxApart];
+        float4 part[kMaxApart];
         float m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml_of[w][h].x);
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < kMaxApart; ++c) {
+          ml[c] = make_float2(-INFINITY, 0.f), part[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (c < (int)ctas) ml[c] = lds_cluster2(shared_of(ml_at, c)), part[c] = lds_cluster4(shared_of(o_at, c));
+        }
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 ml = ml_of[w][h];
-          const float f = ml.x == m ? 1.f : ex2(ml.x - m);  // (a warp without keys: 0 of both; 0 * NaN stays NaN)
-          l += kFp8 ? brought(ml.y, ml.x, m) : f * ml.y;
-          const float4 x = *reinterpret_cast<const float4*>(smem_raw + free_of[w] + (h - h0) * (D * 4) + d * 4);
-          y.x += f * x.x, y.y += f * x.y, y.z += f * x.z, y.w += f * x.w;
+        for (int c = 0; c < kMaxApart; ++c) m = fmaxf(m, ml[c].x);
+        float4 all = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < kMaxApart; ++c) {
+          const float f = ml[c].x == m ? 1.f : ex2(ml[c].x - m);
+          l += kFp8 ? brought(ml[c].y, ml[c].x, m) : f * ml[c].y;
+          all.x += f * part[c].x, all.y += f * part[c].y, all.z += f * part[c].z, all.w += f * part[c].w;
         }
-        if (whole) {
-          T* out = static_cast<T*>(p.a.out) + here.b * p.a.out_seq + (int64_t)(head0 + h) * p.a.out_head + d;
-          const float r[4] = {l == 0.f ? 0.f : y.x / l, l == 0.f ? 0.f : y.y / l, l == 0.f ? 0.f : y.z / l, l == 0.f ? 0.f : y.w / l};
-          Four<T> narrow;
-          narrow.narrow(r);
-          if (p.out_vec)
-            narrow.template store<true>(out);
-          else
-            narrow.template store<false>(out);
-          if (d == 0) {
-            const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
-            if (p.a.lse != nullptr) p.a.lse[here.b * p.a.q_heads + head0 + h] = l2 * 0.693147180559945309f;
-            if (p.weigh) p.lse2[here.b * p.a.q_heads + head0 + h] = l2;
-          }
-        } else {
-          *reinterpret_cast<float4*>(p.o + (rec * kNH + h) * D + d) = y;
-          if (d == 0) p.ml[rec * kNH + h] = make_float2(m, l);
-        }
+        finish(h, d, m, l, all);
       }
-      __syncthreads();
+      cluster.sync();  // (nobody leaves while its memory is read)
+      return;
     }
+    for (int i = threadIdx.x; i < heads * (D / 4); i += kThreads) {
+      const int h = i / (D / 4), d = i % (D / 4) * 4;
+      float m, l;
+      const float4 y = joined(h, d, m, l);
+      if (whole) {
+        finish(h, d, m, l, y);
+      } else {
+        *reinterpret_cast<float4*>(p.o + (rec * kNH + h) * D + d) = y;
+        if (d == 0) p.ml[rec * kNH + h] = make_float2(m, l);
+      }
+    }
+    __syncthreads();
     left -= here.s1 - here.s0;
     if (left <= 0 || !next_segment(p, here, left)) break;
     quarter(here, warp, at, end);
@@ -940,7 +991,11 @@ __global__ void __launch_bounds__(kThreads, 5) paged_finish_kernel(const __grid_
 }
 
 DeviceOnce g_paged_once[kMaxDevices];
-int g_paged_sms[kMaxDevices];
+struct PagedLimits {
+  int sms = 0;
+  int eights[2][2][2] = {};  // clusters of eight CTAs the device holds at once: [e4m3][heads of 128][sixteens of query heads]
+};
+PagedLimits g_paged_limits[kMaxDevices];
 
 template <typename T, bool kFp8, int D, int kNT>
 int setup_one() {
@@ -958,36 +1013,53 @@ int setup_two() {
   if (!r) r = setup_one<T, kFp8, 128, 2>();
   return r;
 }
-int paged_setup(int& sms) {
+template <bool kFp8, int D>
+int eights_of(PagedLimits& limits) {
+  int r = clusters_of(limits.eights[kFp8][D == 128][0], paged_kernel<__nv_bfloat16, kFp8, D, 1, true>, kThreads, paged_smem<kFp8, D>());
+  if (!r) r = clusters_of(limits.eights[kFp8][D == 128][1], paged_kernel<__nv_bfloat16, kFp8, D, 2, true>, kThreads, paged_smem<kFp8, D>());
+  return r;
+}
+int paged_setup(PagedLimits& limits) {
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e);
   if (dev < 0 || dev >= kMaxDevices) return FFTOPK_EDEVICE;
   const int rc = g_paged_once[dev].run([&] {
-    const cudaError_t e2 = cudaDeviceGetAttribute(&g_paged_sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    const cudaError_t e2 = cudaDeviceGetAttribute(&g_paged_limits[dev].sms, cudaDevAttrMultiProcessorCount, dev);
     if (e2 != cudaSuccess) return cuda_fail(e2);
     int r = setup_two<__nv_bfloat16, false>();
     if (!r) r = setup_two<__nv_bfloat16, true>();
     if (!r) r = setup_two<__half, false>();
     if (!r) r = setup_two<__half, true>();
+    if (!r) r = eights_of<false, 64>(g_paged_limits[dev]);
+    if (!r) r = eights_of<false, 128>(g_paged_limits[dev]);
+    if (!r) r = eights_of<true, 64>(g_paged_limits[dev]);
+    if (!r) r = eights_of<true, 128>(g_paged_limits[dev]);
     return r;
   });
-  sms = g_paged_sms[dev];
+  limits = g_paged_limits[dev];
   return rc;
 }
 
 template <typename... A>
-cudaError_t launch(void (*kernel)(A...), int64_t grid, int threads, size_t smem, bool dependent, cudaStream_t stream, const PagedParams& p) {
+cudaError_t launch(void (*kernel)(A...), int64_t grid, int threads, size_t smem, int cluster, bool dependent, cudaStream_t stream, const PagedParams& p) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  if (cluster > 1) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+  } else {
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = dependent ? 1 : 0;
+  cfg.numAttrs = cluster > 1 || dependent ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -1016,7 +1088,8 @@ struct Plan {
   int64_t ctas = 0, finish_ctas = 0, bytes[4] = {}, total = 0;
 };
 int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
-int make_plan(const fftopk_paged* a, int sms, PagedParams& p, Plan& plan) {
+int make_plan(const fftopk_paged* a, const PagedLimits& limits, PagedParams& p, Plan& plan) {
+  const int sms = limits.sms;
   memset(&p, 0, sizeof(p));
   p.a = *a;
   p.group = a->q_heads / a->kv_heads;
@@ -1036,14 +1109,18 @@ int make_plan(const fftopk_paged* a, int sms, PagedParams& p, Plan& plan) {
   const int64_t ctas = (int64_t)sms * form.ctas;
   int64_t runs = ctas / units < blocks / (kMinKeys / keys) ? ctas / units : blocks / (kMinKeys / keys);
   if (runs < 1) runs = 1;
-  // A CTA a sequence and key head, no parts, where the longest is read in less time than the join takes, or nearly, and there are CTAs for the device: one sequence of
-  // 300 (154 KB a key head) 7.4 us, in runs 8.8; of 500 (256 KB) 9.5 and 8.2; 64 of up to 300, 14.5 and 23; 32 of up to 1,500 (768 KB) 31 and 38; 37 with 3 key
-  // heads of up to 2,999 (768 KB) 24 and 20; 40 of up to 2,500 (1.3 MB) 66 and 60
+  // Short tables: a sequence and key head is a piece of work, taken by a cluster - of as many CTAs as fit the device at once and have 128 positions each - that joins
+  // it by itself. What it saves - the search for runs, the second kernel - is worth more than what unequal lengths cost while a CTA reads 200 KB at most, or
+  // 800 KB where there are CTAs for four fifths of the device (in clusters and in equal runs: one sequence of 1,000 8.0 us and 9.3, of 4,096 10.7 and 9.8, of
+  // 16,000 27 and 16; 8 of up to 1,000 8.6 and 13; 37 with 3 key heads of 64 of up to 2,999 16 and 20; 64 of up to 300 15 and 23; 32 of up to 1,500 30 and 39; 40 of
+  // up to 2,500, which are 1.3 MB, 66 and 60)
   const double bytes = (double)bound * a->D * (a->k_scale != nullptr ? 1 : 2) * 2;
-  p.apart = bytes <= 200e3 || (bytes <= 800e3 && a->seqs * units * 5 >= (int64_t)sms * 4);
-  if (p.apart) runs = a->seqs;
+  const int64_t pieces = a->seqs * units, eights = limits.eights[a->k_scale != nullptr][a->D == 128][plan.nt - 1];
+  int apart = 1;
+  while (apart < kMaxApart && pieces * apart * 2 <= ctas && bound / (apart * 2) >= kMinKeys && (apart * 2 < 8 || pieces <= eights)) apart *= 2;
+  if (bytes <= 200e3 * apart || (bytes <= 800e3 * apart && pieces * apart * 5 >= (int64_t)sms * 4)) p.apart = apart, runs = a->seqs;
   p.runs = (int32_t)runs;
-  plan.ctas = runs * units;
+  plan.ctas = runs * units * (p.apart > 1 ? p.apart : 1);
   p.line = (bound + keys - 1) / keys * keys;
   if (runs > 1 && !p.apart) {
     plan.bytes[1] = up256(runs * units * 2 * plan.nh * 8);
@@ -1097,7 +1174,7 @@ int check(const fftopk_paged* a) {
 template <typename T, bool kFp8, int D, int kNT>
 cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {
   const bool whole = p.a.page_size % block_keys<kFp8, D>() == 0;
-  return launch(whole ? paged_kernel<T, kFp8, D, kNT, true> : paged_kernel<T, kFp8, D, kNT, false>, plan.ctas, kThreads, paged_smem<kFp8, D>(), false, stream, p);
+  return launch(whole ? paged_kernel<T, kFp8, D, kNT, true> : paged_kernel<T, kFp8, D, kNT, false>, plan.ctas, kThreads, paged_smem<kFp8, D>(), p.apart, false, stream, p);
 }
 template <typename T, bool kFp8, int D>
 cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t stream) {
@@ -1110,7 +1187,7 @@ cudaError_t launch_paged(const PagedParams& p, const Plan& plan, cudaStream_t st
   cudaError_t e = fp8 ? (d64 ? launch_paged<T, true, 64>(p, plan, stream) : launch_paged<T, true, 128>(p, plan, stream))
                       : d64 ? launch_paged<T, false, 64>(p, plan, stream) : launch_paged<T, false, 128>(p, plan, stream);
   if (e == cudaSuccess && plan.finish_ctas > 0)
-    e = launch(d64 ? paged_finish_kernel<T, 64> : paged_finish_kernel<T, 128>, plan.finish_ctas, kThreads, 0, true, stream, p);
+    e = launch(d64 ? paged_finish_kernel<T, 64> : paged_finish_kernel<T, 128>, plan.finish_ctas, kThreads, 0, 1, true, stream, p);
   return e;
 }
 
@@ -1126,12 +1203,12 @@ int fftopk_paged_workspace_bytes(const fftopk_paged* a, size_t* bytes) {
   *bytes = 0;
   int rc = check(a);
   if (rc || a->seqs == 0 || a->q_heads == 0) return rc;
-  int sms = 0;
-  rc = paged_setup(sms);
+  PagedLimits limits;
+  rc = paged_setup(limits);
   if (rc) return rc;
   PagedParams p;
   Plan plan;
-  rc = make_plan(a, sms, p, plan);
+  rc = make_plan(a, limits, p, plan);
   if (rc == 0) *bytes = (size_t)plan.total;
   return rc;
 }
@@ -1139,12 +1216,12 @@ int fftopk_paged_workspace_bytes(const fftopk_paged* a, size_t* bytes) {
 int fftopk_paged_attention(const fftopk_paged* a, void* workspace, size_t workspace_bytes, uint32_t* status, void* cuda_stream) {
   int rc = check(a);
   if (rc || a->seqs == 0 || a->q_heads == 0) return rc;
-  int sms = 0;
-  rc = paged_setup(sms);
+  PagedLimits limits;
+  rc = paged_setup(limits);
   if (rc) return rc;
   PagedParams p;
   Plan plan;
-  rc = make_plan(a, sms, p, plan);
+  rc = make_plan(a, limits, p, plan);
   if (rc) return rc;
   if (plan.total > 0 && (workspace == nullptr || !on(workspace, 256) || workspace_bytes < (size_t)plan.total)) return FFTOPK_EINVAL;
   if (a->slots <= 1) p.a.k_slot = p.a.v_slot = 0;

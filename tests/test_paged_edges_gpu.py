@@ -56,14 +56,50 @@ def test_many_sequences(B, Hq, longest):
     attend(g, lens, Hq, 1, 8, 64, torch.float16, B % 2 == 0)
 
 
-@pytest.mark.parametrize("Hq,Hk,page,lengths", SHAPES + [(8, 1, 8, (1000, 40)), (12, 1, 8, (333, 600)), (3, 3, 16, (2100, 5))])
+@pytest.mark.parametrize("room,Hq,Hk,page,lengths", [(52000, *x) for x in SHAPES] + [
+    (7000, *x) for x in SHAPES + [(8, 1, 8, (1000, 40)), (12, 1, 8, (333, 600)), (3, 3, 16, (2100, 5))]])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("fp8", [False, True])
-def test_wide_tables(fp8, D, Hq, Hk, page, lengths):
-    """Tables with room for 7,000 positions, most of it unused: runs that hold many sequences and parts of them, several pairs to a warp of the join."""
+def test_wide_tables(fp8, D, room, Hq, Hk, page, lengths):
+    """Tables with room for 7,000 and 52,000 positions, most of it unused: clusters whose CTAs have less than a block each; runs that hold many
+    sequences and parts of them, several pairs to a warp of the join."""
     g = gen(Hq * page + D + 1)
     lens = ragged(g, *lengths) if isinstance(lengths, tuple) else lengths
-    attend(g, lens, Hq, Hk, page, D, torch.bfloat16, fp8, extra=7000 // page)
+    attend(g, lens, Hq, Hk, page, D, torch.bfloat16, fp8, extra=room // page)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_runs_and_their_join_in_a_graph(fp8):
+    """Room for long sequences: equal runs and a second kernel, captured with lengths that change between replays, two graphs side by side."""
+    g = gen(17)
+    page, Hk = 64, 4
+    table, pages = make_pages(g, [13000, 9000, 20000], page)
+    q = rand(g, 3, 32, 128, dtype=torch.bfloat16)
+    k, ks = make_cache(g, pages * page, Hk, 128, torch.bfloat16, fp8)
+    v, vs = make_cache(g, pages * page, Hk, 128, torch.bfloat16, fp8)
+    n = torch.tensor([13000, 9000, 20000], device="cuda", dtype=torch.int32)
+    kw = dict(page_size=page, k_scale=ks, v_scale=vs, return_lse=True)
+    w = [torch.zeros(3, Hk, 20000, device="cuda") for _ in range(3)]
+    paged_attention(q, k, v, table, n, weight_out=w[2], **kw)
+    graphs = []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            r = paged_attention(q, k, v, table, n, weight_out=w[i] if i else None, **kw)
+        graphs.append((graph, r))
+    for lens in ([13000, 9000, 20000], [1, 0, 19999], [0, 0, 0], [12999, 17, 64]):
+        n.copy_(torch.tensor(lens, dtype=torch.int32))
+        for x in w:
+            x.fill_(float("nan"))
+        for graph, _ in graphs:
+            graph.replay()
+        a = paged_attention(q, k, v, table, n, weight_out=w[2], **kw)
+        want, at = paged.attention(q, k, v, table, n, page, None, ks, vs)
+        ref.check_attention(*a, want)
+        for _, r in graphs:
+            assert torch.equal(r[0], a[0]) and torch.equal(r[1], a[1])
+        assert torch.equal(w[1].view(torch.int32), w[2].view(torch.int32))
+        paged.check_weights(w[2], None, n, *paged.weights(q, k, at, want, None, ks))
 
 
 @pytest.mark.parametrize("fp8", [False, True])

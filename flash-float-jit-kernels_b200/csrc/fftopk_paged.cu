@@ -69,6 +69,7 @@ struct PagedParams {
   int32_t apart;      // CTAs of a cluster that takes a sequence, whatever its length: no parts; 0: equal runs
   FastDiv page;
   float scale_log2;
+  int32_t weigh_here;  // the weights are brought up to date by the CTAs that have made the scores: nothing of a sequence is elsewhere
   int32_t stream;   // the rows are more than L2 holds
   int32_t out_vec;  // rows of out start on 8 bytes
   int64_t line;     // positions of a unit of the score workspace
@@ -253,11 +254,12 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   constexpr int kTiles = D / 16;             // of the output: rows of the MMA are channels
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   // (only where a kernel of this call follows, which waits: another one's inputs may be this one's results)
-  if (p.join_ctas > 0 || p.weigh) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.join_ctas > 0 || (p.weigh && !p.weigh_here)) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   __shared__ float2 ml_of[kWarps][kNH];
   __shared__ uint32_t free_of[kWarps];  // the warps' free stages
-  __shared__ float2 joined_ml[kNH];     // of a CTA of a cluster: maximum and sum
+  __shared__ float2 joined_ml[kNH];     // of a CTA: maximum and sum
+  __shared__ float log_sum[kNH];        // of a sequence
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, qd = lane & 3;
   const uint32_t ctas = (uint32_t)max(p.apart, 1), run_unit = blockIdx.x / ctas, rank = blockIdx.x - run_unit * ctas;
@@ -706,7 +708,41 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
       if (d == 0) {
         const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
         if (p.a.lse != nullptr) p.a.lse[here.b * p.a.q_heads + head0 + h] = l2 * 0.693147180559945309f;
-        if (p.weigh) p.lse2[here.b * p.a.q_heads + head0 + h] = l2;
+        if (p.weigh && !p.weigh_here) p.lse2[here.b * p.a.q_heads + head0 + h] = l2;
+      }
+    };
+    // the weights of the segment's positions, from the scores that the CTA has written and the sums of all of the sequence
+    auto weigh = [&]() {
+      if (threadIdx.x < kNH) {
+        float m = -INFINITY, l = 0.f;
+        for (uint32_t c = 0; c < ctas; ++c) {
+          const float2 ml = ctas > 1 ? lds_cluster2(shared_of(smem_u32(&joined_ml[threadIdx.x]), (int)c)) : joined_ml[threadIdx.x];
+          const float top = fmaxf(m, ml.x);
+          l = brought(l, m, top) + brought(ml.y, ml.x, top);
+          m = top;
+        }
+        log_sum[threadIdx.x] = l == 0.f ? INFINITY : m + log2f(l);  // (without keys: everything counts nothing against infinity)
+      }
+      __syncthreads();
+      const float* w = p.a.weight != nullptr ? p.a.weight + here.b * p.a.w_seq + (int64_t)kvh * p.a.w_head : nullptr;
+      float* wo = p.a.weight_out + here.b * p.a.wo_seq + (int64_t)kvh * p.a.wo_head;
+      const float* s = p.scores + (here.b * p.units + unit) * p.line * kNH;
+      const int64_t upto = min((int64_t)here.n, (int64_t)here.s1 * kKeys);
+#pragma unroll 2
+      for (int64_t j = (int64_t)here.s0 * kKeys + threadIdx.x; j < upto; j += kThreads) {
+        if (j < p.a.weight_cols) {
+          float y = w != nullptr ? w[j] : 0.f;
+#pragma unroll
+          for (int i = 0; i < kNH / 4; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(s + j * kNH + 4 * i);
+            const float e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) y += 4 * i + u < heads ? ex2(e[u] - log_sum[4 * i + u]) : 0.f;
+          }
+          wo[j] = y;
+        } else if (p.status) {
+          atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
+        }
       }
     };
     if (ctas > 1) {
@@ -751,6 +787,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
         }
         finish(h, d, m, l, all);
       }
+      if (p.weigh_here) weigh();
       cluster.sync();  // (nobody leaves while its memory is read)
       return;
     }
@@ -760,12 +797,14 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
       const float4 y = joined(h, d, m, l);
       if (whole) {
         finish(h, d, m, l, y);
+        if (d == 0) joined_ml[h] = make_float2(m, l);
       } else {
         *reinterpret_cast<float4*>(p.o + (rec * kNH + h) * D + d) = y;
         if (d == 0) p.ml[rec * kNH + h] = make_float2(m, l);
       }
     }
     __syncthreads();
+    if (p.weigh_here) weigh();  // (one segment a CTA)
     left -= here.s1 - here.s0;
     if (left <= 0 || !next_segment(p, here, left)) break;
     quarter(here, warp, at, end);
@@ -1136,7 +1175,8 @@ int make_plan(const fftopk_paged* a, const PagedLimits& limits, PagedParams& p, 
     if (p.line > 0 && a->seqs * units > ((int64_t)1 << 50) / (p.line * plan.nh)) return FFTOPK_ERANGE;
     plan.bytes[3] = up256(a->seqs * units * p.line * plan.nh * 4);
   }
-  if (p.weigh) {
+  p.weigh_here = p.weigh && p.apart && p.head_blocks == 1;
+  if (p.weigh && !p.weigh_here) {
     int64_t each = (int64_t)sms * 8 * kWarps / a->kv_heads;
     if (each > blocks) each = blocks;
     if (each < 1) each = 1;

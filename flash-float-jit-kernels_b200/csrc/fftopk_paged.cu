@@ -731,15 +731,16 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
 #pragma unroll 2
       for (int64_t j = (int64_t)here.s0 * kKeys + threadIdx.x; j < upto; j += kThreads) {
         if (j < p.a.weight_cols) {
-          float y = w != nullptr ? w[j] : 0.f;
+          const float before = w != nullptr ? w[j] : 0.f;
+          float sum = 0.f;  // (of its own: what has been added up over many calls is far larger than a head's weight, and is rounded once)
 #pragma unroll
           for (int i = 0; i < kNH / 4; ++i) {
             const float4 x = *reinterpret_cast<const float4*>(s + j * kNH + 4 * i);
             const float e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int u = 0; u < 4; ++u) y += 4 * i + u < heads ? ex2(e[u] - log_sum[4 * i + u]) : 0.f;
+            for (int u = 0; u < 4; ++u) sum += 4 * i + u < heads ? ex2(e[u] - log_sum[4 * i + u]) : 0.f;
           }
-          wo[j] = y;
+          wo[j] = before + sum;
         } else if (p.status) {
           atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
         }
@@ -1015,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 5) paged_finish_kernel(const __grid_
               float sum = 0.f;
 #pragma unroll
               for (int n = 0; n < 8; ++n) sum += h8 + n < heads ? ex2(e[n] - all8[n]) : 0.f;
-              wo[j] = y[u] + sum;
+              wo[j] = y[u] + sum;  // (rounded once for every eight heads)
             } else if (j < upto && p.status) {
               atomicOr(p.status, (uint32_t)FFTOPK_ST_BAD_INDEX);
             }

@@ -160,3 +160,22 @@ def test_evict_by_parts_of_a_wider_pool():
         assert torch.equal(got[0].cpu(), kept) and torch.equal(got[1].cpu(), left) and torch.equal(got[2].cpu(), out)
         for x, y in zip(part, data):
             assert torch.equal(x.view(torch.int16), paged.move(y, kept, table[b:b + 1], to[:1], 16).view(torch.int16))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("Hq,page", [(8, 16), (16, 16), (16, 5), (5, 32)])
+@pytest.mark.parametrize("extra", [0, 3000])
+def test_weights_onto_large_ones(fp8, Hq, page, extra):
+    """What many calls have added up is rounded once more by this one (by two eights of heads: twice), not once for every head."""
+    g = gen(Hq * page)
+    lens = [900, 31, 0]
+    table, pages = make_pages(g, lens, page, extra)
+    q = rand(g, 3, Hq, 128, dtype=torch.bfloat16, scale=2.0)
+    k, ks = make_cache(g, pages * page, 1, 128, torch.bfloat16, fp8)
+    v, vs = make_cache(g, pages * page, 1, 128, torch.bfloat16, fp8)
+    n = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    before = 3e4 + 3e4 * torch.rand(3, 1, 900, generator=g, device="cuda")
+    after = torch.full_like(before, float("nan"))
+    paged_attention(q, k, v, table, n, page_size=page, k_scale=ks, v_scale=vs, weight=before, weight_out=after)
+    want, at = paged.attention(q, k, v, table, n, page, None, ks, vs)
+    paged.check_weights(after, before, n, *paged.weights(q, k, at, want, None, ks))

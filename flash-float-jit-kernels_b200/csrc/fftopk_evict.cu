@@ -461,6 +461,12 @@ extern "C" int fftopk_cache_evict(const fftopk_evict* a, uint32_t* status, void*
     return FFTOPK_ERANGE;
   const int64_t units = a->seqs * a->heads;
   if (units * ((a->budget + 7) / 8) > 0x7fffffff) return FFTOPK_ERANGE;
+  // (rows written twice would hold whichever came last; lengths are read while new_lengths are written)
+  if (!rows_apart(a->seqs, a->wo_seq, a->heads, a->wo_head, a->weight_cols) || !rows_apart(a->slots, a->k_slot, a->heads, a->k_head, a->D) ||
+      !rows_apart(a->slots, a->v_slot, a->heads, a->v_head, a->D) || a->lengths == a->new_lengths)
+    return FFTOPK_EINVAL;
+  if (a->k_scale != nullptr && (!rows_apart(a->slots, a->ks_slot, a->heads, a->ks_head, 1) || !rows_apart(a->slots, a->vs_slot, a->heads, a->vs_head, 1)))
+    return FFTOPK_EINVAL;
   int sms = 0;
   const int rc = evict_setup(sms);
   if (rc) return rc;

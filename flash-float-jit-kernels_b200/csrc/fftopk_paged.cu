@@ -1257,6 +1257,9 @@ int fftopk_paged_workspace_bytes(const fftopk_paged* a, size_t* bytes) {
 int fftopk_paged_attention(const fftopk_paged* a, void* workspace, size_t workspace_bytes, uint32_t* status, void* cuda_stream) {
   int rc = check(a);
   if (rc || a->seqs == 0 || a->q_heads == 0) return rc;
+  // (rows written twice would hold whichever came last)
+  if (!rows_apart(a->seqs, a->out_seq, a->q_heads, a->out_head, a->D)) return FFTOPK_EINVAL;
+  if (a->weight_out != nullptr && !rows_apart(a->seqs, a->wo_seq, a->kv_heads, a->wo_head, a->weight_cols)) return FFTOPK_EINVAL;
   PagedLimits limits;
   rc = paged_setup(limits);
   if (rc) return rc;

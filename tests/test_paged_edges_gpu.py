@@ -179,3 +179,33 @@ def test_weights_onto_large_ones(fp8, Hq, page, extra):
     paged_attention(q, k, v, table, n, page_size=page, k_scale=ks, v_scale=vs, weight=before, weight_out=after)
     want, at = paged.attention(q, k, v, table, n, page, None, ks, vs)
     paged.check_weights(after, before, n, *paged.weights(q, k, at, want, None, ks))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_broadcast_views(fp8):
+    """One query for all sequences and heads, one table row for all sequences, weights that key heads share: read as they are. As results
+    they are refused."""
+    g = gen(91)
+    B, Hq, Hk, D, page, n = 3, 8, 2, 64, 16, 150
+    table, pages = make_pages(g, [n], page)
+    table = table.expand(B, -1)
+    q = rand(g, 1, 1, D, dtype=torch.float16, scale=2.0).expand(B, Hq, D)
+    k, ks = make_cache(g, pages * page, Hk, D, torch.float16, fp8)
+    v, vs = make_cache(g, pages * page, Hk, D, torch.float16, fp8)
+    lens = torch.tensor([n, 77, 0], device="cuda", dtype=torch.int32)
+    before = weights(g, B, 1, n).expand(B, Hk, n)
+    after = torch.full((B, Hk, n), float("nan"), device="cuda")
+    scales = dict(page_size=page, k_scale=ks, v_scale=vs)
+    out, lse = paged_attention(q, k, v, table, lens, weight=before, weight_out=after, return_lse=True, **scales)
+    want, at = paged.attention(q, k, v, table, lens, page, None, ks, vs)
+    ref.check_attention(out, lse, want)
+    paged.check_weights(after, before, lens, *paged.weights(q, k, at, want, None, ks))
+    with pytest.raises(RuntimeError):
+        paged_attention(q, k, v, table, lens, weight=before, **scales)
+    with pytest.raises(RuntimeError):
+        paged_attention(q, k, v, table, lens, out=torch.empty_like(out[:1]).expand(B, Hq, D), **scales)
+    to = torch.arange(B * 4, device="cuda", dtype=torch.int32).view(B, 4) % pages
+    with pytest.raises(RuntimeError):
+        cache_evict(k, v, after, table, lens, to, budget=40, weight_out=before, **scales)
+    with pytest.raises(RuntimeError):
+        cache_evict(k[:, :1].expand_as(k), v, after, table, lens, to, budget=40, **scales)

@@ -37,6 +37,14 @@ def test_paged_attention(want, call):
     assert _native.lib().fftopk_paged_workspace_bytes(blob, ctypes.byref(n)) == want and n.value == 0
 
 
+@pytest.mark.parametrize("call", [
+    dict(os=127), dict(os=0), dict(oh=0), dict(oh=-127), dict(wo=A, cols=8, wos=7), dict(wo=A, cols=8, wos=0), dict(w=A, wo=A, cols=1),
+    dict(wo=A, cols=8, wos=16, kv_heads=2, kh=128, woh=7)])
+def test_results_on_one_another(call):
+    """Broadcast views as results: their rows would hold whichever was written last."""
+    assert _native.lib().fftopk_paged_attention(_ARGS.pack(*{**CALL, **call}.values()), None, 0, None, None) == EINVAL
+
+
 def test_without_arguments():
     n = ctypes.c_size_t()
     assert _native.lib().fftopk_paged_attention(None, None, 0, None, None) == EINVAL
@@ -61,6 +69,16 @@ EVICT = dict(k=A, ks=128, kh=128, v=A, vs=128, vh=128, k_scale=0, kss=0, ksh=0, 
     (ERANGE, dict(seqs=1 << 27, budget=1 << 20, to_pages=1 << 16)), (0, dict(seqs=0)), (0, dict(heads=0))])
 def test_cache_evict(want, call):
     assert _native.lib().fftopk_cache_evict(_EVICT.pack(*{**EVICT, **call}.values()), None, None) == want
+
+
+@pytest.mark.parametrize("call", [
+    dict(wos=63), dict(wos=0), dict(heads=2, wos=128, kh=12800, vh=12800, woh=0), dict(heads=2, wos=128, kh=0, vh=12800),
+    dict(heads=2, wos=128, kh=12800, vh=127), dict(ks=0), dict(vs=127), dict(k_scale=A, v_scale=A, kss=0, vss=1),
+    dict(k_scale=A, v_scale=A, kss=1, vss=0), dict()])
+def test_evict_results_on_one_another(call):
+    """Broadcast views as results; and (the last) lengths that would be read while the new ones are written."""
+    blob = _EVICT.pack(*{**EVICT, "new": 2 * A if call else A, **call}.values())
+    assert _native.lib().fftopk_cache_evict(blob, None, None) == EINVAL
 
 
 def test_evict_without_arguments():

@@ -23,7 +23,7 @@ LIB_PATH = LIB_DIR / "libfftopk.so"
 SOURCES = [CSRC / "fftopk_select.cu", CSRC / "fftopk_cp.cu", CSRC / "fftopk_hostio.cu", CSRC / "fftopk_indexer.cu",
            CSRC / "fftopk_rows.cu", CSRC / "fftopk_rows_axes.cu", CSRC / "fftopk_attend.cu",
            CSRC / "fftopk_attend_wide.cu", CSRC / "fftopk_paged.cu", CSRC / "fftopk_evict.cu"]
-HEADERS = [CSRC / "fftopk_device.cuh", CSRC / "fftopk_key.h", CSRC / "fftopk_host.h", CSRC / "fftopk_trace.cuh",
+HEADERS = [CSRC / "fftopk_device.cuh", CSRC / "fftopk_key.h", CSRC / "fftopk_host.h", CSRC / "fftopk_extent.h", CSRC / "fftopk_trace.cuh",
            CSRC / "fftopk_internal.h", CSRC / "fftopk_decide.h", CSRC / "fftopk_merge.cuh", CSRC / "fftopk_rows.cuh", CSRC / "fftopk_head_rows.cuh", CSRC / "fftopk_tcgen05.cuh", CSRC / "fftopk_attend.cuh",
            ROOT.parent / "include" / "fftopk.h"]
 

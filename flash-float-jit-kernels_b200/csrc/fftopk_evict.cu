@@ -17,6 +17,7 @@
 
 #include "../../include/fftopk.h"
 #include "fftopk_attend.cuh"
+#include "fftopk_extent.h"
 #include "fftopk_host.h"
 #include "fftopk_internal.h"
 #include "fftopk_key.h"

@@ -38,6 +38,7 @@
 
 #include "../../include/fftopk.h"
 #include "fftopk_attend.cuh"
+#include "fftopk_extent.h"
 #include "fftopk_host.h"
 #include "fftopk_internal.h"
 #include "fftopk_rows.cuh"

@@ -448,7 +448,7 @@ extern "C" int fftopk_cache_evict(const fftopk_evict* a, uint32_t* status, void*
   if (a->seqs == 0 || a->heads == 0) return FFTOPK_OK;
   if ((a->k_scale != nullptr) != (a->v_scale != nullptr)) return FFTOPK_EINVAL;
   if (!a->lengths || !a->new_lengths || (a->pages > 0 && !a->page_table) || (a->budget > 0 && (!a->to_table || !a->kept))) return FFTOPK_EINVAL;
-  if (a->weight_cols > 0 && (!a->weight || !a->weight_out || a->weight == a->weight_out)) return FFTOPK_EINVAL;
+  if (a->weight_cols > 0 && (!a->weight || !a->weight_out)) return FFTOPK_EINVAL;
   if (a->slots > 0 && (!a->k || !a->v)) return FFTOPK_EINVAL;
   if (!on(a->k, a->elem_bytes) || !on(a->v, a->elem_bytes) || !on(a->k_scale, 4) || !on(a->v_scale, 4) || !on(a->weight, 4) || !on(a->weight_out, 4) ||
       !on(a->page_table, 4) || !on(a->to_table, 4) || !on(a->lengths, 4) || !on(a->new_lengths, 4) || !on(a->kept, 4))
@@ -468,6 +468,8 @@ extern "C" int fftopk_cache_evict(const fftopk_evict* a, uint32_t* status, void*
     return FFTOPK_EINVAL;
   if (a->k_scale != nullptr && (!rows_apart(a->slots, a->ks_slot, a->heads, a->ks_head, 1) || !rows_apart(a->slots, a->vs_slot, a->heads, a->vs_head, 1)))
     return FFTOPK_EINVAL;
+  // (a unit's weights are read while another one's are written)
+  if (rows_meet(a->weight, a->w_seq, a->w_head, a->weight_out, a->wo_seq, a->wo_head, a->seqs, a->heads, a->weight_cols, 4)) return FFTOPK_EINVAL;
   int sms = 0;
   const int rc = evict_setup(sms);
   if (rc) return rc;

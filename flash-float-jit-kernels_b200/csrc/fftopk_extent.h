@@ -17,12 +17,14 @@ inline Wide floor_div(Wide a, Wide b) { return a / b - (a % b != 0 && (a < 0) !=
 // [lo, hi]: with the longest steps in front, hardly any where rows lie side by side.
 inline bool reaches(const Steps* t, int n, Wide x, Wide lo, Wide hi) {
   if (n == 0) return lo <= x && x <= hi;
-  Wide least = 0, most = 0;
-  for (int i = 1; i < n; ++i) {
+  Wide least = 0, most = 0, first_least = 0, first_most = 0;
+  for (int i = n - 1; i >= 0; --i) {
+    if (t[i].lo > t[i].hi) return false;
+    least += first_least, most += first_most;
     const Wide a = t[i].step * t[i].lo, b = t[i].step * t[i].hi;
-    least += a < b ? a : b, most += a < b ? b : a;
+    first_least = a < b ? a : b, first_most = a < b ? b : a;
   }
-  if (t->lo > t->hi) return false;
+  if (x + first_most + most < lo || x + first_least + least > hi) return false;
   if (t->step == 0) return reaches(t + 1, n - 1, x, lo, hi);
   // least element + most >= lo, and element + least <= hi
   const Wide from = lo - most - x, upto = hi - least - x, s = t->step;
@@ -48,6 +50,30 @@ inline bool rows_apart(int64_t seqs, int64_t seq, int64_t heads, int64_t head, i
   const Steps by_seq = {s, 1, (Wide)seqs - 1}, by_head = {-h, 1, (Wide)heads - 1};
   const Steps t[2] = {seq_long ? by_seq : by_head, seq_long ? by_head : by_seq};
   return !reaches(t, 2, 0, 1 - (Wide)width, (Wide)width - 1);
+}
+
+// Has a row of `a` an element in common with a row of `b`? Both are seqs times heads rows of `width` elements of `bytes` each, at strides of their own (in
+// elements); rows in between the other one's are fine.
+inline bool rows_meet(const void* a, int64_t a_seq, int64_t a_head, const void* b, int64_t b_seq, int64_t b_head, int64_t seqs, int64_t heads, int64_t width,
+                      int bytes) {
+  if (seqs <= 0 || heads <= 0 || width <= 0) return false;
+  Steps t[4];
+  int n = 0;
+  auto add = [&](int64_t step, Wide lo, Wide hi) {  // (the longest in front)
+    int i = n++;
+    const Wide s = (Wide)step * bytes, abs = s < 0 ? -s : s;
+    for (; i > 0 && (t[i - 1].step < 0 ? -t[i - 1].step : t[i - 1].step) < abs; --i) t[i] = t[i - 1];
+    t[i] = {s, lo, hi};
+  };
+  auto both = [&](int64_t rows, int64_t of_a, int64_t of_b) {
+    if (of_a == of_b) return add(of_a, 1 - (Wide)rows, (Wide)rows - 1);
+    add(of_b, 0, (Wide)rows - 1);
+    add(of_a, 1 - (Wide)rows, 0);
+  };
+  if (seqs > 1) both(seqs, a_seq, b_seq);  // (the stride of a lone one says nothing)
+  if (heads > 1) both(heads, a_head, b_head);
+  const Wide from = (Wide)reinterpret_cast<uintptr_t>(b) - (Wide)reinterpret_cast<uintptr_t>(a), row = (Wide)width * bytes;
+  return reaches(t, n, from, 1 - row, row - 1);
 }
 
 }  // namespace fftopk

@@ -1261,6 +1261,12 @@ int fftopk_paged_attention(const fftopk_paged* a, void* workspace, size_t worksp
   // (rows written twice would hold whichever came last)
   if (!rows_apart(a->seqs, a->out_seq, a->q_heads, a->out_head, a->D)) return FFTOPK_EINVAL;
   if (a->weight_out != nullptr && !rows_apart(a->seqs, a->wo_seq, a->kv_heads, a->wo_head, a->weight_cols)) return FFTOPK_EINVAL;
+  // (q is read by several CTAs, at different times; weights by other threads than those that write what is elsewhere)
+  if (rows_meet(a->q, a->q_seq, a->q_head, a->out, a->out_seq, a->out_head, a->seqs, a->q_heads, a->D, 2)) return FFTOPK_EINVAL;
+  const bool in_place = a->weight == a->weight_out && (a->seqs == 1 || a->w_seq == a->wo_seq) && (a->kv_heads == 1 || a->w_head == a->wo_head);
+  if (a->weight != nullptr && !in_place &&
+      rows_meet(a->weight, a->w_seq, a->w_head, a->weight_out, a->wo_seq, a->wo_head, a->seqs, a->kv_heads, a->weight_cols, 4))
+    return FFTOPK_EINVAL;
   PagedLimits limits;
   rc = paged_setup(limits);
   if (rc) return rc;

@@ -142,8 +142,8 @@ def cache_evict(
         budget: rows that a key head keeps; a sequence of up to that many keeps (and moves) all of them.
         recent, sinks: of those, the last and the first rows of the sequence, whatever their weight. Between them the largest weights
             stay, of equal ones the lower positions (NaN counts as the largest).
-        weight_out: float32 [B, Hk, N] for the weights of what stays, zeros behind (default: a new tensor; not weight itself, no
-            broadcast view).
+        weight_out: float32 [B, Hk, N] for the weights of what stays, zeros behind (default: a new tensor; apart from weight,
+            no broadcast view).
     Returns:
         (kept, lengths, weight_out): int32 [B, Hk, budget], the positions that stayed in ascending order, -1 behind them; int32 [B],
         the new lengths; the weights. Rows on negative pages or beyond the cache are not copied and show up in kernel_status(), as do

@@ -52,7 +52,8 @@ def paged_attention(
             place; weight_out alone: this call's. Behind a sequence's length weight_out stays as it was. The call then takes
             4 bytes of workspace per query head (rounded up to eights of a key head's) and position the table has room for: hand in a
             page_table as wide as the longest sequence.
-        out: [B, Hq, D] of q's type for the result, apart from q. (Like weight_out no broadcast view.)
+        out: [B, Hq, D] of q's type for the result, apart from q (and weight_out, where it is not weight, from weight): rows in one buffer
+            are fine, on one another they are refused. (Neither is a broadcast view.)
     Returns:
         out, or (out, lse) with lse float32 [B, Hq], the log of the sum of exponentials. A sequence without rows: 0 and -inf.
     """

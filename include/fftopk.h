@@ -482,8 +482,9 @@ int fftopk_sparse_attention(const fftopk_attend* args, uint32_t* status, void* c
  *   lse          fp32 [seqs, q_heads], contiguous, or NULL
  *   weight       fp32 [seqs, kv_heads, weight_cols], inner stride 1, or NULL; weight_out likewise, or NULL: no weights; the two may be
  *                one array, and overlap in no other way
- *   out, lse and weight_out overlap no input, but for weight_out and weight; rows of out, and of weight_out, lie apart (FFTOPK_EINVAL where
- *                two of them have an element in common: no broadcast views, no strides of which one runs into the other's rows)
+ *   out, lse and weight_out overlap no input, but for weight_out and weight; rows of out, and of weight_out, lie apart. FFTOPK_EINVAL where two
+ *                of those rows have an element in common (broadcast views, strides of which one runs into the other's rows), or one of out and one
+ *                of q, or - unless they are one array - one of weight_out and one of weight; rows in between others are fine
  *   strides      in elements; rows of q, k and v start on 16 bytes, slots of k and v less than 2^32 bytes apart (FFTOPK_ERANGE); page_size any
  *                number from 1
  *   workspace    fftopk_paged_workspace_bytes bytes of device memory, 256-byte aligned, any contents; calls that may run at the same
@@ -536,7 +537,8 @@ int fftopk_paged_attention(const fftopk_paged* args, void* workspace, size_t wor
  *   k, v         [slots, heads, D] of elem_bytes (1 or 2) each, D a multiple of 8 up to 256 (FFTOPK_ERANGE otherwise); k_scale, v_scale fp32
  *                [slots, heads], or both NULL; strides in elements
  *   weight, weight_out fp32 [seqs, heads, weight_cols], inner stride 1, apart from one another; rows of weight_out, of a cache, and of scales lie
- *                apart (FFTOPK_EINVAL where two of them have an element in common: no broadcast views, no strides of which one runs into the other's rows)
+ *                apart. FFTOPK_EINVAL where two of those rows, or one of weight and one of weight_out, have an element in common (broadcast views,
+ *                strides of which one runs into the other's rows); rows in between others are fine
  *   page_table   int32 [seqs, pages], to_table int32 [seqs, to_pages], inner stride 1; to_pages * page_size >= budget (FFTOPK_ERANGE otherwise)
  *   kept         int32 [seqs, heads, budget], contiguous; lengths, new_lengths int32 [seqs]; sinks + recent <= budget
  *                No output overlaps an input (the caches aside, see above). Slots of k and v lie less than 2^32 bytes apart (FFTOPK_ERANGE).

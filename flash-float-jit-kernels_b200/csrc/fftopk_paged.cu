@@ -56,7 +56,7 @@ constexpr int kWeighKeys = 128;  // positions that a warp has on their way at a 
 // positions of a run: below that, parts to join cost more than the blocks (one sequence of 1,000, 8 key heads: 8.8 us, with 256 positions 10.7, with 512
 // 15.4; of 4,096: 9.6, 10.3 and 12.3, with 64 11.3)
 constexpr int kMinKeys = 128;
-// Keys of a block, 16 to a product: 8 KB of k and v, so that what goes with a block is done for enough of them (64 sequences of up to 8,192, 8 key heads, with
+// Keys of a block, 16 to a product: 8 KB of k and v (4 KB of e4m3 heads of 64), so that what goes with a block is done for enough of them (64 sequences of up to 8,192, 8 key heads, with
 // 16 keys and with 32: 16 bits, heads of 64 137 us and 128; e4m3, 16 query heads to a key head 187 and 152; up to 16,384, heads of 64 174 and 138)
 template <bool kFp8, int D>
 constexpr int block_keys() {
@@ -226,7 +226,7 @@ struct PagedRing {
   static constexpr int kV = kKeys * kRowBytes, kStage = 2 * kV;
   static constexpr int kStages = 3;
   static constexpr int kScales = kStages * kStage, kScaleStage = kFp8 ? 2 * kKeys * 4 : 0;
-  static constexpr int kBytes = kScales + kStages * (kFp8 ? 256 : 0);  // of a warp
+  static constexpr int kBytes = kScales + kStages * kScaleStage;  // of a warp
   // (rows of 64 bytes: two of them touch all banks already)
   static __device__ __forceinline__ uint32_t k_piece(int row, int piece) { return (uint32_t)(kRowBytes == 64 ? piece : piece ^ (row & 1) << 2); }
   static __device__ __forceinline__ uint32_t v_piece(int row, int piece) { return (uint32_t)(kRowBytes == 64 ? piece ^ (row >> 1 & 3) : piece ^ (row & 7)); }
@@ -309,14 +309,12 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
   const int piece = lane % kLanesRow, sub = lane / kLanesRow;
   const char* const kbase = static_cast<const char*>(p.a.k) + (int64_t)kvh * p.a.k_head * kES + piece * 16;
   const char* const vbase = static_cast<const char*>(p.a.v) + (int64_t)kvh * p.a.v_head * kES + piece * 16;
-  // (blocks of 16: k scales are asked for by the lower lanes, v scales by the upper ones; of 32: both by every lane)
-  const float *sbase[kR] = {};
-  int64_t sstep[kR] = {};
+  static_assert(!kFp8 || kKeys == 32, "e4m3: a lane has a key of the block, and asks for both of its scales");
+  const float *sbase[2] = {};
+  int64_t sstep[2] = {};
   if constexpr (kFp8) {
-    const bool k = kR == 2 || lane < kKeys;
-    sbase[0] = k ? p.a.k_scale + (int64_t)kvh * p.a.ks_head : p.a.v_scale + (int64_t)kvh * p.a.vs_head;
-    sstep[0] = k ? p.a.ks_slot : p.a.vs_slot;
-    if constexpr (kR == 2) sbase[1] = p.a.v_scale + (int64_t)kvh * p.a.vs_head, sstep[1] = p.a.vs_slot;
+    sbase[0] = p.a.k_scale + (int64_t)kvh * p.a.ks_head, sstep[0] = p.a.ks_slot;
+    sbase[1] = p.a.v_scale + (int64_t)kvh * p.a.vs_head, sstep[1] = p.a.vs_slot;
   }
   const uint32_t kstep = (uint32_t)(p.a.k_slot * kES), vstep = (uint32_t)(p.a.v_slot * kES);
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)warp * G::kBytes;
@@ -397,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
           }
           if constexpr (kFp8) {
 #pragma unroll
-            for (int i = 0; i < kR; ++i) copy4(scales + i * 128u, sbase[i] + (uint64_t)(uint32_t)((int)slot + (lane & (kKeys - 1))) * sstep[i]);
+            for (int i = 0; i < 2; ++i) copy4(scales + i * 128u, sbase[i] + (uint64_t)(uint32_t)((int)slot + lane) * sstep[i]);
           }
         } else if (there > 0) {
 #pragma unroll
@@ -407,9 +405,8 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
             copy16_or_zero(data + G::kV + at * G::kRowBytes + G::v_piece(at, piece) * 16u, row_at(vbase, r, vstep), at < there, once);
           }
           if constexpr (kFp8) {
-            const int at = lane & (kKeys - 1);
 #pragma unroll
-            for (int i = 0; i < kR; ++i) copy_or_zero<4>(scales + i * 128u, sbase[i] + (uint64_t)(uint32_t)((int)slot + min(at, there - 1)) * sstep[i], at < there);
+            for (int i = 0; i < 2; ++i) copy_or_zero<4>(scales + i * 128u, sbase[i] + (uint64_t)(uint32_t)((int)slot + min(lane, there - 1)) * sstep[i], lane < there);
           }
         }
       }
@@ -432,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, paged_ctas<kFp8, D, kNT>()) paged_ke
         }
         if constexpr (kFp8) {
 #pragma unroll
-          for (int i = 0; i < kR; ++i) copy_or_zero<4>(scales + i * 128u, sbase[i] + (uint64_t)(uint32_t)max(row, 0) * sstep[i], ok);
+          for (int i = 0; i < 2; ++i) copy_or_zero<4>(scales + i * 128u, sbase[i] + (uint64_t)(uint32_t)max(row, 0) * sstep[i], ok);
         }
       }
     }

@@ -4,8 +4,9 @@
 // to date: weight_out[b, h / g, j] = weight[b, h / g, j] + sum of p_j over the key head's query heads. (The reference ends with indices.)
 //
 // What bounds it is reading the cache: a row of k or v is used by the g heads of its key head alone, g flop a byte in 16 bits, 2 g in e4m3 (64
-// query heads on 8 key heads of 128: 64 sequences of up to 8,192 in bf16 243 us = 6.5 TB/s, of up to 16,384 in e4m3 250 = 6.5; one of 131,072 in bf16
-// 91 = 5.9, of which 5 are the join; one of 100: 5.1).
+// query heads on 8 key heads of 128: 64 sequences of up to 8,192 in bf16 243 us = 6.5 TB/s, of up to 16,384 in e4m3 250 = 6.5 in short runs, 271 to 285 =
+// 5.7 to 6.0 after a second of such calls, when the device is at its power limit and instructions bound it; one of 131,072 in bf16 91 = 5.9, of which 5 are the
+// join; one of 100: 5.1).
 //
 // Work split: the context, 16 or 32 keys a block, of all sequences, sequence after sequence, is one line of blocks. It is cut into equal
 // runs, whatever the lengths; a CTA takes one run for one key head (8 or 16 of its query heads). The CTAs of neighbouring numbers take the same
